@@ -800,6 +800,101 @@ int dressi_tex_profile(dressi_tex_plan* plan, uint32_t iters, char* names,
                        size_t name_stride, float* usec, uint32_t cap,
                        uint32_t* n);
 
+/* ------------------------------------------------------------------------ */
+/* Training a neural shader: group norm and AdamW (no counterpart in the    */
+/* reference, whose graph has its optimizer and no normalisation).          */
+/* ------------------------------------------------------------------------ */
+
+/* Element types of the entry points below. */
+#define DRESSI_F32 0u
+#define DRESSI_BF16 1u
+#define DRESSI_F16 2u
+
+/* Activations: none, max(z, 0), z / (1 + exp(-z)), z Phi(z). */
+#define DRESSI_ACT_NONE 0u
+#define DRESSI_ACT_RELU 1u
+#define DRESSI_ACT_SILU 2u
+#define DRESSI_ACT_GELU 3u
+
+/* Group normalisation of channels-last images with an activation:
+ * y = act((x - mean) rstd w + b), mean and rstd = 1 / sqrt(var + eps) over
+ * the pixels and the n_ch / n_groups channels of each group of each item
+ * (var divides by their number). x is [n_items][n_px][n_ch] of `type` with
+ * the channels next to each other, item_stride and px_stride elements apart;
+ * y is packed. weight / bias [n_ch] of `affine_type`, or NULL for 1 / 0.
+ * mean, rstd [n_items][n_groups]: what the backward pass needs. Sums and
+ * statistics are held in 32 bits. scratch: device memory of at least
+ * dressi_group_norm_scratch bytes (backward: 0 or 1), used by this call
+ * only, so that calls on several streams need several. */
+size_t dressi_group_norm_scratch(uint32_t type, uint32_t n_items,
+                                 uint64_t n_px, uint32_t n_ch,
+                                 uint32_t n_groups, int backward);
+int dressi_group_norm(dressi_ctx* ctx, const void* x, uint32_t type,
+                      uint32_t n_items, uint64_t n_px, uint32_t n_ch,
+                      uint64_t item_stride, uint64_t px_stride,
+                      uint32_t n_groups, const void* weight, const void* bias,
+                      uint32_t affine_type, float eps, uint32_t activation,
+                      void* scratch, size_t scratch_bytes, void* y,
+                      float* mean, float* rstd);
+/* Its gradients: gy packed -> gx packed (of `type`), gw, gb [n_ch] (of
+ * affine_type); any of the three may be NULL. Sums run in a fixed order. */
+int dressi_group_norm_bwd(dressi_ctx* ctx, const void* gy, const void* x,
+                          uint32_t type, uint32_t n_items, uint64_t n_px,
+                          uint32_t n_ch, uint64_t item_stride,
+                          uint64_t px_stride, uint32_t n_groups,
+                          const void* weight, const void* bias,
+                          uint32_t affine_type, uint32_t activation,
+                          const float* mean, const float* rstd, void* scratch,
+                          size_t scratch_bytes, void* gx, void* gw, void* gb);
+
+/* One tensor of an AdamW step: n elements of `type`, packed, updated in
+ * place. Its moments (and its master copy) start at element `state` of the
+ * flat state buffers, a multiple of 32, and take n rounded up to 32; the
+ * filling is zero. `set` names its dressi_adamw_set. */
+typedef struct dressi_adamw_tensor {
+    void* param;
+    const void* grad;
+    uint64_t n;
+    uint64_t state;
+    uint32_t type;
+    uint32_t set;
+} dressi_adamw_tensor;
+/* What tensors share; step counts from 1 for the first. */
+typedef struct dressi_adamw_set {
+    double lr, beta1, beta2, eps, weight_decay;
+    uint64_t step;
+} dressi_adamw_set;
+
+/* One AdamW step over all tensors (decoupled weight decay), computed in 32
+ * bits:
+ *   m = m beta1 + g (1 - beta1);  v = v beta2 + g^2 (1 - beta2)
+ *   p = p (1 - lr wd) - m / (sqrt(v) / sqrt(1 - beta2^t) + eps) lr / (1 - beta1^t)
+ * max_norm > 0: g is the gradient times min(1, max_norm / (|g| + 1e-6)), |g|
+ * the norm over all tensors, which is written to `norm`; this needs
+ * `scratch` of dressi_adamw_scratch bytes. state_bits 32: exp_avg and
+ * exp_avg_sq are float[state_elems], 16-byte aligned. state_bits 8: they are
+ * a byte an element with a scale byte for each 32 in exp_avg_scale /
+ * exp_avg_sq_scale: the largest biased exponent E of the 32, and codes
+ * (bits(|x| 2^-(max(E, T) - T)) + r) >> 20 with T = 14 and the sign in bit 7
+ * for exp_avg, T = 30 for exp_avg_sq; r is a hash of (element, step, seed)
+ * below 2^20. exp_avg_sq above zero has a code above zero; E = 255 stands
+ * for 32 NaN. master (float[state_elems], or NULL): where given, parameters
+ * of 16 bits are roundings of it. */
+size_t dressi_adamw_scratch(void);
+int dressi_adamw_step(dressi_ctx* ctx, const dressi_adamw_tensor* tensors,
+                      uint32_t n_tensors, const dressi_adamw_set* sets,
+                      uint32_t n_sets, uint32_t state_bits,
+                      uint64_t state_elems, void* exp_avg, void* exp_avg_sq,
+                      uint8_t* exp_avg_scale, uint8_t* exp_avg_sq_scale,
+                      float* master, uint32_t seed, float max_norm,
+                      void* scratch, float* norm);
+/* The values that n elements (whole blocks of 32) of 8-bit moments stand
+ * for, as bfloat16, which holds them exactly. */
+int dressi_adamw_values(dressi_ctx* ctx, uint64_t n, const void* exp_avg,
+                        const void* exp_avg_sq, const uint8_t* exp_avg_scale,
+                        const uint8_t* exp_avg_sq_scale, void* exp_avg_bf16,
+                        void* exp_avg_sq_bf16);
+
 #ifdef __cplusplus
 }
 #endif

@@ -44,6 +44,19 @@ class PbrDesc(C.Structure):
                 ("flags", _U)]
 
 
+class AdamwTensor(C.Structure):
+    _fields_ = [("param", _P), ("grad", _P), ("n", C.c_uint64), ("state", C.c_uint64),
+                ("type", _U), ("set", _U)]
+
+
+class AdamwSet(C.Structure):
+    _fields_ = [("lr", C.c_double), ("beta1", C.c_double), ("beta2", C.c_double),
+                ("eps", C.c_double), ("weight_decay", C.c_double), ("step", C.c_uint64)]
+
+
+F32, BF16, F16 = range(3)
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU = range(4)
+
 PBR_KEEP_PRED = 1
 PBR_KEEP_GRAD = 2
 (PBR_LOSS, PBR_PRED, PBR_TARGET, PBR_G_ALBEDO, PBR_G_MR, PBR_G_ENV, PBR_IRR,
@@ -181,6 +194,15 @@ _SIGS = {
     "dressi_tex_buffer": (_I, [_P, _I, C.POINTER(_P), C.POINTER(_S)]),
     "dressi_tex_read": (_I, [_P, _I, _P, _S]),
     "dressi_tex_profile": (_I, [_P, _U, C.c_char_p, _S, _FP, _U, _UP]),
+    "dressi_group_norm_scratch": (_S, [_U, _U, C.c_uint64, _U, _U, _I]),
+    "dressi_group_norm": (_I, [_P, _P, _U, _U, C.c_uint64, _U, C.c_uint64, C.c_uint64, _U, _P, _P,
+                               _U, _F, _U, _P, _S, _P, _P, _P]),
+    "dressi_group_norm_bwd": (_I, [_P, _P, _P, _U, _U, C.c_uint64, _U, C.c_uint64, C.c_uint64, _U,
+                                   _P, _P, _U, _U, _P, _P, _P, _S, _P, _P, _P]),
+    "dressi_adamw_scratch": (_S, []),
+    "dressi_adamw_step": (_I, [_P, _P, _U, _P, _U, _U, C.c_uint64, _P, _P, _P, _P, _P, _U, _F, _P,
+                               _P]),
+    "dressi_adamw_values": (_I, [_P, C.c_uint64, _P, _P, _P, _P, _P, _P]),
 }
 
 EXPORTED = tuple(_SIGS)

@@ -22,13 +22,13 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libdressi_hip.so")
 SOURCES = ["runtime.hip", "raster.hip", "hsr.hip", "aa.hip", "tex.hip", "ds.hip", "surface.hip", "ibl.hip", "pbr.hip",
-           "graph.hip", "executor.hip", "builders.hip", "route.hip"]
+           "graph.hip", "executor.hip", "builders.hip", "route.hip", "group_norm.hip", "adamw.hip"]
 # host-only sources (the examples' asset, geometry and PBR-graph helpers), built with g++;
 # zlib is linked for their deflate streams
 HOST_SOURCES = ["assets.cpp", "jpeg.cpp", "geometry.cpp", "pbr_graph.cpp"]
 HEADERS = ["internal.h", "dressi_math.h", "raster_core.h", "soft_clip.h", "hsr_chain.h",
            "aa_core.h", "plan.h", "ibl_core.h", "graph_ir.h", "route.h", "libm_f32.h",
-           "libm_pow5_table.h", "image_codecs.h", "surface_core.h"]
+           "libm_pow5_table.h", "image_codecs.h", "surface_core.h", "typed.h"]
 ARCH = os.environ.get("DRESSI_OFFLOAD_ARCH", "gfx950")
 
 FLAGS = [

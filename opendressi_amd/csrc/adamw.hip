@@ -1,0 +1,640 @@
+// adamw.hip -- one AdamW step over many parameter tensors at once
+// (dressi_adamw_step), with moments in 32 or in 8 bits.
+//
+// Per element, every operation rounded to float once and in this order, so
+// that the result does not depend on how the work is cut:
+//
+//   g' = g c                     c = min(1, max_norm / (|g|_2 + 1e-6))
+//   m' = m b1 + g' (1 - b1)
+//   v' = v b2 + (g' g') (1 - b2)
+//   p' = p (1 - lr wd) - (m' / (sqrt(v') / sqrt(1 - b2^t) + eps)) (lr / (1 - b1^t))
+//
+// Moments in 8 bits. 32 neighbours share the largest exponent field E of
+// their magnitudes (8 bits). With up = max(E, T) - T the scaled magnitude
+// f = |x| 2^-up has exponent fields of at most T, and its code is
+// (bits(f) + r) >> 20: a float of three mantissa bits with gradual underflow,
+// because the code's subnormals are float's own. T is 14 for the first moment
+// (4 exponent bits and a sign) and 30 for the second (5 exponent bits): one
+// field is left for a rounding that carries. r is uniform in [0, 2^20), a hash
+// of (element, step): the rounding is right on average, without which a second
+// moment that moves by 0.1 % a step would stay where it is, half a step of the
+// code being 3 to 6 %. A second moment above zero never becomes zero: the
+// update would divide by eps. E = 255 (an infinity or a NaN among the 32)
+// makes all 32 NaN. The update itself uses m' and v' as computed, before they
+// are rounded.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "internal.h"
+#include "typed.h"
+
+namespace dressi {
+namespace {
+
+constexpr uint32_t kThreads = 256;
+constexpr uint32_t kLaneElems = 4;  // neighbours of a lane: 16 bytes of float
+constexpr uint32_t kBlock = 32;     // elements that share an exponent
+constexpr int kTop1 = 14, kTop2 = 30;
+constexpr uint32_t kMaxTensors = 72, kMaxSets = 16;
+constexpr uint32_t kMaxPartials = 1024;
+
+struct TensorArg {
+    void* param;
+    const void* grad;
+    uint64_t n;
+    uint64_t state;        // element offset in the flat state buffers
+    uint32_t first_chunk;  // of this launch
+    uint16_t type, set;
+};
+struct SetArg {
+    float b1, omb1, b2, omb2, eps, decay, step_size, inv_bc2;
+    uint32_t key;
+};
+// A launch's tensors: in the kernel arguments, so that no copy to the device
+// and no wait stands between a step's gradients and its kernel. 4 KB at most.
+struct Table {
+    TensorArg t[kMaxTensors];
+    SetArg set[kMaxSets];
+    uint32_t n_tensors, n_chunks;
+};
+static_assert(sizeof(Table) <= 3800, "with the pointers beside it within 4 KB of arguments");
+
+struct State {
+    void* m;
+    void* v;
+    uint8_t* m_scale;
+    uint8_t* v_scale;
+    float* master;
+    const double* partials;  // of the squared norm; null: no clipping
+    uint32_t n_partials;
+    float max_norm;
+    float* norm;
+};
+
+// The tensor that holds `chunk`: the last whose first chunk is not past it.
+// A lane per tensor, one load deep.
+__device__ __forceinline__ uint32_t find_tensor(const Table& tb, uint32_t chunk) {
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t found = 0;
+    for (uint32_t b = 0; b < tb.n_tensors; b += 64) {
+        const uint32_t i = b + lane;
+        const bool at = i < tb.n_tensors && tb.t[i < kMaxTensors ? i : 0].first_chunk <= chunk;
+        found += (uint32_t)__popcll(__ballot(at));
+    }
+    return __builtin_amdgcn_readfirstlane(found - 1);
+}
+
+// ---------------------------------------------------------------------------
+// the squared norm of all gradients
+// ---------------------------------------------------------------------------
+
+// The workgroup's sum of `s`, valid in thread 0.
+__device__ __forceinline__ double block_sum(double s) {
+    __shared__ double part[kThreads / 64];
+    for (int o = 32; o > 0; o >>= 1) {
+        s += __shfl_xor(s, o);
+    }
+    if ((threadIdx.x & 63u) == 0) {
+        part[threadIdx.x >> 6] = s;
+    }
+    __syncthreads();
+    s = part[0];
+    for (uint32_t i = 1; i < kThreads / 64; i++) {
+        s += part[i];
+    }
+    return s;
+}
+
+template <typename T, int ITER>
+__device__ __forceinline__ double chunk_squares(const TensorArg& t, uint64_t at) {
+    const T* g = (const T*)t.grad;
+    double s = 0.0;
+    constexpr uint32_t kStep = kThreads * kLaneElems;
+    const bool vec = ((uintptr_t)g & (kLaneElems * sizeof(T) - 1)) == 0;
+    if (vec && at + (uint64_t)ITER * kStep <= t.n) {
+        float x[ITER][kLaneElems];
+#pragma unroll
+        for (int k = 0; k < ITER; k++) {
+            load_vec<T, kLaneElems>(g + at + (uint64_t)k * kStep + threadIdx.x * kLaneElems, x[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < ITER; k++) {
+#pragma unroll
+            for (uint32_t j = 0; j < kLaneElems; j++) {
+                s = fma((double)x[k][j], (double)x[k][j], s);
+            }
+        }
+    } else {
+        const uint64_t end = std::min<uint64_t>(t.n, at + (uint64_t)ITER * kStep);
+        for (uint64_t i = at + threadIdx.x; i < end; i += kThreads) {
+            const double x = (double)to_float(g[i]);
+            s = fma(x, x, s);
+        }
+    }
+    return s;
+}
+
+// A workgroup's share of sum g^2, in double: a float's square may not be one.
+// One read of the gradients.
+template <int ITER>
+__global__ __launch_bounds__(256) void k_adamw_squares(const Table tb, double* partials) {
+    double s = 0.0;
+    for (uint32_t c = blockIdx.x; c < tb.n_chunks; c += gridDim.x) {
+        const TensorArg& t = tb.t[find_tensor(tb, c)];
+        const uint64_t at = (uint64_t)(c - t.first_chunk) * (ITER * kThreads * kLaneElems);
+        switch (t.type) {
+            case DRESSI_F32:
+                s += chunk_squares<float, ITER>(t, at);
+                break;
+            case DRESSI_BF16:
+                s += chunk_squares<bf16, ITER>(t, at);
+                break;
+            default:
+                s += chunk_squares<f16, ITER>(t, at);
+        }
+    }
+    s = block_sum(s);
+    if (threadIdx.x == 0) {
+        partials[blockIdx.x] = s;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// 8-bit moments
+// ---------------------------------------------------------------------------
+
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// The largest of the 8 lanes that hold a block.
+__device__ __forceinline__ uint32_t block_max(uint32_t x) {
+    x = std::max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xb1, 0xf, 0xf, true));   // lane ^ 1
+    x = std::max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4e, 0xf, 0xf, true));   // lane ^ 2
+    x = std::max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x141, 0xf, 0xf, true));  // 7 - lane
+    return x;
+}
+
+__device__ __forceinline__ int scale_shift(uint32_t field, int top) {
+    return std::max((int)field, top) - top;
+}
+
+__device__ __forceinline__ float decode(uint32_t code, uint32_t field, int top) {
+    const float f = __builtin_ldexpf(__uint_as_float(code << 20), scale_shift(field, top));
+    return field == 255u ? __uint_as_float(0x7fc00000u) : f;
+}
+
+__device__ __forceinline__ uint32_t encode(float x, int up, uint32_t r) {
+    return (__float_as_uint(__builtin_ldexpf(__uint_as_float(abs_bits(x)), -up)) + r) >> 20;
+}
+
+// 32 bits of element i at a step, by two rounds of multiplying and folding.
+__device__ __forceinline__ uint32_t noise(uint64_t i, uint32_t key) {
+    uint32_t x = (uint32_t)i ^ key ^ ((uint32_t)(i >> 32) * 0x85ebca6bu);
+    x = (x ^ (x >> 16)) * 0x7feb352du;
+    x = (x ^ (x >> 15)) * 0x846ca68bu;
+    return x ^ (x >> 16);
+}
+
+struct Moments {
+    float m[kLaneElems], v[kLaneElems];
+};
+
+template <bool Q8>
+__device__ __forceinline__ Moments load_moments(const State& st, uint64_t i) {
+    Moments o;
+    if constexpr (Q8) {
+        const uint32_t cm = *(const uint32_t*)((const uint8_t*)st.m + i);
+        const uint32_t cv = *(const uint32_t*)((const uint8_t*)st.v + i);
+        const uint32_t fm = st.m_scale[i / kBlock], fv = st.v_scale[i / kBlock];
+#pragma unroll
+        for (uint32_t j = 0; j < kLaneElems; j++) {
+            const uint32_t c = (cm >> (8 * j)) & 255u;
+            o.m[j] = __uint_as_float(__float_as_uint(decode(c & 127u, fm, kTop1)) |
+                                     ((c & 128u) << 24));
+            o.v[j] = decode((cv >> (8 * j)) & 255u, fv, kTop2);
+        }
+    } else {
+        load_vec<float, kLaneElems>((const float*)st.m + i, o.m);
+        load_vec<float, kLaneElems>((const float*)st.v + i, o.v);
+    }
+    return o;
+}
+
+// All 64 lanes call this together (the block's maximum crosses lanes); `live`
+// says which hold elements.
+template <bool Q8>
+__device__ __forceinline__ void store_moments(const State& st, uint64_t i, const Moments& o,
+                                              uint32_t key, bool live) {
+    if constexpr (Q8) {
+        uint32_t am = 0, av = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < kLaneElems; j++) {
+            am = std::max(am, abs_bits(o.m[j]));
+            av = std::max(av, abs_bits(o.v[j]));
+        }
+        const uint32_t fm = block_max(am) >> 23, fv = block_max(av) >> 23;
+        const int um = scale_shift(fm, kTop1), uv = scale_shift(fv, kTop2);
+        uint32_t cm = 0, cv = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < kLaneElems; j++) {
+            const uint32_t r = noise(i + j, key);
+            uint32_t a = encode(o.m[j], um, ((r & 0xffffu) << 4) + 8u);
+            uint32_t b = encode(o.v[j], uv, ((r >> 16) << 4) + 8u);
+            b = o.v[j] > 0.f ? std::max(b, 1u) : b;
+            a = fm == 255u ? 0u : a;
+            b = fv == 255u ? 0u : b;
+            cm |= (a | ((__float_as_uint(o.m[j]) >> 24) & 128u)) << (8 * j);
+            cv |= b << (8 * j);
+        }
+        if (live) {
+            *(uint32_t*)((uint8_t*)st.m + i) = cm;
+            *(uint32_t*)((uint8_t*)st.v + i) = cv;
+            if ((threadIdx.x & 7u) == 0) {
+                st.m_scale[i / kBlock] = (uint8_t)fm;
+                st.v_scale[i / kBlock] = (uint8_t)fv;
+            }
+        }
+    } else if (live) {
+        store_vec<float, kLaneElems>((float*)st.m + i, o.m);
+        store_vec<float, kLaneElems>((float*)st.v + i, o.v);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// the step
+// ---------------------------------------------------------------------------
+
+template <bool Q8>
+__device__ __forceinline__ void update(const SetArg& h, float coef, bool clip,
+                                       const float* g, float* p, Moments& o) {
+#pragma unroll
+    for (uint32_t j = 0; j < kLaneElems; j++) {
+        const float x = clip ? g[j] * coef : g[j];
+        o.m[j] = o.m[j] * h.b1 + x * h.omb1;
+        o.v[j] = o.v[j] * h.b2 + (x * x) * h.omb2;
+        const float den = sqrtf(o.v[j]) * h.inv_bc2 + h.eps;
+        p[j] = p[j] * h.decay - (o.m[j] / den) * h.step_size;
+    }
+}
+
+// A chunk of one tensor. FULL: all of its elements are there and aligned for
+// a lane's vector loads, which are all issued before the first is used.
+template <typename T, bool Q8, int ITER, bool FULL>
+__device__ __forceinline__ void step_chunk(const TensorArg& t, const SetArg& h, const State& st,
+                                           uint64_t at, float coef, bool clip) {
+    constexpr uint32_t kStep = kThreads * kLaneElems;
+    T* p = (T*)t.param;
+    const T* g = (const T*)t.grad;
+    const bool wide = !std::is_same<T, float>::value && st.master != nullptr;
+    const uint64_t padded = (t.n + kBlock - 1) / kBlock * kBlock;
+    float gx[ITER][kLaneElems], px[ITER][kLaneElems];
+    Moments mo[ITER];
+#pragma unroll
+    for (int k = 0; k < ITER; k++) {
+        const uint64_t i = at + (uint64_t)k * kStep + threadIdx.x * kLaneElems;
+        if (FULL) {
+            load_vec<T, kLaneElems>(g + i, gx[k]);
+            if (wide) {
+                load_vec<float, kLaneElems>(st.master + t.state + i, px[k]);
+            } else {
+                load_vec<T, kLaneElems>(p + i, px[k]);
+            }
+            mo[k] = load_moments<Q8>(st, t.state + i);
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < kLaneElems; j++) {
+                const bool in = i + j < t.n;
+                gx[k][j] = in ? to_float(g[i + j]) : 0.f;
+                px[k][j] = !in ? 0.f : wide ? st.master[t.state + i + j] : to_float(p[i + j]);
+                mo[k].m[j] = mo[k].v[j] = 0.f;
+            }
+            if (i < padded) {  // a share is padded with zeros to whole blocks
+                mo[k] = load_moments<Q8>(st, t.state + i);
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < ITER; k++) {
+        const uint64_t i = at + (uint64_t)k * kStep + threadIdx.x * kLaneElems;
+        update<Q8>(h, coef, clip, gx[k], px[k], mo[k]);
+        if (!FULL) {
+#pragma unroll
+            for (uint32_t j = 0; j < kLaneElems; j++) {
+                if (i + j >= t.n) {
+                    mo[k].m[j] = mo[k].v[j] = 0.f;  // the padding stays zero
+                }
+            }
+        }
+        store_moments<Q8>(st, t.state + i, mo[k], h.key, FULL || i < padded);
+        if (FULL) {
+            store_vec<T, kLaneElems>(p + i, px[k]);
+            if (wide) {
+                store_vec<float, kLaneElems>(st.master + t.state + i, px[k]);
+            }
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < kLaneElems; j++) {
+                if (i + j < t.n) {
+                    p[i + j] = from_float<T>(px[k][j]);
+                    if (wide) {
+                        st.master[t.state + i + j] = px[k][j];
+                    }
+                }
+            }
+        }
+    }
+}
+
+template <typename T, bool Q8, int ITER>
+__device__ __forceinline__ void step_tensor(const TensorArg& t, const SetArg& h, const State& st,
+                                            uint64_t at, float coef, bool clip) {
+    constexpr uintptr_t kMask = kLaneElems * sizeof(T) - 1;
+    const bool vec = (((uintptr_t)t.param | (uintptr_t)t.grad) & kMask) == 0;
+    if (vec && at + (uint64_t)ITER * kThreads * kLaneElems <= t.n) {
+        step_chunk<T, Q8, ITER, true>(t, h, st, at, coef, clip);
+    } else {
+        step_chunk<T, Q8, ITER, false>(t, h, st, at, coef, clip);
+    }
+}
+
+// A workgroup per chunk of 1024 ITER elements of one tensor: everything is
+// read and written once, so memory bounds it.
+template <bool Q8, int ITER>
+__global__ __launch_bounds__(256) void k_adamw_step(const Table tb, const State st) {
+    float coef = 1.f;
+    const bool clip = st.partials != nullptr;
+    if (clip) {
+        // every workgroup adds the few partials itself: no launch between
+        double s = 0.0;
+        for (uint32_t i = threadIdx.x; i < st.n_partials; i += kThreads) {
+            s += st.partials[i];
+        }
+        const float norm = (float)sqrt(block_sum(s));
+        const float q = st.max_norm / (norm + 1e-6f);
+        coef = q > 1.f ? 1.f : q;  // a NaN stays one
+        if (blockIdx.x == 0 && threadIdx.x == 0) {
+            *st.norm = norm;
+        }
+    }
+    const TensorArg& t = tb.t[find_tensor(tb, blockIdx.x)];
+    const SetArg& h = tb.set[t.set];
+    const uint64_t at = (uint64_t)(blockIdx.x - t.first_chunk) * (ITER * kThreads * kLaneElems);
+    switch (t.type) {
+        case DRESSI_F32:
+            step_tensor<float, Q8, ITER>(t, h, st, at, coef, clip);
+            break;
+        case DRESSI_BF16:
+            step_tensor<bf16, Q8, ITER>(t, h, st, at, coef, clip);
+            break;
+        default:
+            step_tensor<f16, Q8, ITER>(t, h, st, at, coef, clip);
+    }
+}
+
+// The values that 8-bit moments stand for, as bfloat16 (which holds them all:
+// three mantissa bits). 4 elements a lane.
+__global__ __launch_bounds__(256) void k_adamw_values(const State st, uint64_t n, bf16* m,
+                                                      bf16* v) {
+    const uint64_t i = ((uint64_t)blockIdx.x * kThreads + threadIdx.x) * kLaneElems;
+    if (i < n) {
+        const Moments o = load_moments<true>(st, i);
+        store_vec<bf16, kLaneElems>(m + i, o.m);
+        store_vec<bf16, kLaneElems>(v + i, o.v);
+    }
+}
+
+// One launch's worth of tensors: as many as fit the table.
+struct Batch {
+    Table tb;
+    uint32_t iter;
+};
+
+// Elements up to which a workgroup takes 1024 of them, else 4096.
+constexpr uint64_t kSmallTotal = 1ull << 20;
+
+int check_tensors(const dressi_adamw_tensor* t, uint32_t n, uint32_t n_sets, uint64_t state_elems) {
+    for (uint32_t i = 0; i < n; i++) {
+        DRESSI_REQUIRE(t[i].n == 0 || (t[i].param && t[i].grad), "adamw: tensor %u has a NULL pointer", i);
+        DRESSI_REQUIRE(t[i].type <= DRESSI_F16, "adamw: tensor %u has unknown type %u", i, t[i].type);
+        DRESSI_REQUIRE(t[i].set < n_sets, "adamw: tensor %u names set %u of %u", i, t[i].set, n_sets);
+        DRESSI_REQUIRE(t[i].state % kBlock == 0, "adamw: tensor %u's state is not at a multiple of %u",
+                       i, kBlock);
+        const size_t size = t[i].type == DRESSI_F32 ? 4 : 2;
+        DRESSI_REQUIRE(((uintptr_t)t[i].param | (uintptr_t)t[i].grad) % size == 0,
+                       "adamw: tensor %u is not aligned to its type", i);
+        DRESSI_REQUIRE(t[i].n <= (1ull << 40), "adamw: tensor %u is too large", i);
+        const uint64_t padded = (t[i].n + kBlock - 1) / kBlock * kBlock;
+        DRESSI_REQUIRE(t[i].state <= state_elems && padded <= state_elems - t[i].state,
+                       "adamw: tensor %u's share ends past the state buffers", i);
+    }
+    return DRESSI_OK;
+}
+
+int check_set(const dressi_adamw_set& s, uint32_t i) {
+    DRESSI_REQUIRE(s.lr >= 0.0 && std::isfinite(s.lr), "adamw: lr %g of set %u", s.lr, i);
+    DRESSI_REQUIRE(s.beta1 >= 0.0 && s.beta1 < 1.0, "adamw: beta1 %g of set %u", s.beta1, i);
+    DRESSI_REQUIRE(s.beta2 >= 0.0 && s.beta2 < 1.0, "adamw: beta2 %g of set %u", s.beta2, i);
+    DRESSI_REQUIRE(s.eps >= 0.0 && std::isfinite(s.eps), "adamw: eps %g of set %u", s.eps, i);
+    DRESSI_REQUIRE(s.weight_decay >= 0.0 && std::isfinite(s.weight_decay),
+                   "adamw: weight_decay %g of set %u", s.weight_decay, i);
+    DRESSI_REQUIRE(s.step >= 1, "adamw: step 0 of set %u (the first is 1)", i);
+    return DRESSI_OK;
+}
+
+SetArg set_arg(const dressi_adamw_set& s, uint32_t seed) {
+    SetArg a;
+    a.b1 = (float)s.beta1;
+    a.omb1 = (float)(1.0 - s.beta1);
+    a.b2 = (float)s.beta2;
+    a.omb2 = (float)(1.0 - s.beta2);
+    a.eps = (float)s.eps;
+    a.decay = (float)(1.0 - s.lr * s.weight_decay);
+    a.step_size = (float)(s.lr / (1.0 - std::pow(s.beta1, (double)s.step)));
+    a.inv_bc2 = (float)(1.0 / std::sqrt(1.0 - std::pow(s.beta2, (double)s.step)));
+    a.key = (uint32_t)s.step * 0x9e3779b9u + seed * 0x632be5abu + 0x7f4a7c15u;
+    return a;
+}
+
+// Calls f(table) for each launch.
+template <typename F>
+int for_batches(const dressi_adamw_tensor* t, uint32_t n, const dressi_adamw_set* sets,
+                uint32_t seed, uint32_t chunk_elems, F&& f) {
+    Table tb;
+    uint32_t set_of[kMaxSets];
+    uint32_t n_sets = 0;
+    tb.n_tensors = tb.n_chunks = 0;
+    for (uint32_t i = 0; i < n; i++) {
+        if (t[i].n == 0) {
+            continue;
+        }
+        // a tensor's chunks of one launch: more go into further entries
+        uint64_t done = 0;
+        while (done < t[i].n) {
+            uint32_t s = 0;
+            while (s < n_sets && set_of[s] != t[i].set) {
+                s++;
+            }
+            if (tb.n_tensors == kMaxTensors || s == kMaxSets || tb.n_chunks == (1u << 23)) {
+                if (int rc = f(tb)) {
+                    return rc;
+                }
+                tb.n_tensors = tb.n_chunks = n_sets = 0;
+                continue;
+            }
+            if (s == n_sets) {
+                set_of[n_sets++] = t[i].set;
+                tb.set[s] = set_arg(sets[t[i].set], seed);
+            }
+            const uint64_t room = (uint64_t)((1u << 23) - tb.n_chunks) * chunk_elems;
+            const uint64_t take = std::min<uint64_t>(room, t[i].n - done);
+            const size_t size = t[i].type == DRESSI_F32 ? 4 : 2;
+            TensorArg& a = tb.t[tb.n_tensors++];
+            a.param = (char*)t[i].param + done * size;
+            a.grad = (const char*)t[i].grad + done * size;
+            a.n = take;
+            a.state = t[i].state + done;
+            a.first_chunk = tb.n_chunks;
+            a.type = (uint16_t)t[i].type;
+            a.set = (uint16_t)s;
+            tb.n_chunks += (uint32_t)((take + chunk_elems - 1) / chunk_elems);
+            done += take;
+        }
+    }
+    return tb.n_tensors ? f(tb) : DRESSI_OK;
+}
+
+}  // namespace
+}  // namespace dressi
+
+using namespace dressi;
+
+extern "C" {
+
+size_t dressi_adamw_scratch(void) { return kMaxPartials * sizeof(double); }
+
+int dressi_adamw_step(dressi_ctx* ctx, const dressi_adamw_tensor* tensors, uint32_t n_tensors,
+                      const dressi_adamw_set* sets, uint32_t n_sets, uint32_t state_bits,
+                      uint64_t state_elems, void* exp_avg, void* exp_avg_sq,
+                      uint8_t* exp_avg_scale, uint8_t* exp_avg_sq_scale, float* master,
+                      uint32_t seed, float max_norm, void* scratch, float* norm) {
+    DRESSI_REQUIRE(ctx, "NULL context");
+    if (n_tensors == 0) {
+        return DRESSI_OK;
+    }
+    DRESSI_REQUIRE(tensors && sets && n_sets > 0, "adamw: bad arguments");
+    DRESSI_REQUIRE(state_bits == 8 || state_bits == 32, "adamw: state_bits %u is not 8 or 32",
+                   state_bits);
+    DRESSI_REQUIRE((exp_avg && exp_avg_sq) || state_elems == 0, "adamw: NULL state");
+    const bool q8 = state_bits == 8;
+    DRESSI_REQUIRE(!q8 || (exp_avg_scale && exp_avg_sq_scale) || state_elems == 0,
+                   "adamw: 8-bit moments need their scales");
+    const uintptr_t mask = q8 ? 3 : 15;
+    DRESSI_REQUIRE((((uintptr_t)exp_avg | (uintptr_t)exp_avg_sq) & mask) == 0 &&
+                       ((uintptr_t)master & 15) == 0,
+                   "adamw: the state buffers are not aligned");
+    DRESSI_REQUIRE(max_norm >= 0.f, "adamw: max_norm %g", (double)max_norm);
+    const bool clip = max_norm > 0.f;
+    DRESSI_REQUIRE(!clip || (scratch && norm), "adamw: clipping needs scratch and norm");
+    if (int rc = check_tensors(tensors, n_tensors, n_sets, state_elems)) {
+        return rc;
+    }
+    uint64_t total = 0;
+    for (uint32_t i = 0; i < n_tensors; i++) {
+        total += tensors[i].n;
+    }
+    for (uint32_t i = 0; i < n_sets; i++) {
+        if (int rc = check_set(sets[i], i)) {
+            return rc;
+        }
+    }
+    if (total == 0) {
+        return clip ? launch_zero(ctx->stream, norm, sizeof(float)) : DRESSI_OK;
+    }
+    const bool small = total <= kSmallTotal;
+    const uint32_t chunk = kThreads * kLaneElems * (small ? 1 : 4);
+    State st{exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, master, nullptr, 0,
+             max_norm, norm};
+    if (clip) {
+        uint32_t launches = 0;
+        for_batches(tensors, n_tensors, sets, seed, chunk, [&](const Table&) {
+            launches++;
+            return (int)DRESSI_OK;
+        });
+        DRESSI_REQUIRE(launches <= kMaxPartials, "adamw: too many tensors to clip (%u launches)",
+                       launches);
+        const uint32_t share = launches ? kMaxPartials / launches : 1;
+        uint32_t used = 0;
+        const int rc = for_batches(
+            tensors, n_tensors, sets, seed, chunk, [&](const Table& tb) -> int {
+                const uint32_t grid = std::min(tb.n_chunks, std::min(share, 512u));
+                double* out = (double*)scratch + used;
+                if (small) {
+                    hipLaunchKernelGGL(k_adamw_squares<1>, dim3(grid), dim3(kThreads), 0,
+                                       ctx->stream, tb, out);
+                } else {
+                    hipLaunchKernelGGL(k_adamw_squares<4>, dim3(grid), dim3(kThreads), 0,
+                                       ctx->stream, tb, out);
+                }
+                DRESSI_CHECK_LAUNCH();
+                used += grid;
+                return DRESSI_OK;
+            });
+        if (rc) {
+            return rc;
+        }
+        st.partials = (const double*)scratch;
+        st.n_partials = used;
+    }
+    return for_batches(tensors, n_tensors, sets, seed, chunk, [&](const Table& tb) -> int {
+        const dim3 grid(tb.n_chunks), block(kThreads);
+        if (q8 && small) {
+            hipLaunchKernelGGL((k_adamw_step<true, 1>), grid, block, 0, ctx->stream, tb, st);
+        } else if (q8) {
+            hipLaunchKernelGGL((k_adamw_step<true, 4>), grid, block, 0, ctx->stream, tb, st);
+        } else if (small) {
+            hipLaunchKernelGGL((k_adamw_step<false, 1>), grid, block, 0, ctx->stream, tb, st);
+        } else {
+            hipLaunchKernelGGL((k_adamw_step<false, 4>), grid, block, 0, ctx->stream, tb, st);
+        }
+        DRESSI_CHECK_LAUNCH();
+        return DRESSI_OK;
+    });
+}
+
+int dressi_adamw_values(dressi_ctx* ctx, uint64_t n, const void* exp_avg, const void* exp_avg_sq,
+                        const uint8_t* exp_avg_scale, const uint8_t* exp_avg_sq_scale,
+                        void* exp_avg_bf16, void* exp_avg_sq_bf16) {
+    DRESSI_REQUIRE(ctx, "NULL context");
+    if (n == 0) {
+        return DRESSI_OK;
+    }
+    DRESSI_REQUIRE(exp_avg && exp_avg_sq && exp_avg_scale && exp_avg_sq_scale && exp_avg_bf16 &&
+                       exp_avg_sq_bf16,
+                   "adamw: bad arguments");
+    DRESSI_REQUIRE(n % kBlock == 0, "adamw: %llu elements are not whole blocks of %u",
+                   (unsigned long long)n, kBlock);
+    DRESSI_REQUIRE((((uintptr_t)exp_avg | (uintptr_t)exp_avg_sq) & 3) == 0 &&
+                       (((uintptr_t)exp_avg_bf16 | (uintptr_t)exp_avg_sq_bf16) & 7) == 0,
+                   "adamw: the buffers are not aligned");
+    State st{(void*)exp_avg, (void*)exp_avg_sq, (uint8_t*)exp_avg_scale,
+             (uint8_t*)exp_avg_sq_scale, nullptr, nullptr, 0, 0.f, nullptr};
+    // within the launch limit, in whole blocks
+    constexpr uint64_t kPiece = kLaunchThreads * kLaneElems;
+    for (uint64_t at = 0; at < n; at += kPiece) {
+        const uint64_t take = std::min(kPiece, n - at);
+        State s = st;
+        s.m = (uint8_t*)st.m + at;
+        s.v = (uint8_t*)st.v + at;
+        s.m_scale = st.m_scale + at / kBlock;
+        s.v_scale = st.v_scale + at / kBlock;
+        const uint32_t blocks = (uint32_t)((take + kThreads * kLaneElems - 1) / (kThreads * kLaneElems));
+        hipLaunchKernelGGL(k_adamw_values, dim3(blocks), dim3(kThreads), 0, ctx->stream, s, take,
+                           (bf16*)exp_avg_bf16 + at, (bf16*)exp_avg_sq_bf16 + at);
+        DRESSI_CHECK_LAUNCH();
+    }
+    return DRESSI_OK;
+}
+
+}  // extern "C"

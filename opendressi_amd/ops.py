@@ -12,7 +12,7 @@ import ctypes as C
 
 import torch
 
-from ._lib import check, lib
+from ._lib import ACT_GELU, ACT_NONE, ACT_RELU, ACT_SILU, BF16, F16, F32, check, lib
 from .runtime import Context
 
 
@@ -724,3 +724,142 @@ def brdf_lut(ctx: Context, w: int = 256, h: int = 256, n_samples: int = 512,
     out = torch.empty((h, w, 2), dtype=torch.float32, device=device or f"cuda:{ctx.device}")
     check(lib.dressi_brdf_lut(ctx.handle, w, h, n_samples, _ptr(out, "out")))
     return out
+
+
+# ---- group norm with an activation (channels-last images) -------------------
+
+TYPE_CODES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+ACTIVATIONS = {"none": ACT_NONE, "relu": ACT_RELU, "silu": ACT_SILU, "gelu": ACT_GELU}
+
+
+def _typed(ctx: Context, t: torch.Tensor, name: str) -> int:
+    """The element type's code of a tensor on the context's device."""
+    code = TYPE_CODES.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    if t.device.type != "cuda" or t.device.index != ctx.device:
+        raise ValueError(f"{name}: expected a tensor on cuda:{ctx.device}, got one on {t.device}")
+    return code
+
+
+def _pixel_strides(x: torch.Tensor) -> tuple[int, int, int] | None:
+    """(pixels of an item, item stride, pixel stride) of [N, ..., C], or None
+    where its channels are not neighbours or its pixels not evenly spaced."""
+    shape, stride = x.shape, x.stride()
+    if shape[-1] > 1 and stride[-1] != 1:
+        return None
+    n_px, px_stride = 1, shape[-1]
+    for size, step in zip(reversed(shape[1:-1]), reversed(stride[1:-1])):
+        if size == 1:
+            continue
+        if n_px == 1:
+            px_stride = step
+        elif step != px_stride * n_px:
+            return None
+        n_px *= size
+    if px_stride < shape[-1] or (shape[0] > 1 and stride[0] < 0):
+        return None  # pixels that share memory
+    return n_px, stride[0], px_stride
+
+
+def _affine(ctx: Context, c: int, weight, bias) -> int:
+    """Checks weight and bias of c channels; their type's code."""
+    kinds = set()
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is None:
+            continue
+        if t.dim() != 1 or t.shape[0] != c:
+            raise ValueError(f"{name} must be [{c}], got {tuple(t.shape)}")
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+        kinds.add(_typed(ctx, t, name))
+    if len(kinds) > 1:
+        raise TypeError(f"weight is {weight.dtype}, bias {bias.dtype}: they must be of one type")
+    return kinds.pop() if kinds else F32
+
+
+def _norm_args(x: torch.Tensor, groups: int, activation: str) -> int:
+    if x.dim() < 2:
+        raise ValueError(f"x must be [N, ..., C], got {tuple(x.shape)}")
+    if groups < 1 or x.shape[-1] % groups or x.shape[-1] < 1:
+        raise ValueError(f"{x.shape[-1]} channels are not {groups} whole groups")
+    act = ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError(f"unknown activation {activation!r}; one of {', '.join(ACTIVATIONS)}")
+    return act
+
+
+def _addr(t: torch.Tensor | None) -> int | None:
+    return None if t is None else t.data_ptr()
+
+
+def group_norm(ctx: Context, x: torch.Tensor, groups: int, weight: torch.Tensor | None = None,
+               bias: torch.Tensor | None = None, eps: float = 1e-5,
+               activation: str = "none") -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Group normalisation of channels-last images x (N, ..., C) and an
+    activation ("none", "relu", "silu", "gelu"): act((x - mean) rstd w + b),
+    mean and rstd over the pixels and the C / groups channels of each group of
+    each item. float32, bfloat16 or float16, computed in float32; weight and
+    bias (C,) of one type of the three. Returns y (packed), mean and rstd
+    (N, groups) float32. x may have any even pixel stride (a slice of the
+    channels of a wider image); others are packed first."""
+    act = _norm_args(x, groups, activation)
+    code, aff = _typed(ctx, x, "x"), _affine(ctx, x.shape[-1], weight, bias)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean, rstd = torch.zeros((2, x.shape[0], groups), dtype=torch.float32, device=x.device) \
+        if x.numel() == 0 else \
+        torch.empty((2, x.shape[0], groups), dtype=torch.float32, device=x.device)
+    if x.numel() == 0:
+        return y, mean, rstd
+    at = _pixel_strides(x)
+    if at is None:
+        x = x.contiguous()
+        at = _pixel_strides(x)
+    n_px, item, px = at
+    n, c = x.shape[0], x.shape[-1]
+    size = lib.dressi_group_norm_scratch(code, n, n_px, c, groups, 0)
+    scratch = torch.empty(size, dtype=torch.uint8, device=x.device)
+    _prep(ctx)
+    check(lib.dressi_group_norm(ctx.handle, x.data_ptr(), code, n, n_px, c, item, px, groups,
+                                _addr(weight), _addr(bias), aff, eps, act, scratch.data_ptr(),
+                                size, y.data_ptr(), mean.data_ptr(), rstd.data_ptr()))
+    return y, mean, rstd
+
+
+def group_norm_bwd(ctx: Context, gy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor,
+                   rstd: torch.Tensor, groups: int, weight: torch.Tensor | None = None,
+                   bias: torch.Tensor | None = None, activation: str = "none",
+                   need: tuple[bool, bool, bool] = (True, True, True)
+                   ) -> tuple[torch.Tensor | None, torch.Tensor | None, torch.Tensor | None]:
+    """Gradients of group_norm: gy (N, ..., C), and x, mean, rstd of the
+    forward pass -> gx (like x, packed), gw, gb (C,) in the weight's and bias's
+    type (float32 where there is none). `need` says which of the three are
+    wanted; the others are None."""
+    act = _norm_args(x, groups, activation)
+    code, aff = _typed(ctx, x, "x"), _affine(ctx, x.shape[-1], weight, bias)
+    n, c = x.shape[0], x.shape[-1]
+    if gy.shape != x.shape or gy.dtype != x.dtype or gy.device != x.device:
+        raise ValueError(f"gy must be like x: {x.dtype} {tuple(x.shape)}, got {gy.dtype} "
+                         f"{tuple(gy.shape)} on {gy.device}")
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        _ptr(t, name)
+        if t.shape != (n, groups) or t.device != x.device:
+            raise ValueError(f"{name} must be [{n}, {groups}], got {tuple(t.shape)}")
+    kind = next((t.dtype for t in (weight, bias) if t is not None), torch.float32)
+    gx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
+    gw = torch.empty(c, dtype=kind, device=x.device) if need[1] else None
+    gb = torch.empty(c, dtype=kind, device=x.device) if need[2] else None
+    at = _pixel_strides(x)
+    if at is None:
+        x = x.contiguous()
+        at = _pixel_strides(x)
+    gy = gy.contiguous()
+    n_px, item, px = at if x.numel() else (0, 0, c)
+    size = lib.dressi_group_norm_scratch(code, n, n_px, c, groups, 1)
+    scratch = torch.empty(size, dtype=torch.uint8, device=x.device)
+    _prep(ctx)
+    check(lib.dressi_group_norm_bwd(ctx.handle, gy.data_ptr(), x.data_ptr(), code, n, n_px, c,
+                                    item, px, groups, _addr(weight), _addr(bias), aff, act,
+                                    mean.data_ptr(), rstd.data_ptr(), scratch.data_ptr(), size,
+                                    _addr(gx), _addr(gw), _addr(gb)))
+    return gx, gw, gb

@@ -10,6 +10,11 @@
     col     = dr.antialias(col, rast, pos, tri)
     rs      = dr.rasterize_soft(ctx, pos, tri, [H, W], radius_px=3.0)
 
+and, for a neural shader trained through them,
+
+    y   = dr.group_norm(ctx, x, groups=8, weight=w, bias=b, activation="silu")
+    opt = dr.AdamW(ctx, params, lr=1e-3, state_bits=8, max_grad_norm=1.0)
+
 Coordinate conventions follow nvdiffrast (OpenGL clip space, z in [-w, w]);
 the remap to the [0, w] depth range of the reference's rasterizers happens
 inside. Every op runs the library's HIP kernels on the context's device,
@@ -20,6 +25,8 @@ so reference code runs unchanged.
 """
 
 from .context import RasterizeHipContext, RasterizeVulkanContext
+from .norm import group_norm
+from .optim import AdamW
 from .ops import antialias, interpolate, rasterize, rasterize_soft, texture
 
 __all__ = [
@@ -30,4 +37,6 @@ __all__ = [
     "texture",
     "antialias",
     "rasterize_soft",
+    "group_norm",
+    "AdamW",
 ]

@@ -1,0 +1,295 @@
+"""AdamW over many parameter tensors at once, with moments in 32 or in 8 bits:
+the optimizer of what is trained through the surface (vertices, textures,
+environments, a neural shader's weights). No counterpart in the reference's
+surface, whose optimizer is part of its graph.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+import torch
+
+from .._lib import AdamwSet, AdamwTensor, check, lib
+from ..ops import TYPE_CODES, _addr
+from .context import RasterizeHipContext
+
+BLOCK = 32  # elements that share an exponent; a parameter's share is padded to whole ones
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Whether t's elements fill its memory without gaps or overlaps, in
+    whatever order of its dimensions."""
+    if t.is_contiguous():
+        return True
+    step = 1
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != step:
+            return False
+        step *= size
+    return True
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW (decoupled weight decay) in one launch for up to 72 tensors.
+
+    Per element, with gradient g and step t of its parameter:
+
+        m = m beta1 + g (1 - beta1)
+        v = v beta2 + g^2 (1 - beta2)
+        p = p (1 - lr weight_decay)
+            - m / (sqrt(v) / sqrt(1 - beta2^t) + eps) lr / (1 - beta1^t)
+
+    `params` is an iterable of parameters or of groups with their own lr,
+    betas, eps and weight_decay. Parameters are float32, bfloat16 or float16
+    on the context's device, densely stored; they are updated in place, in
+    float32, on torch's current stream.
+
+    state_bits 32 keeps the moments in float32; 8 keeps them in a byte each,
+    with a scale byte for every 32 (2.06 bytes an element in place of 8).
+    Their rounding is random, from a hash of element, step and `seed`, and
+    right on average, so that the slow second moment still moves; the same
+    seed gives the same bits. A gradient that is not finite makes the moments
+    of its 32 neighbours NaN as well.
+
+    master_weights keeps a float32 copy of 16-bit parameters, of which they
+    are roundings; without it a small update of a 16-bit parameter is lost.
+
+    max_grad_norm multiplies the gradients by
+    min(1, max_grad_norm / (norm + 1e-6)), norm the 2-norm over all of them,
+    without a host round trip; `grad_norm` then holds the last step's norm.
+
+    A parameter whose grad is None is left as it is, and so is its step. A
+    step cannot be captured into a graph: it takes the step count from the
+    host."""
+
+    def __init__(self, ctx: RasterizeHipContext, params, lr: float = 1e-3, betas=(0.9, 0.999),
+                 eps: float = 1e-8, weight_decay: float = 1e-2, state_bits: int = 32,
+                 max_grad_norm: float | None = None, master_weights: bool = True, seed: int = 0):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
+        if max_grad_norm is not None and not 0.0 < max_grad_norm < math.inf:
+            raise ValueError(f"max_grad_norm must be above 0, got {max_grad_norm}")
+        self.ctx = ctx
+        self.state_bits = state_bits
+        self.max_grad_norm = max_grad_norm
+        self.master_weights = bool(master_weights)
+        self.seed = int(seed) & 0xffffffff
+        self.grad_norm = None
+        self._params: list[torch.Tensor] = []  # in the order of their shares
+        self._steps: list[int] = []
+        self._groups: list[dict] = []  # each parameter's
+        self._table = (AdamwTensor * 0)()
+        self._total = 0
+        self._moments: tuple[torch.Tensor, torch.Tensor] | None = None
+        self._scales: tuple[torch.Tensor | None, torch.Tensor | None] = (None, None)
+        self.master = None
+        self._scratch = None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    # ---- layout ----
+
+    def add_param_group(self, param_group) -> None:
+        """Adds a group; its parameters' state follows the others', at zero."""
+        group = dict(param_group)
+        group["params"] = [group["params"]] if isinstance(group["params"], torch.Tensor) \
+            else list(group["params"])
+        for p in group["params"]:
+            self._check_param(p)
+        for k, v in self.defaults.items():
+            group.setdefault(k, v)
+        _check_hyper(group)
+        super().add_param_group(group)
+        group = self.param_groups[-1]
+        for p in group["params"]:
+            self._params.append(p)
+            self._steps.append(0)
+            self._groups.append(group)
+        table = (AdamwTensor * len(self._params))()
+        at = 0
+        for i, p in enumerate(self._params):
+            table[i].n, table[i].state = p.numel(), at
+            table[i].type = TYPE_CODES[p.dtype]
+            at += -(-p.numel() // BLOCK) * BLOCK
+        self._grow(at)
+        self._table, self._total = table, at
+
+    def _check_param(self, p) -> None:
+        if not isinstance(p, torch.Tensor):
+            raise TypeError(f"a parameter must be a torch.Tensor, got {type(p).__name__}")
+        if p.dtype not in TYPE_CODES:
+            raise TypeError(f"a parameter must be float32, bfloat16 or float16, got {p.dtype}")
+        if p.device != self.ctx.device:
+            raise ValueError(f"a parameter is on {p.device}, the context on {self.ctx.device}")
+        if not _dense(p):
+            raise ValueError(f"a parameter of shape {tuple(p.shape)} and strides {p.stride()} "
+                             "is not densely stored")
+
+    def _grow(self, total: int) -> None:
+        """State for `total` elements: what is there, then zeros."""
+        dev, old = self.ctx.device, self._total
+
+        def grown(t, n, dtype):
+            new = torch.zeros(n, dtype=dtype, device=dev)
+            if t is not None:
+                new[:t.numel()] = t
+            return new
+
+        kind = torch.float32 if self.state_bits == 32 else torch.uint8
+        m, v = self._moments or (None, None)
+        self._moments = grown(m, total, kind), grown(v, total, kind)
+        if self.state_bits == 8:
+            self._scales = tuple(grown(s, total // BLOCK, torch.uint8) for s in self._scales)
+        if self.master_weights and any(p.dtype != torch.float32 for p in self._params):
+            had = self.master is not None
+            self.master = grown(self.master, total, torch.float32)
+            at = 0
+            for p in self._params:
+                if not had or at >= old:
+                    self.master[at:at + p.numel()] = _flat(p.detach())
+                at += -(-p.numel() // BLOCK) * BLOCK
+        if self._scratch is None:
+            self._scratch = torch.empty(lib.dressi_adamw_scratch(), dtype=torch.uint8, device=dev)
+            if self.max_grad_norm is not None:
+                self.grad_norm = torch.zeros((), device=dev)
+
+    # ---- the step ----
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        """One step with the parameters' present gradients; returns the
+        closure's loss, if there is a closure."""
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW.step cannot be captured into a graph: its step count is "
+                               "the host's")
+        table, steps = self._table, list(self._steps)
+        kept = []  # copies that the launch reads
+        live = []  # entries with a gradient
+        sets: dict[tuple, int] = {}
+        for i, p in enumerate(self._params):
+            g = p.grad
+            if g is None:
+                continue
+            e = table[i]
+            if g.layout is not torch.strided:
+                raise RuntimeError("AdamW: sparse gradients are not supported")
+            if g.numel() != e.n or p.numel() != e.n or TYPE_CODES.get(g.dtype) != e.type \
+                    or p.dtype != g.dtype or g.device != self.ctx.device \
+                    or p.device != g.device:
+                raise ValueError(f"parameter {i} or its gradient changed its size, type or device: "
+                                 f"{p.dtype} {tuple(p.shape)} on {p.device}, {g.dtype} "
+                                 f"{tuple(g.shape)} on {g.device}")
+            same = g.stride() == p.stride()
+            if not (same and g.is_contiguous()) and not _dense(p):
+                raise ValueError(f"parameter {i} is no longer densely stored")
+            if not same:  # into the parameter's own order
+                g = torch.empty_strided(p.shape, p.stride(), dtype=g.dtype,
+                                        device=g.device).copy_(g)
+                kept.append(g)
+            steps[i] += 1
+            e.param, e.grad = p.data_ptr(), g.data_ptr()
+            e.set = sets.setdefault((id(self._groups[i]), steps[i]), len(sets))
+            live.append(i)
+        if not live:
+            return loss
+        group_of = {id(g): g for g in self.param_groups}
+        hyper = (AdamwSet * len(sets))()
+        for (gid, t), k in sets.items():
+            g = group_of[gid]
+            hyper[k] = AdamwSet(g["lr"], *g["betas"], g["eps"], g["weight_decay"], t)
+        if len(live) < len(table):
+            table = (AdamwTensor * len(live))(*(table[i] for i in live))
+        ctx = self.ctx
+        with ctx.lock:
+            ctx._ctx.use_torch_stream()
+            check(lib.dressi_adamw_step(
+                ctx._ctx.handle, table, len(live), hyper, len(hyper), self.state_bits, self._total,
+                self._moments[0].data_ptr(), self._moments[1].data_ptr(),
+                _addr(self._scales[0]), _addr(self._scales[1]), _addr(self.master), self.seed,
+                self.max_grad_norm or 0.0, self._scratch.data_ptr(), _addr(self.grad_norm)))
+        self._steps = steps
+        return loss
+
+    # ---- state ----
+
+    def moments(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """(m, v) of all parameters, flat, in the parameters' order, each
+        parameter's share in its memory order and padded with zeros to a
+        multiple of 32. With 32-bit state they are the optimizer's own
+        float32 buffers, with 8-bit state the values that the codes stand for,
+        in bfloat16, which holds them exactly."""
+        if self.state_bits == 32:
+            return self._moments
+        out = torch.empty((2, self._total), dtype=torch.bfloat16, device=self.ctx.device)
+        with self.ctx.lock:
+            self.ctx._ctx.use_torch_stream()
+            check(lib.dressi_adamw_values(
+                self.ctx._ctx.handle, self._total, self._moments[0].data_ptr(),
+                self._moments[1].data_ptr(), _addr(self._scales[0]), _addr(self._scales[1]),
+                out[0].data_ptr(), out[1].data_ptr()))
+        return out[0], out[1]
+
+    def state_dict(self) -> dict:
+        """Flat state: "step" (one count a parameter), "exp_avg" and
+        "exp_avg_sq" as they are kept (with "exp_avg_scale" and
+        "exp_avg_sq_scale" in 8 bits), "master" where there is one, and the
+        groups' hyperparameters."""
+        out = {"step": list(self._steps), "seed": self.seed,
+               "exp_avg": self._moments[0], "exp_avg_sq": self._moments[1],
+               "param_groups": [{k: v for k, v in g.items() if k != "params"}
+                                for g in self.param_groups]}
+        if self.state_bits == 8:
+            out["exp_avg_scale"], out["exp_avg_sq_scale"] = self._scales
+        if self.master is not None:
+            out["master"] = self.master
+        return out
+
+    def load_state_dict(self, state_dict: dict) -> None:
+        """Takes over the state of an optimizer of the same parameters and
+        state_bits. "seed", "master" and "param_groups" may be missing: then
+        they stay as they are."""
+        steps = [int(t) for t in state_dict["step"]]
+        if len(steps) != len(self._params) or min(steps, default=0) < 0:
+            raise ValueError(f"state of {len(steps)} parameters for {len(self._params)}")
+        named = {"exp_avg": self._moments[0], "exp_avg_sq": self._moments[1]}
+        if self.state_bits == 8:
+            named["exp_avg_scale"], named["exp_avg_sq_scale"] = self._scales
+        if self.master is not None and "master" in state_dict:
+            named["master"] = self.master
+        for k, t in named.items():
+            src = state_dict[k]
+            if src.dtype != t.dtype or src.shape != t.shape:
+                raise ValueError(f"{k} must be {t.dtype} {tuple(t.shape)}, got {src.dtype} "
+                                 f"{tuple(src.shape)}")
+        groups = state_dict.get("param_groups")
+        if groups is not None:
+            if len(groups) != len(self.param_groups):
+                raise ValueError(f"{len(groups)} groups for {len(self.param_groups)}")
+            for g in groups:
+                _check_hyper(g)
+            for mine, g in zip(self.param_groups, groups):
+                mine.update({k: v for k, v in g.items() if k != "params"})
+        for k, t in named.items():
+            t.copy_(state_dict[k])
+        self._steps = steps
+        self.seed = int(state_dict.get("seed", self.seed)) & 0xffffffff
+
+
+def _flat(t: torch.Tensor) -> torch.Tensor:
+    """A densely stored tensor's elements in memory order."""
+    return torch.as_strided(t, (t.numel(),), (1,))
+
+
+def _check_hyper(g: dict) -> None:
+    b1, b2 = g["betas"]
+    for name, v, ok in (("lr", g["lr"], 0.0 <= g["lr"] < math.inf),
+                        ("betas", g["betas"], 0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0),
+                        ("eps", g["eps"], 0.0 <= g["eps"] < math.inf),
+                        ("weight_decay", g["weight_decay"],
+                         0.0 <= g["weight_decay"] < math.inf)):
+        if not ok:
+            raise ValueError(f"invalid {name}: {v}")
