@@ -15,9 +15,10 @@
 // (every workgroup for itself: a launch in between costs more) and then reads
 // the image again.
 //
-// Statistics: a batch of a thread's values gives its mean and the squares
-// about that mean, both from registers, and (count, mean, squares) of two sets
-// are joined exactly; so values far from zero lose nothing to cancellation.
+// Statistics are those of x less a pivot, the group's first value: a batch of a
+// thread's values gives its mean and the squares about that mean, both from
+// registers, and (count, mean, squares) of two sets are joined. So values far
+// from zero lose nothing to cancellation, nor does a pivot far from the rest.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -33,51 +34,83 @@ namespace {
 constexpr uint32_t kMaxThreads = 512;
 constexpr uint32_t kMaxVecs = 256;  // of a workgroup
 constexpr uint32_t kBatch = 4;      // pixels of a thread in flight
-constexpr uint32_t kTargetGroups = 1024;  // workgroups that a launch should have
+constexpr uint32_t kBatchBwd = 4;   // the same of two images
+constexpr uint32_t kTargetGroups = 512;  // workgroups that a launch should have
+constexpr uint32_t kHold = 8;       // pixels that a thread keeps in registers (one pass)
+constexpr uint32_t kItemThreads = 512;  // of a workgroup that holds its pixels
 
-// How an image is cut. A block is a set of whole groups or, where a group has
-// more than kMaxVecs vectors, one part of a group.
+// How an image is cut. A vector of V channels lies in one group, or (split)
+// over several, each channel then counting for itself: a thread has S = 1 or
+// S = V sums. A unit is the fewest groups that whole vectors make up: one, or
+// V over the powers of two in D. A block is a set of whole units or, where a
+// unit of one group has more than kMaxVecs vectors, a part of it.
 struct Cut {
     uint64_t n_px;
     uint64_t item_stride, px_stride;  // of x, in elements
     uint32_t n_items, n_ch, n_groups;
-    uint32_t vpg;        // vectors of a group
+    uint32_t group_ch;   // channels of a group
+    uint32_t unit_vecs;  // vectors of a unit
+    uint32_t upb;        // units of a block (1 where parts > 1)
     uint32_t gpb;        // groups of a block (1 where parts > 1)
     uint32_t parts;      // blocks of a group
     uint32_t n_blocks;
     uint32_t rows;       // pixels that a workgroup takes side by side
+    uint32_t lanes;      // one pass: of a row, a power of two
     uint32_t threads;
     uint32_t chunks;     // of an item
     uint32_t chunk_px;
+    uint32_t stream;     // results go past the caches
 
     // vectors of a block, and its first
     __host__ __device__ uint32_t first_vec(uint32_t b) const {
-        return parts == 1 ? b * gpb * vpg : (b / parts) * vpg + (b % parts) * kMaxVecs;
+        return parts == 1 ? b * upb * unit_vecs : (b / parts) * unit_vecs + (b % parts) * kMaxVecs;
     }
     __host__ __device__ uint32_t vecs(uint32_t b) const {
         if (parts == 1) {
             const uint32_t left = n_groups - b * gpb;
-            return (left < gpb ? left : gpb) * vpg;
+            return left < gpb ? left * unit_vecs / (gpb / upb) : upb * unit_vecs;
         }
-        const uint32_t left = vpg - (b % parts) * kMaxVecs;
+        const uint32_t left = unit_vecs - (b % parts) * kMaxVecs;
         return left < kMaxVecs ? left : kMaxVecs;
     }
+    // groups of a block (or one, of which it is a part), and its first
+    __device__ uint32_t groups(uint32_t b) const {
+        const uint32_t left = n_groups - (parts == 1 ? b * gpb : b / parts);
+        return left < gpb ? left : gpb;
+    }
+    __device__ uint32_t first_group(uint32_t b) const { return parts == 1 ? b * gpb : b / parts; }
     __device__ uint32_t px_of(uint32_t chunk) const {
         const uint64_t left = n_px - (uint64_t)chunk * chunk_px;
         return left < chunk_px ? (uint32_t)left : chunk_px;
     }
 };
 
-Cut make_cut(uint32_t n_items, uint64_t n_px, uint32_t n_ch, uint32_t n_groups, uint32_t v) {
+// The fields that follow from the channels, with `upb_most` units of a block at
+// most; vectors of v channels.
+Cut make_blocks(uint32_t n_items, uint64_t n_px, uint32_t n_ch, uint32_t n_groups, uint32_t v,
+                uint32_t upb_most) {
     Cut c{};
     c.n_px = n_px;
     c.n_items = n_items;
     c.n_ch = n_ch;
     c.n_groups = n_groups;
-    c.vpg = n_ch / n_groups / v;
-    c.parts = div_up(c.vpg, kMaxVecs);
-    c.gpb = c.parts > 1 ? 1 : std::min(n_groups, kMaxVecs / c.vpg);
+    c.group_ch = n_ch / n_groups;
+    uint32_t unit = 1;  // groups
+    while (c.group_ch * unit % v != 0) {
+        unit *= 2;
+    }
+    c.unit_vecs = c.group_ch * unit / v;
+    c.parts = unit == 1 ? div_up(c.unit_vecs, kMaxVecs) : 1;
+    c.upb = c.parts > 1 ? 1
+                        : std::max(1u, std::min({n_groups / unit, kMaxVecs / c.unit_vecs, upb_most}));
+    c.gpb = c.upb * unit;
     c.n_blocks = c.parts > 1 ? n_groups * c.parts : div_up(n_groups, c.gpb);
+    return c;
+}
+
+// For two passes over the image.
+Cut make_cut(uint32_t n_items, uint64_t n_px, uint32_t n_ch, uint32_t n_groups, uint32_t v) {
+    Cut c = make_blocks(n_items, n_px, n_ch, n_groups, v, n_groups);
     const uint32_t most = c.vecs(0);
     c.rows = std::max(1u, kMaxThreads / most);
     c.threads = div_up(c.rows * most, 64) * 64;
@@ -91,6 +124,37 @@ Cut make_cut(uint32_t n_items, uint64_t n_px, uint32_t n_ch, uint32_t n_groups, 
     return c;
 }
 
+// For one pass: a workgroup holds all pixels of a block, at most kHold vectors a
+// thread; a row's vectors lie in one wave. chunks is 0 where
+// they are too many. Blocks take as many groups as leave 256 workgroups: their
+// reads are longer then.
+Cut make_item_cut(uint32_t n_items, uint64_t n_px, uint32_t n_ch, uint32_t n_groups,
+                  uint32_t v) {
+    const uint64_t most = std::max<uint64_t>(1, (uint64_t)n_items * n_groups / 256);
+    for (uint32_t gpb = (uint32_t)std::min<uint64_t>(most, n_groups); gpb > 0; gpb /= 2) {
+        Cut c = make_blocks(n_items, n_px, n_ch, n_groups, v, gpb);
+        if (c.vecs(0) > 64) {
+            continue;
+        }
+        uint32_t lanes = 1;
+        while (lanes < c.vecs(0)) {
+            lanes *= 2;
+        }
+        c.rows = kItemThreads / lanes;
+        if (n_px <= (uint64_t)c.rows * kHold) {
+            // no more rows than pixels, in whole waves
+            const uint64_t need = (n_px * lanes + 63) / 64 * 64;
+            c.threads = (uint32_t)std::min<uint64_t>(kItemThreads, need);
+            c.rows = c.threads / lanes;
+            c.lanes = lanes;
+            c.chunks = 1;
+            c.chunk_px = (uint32_t)n_px;
+            return c;
+        }
+    }
+    return Cut{};
+}
+
 // A thread's place: its vector of the block and the row of pixels it walks.
 struct Place {
     uint32_t vec, row, nv;
@@ -101,22 +165,64 @@ struct Place {
         vec = threadIdx.x - row * nv;
         live = row < c.rows;
     }
+    // pixels of a chunk that the thread takes: its row, then each c.rows on
+    __device__ uint32_t pixels(const Cut& c, uint32_t chunk) const {
+        const uint32_t len = c.px_of(chunk);
+        return live && row < len ? (len - row + c.rows - 1) / c.rows : 0;
+    }
 };
+
+__device__ __forceinline__ float2 shfl_xor(float2 x, uint32_t o) {
+    return make_float2(__shfl_xor(x.x, o), __shfl_xor(x.y, o));
+}
+__device__ __forceinline__ float shfl_xor(float x, uint32_t o) { return __shfl_xor(x, o); }
 
 // (n, mean, squares about it) of two sets joined.
 __device__ __forceinline__ void join(float& n, float& mean, float& m2, float nb, float meanb,
-                                     float m2b) {
-    const float sum = n + nb;
-    if (nb > 0.f) {
-        const float d = meanb - mean, share = nb / sum;
-        mean = fmaf(d, share, mean);
-        m2 += m2b + d * d * (n * share);
-        n = sum;
-    }
+                                     float m2b, float share) {
+    const float d = meanb - mean;
+    mean = fmaf(d, share, mean);
+    m2 += m2b + d * d * (n * share);
 }
 
-__device__ __forceinline__ uint32_t half_up(uint32_t n) {  // the power of two in [n / 2, n)
-    return n <= 1 ? 0u : 1u << (31 - __builtin_clz(n - 1));
+// Sums over a workgroup. Each thread has left S pairs, its vector's channels or
+// groups, in red[s][thread]; sum k is that of the rows and of the `per`
+// entries k per .. of a row, counted through its vectors. use(k, sum) is
+// called by one thread for each of the n sums. A power of two of lanes take
+// one sum; all threads call this.
+template <int S, uint32_t THREADS, typename Use>
+__device__ __forceinline__ void add_all(const float2 (*red)[THREADS], uint32_t rows, uint32_t nv,
+                                        uint32_t per, uint32_t n, Use&& use) {
+    uint32_t lanes = 64;
+    while (lanes > 1 && lanes * n > blockDim.x) {
+        lanes >>= 1;
+    }
+    uint32_t lr = lanes;  // of them, side by side over the rows
+    while (lr > 1 && lr >= 2 * rows) {
+        lr >>= 1;
+    }
+    const uint32_t lq = lanes / lr, lane = threadIdx.x & (lanes - 1);
+    for (uint32_t k = threadIdx.x / lanes; k - threadIdx.x / lanes < n; k += blockDim.x / lanes) {
+        float2 s = make_float2(0.f, 0.f);
+        if (k < n) {
+            for (uint32_t q = lane / lr; q < per; q += lq) {
+                const uint32_t entry = k * per + q, at = entry / S;
+                for (uint32_t r = lane & (lr - 1); r < rows; r += lr) {
+                    const float2 x = red[entry - at * S][r * nv + at];
+                    s.x += x.x;
+                    s.y += x.y;
+                }
+            }
+        }
+        for (uint32_t o = 1; o < lanes; o <<= 1) {
+            const float2 x = shfl_xor(s, o);
+            s.x += x.x;
+            s.y += x.y;
+        }
+        if (k < n && lane == 0) {
+            use(k, s);
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -124,7 +230,7 @@ __device__ __forceinline__ uint32_t half_up(uint32_t n) {  // the power of two i
 // ---------------------------------------------------------------------------
 
 __device__ __forceinline__ float sigmoid(float z) {
-    return 1.f / (1.f + __expf(-z));
+    return __builtin_amdgcn_rcpf(1.f + __expf(-z));  // an ulp of each
 }
 __device__ __forceinline__ float gauss_cdf(float z) {
     return 0.5f * (1.f + erff(z * 0.70710678118654752f));
@@ -163,7 +269,7 @@ __device__ __forceinline__ void act_slopes(uint32_t act, const float (&z)[V], fl
         case DRESSI_ACT_RELU:
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                g[j] = z[j] > 0.f ? g[j] : 0.f * g[j];
+                g[j] *= z[j] > 0.f ? 1.f : 0.f;
             }
             break;
         case DRESSI_ACT_SILU:
@@ -189,143 +295,199 @@ __device__ __forceinline__ void act_slopes(uint32_t act, const float (&z)[V], fl
 // forward
 // ---------------------------------------------------------------------------
 
-template <typename T, int V>
-__global__ __launch_bounds__(kMaxThreads) void k_gn_stats(const T* x, const Cut c, float2* part) {
-    __shared__ float sn[kMaxThreads], smean[kMaxThreads], sm2[kMaxThreads];
-    const Place at(c);
-    const uint32_t item = blockIdx.x / c.chunks, chunk = blockIdx.x - item * c.chunks;
-    float n = 0.f, mean = 0.f, m2 = 0.f;
-    if (at.live) {
-        const T* p = x + (size_t)item * c.item_stride +
-                     ((size_t)chunk * c.chunk_px) * c.px_stride +
-                     (size_t)(c.first_vec(blockIdx.y) + at.vec) * V;
-        const uint32_t len = c.px_of(chunk);
-        uint32_t i = at.row;
-        for (; i + (kBatch - 1) * c.rows < len; i += kBatch * c.rows) {
-            float v[kBatch][V];
+// A thread's first `count` of B vectors, less the pivots, joined to each of
+// its S sets (n, mean, m2): their mean, then the squares about it.
+template <typename T, int V, int S, int B>
+__device__ __forceinline__ void add_batch(const Pack<T, V> (&v)[B], uint32_t count,
+                                          const float (&pivot)[S], float& n, float (&mean)[S],
+                                          float (&m2)[S]) {
+    constexpr int W = V / S;
+    const float values = (float)(count * W), inv = count == B ? 1.f / (B * W) : 1.f / values;
+    float s[S], q[S];
 #pragma unroll
-            for (uint32_t k = 0; k < kBatch; k++) {
-                load_vec<T, V>(p + (size_t)(i + k * c.rows) * c.px_stride, v[k]);
+    for (int g = 0; g < S; g++) {
+        s[g] = q[g] = 0.f;
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < B; k++) {
+        float x[V];
+        unpack(v[k], x);
+#pragma unroll
+        for (int g = 0; g < S; g++) {
+            float t = 0.f;
+#pragma unroll
+            for (int j = 0; j < W; j++) {
+                t += x[g * W + j] - pivot[g];
             }
-            float s = 0.f, q = 0.f;
-#pragma unroll
-            for (uint32_t k = 0; k < kBatch; k++) {
-#pragma unroll
-                for (int j = 0; j < V; j++) {
-                    s += v[k][j];
-                }
-            }
-            s *= 1.f / (kBatch * V);
-#pragma unroll
-            for (uint32_t k = 0; k < kBatch; k++) {
-#pragma unroll
-                for (int j = 0; j < V; j++) {
-                    const float d = v[k][j] - s;
-                    q = fmaf(d, d, q);
-                }
-            }
-            join(n, mean, m2, (float)(kBatch * V), s, q);
-        }
-        for (; i < len; i += c.rows) {
-            float v[V], s = 0.f, q = 0.f;
-            load_vec<T, V>(p + (size_t)i * c.px_stride, v);
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                s += v[j];
-            }
-            s *= 1.f / V;
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                const float d = v[j] - s;
-                q = fmaf(d, d, q);
-            }
-            join(n, mean, m2, (float)V, s, q);
+            s[g] += k < count ? t : 0.f;
         }
     }
-    sn[threadIdx.x] = n;
-    smean[threadIdx.x] = mean;
-    sm2[threadIdx.x] = m2;
-    __syncthreads();
-    // over the rows, then over a group's vectors
-    const uint32_t per = c.parts == 1 ? c.vpg : at.nv;
-    const uint32_t j = at.vec % per;
-    const auto take = [&](uint32_t from) {
-        join(n, mean, m2, sn[from], smean[from], sm2[from]);
-        sn[threadIdx.x] = n;
-        smean[threadIdx.x] = mean;
-        sm2[threadIdx.x] = m2;
-    };
-    for (uint32_t left = c.rows, s = half_up(left); s > 0; left = s, s = half_up(left)) {
-        if (at.row < s && at.row + s < left) {
-            take(threadIdx.x + s * at.nv);
-        }
-        __syncthreads();
+#pragma unroll
+    for (int g = 0; g < S; g++) {
+        s[g] *= inv;
     }
-    for (uint32_t left = per, s = half_up(left); s > 0; left = s, s = half_up(left)) {
-        if (at.row == 0 && j < s && j + s < left) {
-            take(threadIdx.x + s);
+#pragma unroll
+    for (uint32_t k = 0; k < B; k++) {
+        float x[V];
+        unpack(v[k], x);
+#pragma unroll
+        for (int g = 0; g < S; g++) {
+            float t = 0.f;
+#pragma unroll
+            for (int j = 0; j < W; j++) {
+                const float d = (x[g * W + j] - pivot[g]) - s[g];
+                t = fmaf(d, d, t);
+            }
+            q[g] += k < count ? t : 0.f;
         }
-        __syncthreads();
     }
-    if (at.row == 0 && j == 0) {
-        const uint32_t slot = c.parts == 1 ? blockIdx.y * c.gpb + at.vec / per : blockIdx.y;
-        part[((size_t)item * c.n_groups * c.parts + slot) * c.chunks + chunk] =
-            make_float2(mean, m2);
+    const float share = values * __builtin_amdgcn_rcpf(n + values);
+#pragma unroll
+    for (int g = 0; g < S; g++) {
+        join(n, mean[g], m2[g], values, s[g], q[g], share);
+    }
+    n += values;
+}
+
+// B of a thread's pixels, `stride` elements apart; past `count` the last again.
+template <typename T, int V, int B>
+__device__ __forceinline__ void load_batch(const T* p, size_t stride, uint32_t count,
+                                           Pack<T, V> (&v)[B]) {
+#pragma unroll
+    for (uint32_t k = 0; k < B; k++) {
+        v[k] = load_pack<T, V>(p + (k < count ? k : count - 1) * stride);
     }
 }
 
+// The value of a group's first channel at the item's first pixel.
+template <typename T>
+__device__ __forceinline__ float pivot_of(const T* x, const Cut& c, uint32_t item,
+                                          uint32_t group) {
+    return to_float(x[(size_t)item * c.item_stride + (size_t)group * c.group_ch]);
+}
+
+// Group (of the image) of set g of vector `vec`.
+template <int V, int S>
+__device__ __forceinline__ uint32_t group_of(const Cut& c, uint32_t vec, int g) {
+    return (vec * V + g * (V / S)) / c.group_ch;
+}
+
+// The first pass: each chunk's (mean less the pivot, squares) for each group.
+template <typename T, int V, int S>
+__global__ __launch_bounds__(kMaxThreads) void k_gn_stats(const T* x, const Cut c, float2* part) {
+    __shared__ float2 red[S][kMaxThreads];
+    __shared__ float first[S * kMaxVecs];
+    const Place at(c);
+    const uint32_t item = blockIdx.x / c.chunks, chunk = blockIdx.x - item * c.chunks;
+    const uint32_t vec = c.first_vec(blockIdx.y) + at.vec, group0 = c.first_group(blockIdx.y);
+    float n = 0.f, mean[S], m2[S], pivot[S];
+#pragma unroll
+    for (int g = 0; g < S; g++) {
+        mean[g] = m2[g] = pivot[g] = 0.f;
+    }
+    uint32_t left = at.pixels(c, chunk);
+    if (left > 0) {
+        const T* p = x + (size_t)item * c.item_stride +
+                     ((size_t)chunk * c.chunk_px + at.row) * c.px_stride + (size_t)vec * V;
+        const size_t step = (size_t)c.rows * c.px_stride;
+#pragma unroll
+        for (int g = 0; g < S; g++) {
+            pivot[g] = pivot_of(x, c, item, group_of<V, S>(c, vec, g));
+        }
+        uint32_t count = left % kBatch ? left % kBatch : kBatch;
+        while (left > 0) {
+            Pack<T, V> v[kBatch];
+            load_batch<T, V, kBatch>(p, step, count, v);
+            add_batch<T, V, S, kBatch>(v, count, pivot, n, mean, m2);
+            left -= count;
+            p += count * step;
+            count = kBatch;
+        }
+    }
+    // sums and squares about the mean of one of the group's threads: small, so
+    // that they can be added as they are
+    const uint32_t groups = c.groups(blockIdx.y);
+    if (at.row == 0) {
+#pragma unroll
+        for (int g = 0; g < S; g++) {
+            const uint32_t k = group_of<V, S>(c, vec, g) - group0;
+            if (at.vec == 0 || (vec * V + g * (V / S)) % c.group_ch == 0) {
+                first[k] = mean[g];
+            }
+        }
+    }
+    __syncthreads();
+    if (at.live) {
+#pragma unroll
+        for (int g = 0; g < S; g++) {
+            const float d = mean[g] - first[group_of<V, S>(c, vec, g) - group0];
+            red[g][threadIdx.x] = n > 0.f ? make_float2(n * d, fmaf(n * d, d, m2[g]))
+                                          : make_float2(0.f, 0.f);
+        }
+    }
+    __syncthreads();
+    const uint32_t entries = at.nv * S / groups;
+    const float values = (float)c.px_of(chunk) * (float)(entries * (V / S));
+    add_all<S, kMaxThreads>(red, c.rows, at.nv, entries, groups, [&](uint32_t k, float2 s) {
+        const float d = s.x / values;
+        const uint32_t slot = c.parts == 1 ? group0 + k : blockIdx.y;
+        part[((size_t)item * c.n_groups * c.parts + slot) * c.chunks + chunk] =
+            make_float2(first[k] + d, fmaf(-s.x, d, s.y));
+    });
+}
+
 // Lanes that share the joining of one group's chunks: a power of two, so that
-// the workgroup takes all of its groups at once.
-__device__ __forceinline__ uint32_t lanes_of_group(uint32_t threads, uint32_t groups) {
+// the workgroup takes all of its groups at once if it can.
+__device__ __forceinline__ uint32_t lanes_of_group(uint32_t groups) {
     uint32_t l = 64;
-    while (l > 1 && l * groups > threads) {
+    while (l > 1 && l * groups > blockDim.x) {
         l >>= 1;
     }
     return l;
 }
 
-// (mean, 1 / sqrt(var + eps)) of the block's groups into `stat`.
-__device__ __forceinline__ void join_chunks(const Cut& c, uint32_t item, const float2* part,
-                                            int v, float eps, float2* stat) {
-    const uint32_t groups = c.parts == 1 ? c.vecs(blockIdx.y) / c.vpg : 1;
-    const uint32_t first = c.parts == 1 ? blockIdx.y * c.gpb : blockIdx.y / c.parts;
-    const uint32_t lanes = lanes_of_group(blockDim.x, groups);
-    const uint32_t g = threadIdx.x / lanes, lane = threadIdx.x & (lanes - 1);
-    float n = 0.f, mean = 0.f, m2 = 0.f;
-    if (g < groups) {
-        const uint32_t entries = c.parts * c.chunks;
-        const float2* p =
-            part + ((size_t)item * c.n_groups + first + g) * c.parts * c.chunks;
-        const uint32_t b0 = (first + g) * c.parts;
-        for (uint32_t e = lane; e < entries; e += lanes) {
-            const uint32_t chunk = c.parts == 1 ? e : e % c.chunks;
-            const uint32_t vecs = c.parts == 1 ? c.vpg : c.vecs(b0 + e / c.chunks);
-            const float2 q = p[e];
-            join(n, mean, m2, (float)c.px_of(chunk) * (float)(vecs * v), q.x, q.y);
+// (mean, 1 / sqrt(var + eps)) of the block's groups into `stat`: sums and
+// squares about the pivot in double, where their difference loses nothing.
+template <typename T, int V>
+__device__ __forceinline__ void join_chunks(const T* x, const Cut& c, uint32_t item,
+                                            const float2* part, float eps, float2* stat) {
+    const uint32_t groups = c.groups(blockIdx.y), group0 = c.first_group(blockIdx.y);
+    const uint32_t lanes = lanes_of_group(groups), lane = threadIdx.x & (lanes - 1);
+    const double last = (double)c.px_of(c.chunks - 1);
+    for (uint32_t g = threadIdx.x / lanes; g - threadIdx.x / lanes < groups;
+         g += blockDim.x / lanes) {
+        double s = 0.0, q = 0.0;
+        if (g < groups) {
+            const float2* p =
+                part + ((size_t)item * c.n_groups + group0 + g) * c.parts * c.chunks;
+            for (uint32_t k = 0; k < c.parts; k++, p += c.chunks) {
+                const uint32_t ch = c.parts == 1 ? c.group_ch
+                                                 : c.vecs((group0 + g) * c.parts + k) * V;
+                const double full = (double)c.chunk_px * ch, less = last * ch;
+#pragma unroll 8
+                for (uint32_t e = lane; e < c.chunks; e += lanes) {
+                    const double n = e == c.chunks - 1 ? less : full;
+                    const double m = (double)p[e].x, nm = n * m;
+                    s += nm;
+                    q += fma(nm, m, (double)p[e].y);
+                }
+            }
         }
-    }
-    for (uint32_t o = 1; o < lanes; o <<= 1) {
-        const float nb = __shfl_xor(n, o), meanb = __shfl_xor(mean, o), m2b = __shfl_xor(m2, o);
-        // both lanes of a pair join in the same order
-        if (threadIdx.x & o) {
-            float na = nb, ma = meanb, qa = m2b;
-            join(na, ma, qa, n, mean, m2);
-            n = na, mean = ma, m2 = qa;
-        } else {
-            join(n, mean, m2, nb, meanb, m2b);
+        for (uint32_t o = 1; o < lanes; o <<= 1) {
+            s += __shfl_xor(s, o);
+            q += __shfl_xor(q, o);
         }
-    }
-    if (g < groups && lane == 0) {
-        stat[g] = make_float2(mean, 1.f / sqrtf(m2 / n + eps));
+        if (g < groups && lane == 0) {
+            const double n = (double)c.n_px * c.group_ch, mean = s / n;
+            const double m2 = q - s * mean;
+            const float var = m2 < 0.0 ? 0.f : (float)(m2 / n);  // a NaN stays one
+            stat[g] = make_float2(pivot_of(x, c, item, group0 + g) + (float)mean,
+                                  1.f / sqrtf(var + eps));
+        }
     }
     __syncthreads();
 }
 
-__device__ __forceinline__ float load_as_float(const void* p, uint32_t type, size_t i) {
-    return type == DRESSI_F32    ? ((const float*)p)[i]
-           : type == DRESSI_BF16 ? to_float(((const bf16*)p)[i])
-                                 : to_float(((const f16*)p)[i]);
-}
 __device__ __forceinline__ void store_as(void* p, uint32_t type, size_t i, float x) {
     if (type == DRESSI_F32) {
         ((float*)p)[i] = x;
@@ -342,70 +504,255 @@ struct Affine {
     uint32_t type;
 };
 
+// One branch for all V, so that their loads are on their way together.
+template <int V>
+__device__ __forceinline__ void load_channels(const void* p, uint32_t type, uint32_t ch,
+                                              float absent, float (&w)[V]) {
+    if (!p) {
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            w[j] = absent;
+        }
+    } else if (type == DRESSI_F32) {
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            w[j] = ((const float*)p)[ch + j];
+        }
+    } else if (type == DRESSI_BF16) {
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            w[j] = to_float(((const bf16*)p)[ch + j]);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            w[j] = to_float(((const f16*)p)[ch + j]);
+        }
+    }
+}
 template <int V>
 __device__ __forceinline__ void load_affine(const Affine& a, uint32_t ch, float (&w)[V],
                                             float (&b)[V]) {
-#pragma unroll
-    for (int j = 0; j < V; j++) {
-        w[j] = a.weight ? load_as_float(a.weight, a.type, ch + j) : 1.f;
-        b[j] = a.bias ? load_as_float(a.bias, a.type, ch + j) : 0.f;
+    load_channels<V>(a.weight, a.type, ch, 1.f, w);
+    load_channels<V>(a.bias, a.type, ch, 0.f, b);
+}
+
+// V results, past the caches where they are many (they would drive out what
+// the next pass or item still reads).
+template <typename T, int V>
+__device__ __forceinline__ void put(T* p, const float (&x)[V], uint32_t stream) {
+    if (stream) {
+        stream_vec<T, V>(p, x);
+    } else {
+        store_vec<T, V>(p, x);
     }
 }
 
-template <typename T, int V>
+// act((x - mean) ws + b), ws = rstd w
+template <typename T, int V, int S>
+__device__ __forceinline__ void normalise(const Pack<T, V>& x, const float (&mean)[S],
+                                          const float (&ws)[V], const float (&b)[V], uint32_t act,
+                                          T* y, uint32_t stream) {
+    float v[V];
+    unpack(x, v);
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+        v[j] = fmaf(v[j] - mean[j / (V / S)], ws[j], b[j]);
+    }
+    act_values<V>(act, v);
+    put<T, V>(y, v, stream);
+}
+
+// The second pass. It walks the image backwards: what the first pass read
+// last may still be in a cache.
+template <typename T, int V, int S>
 __global__ __launch_bounds__(kMaxThreads) void k_gn_apply(const T* x, const Cut c,
                                                           const float2* part, const Affine aff,
                                                           float eps, uint32_t act, T* y,
                                                           float* mean_out, float* rstd_out) {
-    __shared__ float2 stat[kMaxVecs];
+    __shared__ float2 stat[S * kMaxVecs];
     const Place at(c);
-    const uint32_t item = blockIdx.x / c.chunks, chunk = blockIdx.x - item * c.chunks;
-    join_chunks(c, item, part, V, eps, stat);
-    if (!at.live) {
-        return;
-    }
-    const uint32_t vec = c.first_vec(blockIdx.y) + at.vec;
-    const float2 ms = stat[c.parts == 1 ? at.vec / c.vpg : 0];
-    if (chunk == 0 && at.row == 0 && vec % c.vpg == 0) {
-        mean_out[(size_t)item * c.n_groups + vec / c.vpg] = ms.x;
-        rstd_out[(size_t)item * c.n_groups + vec / c.vpg] = ms.y;
-    }
-    float w[V], b[V];
-    load_affine<V>(aff, vec * V, w, b);
-#pragma unroll
-    for (int j = 0; j < V; j++) {
-        w[j] *= ms.y;
-    }
-    const size_t px0 = (size_t)chunk * c.chunk_px;
+    const uint32_t unit = gridDim.x - 1 - blockIdx.x;
+    const uint32_t item = unit / c.chunks, chunk = unit - item * c.chunks;
+    uint32_t left = at.pixels(c, chunk);
+    const uint32_t vec = c.first_vec(blockIdx.y) + at.vec, group0 = c.first_group(blockIdx.y);
+    const size_t px0 = (size_t)chunk * c.chunk_px + at.row;
     const T* p = x + (size_t)item * c.item_stride + px0 * c.px_stride + (size_t)vec * V;
     T* o = y + ((size_t)item * c.n_px + px0) * c.n_ch + (size_t)vec * V;
-    const uint32_t len = c.px_of(chunk);
-    uint32_t i = at.row;
-    for (; i + (kBatch - 1) * c.rows < len; i += kBatch * c.rows) {
-        float v[kBatch][V];
-#pragma unroll
-        for (uint32_t k = 0; k < kBatch; k++) {
-            load_vec<T, V>(p + (size_t)(i + k * c.rows) * c.px_stride, v[k]);
-        }
-#pragma unroll
-        for (uint32_t k = 0; k < kBatch; k++) {
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                v[k][j] = fmaf(v[k][j] - ms.x, w[j], b[j]);
-            }
-            act_values<V>(act, v[k]);
-            store_vec<T, V>(o + (size_t)(i + k * c.rows) * c.n_ch, v[k]);
+    const size_t step = (size_t)c.rows * c.px_stride, ostep = (size_t)c.rows * c.n_ch;
+    // the first batch and the weights are on their way while the chunks are joined
+    Pack<T, V> v[kBatch];
+    uint32_t count = left < kBatch ? left : kBatch;
+    float w[V], b[V], mean[S];
+    if (left > 0) {
+        load_batch<T, V, kBatch>(p + (left - count) * step, step, count, v);
+        load_affine<V>(aff, vec * V, w, b);
+    }
+    join_chunks<T, V>(x, c, item, part, eps, stat);
+    if (chunk == 0 && (c.parts == 1 || blockIdx.y % c.parts == 0)) {
+        for (uint32_t g = threadIdx.x; g < c.groups(blockIdx.y); g += blockDim.x) {
+            mean_out[(size_t)item * c.n_groups + group0 + g] = stat[g].x;
+            rstd_out[(size_t)item * c.n_groups + group0 + g] = stat[g].y;
         }
     }
-    for (; i < len; i += c.rows) {
-        float v[V];
-        load_vec<T, V>(p + (size_t)i * c.px_stride, v);
+    if (left == 0) {
+        return;
+    }
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-            v[j] = fmaf(v[j] - ms.x, w[j], b[j]);
+    for (int g = 0; g < S; g++) {
+        const float2 ms = stat[group_of<V, S>(c, vec, g) - group0];
+        mean[g] = ms.x;
+#pragma unroll
+        for (int j = 0; j < V / S; j++) {
+            w[g * (V / S) + j] *= ms.y;
         }
-        act_values<V>(act, v);
-        store_vec<T, V>(o + (size_t)i * c.n_ch, v);
+    }
+    while (true) {
+        left -= count;
+#pragma unroll
+        for (uint32_t k = 0; k < kBatch; k++) {
+            if (k < count) {
+                normalise<T, V, S>(v[k], mean, w, b, act, o + (left + k) * ostep, c.stream);
+            }
+        }
+        if (left == 0) {
+            break;
+        }
+        count = left < kBatch ? left : kBatch;
+        load_batch<T, V, kBatch>(p + (left - count) * step, step, count, v);
+    }
+}
+
+// A thread's place in one pass: `lanes` lanes of a wave take a row, so that a
+// sum over rows is one over lanes and then over waves.
+struct ItemPlace {
+    uint32_t vec, row, mine;
+    __device__ ItemPlace(const Cut& c) {
+        vec = threadIdx.x & (c.lanes - 1);
+        row = threadIdx.x / c.lanes;
+        const uint32_t len = (uint32_t)c.n_px;
+        mine = vec < c.vecs(blockIdx.y) && row < len ? (len - row + c.rows - 1) / c.rows : 0;
+    }
+};
+
+__device__ __forceinline__ void accumulate(float& a, float b) { a += b; }
+__device__ __forceinline__ void accumulate(float2& a, float2 b) {
+    a.x += b.x;
+    a.y += b.y;
+}
+
+// The sum of `s` over the thread's group; every thread calls it, those without
+// pixels with 0. `part` is not reused before the next barrier but one.
+template <typename N>
+__device__ __forceinline__ N add_item(const Cut& c, const ItemPlace& at, N s, N (*part)[64]) {
+    const uint32_t waves = blockDim.x / 64, wave = threadIdx.x / 64, per = c.unit_vecs;
+    const bool even = (per & (per - 1)) == 0;
+    for (uint32_t o = c.lanes; o < 64; o *= 2) {
+        accumulate(s, shfl_xor(s, o));
+    }
+    if (even) {
+        for (uint32_t o = 1; o < per; o *= 2) {
+            accumulate(s, shfl_xor(s, o));
+        }
+    }
+    if ((threadIdx.x & 63u) < c.lanes) {
+        part[wave][at.vec] = s;
+    }
+    __syncthreads();
+    if (even) {
+        N sum = part[0][at.vec];
+        for (uint32_t i = 1; i < waves; i++) {
+            accumulate(sum, part[i][at.vec]);
+        }
+        return sum;
+    }
+    if (threadIdx.x < c.lanes) {
+        N sum = part[0][at.vec];
+        for (uint32_t i = 1; i < waves; i++) {
+            accumulate(sum, part[i][at.vec]);
+        }
+        part[0][at.vec] = sum;
+    }
+    __syncthreads();
+    const uint32_t first = at.vec / per * per;
+    N sum = part[0][first];
+    for (uint32_t i = 1; i < per; i++) {
+        // a lane past the block's vectors reads on within the row
+        accumulate(sum, part[0][(first + i) & 63u]);
+    }
+    return sum;
+}
+
+// Both passes where a block's pixels fit its workgroup's registers: x is read
+// once, in one launch.
+template <typename T, int V>
+__global__ __launch_bounds__(kItemThreads) void k_gn_item(const T* x, const Cut c,
+                                                          const Affine aff, float eps,
+                                                          uint32_t act, T* y, float* mean_out,
+                                                          float* rstd_out) {
+    __shared__ float part[2][kItemThreads / 64][64];
+    const ItemPlace at(c);
+    const uint32_t item = blockIdx.x;
+    const uint32_t vec = c.first_vec(blockIdx.y) + at.vec, group = vec / c.unit_vecs;
+    const T* p = x + (size_t)item * c.item_stride + (size_t)at.row * c.px_stride + (size_t)vec * V;
+    T* o = y + ((size_t)item * c.n_px + at.row) * c.n_ch + (size_t)vec * V;
+    const size_t step = (size_t)c.rows * c.px_stride, ostep = (size_t)c.rows * c.n_ch;
+    Pack<T, V> v[kHold];
+#pragma unroll
+    for (uint32_t k = 0; k < kHold; k++) {
+        if (k < at.mine) {
+            v[k] = load_pack<T, V>(p + k * step);
+        }
+    }
+    float w[V], b[V], pivot = 0.f;
+    if (at.mine > 0) {
+        load_affine<V>(aff, vec * V, w, b);
+        pivot = pivot_of(x, c, item, group);
+    }
+    const float values = (float)c.n_px * (float)c.group_ch;
+    float s = 0.f, q = 0.f;
+#pragma unroll
+    for (uint32_t k = 0; k < kHold; k++) {
+        if (k < at.mine) {
+            float f[V];
+            unpack(v[k], f);
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                s += f[j] - pivot;
+            }
+        }
+    }
+    const float d_mean = add_item(c, at, s, part[0]) / values;
+#pragma unroll
+    for (uint32_t k = 0; k < kHold; k++) {
+        if (k < at.mine) {
+            float f[V];
+            unpack(v[k], f);
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                const float d = (f[j] - pivot) - d_mean;
+                q = fmaf(d, d, q);
+            }
+        }
+    }
+    const float rstd = 1.f / sqrtf(add_item(c, at, q, part[1]) / values + eps);
+    if (at.mine == 0) {
+        return;
+    }
+    const float mean[1] = {pivot + d_mean};
+    if (at.row == 0 && at.vec % c.unit_vecs == 0) {
+        mean_out[(size_t)item * c.n_groups + group] = mean[0];
+        rstd_out[(size_t)item * c.n_groups + group] = rstd;
+    }
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+        w[j] *= rstd;
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < kHold; k++) {
+        if (k < at.mine) {
+            normalise<T, V, 1>(v[k], mean, w, b, act, o + k * ostep, c.stream);
+        }
     }
 }
 
@@ -413,9 +760,64 @@ __global__ __launch_bounds__(kMaxThreads) void k_gn_apply(const T* x, const Cut 
 // backward
 // ---------------------------------------------------------------------------
 
-// Per chunk the channels' (sum gz, sum gz xh), and the groups' sums of both
-// weighted.
-template <typename T, int V>
+// What a thread of the backward pass knows of its channels.
+template <int V, int S>
+struct Channels {
+    float mu[S], rstd[S], w[V], b[V];
+
+    __device__ __forceinline__ void load(const Cut& c, const Affine& aff, uint32_t item,
+                                         uint32_t vec, const float* mean, const float* rs) {
+        load_affine<V>(aff, vec * V, w, b);
+#pragma unroll
+        for (int g = 0; g < S; g++) {
+            const size_t at = (size_t)item * c.n_groups + group_of<V, S>(c, vec, g);
+            mu[g] = mean[at];
+            rstd[g] = rs[at];
+        }
+    }
+    // xh and gz of a vector
+    template <typename T>
+    __device__ __forceinline__ void gradients(const Pack<T, V>& x, const Pack<T, V>& gy,
+                                              uint32_t act, float (&xh)[V], float (&gz)[V]) const {
+        float z[V];
+        unpack(x, xh);
+        unpack(gy, gz);
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            xh[j] = (xh[j] - mu[j / (V / S)]) * rstd[j / (V / S)];
+            z[j] = fmaf(xh[j], w[j], b[j]);
+        }
+        act_slopes<V>(act, z, gz);
+    }
+    template <typename T>
+    __device__ __forceinline__ void add(const Pack<T, V>& x, const Pack<T, V>& gy, uint32_t act,
+                                        float (&sa)[V], float (&sb)[V]) const {
+        float xh[V], gz[V];
+        gradients(x, gy, act, xh, gz);
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            sa[j] += gz[j];
+            sb[j] = fmaf(gz[j], xh[j], sb[j]);
+        }
+    }
+    // gx from the groups' means of w gz and w gz xh
+    template <typename T>
+    __device__ __forceinline__ void finish(const Pack<T, V>& x, const Pack<T, V>& gy, uint32_t act,
+                                           const float2 (&m)[S], T* gx, uint32_t stream) const {
+        float xh[V], gz[V];
+        gradients(x, gy, act, xh, gz);
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const int g = j / (V / S);
+            gz[j] = rstd[g] * (fmaf(gz[j], w[j], -m[g].x) - xh[j] * m[g].y);
+        }
+        put<T, V>(gx, gz, stream);
+    }
+};
+
+// The first pass: per chunk the channels' (sum gz, sum gz xh), and the groups'
+// sums of both weighted.
+template <typename T, int V, int S>
 __global__ __launch_bounds__(kMaxThreads) void k_gn_bwd_sums(const T* gy, const T* x, const Cut c,
                                                              const Affine aff, uint32_t act,
                                                              const float* mean, const float* rstd,
@@ -425,51 +827,36 @@ __global__ __launch_bounds__(kMaxThreads) void k_gn_bwd_sums(const T* gy, const 
     const Place at(c);
     const uint32_t item = blockIdx.x / c.chunks, chunk = blockIdx.x - item * c.chunks;
     const uint32_t vec = c.first_vec(blockIdx.y) + at.vec;
-    float sa[V], sb[V], w[V], b[V];
+    float sa[V], sb[V];
 #pragma unroll
     for (int j = 0; j < V; j++) {
         sa[j] = sb[j] = 0.f;
     }
+    Channels<V, S> ch;
+    uint32_t left = at.pixels(c, chunk);
     if (at.live) {
-        load_affine<V>(aff, vec * V, w, b);
-        const float mu = mean[(size_t)item * c.n_groups + vec / c.vpg];
-        const float s = rstd[(size_t)item * c.n_groups + vec / c.vpg];
-        const size_t px0 = (size_t)chunk * c.chunk_px;
+        ch.load(c, aff, item, vec, mean, rstd);
+    }
+    if (left > 0) {
+        const size_t px0 = (size_t)chunk * c.chunk_px + at.row;
         const T* p = x + (size_t)item * c.item_stride + px0 * c.px_stride + (size_t)vec * V;
         const T* q = gy + ((size_t)item * c.n_px + px0) * c.n_ch + (size_t)vec * V;
-        const uint32_t len = c.px_of(chunk);
-        const auto add = [&](float (&xv)[V], float (&gv)[V]) {
-            float z[V];
+        const size_t step = (size_t)c.rows * c.px_stride, qstep = (size_t)c.rows * c.n_ch;
+        uint32_t count = left % kBatchBwd ? left % kBatchBwd : kBatchBwd;
+        while (left > 0) {
+            Pack<T, V> xv[kBatchBwd], gv[kBatchBwd];
+            load_batch<T, V, kBatchBwd>(p, step, count, xv);
+            load_batch<T, V, kBatchBwd>(q, qstep, count, gv);
 #pragma unroll
-            for (int j = 0; j < V; j++) {
-                xv[j] = (xv[j] - mu) * s;
-                z[j] = fmaf(xv[j], w[j], b[j]);
+            for (uint32_t k = 0; k < kBatchBwd; k++) {
+                if (k < count) {
+                    ch.add(xv[k], gv[k], act, sa, sb);
+                }
             }
-            act_slopes<V>(act, z, gv);
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                sa[j] += gv[j];
-                sb[j] = fmaf(gv[j], xv[j], sb[j]);
-            }
-        };
-        uint32_t i = at.row;
-        for (; i + (kBatch - 1) * c.rows < len; i += kBatch * c.rows) {
-            float xv[kBatch][V], gv[kBatch][V];
-#pragma unroll
-            for (uint32_t k = 0; k < kBatch; k++) {
-                load_vec<T, V>(p + (size_t)(i + k * c.rows) * c.px_stride, xv[k]);
-                load_vec<T, V>(q + (size_t)(i + k * c.rows) * c.n_ch, gv[k]);
-            }
-#pragma unroll
-            for (uint32_t k = 0; k < kBatch; k++) {
-                add(xv[k], gv[k]);
-            }
-        }
-        for (; i < len; i += c.rows) {
-            float xv[V], gv[V];
-            load_vec<T, V>(p + (size_t)i * c.px_stride, xv);
-            load_vec<T, V>(q + (size_t)i * c.n_ch, gv);
-            add(xv, gv);
+            left -= count;
+            p += count * step;
+            q += count * qstep;
+            count = kBatchBwd;
         }
     }
 #pragma unroll
@@ -477,164 +864,255 @@ __global__ __launch_bounds__(kMaxThreads) void k_gn_bwd_sums(const T* gy, const 
         red[j][threadIdx.x] = make_float2(sa[j], sb[j]);
     }
     __syncthreads();
-    for (uint32_t left = c.rows, s = half_up(left); s > 0; left = s, s = half_up(left)) {
-        if (at.row < s && at.row + s < left) {
+    float2* o = ch_part + ((size_t)item * c.chunks + chunk) * c.n_ch +
+                (size_t)c.first_vec(blockIdx.y) * V;
+    add_all<V, kMaxThreads>(red, c.rows, at.nv, 1, at.nv * V,
+                            [&](uint32_t k, float2 s) { o[k] = s; });
+    __syncthreads();
+    if (at.live) {
 #pragma unroll
-            for (int j = 0; j < V; j++) {
-                const float2 o = red[j][threadIdx.x + s * at.nv];
-                sa[j] += o.x;
-                sb[j] += o.y;
-                red[j][threadIdx.x] = make_float2(sa[j], sb[j]);
+        for (int g = 0; g < S; g++) {
+            float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int j = g * (V / S); j < (g + 1) * (V / S); j++) {
+                s.x = fmaf(ch.w[j], sa[j], s.x);
+                s.y = fmaf(ch.w[j], sb[j], s.y);
             }
+            red[g][threadIdx.x] = s;
         }
-        __syncthreads();
-    }
-    const uint32_t per = c.parts == 1 ? c.vpg : at.nv;
-    const uint32_t j0 = at.vec % per;
-    float ga = 0.f, gb = 0.f;
-    if (at.row == 0) {
-        float2* o = ch_part + (size_t)blockIdx.x * c.n_ch + (size_t)vec * V;
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-            o[j] = make_float2(sa[j], sb[j]);
-            ga = fmaf(w[j], sa[j], ga);
-            gb = fmaf(w[j], sb[j], gb);
-        }
-        red[0][threadIdx.x] = make_float2(ga, gb);
     }
     __syncthreads();
-    for (uint32_t left = per, s = half_up(left); s > 0; left = s, s = half_up(left)) {
-        if (at.row == 0 && j0 < s && j0 + s < left) {
-            const float2 o = red[0][threadIdx.x + s];
-            ga += o.x;
-            gb += o.y;
-            red[0][threadIdx.x] = make_float2(ga, gb);
+    const uint32_t groups = c.groups(blockIdx.y), group0 = c.first_group(blockIdx.y);
+    add_all<S, kMaxThreads>(red, c.rows, at.nv, at.nv * S / groups, groups,
+                            [&](uint32_t k, float2 s) {
+        const uint32_t slot = c.parts == 1 ? group0 + k : blockIdx.y;
+        group_part[((size_t)item * c.n_groups * c.parts + slot) * c.chunks + chunk] = s;
+    });
+}
+
+// gw and gb of kParamCh channels: the chunks' sums over all items in a fixed
+// order, the workgroup's threads taking shares of the chunks.
+constexpr uint32_t kParamCh = 8;
+struct ParamGrad {
+    const float2* ch_part;
+    size_t n_rows;
+    uint32_t n_ch, type;
+    void* gw;
+    void* gb;
+};
+
+__device__ __forceinline__ void param_grad(const ParamGrad& a, uint32_t block) {
+    __shared__ double2 sum[kMaxThreads / 64][kParamCh];
+    const uint32_t lane = threadIdx.x % kParamCh, row = threadIdx.x / kParamCh;
+    const uint32_t ch = block * kParamCh + lane;
+    double2 s = make_double2(0.0, 0.0);
+    if (ch < a.n_ch) {
+#pragma unroll 8
+        for (size_t r = row; r < a.n_rows; r += blockDim.x / kParamCh) {
+            const float2 q = a.ch_part[r * a.n_ch + ch];
+            s.x += (double)q.x;
+            s.y += (double)q.y;
         }
-        __syncthreads();
     }
-    if (at.row == 0 && j0 == 0) {
-        const uint32_t slot = c.parts == 1 ? blockIdx.y * c.gpb + at.vec / per : blockIdx.y;
-        group_part[((size_t)item * c.n_groups * c.parts + slot) * c.chunks + chunk] =
-            make_float2(ga, gb);
+    for (uint32_t o = kParamCh; o < 64; o *= 2) {
+        s.x += __shfl_xor(s.x, o);
+        s.y += __shfl_xor(s.y, o);
+    }
+    if ((threadIdx.x & 63u) < kParamCh) {
+        sum[threadIdx.x / 64][lane] = s;
+    }
+    __syncthreads();
+    if (row == 0 && ch < a.n_ch) {
+        for (uint32_t r = 1; r < blockDim.x / 64; r++) {
+            s.x += sum[r][lane].x;
+            s.y += sum[r][lane].y;
+        }
+        if (a.gb) {
+            store_as(a.gb, a.type, ch, (float)s.x);
+        }
+        if (a.gw) {
+            store_as(a.gw, a.type, ch, (float)s.y);
+        }
     }
 }
 
-template <typename T, int V>
+__global__ __launch_bounds__(kMaxThreads) void k_gn_param_grad(const ParamGrad a) {
+    param_grad(a, blockIdx.x);
+}
+
+// The second pass, backwards like the forward one. The first `extra`
+// workgroups take gw and gb.
+template <typename T, int V, int S>
 __global__ __launch_bounds__(kMaxThreads) void k_gn_bwd_apply(const T* gy, const T* x, const Cut c,
                                                               const Affine aff, uint32_t act,
                                                               const float* mean, const float* rstd,
-                                                              const float2* group_part, T* gx) {
-    __shared__ float2 mean_of[kMaxVecs];
-    const Place at(c);
-    const uint32_t item = blockIdx.x / c.chunks, chunk = blockIdx.x - item * c.chunks;
-    {
-        const uint32_t groups = c.parts == 1 ? c.vecs(blockIdx.y) / c.vpg : 1;
-        const uint32_t first = c.parts == 1 ? blockIdx.y * c.gpb : blockIdx.y / c.parts;
-        const uint32_t lanes = lanes_of_group(blockDim.x, groups);
-        const uint32_t g = threadIdx.x / lanes, lane = threadIdx.x & (lanes - 1);
-        const uint32_t entries = c.parts * c.chunks;
-        float a = 0.f, b = 0.f;
-        if (g < groups) {
-            const float2* p = group_part + ((size_t)item * c.n_groups + first + g) * entries;
-            for (uint32_t e = lane; e < entries; e += lanes) {
-                a += p[e].x;
-                b += p[e].y;
-            }
+                                                              const float2* group_part, T* gx,
+                                                              const ParamGrad params,
+                                                              uint32_t extra) {
+    __shared__ float2 mean_of[S * kMaxVecs];
+    if (blockIdx.x < extra) {
+        if (blockIdx.y == 0) {
+            param_grad(params, blockIdx.x);
         }
-        for (uint32_t o = 1; o < lanes; o <<= 1) {
-            a += __shfl_xor(a, o);
-            b += __shfl_xor(b, o);
-        }
-        if (g < groups && lane == 0) {
-            const float m = 1.f / ((float)c.n_px * (float)(c.n_ch / c.n_groups));
-            mean_of[g] = make_float2(a * m, b * m);
-        }
-        __syncthreads();
-    }
-    if (!at.live) {
         return;
     }
-    const uint32_t vec = c.first_vec(blockIdx.y) + at.vec;
-    const float2 ab = mean_of[c.parts == 1 ? at.vec / c.vpg : 0];
-    const float mu = mean[(size_t)item * c.n_groups + vec / c.vpg];
-    const float s = rstd[(size_t)item * c.n_groups + vec / c.vpg];
-    float w[V], b[V];
-    load_affine<V>(aff, vec * V, w, b);
-    const size_t px0 = (size_t)chunk * c.chunk_px;
+    const Place at(c);
+    const uint32_t unit = gridDim.x - 1 - blockIdx.x;
+    const uint32_t item = unit / c.chunks, chunk = unit - item * c.chunks;
+    uint32_t left = at.pixels(c, chunk);
+    const uint32_t vec = c.first_vec(blockIdx.y) + at.vec, group0 = c.first_group(blockIdx.y);
+    const size_t px0 = (size_t)chunk * c.chunk_px + at.row;
     const T* p = x + (size_t)item * c.item_stride + px0 * c.px_stride + (size_t)vec * V;
     const size_t at_out = ((size_t)item * c.n_px + px0) * c.n_ch + (size_t)vec * V;
     const T* q = gy + at_out;
     T* o = gx + at_out;
-    const uint32_t len = c.px_of(chunk);
-    const auto grad = [&](float (&xv)[V], float (&gv)[V]) {
-        float z[V];
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-            xv[j] = (xv[j] - mu) * s;
-            z[j] = fmaf(xv[j], w[j], b[j]);
-        }
-        act_slopes<V>(act, z, gv);
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-            gv[j] = s * (fmaf(gv[j], w[j], -ab.x) - xv[j] * ab.y);
-        }
-    };
-    uint32_t i = at.row;
-    for (; i + (kBatch - 1) * c.rows < len; i += kBatch * c.rows) {
-        float xv[kBatch][V], gv[kBatch][V];
-#pragma unroll
-        for (uint32_t k = 0; k < kBatch; k++) {
-            load_vec<T, V>(p + (size_t)(i + k * c.rows) * c.px_stride, xv[k]);
-            load_vec<T, V>(q + (size_t)(i + k * c.rows) * c.n_ch, gv[k]);
-        }
-#pragma unroll
-        for (uint32_t k = 0; k < kBatch; k++) {
-            grad(xv[k], gv[k]);
-            store_vec<T, V>(o + (size_t)(i + k * c.rows) * c.n_ch, gv[k]);
-        }
+    const size_t step = (size_t)c.rows * c.px_stride, qstep = (size_t)c.rows * c.n_ch;
+    Pack<T, V> xv[kBatchBwd], gv[kBatchBwd];
+    uint32_t count = left < kBatchBwd ? left : kBatchBwd;
+    Channels<V, S> ch;
+    if (left > 0) {
+        load_batch<T, V, kBatchBwd>(p + (left - count) * step, step, count, xv);
+        load_batch<T, V, kBatchBwd>(q + (left - count) * qstep, qstep, count, gv);
+        ch.load(c, aff, item, vec, mean, rstd);
     }
-    for (; i < len; i += c.rows) {
-        float xv[V], gv[V];
-        load_vec<T, V>(p + (size_t)i * c.px_stride, xv);
-        load_vec<T, V>(q + (size_t)i * c.n_ch, gv);
-        grad(xv, gv);
-        store_vec<T, V>(o + (size_t)i * c.n_ch, gv);
-    }
-}
-
-// gw, gb: the chunks' channel sums over all items, in a fixed order; 32
-// channels and 32 shares of the chunks a workgroup.
-__global__ __launch_bounds__(1024) void k_gn_param_grad(const float2* ch_part, size_t n_rows,
-                                                        uint32_t n_ch, uint32_t type, void* gw,
-                                                        void* gb) {
-    __shared__ double sa[32][33], sb[32][33];
-    const uint32_t lane = threadIdx.x & 31u, row = threadIdx.x >> 5;
-    const uint32_t ch = blockIdx.x * 32 + lane;
-    double a = 0.0, b = 0.0;
-    if (ch < n_ch) {
-#pragma unroll 4
-        for (size_t r = row; r < n_rows; r += 32) {
-            const float2 q = ch_part[r * n_ch + ch];
-            a += (double)q.x;
-            b += (double)q.y;
-        }
-    }
-    sa[row][lane] = a;
-    sb[row][lane] = b;
-    __syncthreads();
-    for (uint32_t s = 16; s > 0; s >>= 1) {
-        if (row < s) {
-            sa[row][lane] += sa[row + s][lane];
-            sb[row][lane] += sb[row + s][lane];
+    {
+        const uint32_t groups = c.groups(blockIdx.y), entries = c.parts * c.chunks;
+        const uint32_t lanes = lanes_of_group(groups), lane = threadIdx.x & (lanes - 1);
+        const float inv = 1.f / ((float)c.n_px * (float)c.group_ch);
+        for (uint32_t g = threadIdx.x / lanes; g - threadIdx.x / lanes < groups;
+             g += blockDim.x / lanes) {
+            float2 s = make_float2(0.f, 0.f);
+            if (g < groups) {
+                const float2* e0 = group_part + ((size_t)item * c.n_groups + group0 + g) * entries;
+#pragma unroll 8
+                for (uint32_t e = lane; e < entries; e += lanes) {
+                    accumulate(s, e0[e]);
+                }
+            }
+            for (uint32_t d = 1; d < lanes; d <<= 1) {
+                accumulate(s, shfl_xor(s, d));
+            }
+            if (g < groups && lane == 0) {
+                mean_of[g] = make_float2(s.x * inv, s.y * inv);
+            }
         }
         __syncthreads();
     }
-    if (row == 0 && ch < n_ch) {
-        if (gb) {
-            store_as(gb, type, ch, (float)sa[0][lane]);
+    if (left == 0) {
+        return;
+    }
+    float2 m[S];
+#pragma unroll
+    for (int g = 0; g < S; g++) {
+        m[g] = mean_of[group_of<V, S>(c, vec, g) - group0];
+    }
+    while (true) {
+        left -= count;
+#pragma unroll
+        for (uint32_t k = 0; k < kBatchBwd; k++) {
+            if (k < count) {
+                ch.finish(xv[k], gv[k], act, m, o + (left + k) * qstep, c.stream);
+            }
         }
-        if (gw) {
-            store_as(gw, type, ch, (float)sb[0][lane]);
+        if (left == 0) {
+            break;
+        }
+        count = left < kBatchBwd ? left : kBatchBwd;
+        load_batch<T, V, kBatchBwd>(p + (left - count) * step, step, count, xv);
+        load_batch<T, V, kBatchBwd>(q + (left - count) * qstep, qstep, count, gv);
+    }
+}
+
+// Both passes where a block's pixels fit its workgroup's registers. ch_part
+// (null for one item: gw and gb are whole then) gets the item's channel sums.
+template <typename T, int V>
+__global__ __launch_bounds__(kItemThreads) void k_gn_bwd_item(
+        const T* gy, const T* x, const Cut c, const Affine aff, uint32_t act, const float* mean,
+        const float* rstd, float2* ch_part, T* gx, void* gw, void* gb) {
+    constexpr uint32_t kWaves = kItemThreads / 64;
+    __shared__ float2 part[kWaves][64];
+    __shared__ float2 chs[kWaves][V][64];
+    const ItemPlace at(c);
+    const uint32_t item = blockIdx.x;
+    const uint32_t vec = c.first_vec(blockIdx.y) + at.vec;
+    const T* p = x + (size_t)item * c.item_stride + (size_t)at.row * c.px_stride + (size_t)vec * V;
+    const size_t at_out = ((size_t)item * c.n_px + at.row) * c.n_ch + (size_t)vec * V;
+    const T* q = gy + at_out;
+    T* o = gx + at_out;
+    const size_t step = (size_t)c.rows * c.px_stride, qstep = (size_t)c.rows * c.n_ch;
+    Pack<T, V> xv[kHold], gv[kHold];
+#pragma unroll
+    for (uint32_t k = 0; k < kHold; k++) {
+        if (k < at.mine) {
+            xv[k] = load_pack<T, V>(p + k * step);
+            gv[k] = load_pack<T, V>(q + k * qstep);
+        }
+    }
+    float sa[V], sb[V];
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+        sa[j] = sb[j] = 0.f;
+    }
+    Channels<V, 1> ch;
+    float2 g = make_float2(0.f, 0.f);
+    if (at.mine > 0) {
+        ch.load(c, aff, item, vec, mean, rstd);
+#pragma unroll
+        for (uint32_t k = 0; k < kHold; k++) {
+            if (k < at.mine) {
+                ch.add(xv[k], gv[k], act, sa, sb);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            g.x = fmaf(ch.w[j], sa[j], g.x);
+            g.y = fmaf(ch.w[j], sb[j], g.y);
+        }
+    }
+    const uint32_t wave = threadIdx.x / 64;
+    if (ch_part || gw || gb) {
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            float2 s = make_float2(sa[j], sb[j]);
+            for (uint32_t d = c.lanes; d < 64; d *= 2) {
+                accumulate(s, shfl_xor(s, d));
+            }
+            if ((threadIdx.x & 63u) < c.lanes) {
+                chs[wave][j][at.vec] = s;
+            }
+        }
+    }
+    g = add_item(c, at, g, part);  // its barrier is chs's too
+    if (ch_part || gw || gb) {
+        const uint32_t n = c.vecs(blockIdx.y);
+        for (uint32_t i = threadIdx.x; i < n * V; i += blockDim.x) {
+            const uint32_t v = i / V, j = i - v * V;
+            float2 s = chs[0][j][v];
+            for (uint32_t k = 1; k < blockDim.x / 64; k++) {
+                accumulate(s, chs[k][j][v]);
+            }
+            const uint32_t chan = c.first_vec(blockIdx.y) * V + i;
+            if (ch_part) {
+                ch_part[(size_t)item * c.n_ch + chan] = s;
+            } else {
+                if (gb) {
+                    store_as(gb, aff.type, chan, s.x);
+                }
+                if (gw) {
+                    store_as(gw, aff.type, chan, s.y);
+                }
+            }
+        }
+    }
+    if (at.mine == 0 || !gx) {
+        return;
+    }
+    const float inv = 1.f / ((float)c.n_px * (float)c.group_ch);
+    const float2 m[1] = {make_float2(g.x * inv, g.y * inv)};
+#pragma unroll
+    for (uint32_t k = 0; k < kHold; k++) {
+        if (k < at.mine) {
+            ch.finish(xv[k], gv[k], act, m, o + k * qstep, c.stream);
         }
     }
 }
@@ -643,19 +1121,25 @@ __global__ __launch_bounds__(1024) void k_gn_param_grad(const float2* ch_part, s
 // host
 // ---------------------------------------------------------------------------
 
-// The widest vector that a group's channels, the strides and the pointers
-// allow, 16 bytes at most. A vector never straddles groups.
-uint32_t vec_width(uint32_t type, uint32_t n_ch, uint32_t n_groups, uint64_t item_stride,
-                   uint64_t px_stride, std::initializer_list<const void*> ptrs) {
+// How wide a thread's vectors are: 16 bytes at most, as the channels, the
+// strides and the pointers allow. `whole`: a vector that no group's edge cuts.
+struct Width {
+    uint32_t any, whole;
+};
+Width vec_width(uint32_t type, uint32_t n_ch, uint32_t n_groups, uint64_t item_stride,
+                uint64_t px_stride, std::initializer_list<const void*> ptrs) {
     const uint32_t size = (uint32_t)type_bytes(type);
-    uint64_t bits = (uint64_t)(n_ch / n_groups) | item_stride | px_stride | (16u / size);
-    uint32_t v = (uint32_t)(bits & (~bits + 1));
+    const auto low_bit = [](uint64_t x) { return (uint32_t)(x & (~x + 1)); };
+    uint32_t v = low_bit((uint64_t)n_ch | item_stride | px_stride | (16u / size));
     for (const void* p : ptrs) {
         while (v > 1 && (uintptr_t)p % ((size_t)v * size) != 0) {
             v >>= 1;
         }
     }
-    return v;
+    const uint32_t group_ch = n_ch / n_groups, whole = std::min(v, low_bit(group_ch));
+    // a unit of several groups has to fit a workgroup
+    const uint32_t unit = v / whole;
+    return {unit > 1 && group_ch * unit / v > kMaxVecs ? whole : v, whole};
 }
 
 struct Scratch {
@@ -682,6 +1166,7 @@ int check_shape(const char* what, uint32_t type, uint32_t n_items, uint64_t n_px
     return DRESSI_OK;
 }
 
+// f(a vector's type, whether a group's edge may cut it)
 template <typename F>
 int for_width(uint32_t type, uint32_t v, F&& f) {
     switch (type) {
@@ -701,39 +1186,71 @@ int for_width(uint32_t type, uint32_t v, F&& f) {
 }
 
 template <typename T, int V>
+int launch_item(hipStream_t s, const Cut& c, const void* x, const Affine& aff, float eps,
+                uint32_t act, void* y, float* mean, float* rstd) {
+    hipLaunchKernelGGL((k_gn_item<T, V>), dim3(c.n_items, c.n_blocks), dim3(c.threads), 0, s,
+                       (const T*)x, c, aff, eps, act, (T*)y, mean, rstd);
+    DRESSI_CHECK_LAUNCH();
+    return DRESSI_OK;
+}
+
+template <typename T, int V, int S>
 int launch_forward(hipStream_t s, const Cut& c, const void* x, const Affine& aff, float eps,
                    uint32_t act, void* scratch, void* y, float* mean, float* rstd) {
     const dim3 grid(c.n_items * c.chunks, c.n_blocks), block(c.threads);
-    hipLaunchKernelGGL((k_gn_stats<T, V>), grid, block, 0, s, (const T*)x, c, (float2*)scratch);
+    hipLaunchKernelGGL((k_gn_stats<T, V, S>), grid, block, 0, s, (const T*)x, c,
+                       (float2*)scratch);
     DRESSI_CHECK_LAUNCH();
-    hipLaunchKernelGGL((k_gn_apply<T, V>), grid, block, 0, s, (const T*)x, c,
+    hipLaunchKernelGGL((k_gn_apply<T, V, S>), grid, block, 0, s, (const T*)x, c,
                        (const float2*)scratch, aff, eps, act, (T*)y, mean, rstd);
     DRESSI_CHECK_LAUNCH();
     return DRESSI_OK;
 }
 
+int launch_param_grad(hipStream_t s, const ParamGrad& a) {
+    hipLaunchKernelGGL(k_gn_param_grad, dim3(div_up(a.n_ch, kParamCh)), dim3(kMaxThreads), 0, s, a);
+    DRESSI_CHECK_LAUNCH();
+    return DRESSI_OK;
+}
+
 template <typename T, int V>
+int launch_bwd_item(hipStream_t s, const Cut& c, const void* gy, const void* x, const Affine& aff,
+                    uint32_t act, const float* mean, const float* rstd, void* scratch, void* gx,
+                    void* gw, void* gb) {
+    const bool sums = c.n_items > 1 && (gw || gb);  // the items' are added afterwards
+    hipLaunchKernelGGL((k_gn_bwd_item<T, V>), dim3(c.n_items, c.n_blocks), dim3(c.threads), 0, s,
+                       (const T*)gy, (const T*)x, c, aff, act, mean, rstd,
+                       sums ? (float2*)scratch : nullptr, (T*)gx, gw, gb);
+    DRESSI_CHECK_LAUNCH();
+    return sums ? launch_param_grad(s, ParamGrad{(const float2*)scratch, c.n_items, c.n_ch,
+                                                 aff.type, gw, gb})
+                : DRESSI_OK;
+}
+
+template <typename T, int V, int S>
 int launch_backward(hipStream_t s, const Cut& c, const void* gy, const void* x, const Affine& aff,
                     uint32_t act, const float* mean, const float* rstd, void* scratch, void* gx,
                     void* gw, void* gb) {
     const dim3 grid(c.n_items * c.chunks, c.n_blocks), block(c.threads);
     float2* group_part = (float2*)scratch;
     float2* ch_part = (float2*)((char*)scratch + scratch_of(c, true).group_part);
-    hipLaunchKernelGGL((k_gn_bwd_sums<T, V>), grid, block, 0, s, (const T*)gy, (const T*)x, c, aff,
-                       act, mean, rstd, group_part, ch_part);
+    const ParamGrad params{ch_part, (size_t)c.n_items * c.chunks, c.n_ch, aff.type, gw, gb};
+    hipLaunchKernelGGL((k_gn_bwd_sums<T, V, S>), grid, block, 0, s, (const T*)gy, (const T*)x, c,
+                       aff, act, mean, rstd, group_part, ch_part);
     DRESSI_CHECK_LAUNCH();
-    if (gx) {
-        hipLaunchKernelGGL((k_gn_bwd_apply<T, V>), grid, block, 0, s, (const T*)gy, (const T*)x, c,
-                           aff, act, mean, rstd, group_part, (T*)gx);
-        DRESSI_CHECK_LAUNCH();
+    if (!gx) {
+        return gw || gb ? launch_param_grad(s, params) : DRESSI_OK;
     }
-    if (gw || gb) {
-        hipLaunchKernelGGL(k_gn_param_grad, dim3(div_up(c.n_ch, 32)), dim3(1024), 0, s, ch_part,
-                           (size_t)c.n_items * c.chunks, c.n_ch, aff.type, gw, gb);
-        DRESSI_CHECK_LAUNCH();
-    }
+    const uint32_t extra = gw || gb ? div_up(c.n_ch, kParamCh) : 0;
+    hipLaunchKernelGGL((k_gn_bwd_apply<T, V, S>), dim3(grid.x + extra, grid.y), block, 0, s,
+                       (const T*)gy, (const T*)x, c, aff, act, mean, rstd, group_part, (T*)gx,
+                       params, extra);
+    DRESSI_CHECK_LAUNCH();
     return DRESSI_OK;
 }
+
+// Bytes of an image from which results go past the caches.
+constexpr uint64_t kStreamBytes = 32ull << 20;
 
 }  // namespace
 }  // namespace dressi
@@ -748,8 +1265,9 @@ size_t dressi_group_norm_scratch(uint32_t type, uint32_t n_items, uint64_t n_px,
         n_ch % n_groups != 0) {
         return 0;
     }
+    // whatever vectors the pointers allow, and either way of cutting
     size_t most = 0;
-    for (uint32_t v = 1; v <= 16u / type_bytes(type) && n_ch / n_groups % v == 0; v *= 2) {
+    for (uint32_t v = 1; v <= 16u / type_bytes(type) && n_ch % v == 0; v *= 2) {
         most = std::max(most,
                         scratch_of(make_cut(n_items, n_px, n_ch, n_groups, v), backward != 0).bytes);
     }
@@ -771,16 +1289,33 @@ int dressi_group_norm(dressi_ctx* ctx, const void* x, uint32_t type, uint32_t n_
     }
     DRESSI_REQUIRE(x && y && mean && rstd && scratch, "group_norm: bad arguments");
     DRESSI_REQUIRE(px_stride >= n_ch || n_px == 1, "group_norm: pixels overlap");
-    const uint32_t v = vec_width(type, n_ch, n_groups, n_items > 1 ? item_stride : 0,
-                                 n_px > 1 ? px_stride : 0, {x, y});
-    Cut c = make_cut(n_items, n_px, n_ch, n_groups, v);
-    c.item_stride = item_stride;
-    c.px_stride = px_stride;
+    const Width v = vec_width(type, n_ch, n_groups, n_items > 1 ? item_stride : 0,
+                              n_px > 1 ? px_stride : 0, {x, y});
+    const auto place = [&](Cut& c) {
+        c.item_stride = item_stride;
+        c.px_stride = px_stride;
+        c.stream = (uint64_t)n_items * n_px * n_ch * type_bytes(type) >= kStreamBytes;
+    };
+    Cut c = make_item_cut(n_items, n_px, n_ch, n_groups, v.whole);
+    if (c.chunks) {
+        place(c);
+        return for_width(type, v.whole, [&](auto w) {
+            using T = std::remove_reference_t<decltype(w.v[0])>;
+            return launch_item<T, sizeof(w) / sizeof(T)>(ctx->stream, c, x, aff, eps, activation, y,
+                                                         mean, rstd);
+        });
+    }
+    c = make_cut(n_items, n_px, n_ch, n_groups, v.any);
+    place(c);
     DRESSI_REQUIRE(scratch_bytes >= scratch_of(c, false).bytes, "group_norm: scratch too small");
-    return for_width(type, v, [&](auto w) {
+    return for_width(type, v.any, [&](auto w) {
         using T = std::remove_reference_t<decltype(w.v[0])>;
-        return launch_forward<T, sizeof(w) / sizeof(T)>(ctx->stream, c, x, aff, eps, activation,
-                                                        scratch, y, mean, rstd);
+        constexpr int V = sizeof(w) / sizeof(T);
+        return v.any == v.whole
+                   ? launch_forward<T, V, 1>(ctx->stream, c, x, aff, eps, activation, scratch, y,
+                                             mean, rstd)
+                   : launch_forward<T, V, V>(ctx->stream, c, x, aff, eps, activation, scratch, y,
+                                             mean, rstd);
     });
 }
 
@@ -798,27 +1333,43 @@ int dressi_group_norm_bwd(dressi_ctx* ctx, const void* gy, const void* x, uint32
     }
     if (n_items == 0 || n_px == 0) {
         // sums of nothing
-        for (void* p : {gw, gb}) {
-            if (p) {
-                hipLaunchKernelGGL(k_gn_param_grad, dim3(div_up(n_ch, 32)), dim3(1024), 0,
-                                   ctx->stream, nullptr, (size_t)0, n_ch, affine_type, p, nullptr);
-                DRESSI_CHECK_LAUNCH();
-            }
+        if (gw || gb) {
+            return launch_param_grad(ctx->stream, ParamGrad{nullptr, 0, n_ch, affine_type, gw, gb});
         }
         return DRESSI_OK;
     }
     DRESSI_REQUIRE(gy && x && mean && rstd && scratch, "group_norm_bwd: bad arguments");
     DRESSI_REQUIRE(px_stride >= n_ch || n_px == 1, "group_norm_bwd: pixels overlap");
-    const uint32_t v = vec_width(type, n_ch, n_groups, n_items > 1 ? item_stride : 0,
-                                 n_px > 1 ? px_stride : 0, {gy, x, gx});
-    Cut c = make_cut(n_items, n_px, n_ch, n_groups, v);
-    c.item_stride = item_stride;
-    c.px_stride = px_stride;
+    const Width v = vec_width(type, n_ch, n_groups, n_items > 1 ? item_stride : 0,
+                              n_px > 1 ? px_stride : 0, {gy, x, gx});
+    const auto place = [&](Cut& c) {
+        c.item_stride = item_stride;
+        c.px_stride = px_stride;
+        c.stream = (uint64_t)n_items * n_px * n_ch * type_bytes(type) >= kStreamBytes;
+    };
+    Cut c = make_item_cut(n_items, n_px, n_ch, n_groups, v.whole);
+    if (c.chunks) {
+        place(c);
+        DRESSI_REQUIRE(scratch_bytes >= scratch_of(c, true).ch_part,
+                       "group_norm_bwd: scratch too small");
+        return for_width(type, v.whole, [&](auto w) {
+            using T = std::remove_reference_t<decltype(w.v[0])>;
+            return launch_bwd_item<T, sizeof(w) / sizeof(T)>(ctx->stream, c, gy, x, aff,
+                                                             activation, mean, rstd, scratch, gx,
+                                                             gw, gb);
+        });
+    }
+    c = make_cut(n_items, n_px, n_ch, n_groups, v.any);
+    place(c);
     DRESSI_REQUIRE(scratch_bytes >= scratch_of(c, true).bytes, "group_norm_bwd: scratch too small");
-    return for_width(type, v, [&](auto w) {
+    return for_width(type, v.any, [&](auto w) {
         using T = std::remove_reference_t<decltype(w.v[0])>;
-        return launch_backward<T, sizeof(w) / sizeof(T)>(ctx->stream, c, gy, x, aff, activation,
-                                                         mean, rstd, scratch, gx, gw, gb);
+        constexpr int V = sizeof(w) / sizeof(T);
+        return v.any == v.whole
+                   ? launch_backward<T, V, 1>(ctx->stream, c, gy, x, aff, activation, mean, rstd,
+                                              scratch, gx, gw, gb)
+                   : launch_backward<T, V, V>(ctx->stream, c, gy, x, aff, activation, mean, rstd,
+                                              scratch, gx, gw, gb);
     });
 }
 
