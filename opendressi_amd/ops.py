@@ -737,7 +737,7 @@ def _typed(ctx: Context, t: torch.Tensor, name: str) -> int:
     code = TYPE_CODES.get(t.dtype)
     if code is None:
         raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
-    if t.device.type != "cuda" or t.device.index != ctx.device:
+    if t.get_device() != ctx.device:  # -1 for the host
         raise ValueError(f"{name}: expected a tensor on cuda:{ctx.device}, got one on {t.device}")
     return code
 
@@ -764,7 +764,7 @@ def _pixel_strides(x: torch.Tensor) -> tuple[int, int, int] | None:
 
 def _affine(ctx: Context, c: int, weight, bias) -> int:
     """Checks weight and bias of c channels; their type's code."""
-    kinds = set()
+    kind = None
     for t, name in ((weight, "weight"), (bias, "bias")):
         if t is None:
             continue
@@ -772,10 +772,12 @@ def _affine(ctx: Context, c: int, weight, bias) -> int:
             raise ValueError(f"{name} must be [{c}], got {tuple(t.shape)}")
         if not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous")
-        kinds.add(_typed(ctx, t, name))
-    if len(kinds) > 1:
-        raise TypeError(f"weight is {weight.dtype}, bias {bias.dtype}: they must be of one type")
-    return kinds.pop() if kinds else F32
+        code = _typed(ctx, t, name)
+        if kind is not None and code != kind:
+            raise TypeError(f"weight is {weight.dtype}, bias {bias.dtype}: they must be of one "
+                            "type")
+        kind = code
+    return F32 if kind is None else kind
 
 
 def _norm_args(x: torch.Tensor, groups: int, activation: str) -> int:
@@ -805,18 +807,18 @@ def group_norm(ctx: Context, x: torch.Tensor, groups: int, weight: torch.Tensor 
     channels of a wider image); others are packed first."""
     act = _norm_args(x, groups, activation)
     code, aff = _typed(ctx, x, "x"), _affine(ctx, x.shape[-1], weight, bias)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean, rstd = torch.zeros((2, x.shape[0], groups), dtype=torch.float32, device=x.device) \
-        if x.numel() == 0 else \
-        torch.empty((2, x.shape[0], groups), dtype=torch.float32, device=x.device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    n, c = x.shape[0], x.shape[-1]
     if x.numel() == 0:
+        mean, rstd = torch.zeros((2, n, groups), dtype=torch.float32, device=x.device)
         return y, mean, rstd
+    mean = torch.empty((n, groups), dtype=torch.float32, device=x.device)
+    rstd = torch.empty_like(mean)
     at = _pixel_strides(x)
     if at is None:
         x = x.contiguous()
         at = _pixel_strides(x)
     n_px, item, px = at
-    n, c = x.shape[0], x.shape[-1]
     size = lib.dressi_group_norm_scratch(code, n, n_px, c, groups, 0)
     scratch = torch.empty(size, dtype=torch.uint8, device=x.device)
     _prep(ctx)
@@ -845,10 +847,10 @@ def group_norm_bwd(ctx: Context, gy: torch.Tensor, x: torch.Tensor, mean: torch.
         _ptr(t, name)
         if t.shape != (n, groups) or t.device != x.device:
             raise ValueError(f"{name} must be [{n}, {groups}], got {tuple(t.shape)}")
-    kind = next((t.dtype for t in (weight, bias) if t is not None), torch.float32)
-    gx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
-    gw = torch.empty(c, dtype=kind, device=x.device) if need[1] else None
-    gb = torch.empty(c, dtype=kind, device=x.device) if need[2] else None
+    gx = torch.empty_like(x, memory_format=torch.contiguous_format) if need[0] else None
+    some = weight if weight is not None else bias
+    gw, gb = (None if not wanted else torch.empty(c, dtype=torch.float32, device=x.device)
+              if some is None else torch.empty_like(some) for wanted in need[1:])
     at = _pixel_strides(x)
     if at is None:
         x = x.contiguous()

@@ -7,6 +7,7 @@ one stream; every op and plan created from it is stream-ordered on it.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import numpy as np
 
@@ -18,6 +19,15 @@ _FP = C.POINTER(C.c_float)
 def _fp(a: np.ndarray):
     assert a.dtype == np.float32 and a.flags["C_CONTIGUOUS"]
     return a.ctypes.data_as(_FP)
+
+
+@functools.cache
+def _torch_stream():
+    """device index -> the handle of torch's current stream there: without the
+    Stream object (a microsecond) where this torch has the call for it."""
+    import torch
+    return getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+        (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 class Context:
@@ -48,8 +58,7 @@ class Context:
 
     def use_torch_stream(self) -> None:
         """Order this context's work on torch's current HIP stream."""
-        import torch
-        self.set_stream(torch.cuda.current_stream(self.device).cuda_stream)
+        check(lib.dressi_ctx_set_stream(self.handle, _torch_stream()(self.device)))
 
     def synchronize(self) -> None:
         check(lib.dressi_ctx_synchronize(self.handle))

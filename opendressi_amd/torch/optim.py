@@ -5,15 +5,19 @@ surface, whose optimizer is part of its graph.
 """
 from __future__ import annotations
 
-import ctypes as C
 import math
+from collections import OrderedDict
 
+import numpy as np
 import torch
 
 from .._lib import AdamwSet, AdamwTensor, check, lib
 from ..ops import TYPE_CODES, _addr
 from .context import RasterizeHipContext
 
+# an entry of the table of parameters (dressi_adamw_tensor)
+_ENTRY = np.dtype([("param", "<u8"), ("grad", "<u8"), ("n", "<u8"), ("state", "<u8"),
+                   ("type", "<u4"), ("set", "<u4")])
 BLOCK = 32  # elements that share an exponent; a parameter's share is padded to whole ones
 
 
@@ -61,7 +65,8 @@ class AdamW(torch.optim.Optimizer):
 
     A parameter whose grad is None is left as it is, and so is its step. A
     step cannot be captured into a graph: it takes the step count from the
-    host."""
+    host. Hooks registered on the optimizer run; torch's global optimizer
+    hooks do not."""
 
     def __init__(self, ctx: RasterizeHipContext, params, lr: float = 1e-3, betas=(0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float = 1e-2, state_bits: int = 32,
@@ -79,7 +84,11 @@ class AdamW(torch.optim.Optimizer):
         self._params: list[torch.Tensor] = []  # in the order of their shares
         self._steps: list[int] = []
         self._groups: list[dict] = []  # each parameter's
-        self._table = (AdamwTensor * 0)()
+        self._pre_hooks: OrderedDict = OrderedDict()
+        self._post_hooks: OrderedDict = OrderedDict()
+        self._expect: list[tuple] = []  # each parameter with its size and type
+        self._sets: list[tuple[dict, int]] = []  # each group with the place of its first parameter
+        self._even = True  # every group's parameters have taken the same steps
         self._total = 0
         self._moments: tuple[torch.Tensor, torch.Tensor] | None = None
         self._scales: tuple[torch.Tensor | None, torch.Tensor | None] = (None, None)
@@ -101,18 +110,23 @@ class AdamW(torch.optim.Optimizer):
         _check_hyper(group)
         super().add_param_group(group)
         group = self.param_groups[-1]
+        if group["params"]:
+            self._sets.append((group, len(self._params)))
         for p in group["params"]:
             self._params.append(p)
             self._steps.append(0)
             self._groups.append(group)
-        table = (AdamwTensor * len(self._params))()
         at = 0
+        table = (AdamwTensor * len(self._params))()
+        view = np.frombuffer(table, dtype=_ENTRY) if len(table) else np.empty(0, _ENTRY)
         for i, p in enumerate(self._params):
-            table[i].n, table[i].state = p.numel(), at
-            table[i].type = TYPE_CODES[p.dtype]
+            view[i] = (0, 0, p.numel(), at, TYPE_CODES[p.dtype], 0)
             at += -(-p.numel() // BLOCK) * BLOCK
+        for k, (_, first) in enumerate(self._sets):
+            view["set"][first:] = k
         self._grow(at)
-        self._table, self._total = table, at
+        self._expect = [(p, p.numel(), p.dtype) for p in self._params]
+        self._table, self._view, self._total = table, view, at
 
     def _check_param(self, p) -> None:
         if not isinstance(p, torch.Tensor):
@@ -155,10 +169,39 @@ class AdamW(torch.optim.Optimizer):
 
     # ---- the step ----
 
-    @torch.no_grad()
     def step(self, closure=None):
         """One step with the parameters' present gradients; returns the
         closure's loss, if there is a closure."""
+        if not self._pre_hooks and not self._post_hooks:
+            return self._step(closure)
+        args, kwargs = (closure,), {}
+        for hook in list(self._pre_hooks.values()):
+            new = hook(self, args, kwargs)
+            if new is not None:
+                args, kwargs = new
+        loss = self._step(*args, **kwargs)
+        for hook in list(self._post_hooks.values()):
+            hook(self, args, kwargs)
+        return loss
+
+    # torch would wrap step for its hooks and profiler label, 7 us a call; a torch that does not
+    # know this mark wraps it all the same
+    step.hooked = True
+
+    def register_step_pre_hook(self, hook):
+        """hook(optimizer, args, kwargs) before each step; it may return new
+        (args, kwargs). Returns a handle whose remove() takes it out."""
+        handle = torch.utils.hooks.RemovableHandle(self._pre_hooks)
+        self._pre_hooks[handle.id] = hook
+        return handle
+
+    def register_step_post_hook(self, hook):
+        """hook(optimizer, args, kwargs) after each step."""
+        handle = torch.utils.hooks.RemovableHandle(self._post_hooks)
+        self._post_hooks[handle.id] = hook
+        return handle
+
+    def _step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -166,43 +209,47 @@ class AdamW(torch.optim.Optimizer):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("AdamW.step cannot be captured into a graph: its step count is "
                                "the host's")
-        table, steps = self._table, list(self._steps)
+        dev = self.ctx.device.index
         kept = []  # copies that the launch reads
-        live = []  # entries with a gradient
-        sets: dict[tuple, int] = {}
-        for i, p in enumerate(self._params):
+        live, params, grads = [], [], []
+        for i, (p, n, kind) in enumerate(self._expect):
             g = p.grad
             if g is None:
                 continue
-            e = table[i]
-            if g.layout is not torch.strided:
-                raise RuntimeError("AdamW: sparse gradients are not supported")
-            if g.numel() != e.n or p.numel() != e.n or TYPE_CODES.get(g.dtype) != e.type \
-                    or p.dtype != g.dtype or g.device != self.ctx.device \
-                    or p.device != g.device:
-                raise ValueError(f"parameter {i} or its gradient changed its size, type or device: "
-                                 f"{p.dtype} {tuple(p.shape)} on {p.device}, {g.dtype} "
-                                 f"{tuple(g.shape)} on {g.device}")
-            same = g.stride() == p.stride()
-            if not (same and g.is_contiguous()) and not _dense(p):
-                raise ValueError(f"parameter {i} is no longer densely stored")
-            if not same:  # into the parameter's own order
-                g = torch.empty_strided(p.shape, p.stride(), dtype=g.dtype,
-                                        device=g.device).copy_(g)
+            # a parameter's and its gradient's storage may have been replaced
+            if (g.dtype is not kind or p.dtype is not kind or g.numel() != n or p.numel() != n
+                    or g.get_device() != dev or p.get_device() != dev
+                    or g.layout is not torch.strided
+                    or not (g.is_contiguous() and p.is_contiguous())):
+                g = self._reorder(i, p, g, n, kind)
                 kept.append(g)
-            steps[i] += 1
-            e.param, e.grad = p.data_ptr(), g.data_ptr()
-            e.set = sets.setdefault((id(self._groups[i]), steps[i]), len(sets))
             live.append(i)
+            params.append(p.data_ptr())
+            grads.append(g.data_ptr())
         if not live:
             return loss
-        group_of = {id(g): g for g in self.param_groups}
-        hyper = (AdamwSet * len(sets))()
-        for (gid, t), k in sets.items():
-            g = group_of[gid]
-            hyper[k] = AdamwSet(g["lr"], *g["betas"], g["eps"], g["weight_decay"], t)
-        if len(live) < len(table):
-            table = (AdamwTensor * len(live))(*(table[i] for i in live))
+        every = len(live) == len(self._expect)
+        steps = self._steps
+        if every and self._even:
+            # all in step: a set for each group, as the table has it
+            now = [t + 1 for t in steps]
+            sets = [(g, steps[at] + 1) for g, at in self._sets]
+            table, view = self._table, self._view
+        else:
+            now = list(steps)
+            index, sets, of = {}, [], []
+            for i in live:
+                now[i] += 1
+                k = index.setdefault((id(self._groups[i]), now[i]), len(sets))
+                if k == len(sets):
+                    sets.append((self._groups[i], now[i]))
+                of.append(k)
+            view = self._view[live].copy()
+            view["set"] = of
+            table = (AdamwTensor * len(live)).from_buffer(view)
+        view["param"], view["grad"] = params, grads
+        hyper = (AdamwSet * len(sets))(*(
+            (g["lr"], *g["betas"], g["eps"], g["weight_decay"], t) for g, t in sets))
         ctx = self.ctx
         with ctx.lock:
             ctx._ctx.use_torch_stream()
@@ -211,8 +258,27 @@ class AdamW(torch.optim.Optimizer):
                 self._moments[0].data_ptr(), self._moments[1].data_ptr(),
                 _addr(self._scales[0]), _addr(self._scales[1]), _addr(self.master), self.seed,
                 self.max_grad_norm or 0.0, self._scratch.data_ptr(), _addr(self.grad_norm)))
-        self._steps = steps
+        self._steps = now
+        self._even = self._even and every
         return loss
+
+    def _reorder(self, i: int, p, g, n: int, kind) -> torch.Tensor:
+        """The gradient in its parameter's memory order; refuses what the
+        kernel cannot take."""
+        if g.layout is not torch.strided:
+            raise RuntimeError("AdamW: sparse gradients are not supported")
+        if g.numel() != n or p.numel() != n or g.dtype is not kind or p.dtype is not kind \
+                or g.device != self.ctx.device or p.device != g.device:
+            raise ValueError(f"parameter {i} or its gradient changed its size, type or device: "
+                             f"{p.dtype} {tuple(p.shape)} on {p.device}, {g.dtype} "
+                             f"{tuple(g.shape)} on {g.device}")
+        if not _dense(p):
+            raise ValueError(f"parameter {i} is no longer densely stored")
+        if g.stride() == p.stride():
+            return g
+        with torch.no_grad():
+            return torch.empty_strided(p.shape, p.stride(), dtype=g.dtype,
+                                       device=g.device).copy_(g)
 
     # ---- state ----
 
@@ -276,6 +342,8 @@ class AdamW(torch.optim.Optimizer):
         for k, t in named.items():
             t.copy_(state_dict[k])
         self._steps = steps
+        ends = [at for _, at in self._sets[1:]] + [len(steps)]
+        self._even = all(len(set(steps[a:b])) == 1 for (_, a), b in zip(self._sets, ends))
         self.seed = int(state_dict.get("seed", self.seed)) & 0xffffffff
 
 

@@ -393,6 +393,47 @@ def test_group_added_later(ctx):
     assert torch.allclose(b, torch.full_like(b, -0.5)) and torch.allclose(a, torch.full_like(a, -0.2))
 
 
+def test_hooks_closures_and_schedulers(ctx):
+    import opendressi_amd.torch as dr
+    p = torch.zeros(8, device="cuda", requires_grad=True)
+    opt = dr.AdamW(ctx, [p], lr=0.5, weight_decay=0.0)
+    sched = torch.optim.lr_scheduler.StepLR(opt, 1, 0.5)
+    seen = []
+    pre = opt.register_step_pre_hook(lambda o, a, k: seen.append("pre"))
+    opt.register_step_post_hook(lambda o, a, k: seen.append("post"))
+
+    def closure():
+        opt.zero_grad()
+        loss = p.sum()
+        loss.backward()
+        seen.append("loss")
+        return loss
+
+    assert float(opt.step(closure)) == 0.0
+    sched.step()
+    pre.remove()
+    opt.step()
+    assert seen == ["pre", "loss", "post", "post"]
+    assert torch.allclose(p.detach(), torch.full_like(p, -0.75))
+
+
+def test_state_is_freed(ctx):
+    """Nothing but the optimizer holds its state."""
+    import gc
+
+    import opendressi_amd.torch as dr
+    p = torch.zeros(1 << 22, device="cuda")
+    gc.disable()
+    try:
+        before = torch.cuda.memory_allocated()
+        opt = dr.AdamW(ctx, [p])
+        assert torch.cuda.memory_allocated() >= before + 8 * p.numel()
+        del opt
+        assert torch.cuda.memory_allocated() == before
+    finally:
+        gc.enable()
+
+
 def test_refusals(ctx):
     import opendressi_amd.torch as dr
     p = torch.zeros(8, device="cuda")
