@@ -824,11 +824,14 @@ int dressi_tex_profile(dressi_tex_plan* plan, uint32_t iters, char* names,
  * y is packed. weight / bias [n_ch] of `affine_type`, or NULL for 1 / 0.
  * mean, rstd [n_items][n_groups]: what the backward pass needs. Sums and
  * statistics are held in 32 bits. scratch: device memory of at least
- * dressi_group_norm_scratch bytes (backward: 0 or 1), used by this call
- * only, so that calls on several streams need several. */
+ * dressi_group_norm_scratch bytes (addresses: those of the call's images, x
+ * and y, or gy, x and gx, or-ed together; backward: 0 or 1), used by this
+ * call only, so that calls on several streams need several. */
 size_t dressi_group_norm_scratch(uint32_t type, uint32_t n_items,
                                  uint64_t n_px, uint32_t n_ch,
-                                 uint32_t n_groups, int backward);
+                                 uint64_t item_stride, uint64_t px_stride,
+                                 uint32_t n_groups, uint64_t addresses,
+                                 int backward);
 int dressi_group_norm(dressi_ctx* ctx, const void* x, uint32_t type,
                       uint32_t n_items, uint64_t n_px, uint32_t n_ch,
                       uint64_t item_stride, uint64_t px_stride,
@@ -848,12 +851,16 @@ int dressi_group_norm_bwd(dressi_ctx* ctx, const void* gy, const void* x,
                           size_t scratch_bytes, void* gx, void* gw, void* gb);
 
 /* One tensor of an AdamW step: n elements of `type`, packed, updated in
- * place. Its moments (and its master copy) start at element `state` of the
- * flat state buffers, a multiple of 32, and take n rounded up to 32; the
- * filling is zero. `set` names its dressi_adamw_set. */
+ * place. Its moments start at element `state` of the flat state buffers, a
+ * multiple of 32, and take n rounded up to 32; the filling is zero. master
+ * (n floats, 16-byte aligned, or NULL; not looked at for DRESSI_F32): the
+ * float copy of which a 16-bit parameter is the rounding. Where it is not,
+ * the parameter has been written since, and the copy takes its value. `set`
+ * names its dressi_adamw_set. */
 typedef struct dressi_adamw_tensor {
     void* param;
     const void* grad;
+    float* master;
     uint64_t n;
     uint64_t state;
     uint32_t type;
@@ -878,16 +885,16 @@ typedef struct dressi_adamw_set {
  * (bits(|x| 2^-(max(E, T) - T)) + r) >> 20 with T = 14 and the sign in bit 7
  * for exp_avg, T = 30 for exp_avg_sq; r is a hash of (element, step, seed)
  * below 2^20. exp_avg_sq above zero has a code above zero; E = 255 stands
- * for 32 NaN. master (float[state_elems], or NULL): where given, parameters
- * of 16 bits are roundings of it. */
+ * for 32 NaN. The steps' counts and rates are arguments: a step captured into
+ * a graph would repeat them. */
 size_t dressi_adamw_scratch(void);
 int dressi_adamw_step(dressi_ctx* ctx, const dressi_adamw_tensor* tensors,
                       uint32_t n_tensors, const dressi_adamw_set* sets,
                       uint32_t n_sets, uint32_t state_bits,
                       uint64_t state_elems, void* exp_avg, void* exp_avg_sq,
                       uint8_t* exp_avg_scale, uint8_t* exp_avg_sq_scale,
-                      float* master, uint32_t seed, float max_norm,
-                      void* scratch, float* norm);
+                      uint32_t seed, float max_norm, void* scratch,
+                      float* norm);
 /* The values that n elements (whole blocks of 32) of 8-bit moments stand
  * for, as bfloat16, which holds them exactly. */
 int dressi_adamw_values(dressi_ctx* ctx, uint64_t n, const void* exp_avg,

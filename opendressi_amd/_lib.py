@@ -45,7 +45,7 @@ class PbrDesc(C.Structure):
 
 
 class AdamwTensor(C.Structure):
-    _fields_ = [("param", _P), ("grad", _P), ("n", C.c_uint64), ("state", C.c_uint64),
+    _fields_ = [("param", _P), ("grad", _P), ("master", _P), ("n", C.c_uint64), ("state", C.c_uint64),
                 ("type", _U), ("set", _U)]
 
 
@@ -194,13 +194,14 @@ _SIGS = {
     "dressi_tex_buffer": (_I, [_P, _I, C.POINTER(_P), C.POINTER(_S)]),
     "dressi_tex_read": (_I, [_P, _I, _P, _S]),
     "dressi_tex_profile": (_I, [_P, _U, C.c_char_p, _S, _FP, _U, _UP]),
-    "dressi_group_norm_scratch": (_S, [_U, _U, C.c_uint64, _U, _U, _I]),
+    "dressi_group_norm_scratch": (_S, [_U, _U, C.c_uint64, _U, C.c_uint64, C.c_uint64, _U,
+                                       C.c_uint64, _I]),
     "dressi_group_norm": (_I, [_P, _P, _U, _U, C.c_uint64, _U, C.c_uint64, C.c_uint64, _U, _P, _P,
                                _U, _F, _U, _P, _S, _P, _P, _P]),
     "dressi_group_norm_bwd": (_I, [_P, _P, _P, _U, _U, C.c_uint64, _U, C.c_uint64, C.c_uint64, _U,
                                    _P, _P, _U, _U, _P, _P, _P, _S, _P, _P, _P]),
     "dressi_adamw_scratch": (_S, []),
-    "dressi_adamw_step": (_I, [_P, _P, _U, _P, _U, _U, C.c_uint64, _P, _P, _P, _P, _P, _U, _F, _P,
+    "dressi_adamw_step": (_I, [_P, _P, _U, _P, _U, _U, C.c_uint64, _P, _P, _P, _P, _U, _F, _P,
                                _P]),
     "dressi_adamw_values": (_I, [_P, C.c_uint64, _P, _P, _P, _P, _P, _P]),
 }

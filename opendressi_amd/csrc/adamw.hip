@@ -38,12 +38,13 @@ constexpr uint32_t kThreads = 256;
 constexpr uint32_t kLaneElems = 4;  // neighbours of a lane: 16 bytes of float
 constexpr uint32_t kBlock = 32;     // elements that share an exponent
 constexpr int kTop1 = 14, kTop2 = 30;
-constexpr uint32_t kMaxTensors = 72, kMaxSets = 16;
+constexpr uint32_t kMaxTensors = 64, kMaxSets = 16;
 constexpr uint32_t kMaxPartials = 1024;
 
 struct TensorArg {
     void* param;
     const void* grad;
+    float* master;         // of 16-bit parameters, or null
     uint64_t n;
     uint64_t state;        // element offset in the flat state buffers
     uint32_t first_chunk;  // of this launch
@@ -67,7 +68,6 @@ struct State {
     void* v;
     uint8_t* m_scale;
     uint8_t* v_scale;
-    float* master;
     const double* partials;  // of the squared norm; null: no clipping
     uint32_t n_partials;
     float max_norm;
@@ -77,14 +77,10 @@ struct State {
 // The tensor that holds `chunk`: the last whose first chunk is not past it.
 // A lane per tensor, one load deep.
 __device__ __forceinline__ uint32_t find_tensor(const Table& tb, uint32_t chunk) {
+    static_assert(kMaxTensors == 64, "a tensor a lane");
     const uint32_t lane = threadIdx.x & 63u;
-    uint32_t found = 0;
-    for (uint32_t b = 0; b < tb.n_tensors; b += 64) {
-        const uint32_t i = b + lane;
-        const bool at = i < tb.n_tensors && tb.t[i < kMaxTensors ? i : 0].first_chunk <= chunk;
-        found += (uint32_t)__popcll(__ballot(at));
-    }
-    return __builtin_amdgcn_readfirstlane(found - 1);
+    const bool at = lane < tb.n_tensors && tb.t[lane].first_chunk <= chunk;
+    return __builtin_amdgcn_readfirstlane((uint32_t)__popcll(__ballot(at)) - 1);
 }
 
 // ---------------------------------------------------------------------------
@@ -279,6 +275,14 @@ __device__ __forceinline__ void update(const SetArg& h, float coef, bool clip,
     }
 }
 
+// A parameter's value: its master's, unless it is no longer the master's
+// rounding. Then someone else has written it since the last step (a clamp, a
+// checkpoint) and it counts.
+template <typename T>
+__device__ __forceinline__ float newest(float param, float master) {
+    return to_float(from_float<T>(master)) == param ? master : param;
+}
+
 // A chunk of one tensor. FULL: all of its elements are there and aligned for
 // a lane's vector loads, which are all issued before the first is used.
 template <typename T, bool Q8, int ITER, bool FULL>
@@ -287,7 +291,7 @@ __device__ __forceinline__ void step_chunk(const TensorArg& t, const SetArg& h, 
     constexpr uint32_t kStep = kThreads * kLaneElems;
     T* p = (T*)t.param;
     const T* g = (const T*)t.grad;
-    const bool wide = !std::is_same<T, float>::value && st.master != nullptr;
+    const bool wide = !std::is_same<T, float>::value && t.master != nullptr;
     const uint64_t padded = (t.n + kBlock - 1) / kBlock * kBlock;
     float gx[ITER][kLaneElems], px[ITER][kLaneElems];
     Moments mo[ITER];
@@ -296,10 +300,14 @@ __device__ __forceinline__ void step_chunk(const TensorArg& t, const SetArg& h, 
         const uint64_t i = at + (uint64_t)k * kStep + threadIdx.x * kLaneElems;
         if (FULL) {
             load_vec<T, kLaneElems>(g + i, gx[k]);
+            load_vec<T, kLaneElems>(p + i, px[k]);
             if (wide) {
-                load_vec<float, kLaneElems>(st.master + t.state + i, px[k]);
-            } else {
-                load_vec<T, kLaneElems>(p + i, px[k]);
+                float ms[kLaneElems];
+                load_vec<float, kLaneElems>(t.master + i, ms);
+#pragma unroll
+                for (uint32_t j = 0; j < kLaneElems; j++) {
+                    px[k][j] = newest<T>(px[k][j], ms[j]);
+                }
             }
             mo[k] = load_moments<Q8>(st, t.state + i);
         } else {
@@ -307,7 +315,10 @@ __device__ __forceinline__ void step_chunk(const TensorArg& t, const SetArg& h, 
             for (uint32_t j = 0; j < kLaneElems; j++) {
                 const bool in = i + j < t.n;
                 gx[k][j] = in ? to_float(g[i + j]) : 0.f;
-                px[k][j] = !in ? 0.f : wide ? st.master[t.state + i + j] : to_float(p[i + j]);
+                px[k][j] = in ? to_float(p[i + j]) : 0.f;
+                if (in && wide) {
+                    px[k][j] = newest<T>(px[k][j], t.master[i + j]);
+                }
                 mo[k].m[j] = mo[k].v[j] = 0.f;
             }
             if (i < padded) {  // a share is padded with zeros to whole blocks
@@ -331,7 +342,7 @@ __device__ __forceinline__ void step_chunk(const TensorArg& t, const SetArg& h, 
         if (FULL) {
             store_vec<T, kLaneElems>(p + i, px[k]);
             if (wide) {
-                store_vec<float, kLaneElems>(st.master + t.state + i, px[k]);
+                store_vec<float, kLaneElems>(t.master + i, px[k]);
             }
         } else {
 #pragma unroll
@@ -339,7 +350,7 @@ __device__ __forceinline__ void step_chunk(const TensorArg& t, const SetArg& h, 
                 if (i + j < t.n) {
                     p[i + j] = from_float<T>(px[k][j]);
                     if (wide) {
-                        st.master[t.state + i + j] = px[k][j];
+                        t.master[i + j] = px[k][j];
                     }
                 }
             }
@@ -427,6 +438,8 @@ int check_tensors(const dressi_adamw_tensor* t, uint32_t n, uint32_t n_sets, uin
         const size_t size = t[i].type == DRESSI_F32 ? 4 : 2;
         DRESSI_REQUIRE(((uintptr_t)t[i].param | (uintptr_t)t[i].grad) % size == 0,
                        "adamw: tensor %u is not aligned to its type", i);
+        DRESSI_REQUIRE(((uintptr_t)t[i].master & 15) == 0,
+                       "adamw: tensor %u's master is not aligned", i);
         DRESSI_REQUIRE(t[i].n <= (1ull << 40), "adamw: tensor %u is too large", i);
         const uint64_t padded = (t[i].n + kBlock - 1) / kBlock * kBlock;
         DRESSI_REQUIRE(t[i].state <= state_elems && padded <= state_elems - t[i].state,
@@ -496,6 +509,7 @@ int for_batches(const dressi_adamw_tensor* t, uint32_t n, const dressi_adamw_set
             TensorArg& a = tb.t[tb.n_tensors++];
             a.param = (char*)t[i].param + done * size;
             a.grad = (const char*)t[i].grad + done * size;
+            a.master = t[i].master ? t[i].master + done : nullptr;
             a.n = take;
             a.state = t[i].state + done;
             a.first_chunk = tb.n_chunks;
@@ -520,8 +534,8 @@ size_t dressi_adamw_scratch(void) { return kMaxPartials * sizeof(double); }
 int dressi_adamw_step(dressi_ctx* ctx, const dressi_adamw_tensor* tensors, uint32_t n_tensors,
                       const dressi_adamw_set* sets, uint32_t n_sets, uint32_t state_bits,
                       uint64_t state_elems, void* exp_avg, void* exp_avg_sq,
-                      uint8_t* exp_avg_scale, uint8_t* exp_avg_sq_scale, float* master,
-                      uint32_t seed, float max_norm, void* scratch, float* norm) {
+                      uint8_t* exp_avg_scale, uint8_t* exp_avg_sq_scale, uint32_t seed,
+                      float max_norm, void* scratch, float* norm) {
     DRESSI_REQUIRE(ctx, "NULL context");
     if (n_tensors == 0) {
         return DRESSI_OK;
@@ -534,8 +548,7 @@ int dressi_adamw_step(dressi_ctx* ctx, const dressi_adamw_tensor* tensors, uint3
     DRESSI_REQUIRE(!q8 || (exp_avg_scale && exp_avg_sq_scale) || state_elems == 0,
                    "adamw: 8-bit moments need their scales");
     const uintptr_t mask = q8 ? 3 : 15;
-    DRESSI_REQUIRE((((uintptr_t)exp_avg | (uintptr_t)exp_avg_sq) & mask) == 0 &&
-                       ((uintptr_t)master & 15) == 0,
+    DRESSI_REQUIRE((((uintptr_t)exp_avg | (uintptr_t)exp_avg_sq) & mask) == 0,
                    "adamw: the state buffers are not aligned");
     DRESSI_REQUIRE(max_norm >= 0.f, "adamw: max_norm %g", (double)max_norm);
     const bool clip = max_norm > 0.f;
@@ -557,8 +570,7 @@ int dressi_adamw_step(dressi_ctx* ctx, const dressi_adamw_tensor* tensors, uint3
     }
     const bool small = total <= (q8 ? kSmallTotal8 : kSmallTotal);
     const uint32_t chunk = kThreads * kLaneElems * (small ? 1 : 4);
-    State st{exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, master, nullptr, 0,
-             max_norm, norm};
+    State st{exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, nullptr, 0, max_norm, norm};
     if (clip) {
         uint32_t launches = 0;
         for_batches(tensors, n_tensors, sets, seed, chunk, [&](const Table&) {
@@ -622,7 +634,7 @@ int dressi_adamw_values(dressi_ctx* ctx, uint64_t n, const void* exp_avg, const 
                        (((uintptr_t)exp_avg_bf16 | (uintptr_t)exp_avg_sq_bf16) & 7) == 0,
                    "adamw: the buffers are not aligned");
     State st{(void*)exp_avg, (void*)exp_avg_sq, (uint8_t*)exp_avg_scale,
-             (uint8_t*)exp_avg_sq_scale, nullptr, nullptr, 0, 0.f, nullptr};
+             (uint8_t*)exp_avg_sq_scale, nullptr, 0, 0.f, nullptr};
     // within the launch limit, in whole blocks
     constexpr uint64_t kPiece = kLaunchThreads * kLaneElems;
     for (uint64_t at = 0; at < n; at += kPiece) {

@@ -713,8 +713,8 @@ __global__ __launch_bounds__(kItemThreads) void k_gn_item(const T* x, const Cut 
                                                           float* rstd_out) {
     __shared__ float part[2][kItemThreads / 64][64];
     const ItemPlace at(c);
-    const uint32_t item = blockIdx.x;
     const uint32_t vec = c.first_vec(blockIdx.y) + at.vec, group = vec / c.unit_vecs;
+    const uint32_t item = blockIdx.x;
     const T* p = x + (size_t)item * c.item_stride + (size_t)at.row * c.px_stride + (size_t)vec * V;
     T* o = y + ((size_t)item * c.n_px + at.row) * c.n_ch + (size_t)vec * V;
     const size_t step = (size_t)c.rows * c.px_stride, ostep = (size_t)c.rows * c.n_ch;
@@ -836,9 +836,10 @@ struct Channels {
     }
 };
 
-// The first pass: per chunk the channels' (sum gz, sum gz xh), and the groups'
-// sums of both weighted.
-template <typename T, int V, int S>
+// The first pass: per chunk the groups' sums of w gz and w gz xh, and for all
+// chunks of a workgroup the channels' sums of gz and gz xh. MANY: it takes every
+// gridDim.x-th chunk of all items'; else it has one.
+template <typename T, int V, int S, bool MANY>
 __global__ __launch_bounds__(kMaxThreads) void k_gn_bwd_sums(const T* gy, const T* x, const Cut c,
                                                              const Affine aff, uint32_t act,
                                                              const float* mean, const float* rstd,
@@ -846,69 +847,82 @@ __global__ __launch_bounds__(kMaxThreads) void k_gn_bwd_sums(const T* gy, const 
                                                              float2* ch_part) {
     __shared__ float2 red[V][kMaxThreads];
     const Place at(c);
-    const uint32_t item = blockIdx.x / c.chunks, chunk = blockIdx.x - item * c.chunks;
     const uint32_t vec = c.first_vec(blockIdx.y) + at.vec;
-    float sa[V], sb[V];
+    const uint32_t groups = c.groups(blockIdx.y), group0 = c.first_group(blockIdx.y);
+    const size_t step = (size_t)c.rows * c.px_stride, qstep = (size_t)c.rows * c.n_ch;
+    float a[V], b[V], sa[V], sb[V];
 #pragma unroll
     for (int j = 0; j < V; j++) {
         sa[j] = sb[j] = 0.f;
     }
-    Channels<V, S> ch;
-    uint32_t left = at.pixels(c, chunk);
-    if (at.live) {
-        ch.load(c, aff, item, vec, mean, rstd);
-    }
-    if (left > 0) {
-        const size_t px0 = (size_t)chunk * c.chunk_px + at.row;
-        const T* p = x + (size_t)item * c.item_stride + px0 * c.px_stride + (size_t)vec * V;
-        const T* q = gy + ((size_t)item * c.n_px + px0) * c.n_ch + (size_t)vec * V;
-        const size_t step = (size_t)c.rows * c.px_stride, qstep = (size_t)c.rows * c.n_ch;
-        uint32_t count = left % kBatchBwd ? left % kBatchBwd : kBatchBwd;
-        while (left > 0) {
-            Pack<T, V> xv[kBatchBwd], gv[kBatchBwd];
-            load_batch<T, V, kBatchBwd>(p, step, count, xv);
-            load_batch<T, V, kBatchBwd>(q, qstep, count, gv);
+    for (uint32_t unit = blockIdx.x; unit < c.n_items * c.chunks; unit += gridDim.x) {
+        const uint32_t item = unit / c.chunks, chunk = unit - item * c.chunks;
 #pragma unroll
-            for (uint32_t k = 0; k < kBatchBwd; k++) {
-                if (k < count) {
-                    ch.add(xv[k], gv[k], act, sa, sb);
+        for (int j = 0; j < V; j++) {
+            a[j] = b[j] = 0.f;
+        }
+        Channels<V, S> ch;
+        uint32_t left = at.pixels(c, chunk);
+        if (left > 0) {
+            ch.load(c, aff, item, vec, mean, rstd);
+            const size_t px0 = (size_t)chunk * c.chunk_px + at.row;
+            const T* p = x + (size_t)item * c.item_stride + px0 * c.px_stride + (size_t)vec * V;
+            const T* q = gy + ((size_t)item * c.n_px + px0) * c.n_ch + (size_t)vec * V;
+            uint32_t count = left % kBatchBwd ? left % kBatchBwd : kBatchBwd;
+            while (left > 0) {
+                Pack<T, V> xv[kBatchBwd], gv[kBatchBwd];
+                load_batch<T, V, kBatchBwd>(p, step, count, xv);
+                load_batch<T, V, kBatchBwd>(q, qstep, count, gv);
+#pragma unroll
+                for (uint32_t k = 0; k < kBatchBwd; k++) {
+                    if (k < count) {
+                        ch.add(xv[k], gv[k], act, a, b);
+                    }
                 }
+                left -= count;
+                p += count * step;
+                q += count * qstep;
+                count = kBatchBwd;
             }
-            left -= count;
-            p += count * step;
-            q += count * qstep;
-            count = kBatchBwd;
+        }
+        if (at.live) {
+#pragma unroll
+            for (int g = 0; g < S; g++) {
+                float2 s = make_float2(0.f, 0.f);
+                if (at.pixels(c, chunk) > 0) {
+#pragma unroll
+                    for (int j = g * (V / S); j < (g + 1) * (V / S); j++) {
+                        s.x = fmaf(ch.w[j], a[j], s.x);
+                        s.y = fmaf(ch.w[j], b[j], s.y);
+                    }
+                }
+                red[g][threadIdx.x] = s;
+            }
+        }
+#pragma unroll
+        for (int j = 0; MANY && j < V; j++) {
+            sa[j] += a[j];
+            sb[j] += b[j];
+        }
+        __syncthreads();
+        add_all<S, kMaxThreads>(red, c.rows, at.nv, at.nv * S / groups, groups,
+                                [&](uint32_t k, float2 s) {
+            const uint32_t slot = c.parts == 1 ? group0 + k : blockIdx.y;
+            group_part[((size_t)item * c.n_groups * c.parts + slot) * c.chunks + chunk] = s;
+        });
+        __syncthreads();
+        if (!MANY) {
+            break;
         }
     }
 #pragma unroll
     for (int j = 0; j < V; j++) {
-        red[j][threadIdx.x] = make_float2(sa[j], sb[j]);
+        red[j][threadIdx.x] = MANY ? make_float2(sa[j], sb[j]) : make_float2(a[j], b[j]);
     }
     __syncthreads();
-    float2* o = ch_part + ((size_t)item * c.chunks + chunk) * c.n_ch +
-                (size_t)c.first_vec(blockIdx.y) * V;
+    float2* o = ch_part + (size_t)blockIdx.x * c.n_ch + (size_t)c.first_vec(blockIdx.y) * V;
     add_all<V, kMaxThreads>(red, c.rows, at.nv, 1, at.nv * V,
                             [&](uint32_t k, float2 s) { o[k] = s; });
-    __syncthreads();
-    if (at.live) {
-#pragma unroll
-        for (int g = 0; g < S; g++) {
-            float2 s = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int j = g * (V / S); j < (g + 1) * (V / S); j++) {
-                s.x = fmaf(ch.w[j], sa[j], s.x);
-                s.y = fmaf(ch.w[j], sb[j], s.y);
-            }
-            red[g][threadIdx.x] = s;
-        }
-    }
-    __syncthreads();
-    const uint32_t groups = c.groups(blockIdx.y), group0 = c.first_group(blockIdx.y);
-    add_all<S, kMaxThreads>(red, c.rows, at.nv, at.nv * S / groups, groups,
-                            [&](uint32_t k, float2 s) {
-        const uint32_t slot = c.parts == 1 ? group0 + k : blockIdx.y;
-        group_part[((size_t)item * c.n_groups * c.parts + slot) * c.chunks + chunk] = s;
-    });
 }
 
 // gw and gb of kParamCh channels: the chunks' sums over all items in a fixed
@@ -1045,86 +1059,94 @@ __global__ __launch_bounds__(kMaxThreads) void k_gn_bwd_apply(const T* gy, const
     }
 }
 
-// Both passes where a block's pixels fit its workgroup's registers. ch_part
-// (null for one item: gw and gb are whole then) gets the item's channel sums.
+// Both passes where a block's pixels fit its workgroup's registers. A workgroup
+// takes every gridDim.x-th item; ch_part (null for one workgroup a block: gw
+// and gb are whole then) gets its items' channel sums.
 template <typename T, int V>
 __global__ __launch_bounds__(kItemThreads) void k_gn_bwd_item(
         const T* gy, const T* x, const Cut c, const Affine aff, uint32_t act, const float* mean,
         const float* rstd, float2* ch_part, T* gx, void* gw, void* gb) {
-    constexpr uint32_t kWaves = kItemThreads / 64;
-    __shared__ float2 part[kWaves][64];
+    __shared__ float2 part[2][kItemThreads / 64][64];
     __shared__ float2 red[V][kItemThreads];
     const ItemPlace at(c);
-    const uint32_t item = blockIdx.x;
     const uint32_t vec = c.first_vec(blockIdx.y) + at.vec;
-    const T* p = x + (size_t)item * c.item_stride + (size_t)at.row * c.px_stride + (size_t)vec * V;
-    const size_t at_out = ((size_t)item * c.n_px + at.row) * c.n_ch + (size_t)vec * V;
-    const T* q = gy + at_out;
-    T* o = gx + at_out;
     const size_t step = (size_t)c.rows * c.px_stride, qstep = (size_t)c.rows * c.n_ch;
-    Pack<T, V> xv[kHoldBwd], gv[kHoldBwd];
-#pragma unroll
-    for (uint32_t k = 0; k < kHoldBwd; k++) {
-        if (k < at.mine) {
-            xv[k] = load_pack<T, V>(p + k * step);
-            gv[k] = load_pack<T, V>(q + k * qstep);
-        }
-    }
+    const float inv = 1.f / ((float)c.n_px * (float)c.group_ch);
     float sa[V], sb[V];
 #pragma unroll
     for (int j = 0; j < V; j++) {
         sa[j] = sb[j] = 0.f;
     }
     Channels<V, 1> ch;
-    float2 g = make_float2(0.f, 0.f);
-    if (at.mine > 0) {
-        ch.load(c, aff, item, vec, mean, rstd);
+    uint32_t turn = 0;
+    for (uint32_t item = blockIdx.x; item < c.n_items; item += gridDim.x, turn ^= 1) {
+        const T* p = x + (size_t)item * c.item_stride + (size_t)at.row * c.px_stride +
+                     (size_t)vec * V;
+        const size_t at_out = ((size_t)item * c.n_px + at.row) * c.n_ch + (size_t)vec * V;
+        const T* q = gy + at_out;
+        Pack<T, V> xv[kHoldBwd], gv[kHoldBwd];
 #pragma unroll
         for (uint32_t k = 0; k < kHoldBwd; k++) {
             if (k < at.mine) {
-                ch.add(xv[k], gv[k], act, sa, sb);
+                xv[k] = load_pack<T, V>(p + k * step);
+                gv[k] = load_pack<T, V>(q + k * qstep);
             }
         }
+        float2 g = make_float2(0.f, 0.f);
+        if (at.mine > 0) {
+            float a[V], b[V];
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-            g.x = fmaf(ch.w[j], sa[j], g.x);
-            g.y = fmaf(ch.w[j], sb[j], g.y);
-        }
-    }
-    if (ch_part || gw || gb) {
+            for (int j = 0; j < V; j++) {
+                a[j] = b[j] = 0.f;
+            }
+            ch.load(c, aff, item, vec, mean, rstd);
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-            red[j][threadIdx.x] = make_float2(sa[j], sb[j]);
+            for (uint32_t k = 0; k < kHoldBwd; k++) {
+                if (k < at.mine) {
+                    ch.add(xv[k], gv[k], act, a, b);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                g.x = fmaf(ch.w[j], a[j], g.x);
+                g.y = fmaf(ch.w[j], b[j], g.y);
+                sa[j] += a[j];
+                sb[j] += b[j];
+            }
+        }
+        g = add_item(c, at, g, part[turn]);
+        if (at.mine > 0 && gx) {
+            const float2 m[1] = {make_float2(g.x * inv, g.y * inv)};
+#pragma unroll
+            for (uint32_t k = 0; k < kHoldBwd; k++) {
+                if (k < at.mine) {
+                    ch.finish(xv[k], gv[k], act, m, gx + at_out + k * qstep, c.stream);
+                }
+            }
         }
     }
-    g = add_item(c, at, g, part);  // its barrier is red's too
-    if (ch_part || gw || gb) {
-        const uint32_t ch0 = c.first_vec(blockIdx.y) * V;
-        add_all<V, kItemThreads>(red, c.rows, c.lanes, 1, c.vecs(blockIdx.y) * V,
-                                 [&](uint32_t k, float2 s) {
-            if (ch_part) {
-                ch_part[(size_t)item * c.n_ch + ch0 + k] = s;
-                return;
-            }
-            if (gb) {
-                store_as(gb, aff.type, ch0 + k, s.x);
-            }
-            if (gw) {
-                store_as(gw, aff.type, ch0 + k, s.y);
-            }
-        });
-    }
-    if (at.mine == 0 || !gx) {
+    if (!ch_part && !gw && !gb) {
         return;
     }
-    const float inv = 1.f / ((float)c.n_px * (float)c.group_ch);
-    const float2 m[1] = {make_float2(g.x * inv, g.y * inv)};
 #pragma unroll
-    for (uint32_t k = 0; k < kHoldBwd; k++) {
-        if (k < at.mine) {
-            ch.finish(xv[k], gv[k], act, m, o + k * qstep, c.stream);
-        }
+    for (int j = 0; j < V; j++) {
+        red[j][threadIdx.x] = make_float2(sa[j], sb[j]);
     }
+    __syncthreads();
+    const uint32_t ch0 = c.first_vec(blockIdx.y) * V;
+    add_all<V, kItemThreads>(red, c.rows, c.lanes, 1, c.vecs(blockIdx.y) * V,
+                             [&](uint32_t k, float2 s) {
+        if (ch_part) {
+            ch_part[(size_t)blockIdx.x * c.n_ch + ch0 + k] = s;
+            return;
+        }
+        if (gb) {
+            store_as(gb, aff.type, ch0 + k, s.x);
+        }
+        if (gw) {
+            store_as(gw, aff.type, ch0 + k, s.y);
+        }
+    });
 }
 
 // ---------------------------------------------------------------------------
@@ -1132,35 +1154,72 @@ __global__ __launch_bounds__(kItemThreads) void k_gn_bwd_item(
 // ---------------------------------------------------------------------------
 
 // How wide a thread's vectors are: 16 bytes at most, as the channels, the
-// strides and the pointers allow. `whole`: a vector that no group's edge cuts.
+// strides and the images' addresses (or-ed) allow. `whole`: a vector that no group's edge cuts.
 struct Width {
     uint32_t any, whole;
 };
 Width vec_width(uint32_t type, uint32_t n_ch, uint32_t n_groups, uint64_t item_stride,
-                uint64_t px_stride, std::initializer_list<const void*> ptrs) {
+                uint64_t px_stride, uint64_t addresses) {
     const uint32_t size = (uint32_t)type_bytes(type);
     const auto low_bit = [](uint64_t x) { return (uint32_t)(x & (~x + 1)); };
-    uint32_t v = low_bit((uint64_t)n_ch | item_stride | px_stride | (16u / size));
-    for (const void* p : ptrs) {
-        while (v > 1 && (uintptr_t)p % ((size_t)v * size) != 0) {
-            v >>= 1;
-        }
-    }
+    const uint32_t v =
+        low_bit((uint64_t)n_ch | item_stride | px_stride | addresses / size | (16u / size));
     const uint32_t group_ch = n_ch / n_groups, whole = std::min(v, low_bit(group_ch));
     // a unit of several groups has to fit a workgroup
     const uint32_t unit = v / whole;
     return {unit > 1 && group_ch * unit / v > kMaxVecs ? whole : v, whole};
 }
 
+// Workgroups of a block whose channel sums are added afterwards: few, where
+// the units (chunks, or items in one pass) are many.
+uint32_t sum_rows(uint64_t units, const Cut& c) {
+    const uint64_t most = std::max(1u, 2048 / c.n_blocks);
+    const uint64_t each = (units + most - 1) / most;
+    return (uint32_t)((units + each - 1) / each);
+}
+
+// Bytes of the chunks' and of the channels' sums.
 struct Scratch {
     size_t group_part, ch_part, bytes;
 };
-Scratch scratch_of(const Cut& c, bool backward) {
+Scratch scratch_of(const Cut& c, bool whole, bool backward) {
     Scratch s;
-    s.group_part = sizeof(float2) * (size_t)c.n_items * c.n_groups * c.parts * c.chunks;
-    s.ch_part = backward ? sizeof(float2) * (size_t)c.n_items * c.chunks * c.n_ch : 0;
+    s.group_part =
+        whole ? 0 : sizeof(float2) * (size_t)c.n_items * c.n_groups * c.parts * c.chunks;
+    s.ch_part = backward ? sizeof(float2) * sum_rows((uint64_t)c.n_items * c.chunks, c) * c.n_ch : 0;
     s.bytes = s.group_part + s.ch_part;
     return s;
+}
+
+// Bytes of an image from which results go past the caches. Forward with them and
+// without takes 73 and 87 us for 1024 x 1024 x 64 bfloat16, 25.3 and 26.1 for
+// 512 x 512 x 64; with a pass after it that reads the result 125 and 127, 37 and 37.
+constexpr uint64_t kStreamBytes = 32ull << 20;
+
+// How a call is cut: in one pass if it can be.
+struct Plan {
+    Cut c;
+    uint32_t v;
+    bool whole, split;
+};
+Plan make_plan(uint32_t type, uint32_t n_items, uint64_t n_px, uint32_t n_ch, uint64_t item_stride,
+               uint64_t px_stride, uint32_t n_groups, uint64_t addresses, uint32_t hold) {
+    const Width w = vec_width(type, n_ch, n_groups, n_items > 1 ? item_stride : 0,
+                              n_px > 1 ? px_stride : 0, addresses);
+    Plan p;
+    p.v = w.whole;
+    p.split = false;
+    p.c = make_item_cut(n_items, n_px, n_ch, n_groups, w.whole, hold);
+    p.whole = p.c.chunks != 0;
+    if (!p.whole) {
+        p.v = w.any;
+        p.split = w.any != w.whole;
+        p.c = make_cut(n_items, n_px, n_ch, n_groups, w.any);
+    }
+    p.c.item_stride = item_stride;
+    p.c.px_stride = px_stride;
+    p.c.stream = (uint64_t)n_items * n_px * n_ch * type_bytes(type) >= kStreamBytes;
+    return p;
 }
 
 int check_shape(const char* what, uint32_t type, uint32_t n_items, uint64_t n_px, uint32_t n_ch,
@@ -1172,7 +1231,7 @@ int check_shape(const char* what, uint32_t type, uint32_t n_items, uint64_t n_px
     DRESSI_REQUIRE(n_groups > 0 && n_ch % n_groups == 0 && n_ch > 0,
                    "%s: %u channels are not %u whole groups", what, n_ch, n_groups);
     DRESSI_REQUIRE(n_px <= (1ull << 40), "%s: too many pixels", what);
-    DRESSI_REQUIRE(n_items <= (1u << 20), "%s: too many items", what);
+    DRESSI_REQUIRE(n_items <= (1u << 31), "%s: too many items", what);
     return DRESSI_OK;
 }
 
@@ -1198,22 +1257,36 @@ int for_width(uint32_t type, uint32_t v, F&& f) {
 template <typename T, int V>
 int launch_item(hipStream_t s, const Cut& c, const void* x, const Affine& aff, float eps,
                 uint32_t act, void* y, float* mean, float* rstd) {
-    hipLaunchKernelGGL((k_gn_item<T, V>), dim3(c.n_items, c.n_blocks), dim3(c.threads), 0, s,
-                       (const T*)x, c, aff, eps, act, (T*)y, mean, rstd);
-    DRESSI_CHECK_LAUNCH();
+    const uint32_t most = (uint32_t)(kLaunchThreads / kItemThreads);  // items of a launch
+    for (uint32_t i = 0; i < c.n_items; i += most) {
+        hipLaunchKernelGGL((k_gn_item<T, V>), dim3(std::min(most, c.n_items - i), c.n_blocks),
+                           dim3(c.threads), 0, s, (const T*)x + (size_t)i * c.item_stride, c, aff,
+                           eps, act, (T*)y + (size_t)i * c.n_px * c.n_ch,
+                           mean + (size_t)i * c.n_groups, rstd + (size_t)i * c.n_groups);
+        DRESSI_CHECK_LAUNCH();
+    }
     return DRESSI_OK;
+}
+
+// Items of a launch whose workgroups each take a chunk of one.
+uint32_t items_at_once(const Cut& c) {
+    return (uint32_t)std::max<uint64_t>(1, kLaunchThreads / kMaxThreads / c.chunks);
 }
 
 template <typename T, int V, int S>
 int launch_forward(hipStream_t s, const Cut& c, const void* x, const Affine& aff, float eps,
                    uint32_t act, void* scratch, void* y, float* mean, float* rstd) {
-    const dim3 grid(c.n_items * c.chunks, c.n_blocks), block(c.threads);
-    hipLaunchKernelGGL((k_gn_stats<T, V, S>), grid, block, 0, s, (const T*)x, c,
-                       (float2*)scratch);
-    DRESSI_CHECK_LAUNCH();
-    hipLaunchKernelGGL((k_gn_apply<T, V, S>), grid, block, 0, s, (const T*)x, c,
-                       (const float2*)scratch, aff, eps, act, (T*)y, mean, rstd);
-    DRESSI_CHECK_LAUNCH();
+    const uint32_t most = items_at_once(c);
+    for (uint32_t i = 0; i < c.n_items; i += most) {
+        const dim3 grid(std::min(most, c.n_items - i) * c.chunks, c.n_blocks), block(c.threads);
+        const T* xi = (const T*)x + (size_t)i * c.item_stride;
+        hipLaunchKernelGGL((k_gn_stats<T, V, S>), grid, block, 0, s, xi, c, (float2*)scratch);
+        DRESSI_CHECK_LAUNCH();
+        hipLaunchKernelGGL((k_gn_apply<T, V, S>), grid, block, 0, s, xi, c, (const float2*)scratch,
+                           aff, eps, act, (T*)y + (size_t)i * c.n_px * c.n_ch,
+                           mean + (size_t)i * c.n_groups, rstd + (size_t)i * c.n_groups);
+        DRESSI_CHECK_LAUNCH();
+    }
     return DRESSI_OK;
 }
 
@@ -1227,13 +1300,14 @@ template <typename T, int V>
 int launch_bwd_item(hipStream_t s, const Cut& c, const void* gy, const void* x, const Affine& aff,
                     uint32_t act, const float* mean, const float* rstd, void* scratch, void* gx,
                     void* gw, void* gb) {
-    const bool sums = c.n_items > 1 && (gw || gb);  // the items' are added afterwards
-    hipLaunchKernelGGL((k_gn_bwd_item<T, V>), dim3(c.n_items, c.n_blocks), dim3(c.threads), 0, s,
+    const uint32_t rows = sum_rows(c.n_items, c);
+    const bool sums = rows > 1 && (gw || gb);  // the workgroups' are added afterwards
+    hipLaunchKernelGGL((k_gn_bwd_item<T, V>), dim3(rows, c.n_blocks), dim3(c.threads), 0, s,
                        (const T*)gy, (const T*)x, c, aff, act, mean, rstd,
                        sums ? (float2*)scratch : nullptr, (T*)gx, gw, gb);
     DRESSI_CHECK_LAUNCH();
-    return sums ? launch_param_grad(s, ParamGrad{(const float2*)scratch, c.n_items, c.n_ch,
-                                                 aff.type, gw, gb})
+    return sums ? launch_param_grad(s, ParamGrad{(const float2*)scratch, rows, c.n_ch, aff.type,
+                                                 gw, gb})
                 : DRESSI_OK;
 }
 
@@ -1241,26 +1315,33 @@ template <typename T, int V, int S>
 int launch_backward(hipStream_t s, const Cut& c, const void* gy, const void* x, const Affine& aff,
                     uint32_t act, const float* mean, const float* rstd, void* scratch, void* gx,
                     void* gw, void* gb) {
-    const dim3 grid(c.n_items * c.chunks, c.n_blocks), block(c.threads);
+    const uint32_t rows = sum_rows((uint64_t)c.n_items * c.chunks, c);
+    const dim3 block(c.threads);
     float2* group_part = (float2*)scratch;
-    float2* ch_part = (float2*)((char*)scratch + scratch_of(c, true).group_part);
-    const ParamGrad params{ch_part, (size_t)c.n_items * c.chunks, c.n_ch, aff.type, gw, gb};
-    hipLaunchKernelGGL((k_gn_bwd_sums<T, V, S>), grid, block, 0, s, (const T*)gy, (const T*)x, c,
+    float2* ch_part = (float2*)((char*)scratch + scratch_of(c, false, true).group_part);
+    const ParamGrad params{ch_part, rows, c.n_ch, aff.type, gw, gb};
+    const auto sums = rows < (uint64_t)c.n_items * c.chunks ? k_gn_bwd_sums<T, V, S, true>
+                                                            : k_gn_bwd_sums<T, V, S, false>;
+    hipLaunchKernelGGL(sums, dim3(rows, c.n_blocks), block, 0, s, (const T*)gy, (const T*)x, c,
                        aff, act, mean, rstd, group_part, ch_part);
     DRESSI_CHECK_LAUNCH();
     if (!gx) {
         return gw || gb ? launch_param_grad(s, params) : DRESSI_OK;
     }
-    const uint32_t extra = gw || gb ? div_up(c.n_ch, kParamCh) : 0;
-    hipLaunchKernelGGL((k_gn_bwd_apply<T, V, S>), dim3(grid.x + extra, grid.y), block, 0, s,
-                       (const T*)gy, (const T*)x, c, aff, act, mean, rstd, group_part, (T*)gx,
-                       params, extra);
-    DRESSI_CHECK_LAUNCH();
+    const uint32_t most = items_at_once(c);
+    for (uint32_t i = 0; i < c.n_items; i += most) {
+        const uint32_t items = std::min(most, c.n_items - i);
+        const uint32_t extra = i + items == c.n_items && (gw || gb) ? div_up(c.n_ch, kParamCh) : 0;
+        const size_t at = (size_t)i * c.n_px * c.n_ch, g = (size_t)i * c.n_groups;
+        hipLaunchKernelGGL((k_gn_bwd_apply<T, V, S>), dim3(items * c.chunks + extra, c.n_blocks),
+                           block, 0, s, (const T*)gy + at,
+                           (const T*)x + (size_t)i * c.item_stride, c, aff, act, mean + g,
+                           rstd + g, group_part + g * c.parts * c.chunks, (T*)gx + at, params,
+                           extra);
+        DRESSI_CHECK_LAUNCH();
+    }
     return DRESSI_OK;
 }
-
-// Bytes of an image from which results go past the caches.
-constexpr uint64_t kStreamBytes = 32ull << 20;
 
 }  // namespace
 }  // namespace dressi
@@ -1270,18 +1351,15 @@ using namespace dressi;
 extern "C" {
 
 size_t dressi_group_norm_scratch(uint32_t type, uint32_t n_items, uint64_t n_px, uint32_t n_ch,
-                                 uint32_t n_groups, int backward) {
+                                 uint64_t item_stride, uint64_t px_stride, uint32_t n_groups,
+                                 uint64_t addresses, int backward) {
     if (type > DRESSI_F16 || n_items == 0 || n_px == 0 || n_ch == 0 || n_groups == 0 ||
         n_ch % n_groups != 0) {
         return 0;
     }
-    // whatever vectors the pointers allow, and either way of cutting
-    size_t most = 0;
-    for (uint32_t v = 1; v <= 16u / type_bytes(type) && n_ch % v == 0; v *= 2) {
-        most = std::max(most,
-                        scratch_of(make_cut(n_items, n_px, n_ch, n_groups, v), backward != 0).bytes);
-    }
-    return most;
+    const Plan p = make_plan(type, n_items, n_px, n_ch, item_stride, px_stride, n_groups,
+                             addresses, backward ? kHoldBwd : kHold);
+    return scratch_of(p.c, p.whole, backward != 0).bytes;
 }
 
 int dressi_group_norm(dressi_ctx* ctx, const void* x, uint32_t type, uint32_t n_items,
@@ -1294,38 +1372,27 @@ int dressi_group_norm(dressi_ctx* ctx, const void* x, uint32_t type, uint32_t n_
     if (int rc = check_shape("group_norm", type, n_items, n_px, n_ch, n_groups, activation, aff)) {
         return rc;
     }
+    DRESSI_REQUIRE(eps >= 0.f && std::isfinite(eps), "group_norm: eps %g", (double)eps);
     if (n_items == 0 || n_px == 0) {
         return DRESSI_OK;
     }
-    DRESSI_REQUIRE(x && y && mean && rstd && scratch, "group_norm: bad arguments");
+    DRESSI_REQUIRE(x && y && mean && rstd, "group_norm: bad arguments");
     DRESSI_REQUIRE(px_stride >= n_ch || n_px == 1, "group_norm: pixels overlap");
-    const Width v = vec_width(type, n_ch, n_groups, n_items > 1 ? item_stride : 0,
-                              n_px > 1 ? px_stride : 0, {x, y});
-    const auto place = [&](Cut& c) {
-        c.item_stride = item_stride;
-        c.px_stride = px_stride;
-        c.stream = (uint64_t)n_items * n_px * n_ch * type_bytes(type) >= kStreamBytes;
-    };
-    Cut c = make_item_cut(n_items, n_px, n_ch, n_groups, v.whole, kHold);
-    if (c.chunks) {
-        place(c);
-        return for_width(type, v.whole, [&](auto w) {
-            using T = std::remove_reference_t<decltype(w.v[0])>;
-            return launch_item<T, sizeof(w) / sizeof(T)>(ctx->stream, c, x, aff, eps, activation, y,
-                                                         mean, rstd);
-        });
-    }
-    c = make_cut(n_items, n_px, n_ch, n_groups, v.any);
-    place(c);
-    DRESSI_REQUIRE(scratch_bytes >= scratch_of(c, false).bytes, "group_norm: scratch too small");
-    return for_width(type, v.any, [&](auto w) {
+    const uint64_t addresses = (uintptr_t)x | (uintptr_t)y;
+    DRESSI_REQUIRE(addresses % type_bytes(type) == 0, "group_norm: not aligned to its type");
+    const Plan p = make_plan(type, n_items, n_px, n_ch, item_stride, px_stride, n_groups,
+                             addresses, kHold);
+    const size_t need = scratch_of(p.c, p.whole, false).bytes;
+    DRESSI_REQUIRE(need == 0 || (scratch && scratch_bytes >= need), "group_norm: scratch too small");
+    return for_width(type, p.v, [&](auto w) {
         using T = std::remove_reference_t<decltype(w.v[0])>;
         constexpr int V = sizeof(w) / sizeof(T);
-        return v.any == v.whole
-                   ? launch_forward<T, V, 1>(ctx->stream, c, x, aff, eps, activation, scratch, y,
-                                             mean, rstd)
-                   : launch_forward<T, V, V>(ctx->stream, c, x, aff, eps, activation, scratch, y,
-                                             mean, rstd);
+        hipStream_t s = ctx->stream;
+        return p.whole ? launch_item<T, V>(s, p.c, x, aff, eps, activation, y, mean, rstd)
+               : p.split
+                   ? launch_forward<T, V, V>(s, p.c, x, aff, eps, activation, scratch, y, mean, rstd)
+                   : launch_forward<T, V, 1>(s, p.c, x, aff, eps, activation, scratch, y, mean,
+                                             rstd);
     });
 }
 
@@ -1341,45 +1408,33 @@ int dressi_group_norm_bwd(dressi_ctx* ctx, const void* gy, const void* x, uint32
                              aff)) {
         return rc;
     }
-    if (n_items == 0 || n_px == 0) {
-        // sums of nothing
-        if (gw || gb) {
-            return launch_param_grad(ctx->stream, ParamGrad{nullptr, 0, n_ch, affine_type, gw, gb});
-        }
+    if (!gx && !gw && !gb) {
         return DRESSI_OK;
     }
-    DRESSI_REQUIRE(gy && x && mean && rstd && scratch, "group_norm_bwd: bad arguments");
-    DRESSI_REQUIRE(px_stride >= n_ch || n_px == 1, "group_norm_bwd: pixels overlap");
-    const Width v = vec_width(type, n_ch, n_groups, n_items > 1 ? item_stride : 0,
-                              n_px > 1 ? px_stride : 0, {gy, x, gx});
-    const auto place = [&](Cut& c) {
-        c.item_stride = item_stride;
-        c.px_stride = px_stride;
-        c.stream = (uint64_t)n_items * n_px * n_ch * type_bytes(type) >= kStreamBytes;
-    };
-    Cut c = make_item_cut(n_items, n_px, n_ch, n_groups, v.whole, kHoldBwd);
-    if (c.chunks) {
-        place(c);
-        DRESSI_REQUIRE(scratch_bytes >= scratch_of(c, true).ch_part,
-                       "group_norm_bwd: scratch too small");
-        return for_width(type, v.whole, [&](auto w) {
-            using T = std::remove_reference_t<decltype(w.v[0])>;
-            return launch_bwd_item<T, sizeof(w) / sizeof(T)>(ctx->stream, c, gy, x, aff,
-                                                             activation, mean, rstd, scratch, gx,
-                                                             gw, gb);
-        });
+    if (n_items == 0 || n_px == 0) {
+        // sums of nothing
+        return gw || gb ? launch_param_grad(ctx->stream,
+                                            ParamGrad{nullptr, 0, n_ch, affine_type, gw, gb})
+                        : DRESSI_OK;
     }
-    c = make_cut(n_items, n_px, n_ch, n_groups, v.any);
-    place(c);
-    DRESSI_REQUIRE(scratch_bytes >= scratch_of(c, true).bytes, "group_norm_bwd: scratch too small");
-    return for_width(type, v.any, [&](auto w) {
+    DRESSI_REQUIRE(gy && x && mean && rstd, "group_norm_bwd: bad arguments");
+    DRESSI_REQUIRE(px_stride >= n_ch || n_px == 1, "group_norm_bwd: pixels overlap");
+    const uint64_t addresses = (uintptr_t)gy | (uintptr_t)x | (uintptr_t)gx;
+    DRESSI_REQUIRE(addresses % type_bytes(type) == 0, "group_norm_bwd: not aligned to its type");
+    const Plan p = make_plan(type, n_items, n_px, n_ch, item_stride, px_stride, n_groups,
+                             addresses, kHoldBwd);
+    DRESSI_REQUIRE(scratch && scratch_bytes >= scratch_of(p.c, p.whole, true).bytes,
+                   "group_norm_bwd: scratch too small");
+    return for_width(type, p.v, [&](auto w) {
         using T = std::remove_reference_t<decltype(w.v[0])>;
         constexpr int V = sizeof(w) / sizeof(T);
-        return v.any == v.whole
-                   ? launch_backward<T, V, 1>(ctx->stream, c, gy, x, aff, activation, mean, rstd,
-                                              scratch, gx, gw, gb)
-                   : launch_backward<T, V, V>(ctx->stream, c, gy, x, aff, activation, mean, rstd,
-                                              scratch, gx, gw, gb);
+        hipStream_t s = ctx->stream;
+        return p.whole ? launch_bwd_item<T, V>(s, p.c, gy, x, aff, activation, mean, rstd, scratch,
+                                               gx, gw, gb)
+               : p.split ? launch_backward<T, V, V>(s, p.c, gy, x, aff, activation, mean, rstd,
+                                                    scratch, gx, gw, gb)
+                         : launch_backward<T, V, 1>(s, p.c, gy, x, aff, activation, mean, rstd,
+                                                    scratch, gx, gw, gb);
     });
 }
 

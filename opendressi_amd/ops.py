@@ -819,7 +819,8 @@ def group_norm(ctx: Context, x: torch.Tensor, groups: int, weight: torch.Tensor 
         x = x.contiguous()
         at = _pixel_strides(x)
     n_px, item, px = at
-    size = lib.dressi_group_norm_scratch(code, n, n_px, c, groups, 0)
+    size = lib.dressi_group_norm_scratch(code, n, n_px, c, item, px, groups,
+                                         x.data_ptr() | y.data_ptr(), 0)
     scratch = torch.empty(size, dtype=torch.uint8, device=x.device)
     _prep(ctx)
     check(lib.dressi_group_norm(ctx.handle, x.data_ptr(), code, n, n_px, c, item, px, groups,
@@ -857,7 +858,8 @@ def group_norm_bwd(ctx: Context, gy: torch.Tensor, x: torch.Tensor, mean: torch.
         at = _pixel_strides(x)
     gy = gy.contiguous()
     n_px, item, px = at if x.numel() else (0, 0, c)
-    size = lib.dressi_group_norm_scratch(code, n, n_px, c, groups, 1)
+    size = lib.dressi_group_norm_scratch(code, n, n_px, c, item, px, groups,
+                                         gy.data_ptr() | x.data_ptr() | (_addr(gx) or 0), 1)
     scratch = torch.empty(size, dtype=torch.uint8, device=x.device)
     _prep(ctx)
     check(lib.dressi_group_norm_bwd(ctx.handle, gy.data_ptr(), x.data_ptr(), code, n, n_px, c,

@@ -16,8 +16,8 @@ from ..ops import TYPE_CODES, _addr
 from .context import RasterizeHipContext
 
 # an entry of the table of parameters (dressi_adamw_tensor)
-_ENTRY = np.dtype([("param", "<u8"), ("grad", "<u8"), ("n", "<u8"), ("state", "<u8"),
-                   ("type", "<u4"), ("set", "<u4")])
+_ENTRY = np.dtype([("param", "<u8"), ("grad", "<u8"), ("master", "<u8"), ("n", "<u8"),
+                   ("state", "<u8"), ("type", "<u4"), ("set", "<u4")])
 BLOCK = 32  # elements that share an exponent; a parameter's share is padded to whole ones
 
 
@@ -35,7 +35,7 @@ def _dense(t: torch.Tensor) -> bool:
 
 
 class AdamW(torch.optim.Optimizer):
-    """AdamW (decoupled weight decay) in one launch for up to 72 tensors.
+    """AdamW (decoupled weight decay) in one launch for up to 64 tensors.
 
     Per element, with gradient g and step t of its parameter:
 
@@ -58,6 +58,8 @@ class AdamW(torch.optim.Optimizer):
 
     master_weights keeps a float32 copy of 16-bit parameters, of which they
     are roundings; without it a small update of a 16-bit parameter is lost.
+    Where such a parameter is written by others between steps (clamped,
+    loaded), the copy takes the new value.
 
     max_grad_norm multiplies the gradients by
     min(1, max_grad_norm / (norm + 1e-6)), norm the 2-norm over all of them,
@@ -120,11 +122,17 @@ class AdamW(torch.optim.Optimizer):
         table = (AdamwTensor * len(self._params))()
         view = np.frombuffer(table, dtype=_ENTRY) if len(table) else np.empty(0, _ENTRY)
         for i, p in enumerate(self._params):
-            view[i] = (0, 0, p.numel(), at, TYPE_CODES[p.dtype], 0)
-            at += -(-p.numel() // BLOCK) * BLOCK
+            view[i] = (0, 0, 0, p.numel(), at, TYPE_CODES[p.dtype], 0)
+            at += _share(p)
         for k, (_, first) in enumerate(self._sets):
             view["set"][first:] = k
         self._grow(at)
+        if self.master is not None:
+            where = self.master.data_ptr()
+            for i, p in enumerate(self._params):
+                if p.dtype != torch.float32:
+                    view["master"][i] = where
+                    where += 4 * _share(p)
         self._expect = [(p, p.numel(), p.dtype) for p in self._params]
         self._table, self._view, self._total = table, view, at
 
@@ -140,8 +148,9 @@ class AdamW(torch.optim.Optimizer):
                              "is not densely stored")
 
     def _grow(self, total: int) -> None:
-        """State for `total` elements: what is there, then zeros."""
-        dev, old = self.ctx.device, self._total
+        """State for `total` elements: what is there, then zeros (and the new
+        16-bit parameters' master copies)."""
+        dev = self.ctx.device
 
         def grown(t, n, dtype):
             new = torch.zeros(n, dtype=dtype, device=dev)
@@ -154,14 +163,15 @@ class AdamW(torch.optim.Optimizer):
         self._moments = grown(m, total, kind), grown(v, total, kind)
         if self.state_bits == 8:
             self._scales = tuple(grown(s, total // BLOCK, torch.uint8) for s in self._scales)
-        if self.master_weights and any(p.dtype != torch.float32 for p in self._params):
-            had = self.master is not None
-            self.master = grown(self.master, total, torch.float32)
+        narrow = [p for p in self._params if p.dtype != torch.float32]
+        if self.master_weights and narrow:
+            old = 0 if self.master is None else self.master.numel()
+            self.master = grown(self.master, sum(map(_share, narrow)), torch.float32)
             at = 0
-            for p in self._params:
-                if not had or at >= old:
+            for p in narrow:
+                if at >= old:
                     self.master[at:at + p.numel()] = _flat(p.detach())
-                at += -(-p.numel() // BLOCK) * BLOCK
+                at += _share(p)
         if self._scratch is None:
             self._scratch = torch.empty(lib.dressi_adamw_scratch(), dtype=torch.uint8, device=dev)
             if self.max_grad_norm is not None:
@@ -256,8 +266,8 @@ class AdamW(torch.optim.Optimizer):
             check(lib.dressi_adamw_step(
                 ctx._ctx.handle, table, len(live), hyper, len(hyper), self.state_bits, self._total,
                 self._moments[0].data_ptr(), self._moments[1].data_ptr(),
-                _addr(self._scales[0]), _addr(self._scales[1]), _addr(self.master), self.seed,
-                self.max_grad_norm or 0.0, self._scratch.data_ptr(), _addr(self.grad_norm)))
+                _addr(self._scales[0]), _addr(self._scales[1]), self.seed, self.max_grad_norm or 0.0,
+                self._scratch.data_ptr(), _addr(self.grad_norm)))
         self._steps = now
         self._even = self._even and every
         return loss
@@ -302,8 +312,9 @@ class AdamW(torch.optim.Optimizer):
     def state_dict(self) -> dict:
         """Flat state: "step" (one count a parameter), "exp_avg" and
         "exp_avg_sq" as they are kept (with "exp_avg_scale" and
-        "exp_avg_sq_scale" in 8 bits), "master" where there is one, and the
-        groups' hyperparameters."""
+        "exp_avg_sq_scale" in 8 bits), "master" where there is one (the
+        16-bit parameters' copies, laid out like the moments), and the groups'
+        hyperparameters."""
         out = {"step": list(self._steps), "seed": self.seed,
                "exp_avg": self._moments[0], "exp_avg_sq": self._moments[1],
                "param_groups": [{k: v for k, v in g.items() if k != "params"}
@@ -345,6 +356,11 @@ class AdamW(torch.optim.Optimizer):
         ends = [at for _, at in self._sets[1:]] + [len(steps)]
         self._even = all(len(set(steps[a:b])) == 1 for (_, a), b in zip(self._sets, ends))
         self.seed = int(state_dict.get("seed", self.seed)) & 0xffffffff
+
+
+def _share(p: torch.Tensor) -> int:
+    """Elements of the flat buffers that belong to a parameter."""
+    return -(-p.numel() // BLOCK) * BLOCK
 
 
 def _flat(t: torch.Tensor) -> torch.Tensor:

@@ -393,6 +393,49 @@ def test_group_added_later(ctx):
     assert torch.allclose(b, torch.full_like(b, -0.5)) and torch.allclose(a, torch.full_like(a, -0.2))
 
 
+@pytest.mark.parametrize("kind", TYPES[1:], ids=str)
+def test_parameters_written_between_steps(ctx, kind):
+    """A 16-bit parameter that is clamped or replaced between steps keeps what was written: the
+    next step starts from it, not from the old master copy."""
+    import opendressi_amd.torch as dr
+    rng = np.random.default_rng(8)
+    p = torch.tensor(_values(rng, 3001)).to(kind).cuda()
+    opt = dr.AdamW(ctx, [p], lr=1e-2, weight_decay=0.0)
+    for t in range(4):
+        p.grad = torch.tensor(_values(rng, 3001)).to(kind).cuda()
+        if t == 1:
+            p.data.clamp_(-0.5, 0.5)
+        if t == 2:
+            p.data = torch.tensor(_values(rng, 3001)).to(kind).cuda()
+        before = torch.where(opt.master[:3001].to(kind) == p, opt.master[:3001], p.float()).clone()
+        opt.step()
+        # no update is larger than lr times (1 - b1) / sqrt(1 - b2), about 3.2
+        assert ((opt.master[:3001] - before).abs() <= 3.3e-2).all(), t
+        assert torch.equal(opt.master[:3001].to(kind), p)
+
+
+def test_mixed_types(ctx):
+    """Master copies for the 16-bit parameters alone, each at its place."""
+    import opendressi_amd.torch as dr
+    rng = np.random.default_rng(9)
+    sizes, kinds = (100, 33, 64, 7), (torch.float32, torch.bfloat16, torch.float32, torch.float16)
+    ps = [torch.tensor(_values(rng, n)).to(k).cuda() for n, k in zip(sizes, kinds)]
+    alone = [p.clone() for p in ps]
+    opts = [dr.AdamW(ctx, [p], lr=1e-2) for p in alone]
+    opt = dr.AdamW(ctx, ps[:2], lr=1e-2)
+    opt.add_param_group({"params": ps[2:]})
+    assert opt.master.numel() == 64 + 32
+    for _ in range(3):
+        for p, q, o in zip(ps, alone, opts):
+            p.grad = torch.tensor(_values(rng, p.numel())).to(p.dtype).cuda()
+            q.grad = p.grad.clone()
+            o.step()
+        opt.step()
+    for p, q in zip(ps, alone):
+        assert torch.equal(p, q)
+    assert torch.equal(opt.master[64:71], opts[3].master[:7])
+
+
 def test_hooks_closures_and_schedulers(ctx):
     import opendressi_amd.torch as dr
     p = torch.zeros(8, device="cuda", requires_grad=True)

@@ -147,6 +147,16 @@ def test_against_float64(ctx, shape, groups, kind, act):
     _check(x, gy, w, b, groups, 1e-5, act, _run(ctx, x, gy, w, b, groups, 1e-5, act))
 
 
+@pytest.mark.parametrize("shape,groups", [((5000, 8), 2), ((2100, 5, 24), 3), ((2500, 1100), 1),
+                                          ((600, 70, 33), 3), ((2300, 9, 520), 1)], ids=str)
+@pytest.mark.parametrize("kind", TYPES, ids=str)
+def test_many_items(ctx, shape, groups, kind):
+    """More items than workgroups whose channel sums are added: each takes several."""
+    print(f"[group_norm items] {shape} {groups} {kind}", flush=True)
+    x, gy, w, b = _inputs(shape, kind, 12)
+    _check(x, gy, w, b, groups, 1e-5, "silu", _run(ctx, x, gy, w, b, groups, 1e-5, "silu"))
+
+
 @pytest.mark.parametrize("offset", [0.0, 300.0, -3e4])
 @pytest.mark.parametrize("shape,groups", [((2, 64, 65, 32), 4), ((1, 30, 30, 5), 1),
                                           ((1, 300, 300, 8), 1)], ids=str)
