@@ -885,8 +885,12 @@ typedef struct dressi_adamw_set {
  * (bits(|x| 2^-(max(E, T) - T)) + r) >> 20 with T = 14 and the sign in bit 7
  * for exp_avg, T = 30 for exp_avg_sq; r is a hash of (element, step, seed)
  * below 2^20. exp_avg_sq above zero has a code above zero; E = 255 stands
- * for 32 NaN. The steps' counts and rates are arguments: a step captured into
- * a graph would repeat them. */
+ * for 32 NaN. steps, device_sets: both NULL, or the sets' step counts on the
+ * device, which the call advances in place of reading dressi_adamw_set.step,
+ * and dressi_adamw_set_bytes of device memory for each set: then a step
+ * captured into a graph goes on counting when it is replayed (at the rates of
+ * the capture). */
+size_t dressi_adamw_set_bytes(void);
 size_t dressi_adamw_scratch(void);
 int dressi_adamw_step(dressi_ctx* ctx, const dressi_adamw_tensor* tensors,
                       uint32_t n_tensors, const dressi_adamw_set* sets,
@@ -894,7 +898,7 @@ int dressi_adamw_step(dressi_ctx* ctx, const dressi_adamw_tensor* tensors,
                       uint64_t state_elems, void* exp_avg, void* exp_avg_sq,
                       uint8_t* exp_avg_scale, uint8_t* exp_avg_sq_scale,
                       uint32_t seed, float max_norm, void* scratch,
-                      float* norm);
+                      float* norm, uint64_t* steps, void* device_sets);
 /* The values that n elements (whole blocks of 32) of 8-bit moments stand
  * for, as bfloat16, which holds them exactly. */
 int dressi_adamw_values(dressi_ctx* ctx, uint64_t n, const void* exp_avg,

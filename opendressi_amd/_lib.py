@@ -201,8 +201,9 @@ _SIGS = {
     "dressi_group_norm_bwd": (_I, [_P, _P, _P, _U, _U, C.c_uint64, _U, C.c_uint64, C.c_uint64, _U,
                                    _P, _P, _U, _U, _P, _P, _P, _S, _P, _P, _P]),
     "dressi_adamw_scratch": (_S, []),
+    "dressi_adamw_set_bytes": (_S, []),
     "dressi_adamw_step": (_I, [_P, _P, _U, _P, _U, _U, C.c_uint64, _P, _P, _P, _P, _U, _F, _P,
-                               _P]),
+                               _P, _P, _P]),
     "dressi_adamw_values": (_I, [_P, C.c_uint64, _P, _P, _P, _P, _P, _P]),
 }
 

@@ -64,6 +64,7 @@ struct Table {
 static_assert(sizeof(Table) <= 3800, "with the pointers beside it within 4 KB of arguments");
 
 struct State {
+    const SetArg* sets;  // on the device, or null: the table's
     void* m;
     void* v;
     uint8_t* m_scale;
@@ -197,26 +198,45 @@ struct Moments {
     float m[kLaneElems], v[kLaneElems];
 };
 
+// A lane's moments as they lie in memory.
 template <bool Q8>
-__device__ __forceinline__ Moments load_moments(const State& st, uint64_t i) {
-    Moments o;
-    if constexpr (Q8) {
-        const uint32_t cm = *(const uint32_t*)((const uint8_t*)st.m + i);
-        const uint32_t cv = *(const uint32_t*)((const uint8_t*)st.v + i);
-        const uint32_t fm = st.m_scale[i / kBlock], fv = st.v_scale[i / kBlock];
+struct RawMoments {
+    Pack<float, kLaneElems> m, v;
+    __device__ __forceinline__ void load(const State& st, uint64_t i) {
+        m = load_pack<float, kLaneElems>((const float*)st.m + i);
+        v = load_pack<float, kLaneElems>((const float*)st.v + i);
+    }
+    __device__ __forceinline__ void clear() { m = v = {}; }
+    __device__ __forceinline__ Moments values() const {
+        Moments o;
+        unpack(m, o.m);
+        unpack(v, o.v);
+        return o;
+    }
+};
+template <>
+struct RawMoments<true> {
+    uint32_t m, v;  // four codes each
+    uint8_t m_scale, v_scale;
+    __device__ __forceinline__ void load(const State& st, uint64_t i) {
+        m = *(const uint32_t*)((const uint8_t*)st.m + i);
+        v = *(const uint32_t*)((const uint8_t*)st.v + i);
+        m_scale = st.m_scale[i / kBlock];
+        v_scale = st.v_scale[i / kBlock];
+    }
+    __device__ __forceinline__ void clear() { m = v = m_scale = v_scale = 0; }
+    __device__ __forceinline__ Moments values() const {
+        Moments o;
 #pragma unroll
         for (uint32_t j = 0; j < kLaneElems; j++) {
-            const uint32_t c = (cm >> (8 * j)) & 255u;
-            o.m[j] = __uint_as_float(__float_as_uint(decode(c & 127u, fm, kTop1)) |
+            const uint32_t c = (m >> (8 * j)) & 255u;
+            o.m[j] = __uint_as_float(__float_as_uint(decode(c & 127u, m_scale, kTop1)) |
                                      ((c & 128u) << 24));
-            o.v[j] = decode((cv >> (8 * j)) & 255u, fv, kTop2);
+            o.v[j] = decode((v >> (8 * j)) & 255u, v_scale, kTop2);
         }
-    } else {
-        load_vec<float, kLaneElems>((const float*)st.m + i, o.m);
-        load_vec<float, kLaneElems>((const float*)st.v + i, o.v);
+        return o;
     }
-    return o;
-}
+};
 
 // All 64 lanes call this together (the block's maximum crosses lanes); `live`
 // says which hold elements.
@@ -262,9 +282,8 @@ __device__ __forceinline__ void store_moments(const State& st, uint64_t i, const
 // the step
 // ---------------------------------------------------------------------------
 
-template <bool Q8>
-__device__ __forceinline__ void update(const SetArg& h, float coef, bool clip,
-                                       const float* g, float* p, Moments& o) {
+__device__ __forceinline__ void update(const SetArg& h, float coef, bool clip, const float* g,
+                                       float* p, Moments& o) {
 #pragma unroll
     for (uint32_t j = 0; j < kLaneElems; j++) {
         const float x = clip ? g[j] * coef : g[j];
@@ -293,64 +312,66 @@ __device__ __forceinline__ void step_chunk(const TensorArg& t, const SetArg& h, 
     const T* g = (const T*)t.grad;
     const bool wide = !std::is_same<T, float>::value && t.master != nullptr;
     const uint64_t padded = (t.n + kBlock - 1) / kBlock * kBlock;
-    float gx[ITER][kLaneElems], px[ITER][kLaneElems];
-    Moments mo[ITER];
+    Pack<T, kLaneElems> gv[ITER], pv[ITER];
+    Pack<float, kLaneElems> mv[ITER];
+    RawMoments<Q8> raw[ITER];
 #pragma unroll
     for (int k = 0; k < ITER; k++) {
         const uint64_t i = at + (uint64_t)k * kStep + threadIdx.x * kLaneElems;
         if (FULL) {
-            load_vec<T, kLaneElems>(g + i, gx[k]);
-            load_vec<T, kLaneElems>(p + i, px[k]);
+            gv[k] = load_pack<T, kLaneElems>(g + i);
+            pv[k] = load_pack<T, kLaneElems>(p + i);
             if (wide) {
-                float ms[kLaneElems];
-                load_vec<float, kLaneElems>(t.master + i, ms);
-#pragma unroll
-                for (uint32_t j = 0; j < kLaneElems; j++) {
-                    px[k][j] = newest<T>(px[k][j], ms[j]);
-                }
+                mv[k] = load_pack<float, kLaneElems>(t.master + i);
             }
-            mo[k] = load_moments<Q8>(st, t.state + i);
+            raw[k].load(st, t.state + i);
         } else {
 #pragma unroll
             for (uint32_t j = 0; j < kLaneElems; j++) {
                 const bool in = i + j < t.n;
-                gx[k][j] = in ? to_float(g[i + j]) : 0.f;
-                px[k][j] = in ? to_float(p[i + j]) : 0.f;
-                if (in && wide) {
-                    px[k][j] = newest<T>(px[k][j], t.master[i + j]);
-                }
-                mo[k].m[j] = mo[k].v[j] = 0.f;
+                gv[k].v[j] = in ? g[i + j] : (T)0.f;
+                pv[k].v[j] = in ? p[i + j] : (T)0.f;
+                mv[k].v[j] = in && wide ? t.master[i + j] : 0.f;
             }
+            raw[k].clear();
             if (i < padded) {  // a share is padded with zeros to whole blocks
-                mo[k] = load_moments<Q8>(st, t.state + i);
+                raw[k].load(st, t.state + i);
             }
         }
     }
 #pragma unroll
     for (int k = 0; k < ITER; k++) {
         const uint64_t i = at + (uint64_t)k * kStep + threadIdx.x * kLaneElems;
-        update<Q8>(h, coef, clip, gx[k], px[k], mo[k]);
+        float gx[kLaneElems], px[kLaneElems];
+        unpack(gv[k], gx);
+        unpack(pv[k], px);
+#pragma unroll
+        for (uint32_t j = 0; wide && j < kLaneElems; j++) {
+            px[j] = newest<T>(px[j], mv[k].v[j]);
+        }
+        Moments o = raw[k].values();
+        update(h, coef, clip, gx, px, o);
         if (!FULL) {
 #pragma unroll
             for (uint32_t j = 0; j < kLaneElems; j++) {
                 if (i + j >= t.n) {
-                    mo[k].m[j] = mo[k].v[j] = 0.f;  // the padding stays zero
+                    o.m[j] = o.v[j] = 0.f;  // the padding stays zero
                 }
             }
         }
-        store_moments<Q8>(st, t.state + i, mo[k], h.key, FULL || i < padded);
+        store_moments<Q8>(st, t.state + i, o, h.key, FULL || i < padded);
         if (FULL) {
-            store_vec<T, kLaneElems>(p + i, px[k]);
+            store_vec<T, kLaneElems>(p + i, px);
             if (wide) {
-                store_vec<float, kLaneElems>(t.master + i, px[k]);
+                store_vec<float, kLaneElems>(t.master + i, px);
             }
         } else {
 #pragma unroll
             for (uint32_t j = 0; j < kLaneElems; j++) {
                 if (i + j < t.n) {
-                    p[i + j] = from_float<T>(px[k][j]);
+                    p[i + j] = from_float<T>(px[j]);
                     if (wide) {
-                        t.master[i + j] = px[k][j];
+                        t.master[i + j] = px[j];
                     }
                 }
             }
@@ -390,7 +411,7 @@ __global__ __launch_bounds__(256) void k_adamw_step(const Table tb, const State 
         }
     }
     const TensorArg& t = tb.t[find_tensor(tb, blockIdx.x)];
-    const SetArg& h = tb.set[t.set];
+    const SetArg h = st.sets ? st.sets[t.set] : tb.set[t.set];
     const uint64_t at = (uint64_t)(blockIdx.x - t.first_chunk) * (ITER * kThreads * kLaneElems);
     switch (t.type) {
         case DRESSI_F32:
@@ -404,28 +425,51 @@ __global__ __launch_bounds__(256) void k_adamw_step(const Table tb, const State 
     }
 }
 
+// What follows from a set's rates at step t.
+__host__ __device__ inline SetArg set_arg(const dressi_adamw_set& s, uint64_t step, uint32_t seed) {
+    SetArg a;
+    a.b1 = (float)s.beta1;
+    a.omb1 = (float)(1.0 - s.beta1);
+    a.b2 = (float)s.beta2;
+    a.omb2 = (float)(1.0 - s.beta2);
+    a.eps = (float)s.eps;
+    a.decay = (float)(1.0 - s.lr * s.weight_decay);
+    a.step_size = (float)(s.lr / (1.0 - pow(s.beta1, (double)step)));
+    a.inv_bc2 = (float)(1.0 / sqrt(1.0 - pow(s.beta2, (double)step)));
+    a.key = (uint32_t)step * 0x9e3779b9u + seed * 0x632be5abu + 0x7f4a7c15u;
+    return a;
+}
+
+// Steps that a graph may repeat: their count is on the device. One thread, a
+// launch for each set: it is counted once, before the step's kernels read it.
+__global__ __launch_bounds__(64) void k_adamw_tick(const dressi_adamw_set set, uint32_t seed,
+                                                   uint64_t* step, SetArg* out) {
+    if (threadIdx.x == 0) {
+        *step += 1;
+        *out = set_arg(set, *step, seed);
+    }
+}
+
 // The values that 8-bit moments stand for, as bfloat16 (which holds them all:
 // three mantissa bits). 4 elements a lane.
 __global__ __launch_bounds__(256) void k_adamw_values(const State st, uint64_t n, bf16* m,
                                                       bf16* v) {
     const uint64_t i = ((uint64_t)blockIdx.x * kThreads + threadIdx.x) * kLaneElems;
     if (i < n) {
-        const Moments o = load_moments<true>(st, i);
+        RawMoments<true> raw;
+        raw.load(st, i);
+        const Moments o = raw.values();
         store_vec<bf16, kLaneElems>(m + i, o.m);
         store_vec<bf16, kLaneElems>(v + i, o.v);
     }
 }
 
-// One launch's worth of tensors: as many as fit the table.
-struct Batch {
-    Table tb;
-    uint32_t iter;
-};
-
-// Elements up to which a workgroup takes 1024 of them, else 4096: more workgroups
-// against more loads in flight in each. 8-bit moments take 25.7 and 27.8 us at
-// 2^23 elements, 802 and 779 at 2^28; 32-bit ones the same at 2^22, and 4096
-// leaves a quarter of the sums of a clipped norm (61 and 54 us at 2^23).
+// Elements up to which a workgroup takes 1024 of them, else 4096 (8-bit moments,
+// which take more registers: 2048): more workgroups against more loads in flight
+// in each. 8-bit moments take 25.7 us so and 27.8 with 4096 at 2^23 elements, 802
+// and 779 at 2^28 (bfloat16 parameters, 2^27: 448 us with 2048, 451 with 4096);
+// 32-bit ones the same at 2^22, and 4096 leaves a quarter of the sums of a clipped
+// norm (61 and 54 us at 2^23).
 constexpr uint64_t kSmallTotal = 1ull << 20, kSmallTotal8 = 1ull << 23;
 
 int check_tensors(const dressi_adamw_tensor* t, uint32_t n, uint32_t n_sets, uint64_t state_elems) {
@@ -448,35 +492,22 @@ int check_tensors(const dressi_adamw_tensor* t, uint32_t n, uint32_t n_sets, uin
     return DRESSI_OK;
 }
 
-int check_set(const dressi_adamw_set& s, uint32_t i) {
+int check_set(const dressi_adamw_set& s, uint32_t i, bool on_device) {
     DRESSI_REQUIRE(s.lr >= 0.0 && std::isfinite(s.lr), "adamw: lr %g of set %u", s.lr, i);
     DRESSI_REQUIRE(s.beta1 >= 0.0 && s.beta1 < 1.0, "adamw: beta1 %g of set %u", s.beta1, i);
     DRESSI_REQUIRE(s.beta2 >= 0.0 && s.beta2 < 1.0, "adamw: beta2 %g of set %u", s.beta2, i);
     DRESSI_REQUIRE(s.eps >= 0.0 && std::isfinite(s.eps), "adamw: eps %g of set %u", s.eps, i);
     DRESSI_REQUIRE(s.weight_decay >= 0.0 && std::isfinite(s.weight_decay),
                    "adamw: weight_decay %g of set %u", s.weight_decay, i);
-    DRESSI_REQUIRE(s.step >= 1, "adamw: step 0 of set %u (the first is 1)", i);
+    DRESSI_REQUIRE(on_device || s.step >= 1, "adamw: step 0 of set %u (the first is 1)", i);
     return DRESSI_OK;
 }
 
-SetArg set_arg(const dressi_adamw_set& s, uint32_t seed) {
-    SetArg a;
-    a.b1 = (float)s.beta1;
-    a.omb1 = (float)(1.0 - s.beta1);
-    a.b2 = (float)s.beta2;
-    a.omb2 = (float)(1.0 - s.beta2);
-    a.eps = (float)s.eps;
-    a.decay = (float)(1.0 - s.lr * s.weight_decay);
-    a.step_size = (float)(s.lr / (1.0 - std::pow(s.beta1, (double)s.step)));
-    a.inv_bc2 = (float)(1.0 / std::sqrt(1.0 - std::pow(s.beta2, (double)s.step)));
-    a.key = (uint32_t)s.step * 0x9e3779b9u + seed * 0x632be5abu + 0x7f4a7c15u;
-    return a;
-}
-
-// Calls f(table) for each launch.
+// Calls f(table) for each launch. on_device: the entries keep their sets' own
+// numbers.
 template <typename F>
 int for_batches(const dressi_adamw_tensor* t, uint32_t n, const dressi_adamw_set* sets,
-                uint32_t seed, uint32_t chunk_elems, F&& f) {
+                bool on_device, uint32_t seed, uint32_t chunk_elems, F&& f) {
     Table tb;
     uint32_t set_of[kMaxSets];
     uint32_t n_sets = 0;
@@ -489,7 +520,7 @@ int for_batches(const dressi_adamw_tensor* t, uint32_t n, const dressi_adamw_set
         uint64_t done = 0;
         while (done < t[i].n) {
             uint32_t s = 0;
-            while (s < n_sets && set_of[s] != t[i].set) {
+            while (!on_device && s < n_sets && set_of[s] != t[i].set) {
                 s++;
             }
             if (tb.n_tensors == kMaxTensors || s == kMaxSets || tb.n_chunks == (1u << 23)) {
@@ -499,9 +530,11 @@ int for_batches(const dressi_adamw_tensor* t, uint32_t n, const dressi_adamw_set
                 tb.n_tensors = tb.n_chunks = n_sets = 0;
                 continue;
             }
-            if (s == n_sets) {
+            if (on_device) {
+                s = t[i].set;
+            } else if (s == n_sets) {
                 set_of[n_sets++] = t[i].set;
-                tb.set[s] = set_arg(sets[t[i].set], seed);
+                tb.set[s] = set_arg(sets[t[i].set], sets[t[i].set].step, seed);
             }
             const uint64_t room = (uint64_t)((1u << 23) - tb.n_chunks) * chunk_elems;
             const uint64_t take = std::min<uint64_t>(room, t[i].n - done);
@@ -529,13 +562,16 @@ using namespace dressi;
 
 extern "C" {
 
+size_t dressi_adamw_set_bytes(void) { return sizeof(SetArg); }
+
 size_t dressi_adamw_scratch(void) { return kMaxPartials * sizeof(double); }
 
 int dressi_adamw_step(dressi_ctx* ctx, const dressi_adamw_tensor* tensors, uint32_t n_tensors,
                       const dressi_adamw_set* sets, uint32_t n_sets, uint32_t state_bits,
                       uint64_t state_elems, void* exp_avg, void* exp_avg_sq,
                       uint8_t* exp_avg_scale, uint8_t* exp_avg_sq_scale, uint32_t seed,
-                      float max_norm, void* scratch, float* norm) {
+                      float max_norm, void* scratch, float* norm, uint64_t* steps,
+                      void* device_sets) {
     DRESSI_REQUIRE(ctx, "NULL context");
     if (n_tensors == 0) {
         return DRESSI_OK;
@@ -550,6 +586,8 @@ int dressi_adamw_step(dressi_ctx* ctx, const dressi_adamw_tensor* tensors, uint3
     const uintptr_t mask = q8 ? 3 : 15;
     DRESSI_REQUIRE((((uintptr_t)exp_avg | (uintptr_t)exp_avg_sq) & mask) == 0,
                    "adamw: the state buffers are not aligned");
+    DRESSI_REQUIRE(!steps == !device_sets && n_sets <= 65536, "adamw: bad sets");
+    const bool on_device = steps != nullptr;
     DRESSI_REQUIRE(max_norm >= 0.f, "adamw: max_norm %g", (double)max_norm);
     const bool clip = max_norm > 0.f;
     DRESSI_REQUIRE(!clip || (scratch && norm), "adamw: clipping needs scratch and norm");
@@ -561,7 +599,7 @@ int dressi_adamw_step(dressi_ctx* ctx, const dressi_adamw_tensor* tensors, uint3
         total += tensors[i].n;
     }
     for (uint32_t i = 0; i < n_sets; i++) {
-        if (int rc = check_set(sets[i], i)) {
+        if (int rc = check_set(sets[i], i, steps != nullptr)) {
             return rc;
         }
     }
@@ -569,11 +607,17 @@ int dressi_adamw_step(dressi_ctx* ctx, const dressi_adamw_tensor* tensors, uint3
         return clip ? launch_zero(ctx->stream, norm, sizeof(float)) : DRESSI_OK;
     }
     const bool small = total <= (q8 ? kSmallTotal8 : kSmallTotal);
-    const uint32_t chunk = kThreads * kLaneElems * (small ? 1 : 4);
-    State st{exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, nullptr, 0, max_norm, norm};
+    const uint32_t iter = small ? 1 : q8 ? 2 : 4;
+    const uint32_t chunk = kThreads * kLaneElems * iter;
+    for (uint32_t i = 0; on_device && i < n_sets; i++) {
+        hipLaunchKernelGGL(k_adamw_tick, dim3(1), dim3(64), 0, ctx->stream, sets[i], seed,
+                           steps + i, (SetArg*)device_sets + i);
+        DRESSI_CHECK_LAUNCH();
+    }
+    State st{(const SetArg*)device_sets, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, nullptr, 0, max_norm, norm};
     if (clip) {
         uint32_t launches = 0;
-        for_batches(tensors, n_tensors, sets, seed, chunk, [&](const Table&) {
+        for_batches(tensors, n_tensors, sets, on_device, seed, chunk, [&](const Table&) {
             launches++;
             return (int)DRESSI_OK;
         });
@@ -582,16 +626,13 @@ int dressi_adamw_step(dressi_ctx* ctx, const dressi_adamw_tensor* tensors, uint3
         const uint32_t share = launches ? kMaxPartials / launches : 1;
         uint32_t used = 0;
         const int rc = for_batches(
-            tensors, n_tensors, sets, seed, chunk, [&](const Table& tb) -> int {
+            tensors, n_tensors, sets, on_device, seed, chunk, [&](const Table& tb) -> int {
                 const uint32_t grid = std::min(tb.n_chunks, std::min(share, 512u));
                 double* out = (double*)scratch + used;
-                if (small) {
-                    hipLaunchKernelGGL(k_adamw_squares<1>, dim3(grid), dim3(kThreads), 0,
-                                       ctx->stream, tb, out);
-                } else {
-                    hipLaunchKernelGGL(k_adamw_squares<4>, dim3(grid), dim3(kThreads), 0,
-                                       ctx->stream, tb, out);
-                }
+                const auto squares = iter == 1   ? k_adamw_squares<1>
+                                     : iter == 2 ? k_adamw_squares<2>
+                                                 : k_adamw_squares<4>;
+                hipLaunchKernelGGL(squares, dim3(grid), dim3(kThreads), 0, ctx->stream, tb, out);
                 DRESSI_CHECK_LAUNCH();
                 used += grid;
                 return DRESSI_OK;
@@ -602,17 +643,10 @@ int dressi_adamw_step(dressi_ctx* ctx, const dressi_adamw_tensor* tensors, uint3
         st.partials = (const double*)scratch;
         st.n_partials = used;
     }
-    return for_batches(tensors, n_tensors, sets, seed, chunk, [&](const Table& tb) -> int {
-        const dim3 grid(tb.n_chunks), block(kThreads);
-        if (q8 && small) {
-            hipLaunchKernelGGL((k_adamw_step<true, 1>), grid, block, 0, ctx->stream, tb, st);
-        } else if (q8) {
-            hipLaunchKernelGGL((k_adamw_step<true, 4>), grid, block, 0, ctx->stream, tb, st);
-        } else if (small) {
-            hipLaunchKernelGGL((k_adamw_step<false, 1>), grid, block, 0, ctx->stream, tb, st);
-        } else {
-            hipLaunchKernelGGL((k_adamw_step<false, 4>), grid, block, 0, ctx->stream, tb, st);
-        }
+    return for_batches(tensors, n_tensors, sets, on_device, seed, chunk, [&](const Table& tb) -> int {
+        const auto step = q8 ? (small ? k_adamw_step<true, 1> : k_adamw_step<true, 2>)
+                             : (small ? k_adamw_step<false, 1> : k_adamw_step<false, 4>);
+        hipLaunchKernelGGL(step, dim3(tb.n_chunks), dim3(kThreads), 0, ctx->stream, tb, st);
         DRESSI_CHECK_LAUNCH();
         return DRESSI_OK;
     });
@@ -633,7 +667,7 @@ int dressi_adamw_values(dressi_ctx* ctx, uint64_t n, const void* exp_avg, const 
     DRESSI_REQUIRE((((uintptr_t)exp_avg | (uintptr_t)exp_avg_sq) & 3) == 0 &&
                        (((uintptr_t)exp_avg_bf16 | (uintptr_t)exp_avg_sq_bf16) & 7) == 0,
                    "adamw: the buffers are not aligned");
-    State st{(void*)exp_avg, (void*)exp_avg_sq, (uint8_t*)exp_avg_scale,
+    State st{nullptr, (void*)exp_avg, (void*)exp_avg_sq, (uint8_t*)exp_avg_scale,
              (uint8_t*)exp_avg_sq_scale, nullptr, 0, 0.f, nullptr};
     // within the launch limit, in whole blocks
     constexpr uint64_t kPiece = kLaunchThreads * kLaneElems;

@@ -65,14 +65,17 @@ class AdamW(torch.optim.Optimizer):
     min(1, max_grad_norm / (norm + 1e-6)), norm the 2-norm over all of them,
     without a host round trip; `grad_norm` then holds the last step's norm.
 
-    A parameter whose grad is None is left as it is, and so is its step. A
-    step cannot be captured into a graph: it takes the step count from the
-    host. Hooks registered on the optimizer run; torch's global optimizer
+    A parameter whose grad is None is left as it is, and so is its step.
+
+    capturable keeps the step counts on the device, so that a step can be
+    captured into a graph (at the learning rates of the capture); every
+    parameter then needs a gradient in every step. Hooks registered on the optimizer run; torch's global optimizer
     hooks do not."""
 
     def __init__(self, ctx: RasterizeHipContext, params, lr: float = 1e-3, betas=(0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float = 1e-2, state_bits: int = 32,
-                 max_grad_norm: float | None = None, master_weights: bool = True, seed: int = 0):
+                 max_grad_norm: float | None = None, master_weights: bool = True, seed: int = 0,
+                 capturable: bool = False):
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
         if max_grad_norm is not None and not 0.0 < max_grad_norm < math.inf:
@@ -82,6 +85,7 @@ class AdamW(torch.optim.Optimizer):
         self.max_grad_norm = max_grad_norm
         self.master_weights = bool(master_weights)
         self.seed = int(seed) & 0xffffffff
+        self.capturable = bool(capturable)
         self.grad_norm = None
         self._params: list[torch.Tensor] = []  # in the order of their shares
         self._steps: list[int] = []
@@ -96,6 +100,7 @@ class AdamW(torch.optim.Optimizer):
         self._scales: tuple[torch.Tensor | None, torch.Tensor | None] = (None, None)
         self.master = None
         self._scratch = None
+        self._counts = self._device_sets = None  # of the sets, where capturable
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     # ---- layout ----
@@ -126,6 +131,13 @@ class AdamW(torch.optim.Optimizer):
             at += _share(p)
         for k, (_, first) in enumerate(self._sets):
             view["set"][first:] = k
+        if self.capturable:
+            new = torch.zeros(len(self._sets), dtype=torch.int64, device=self.ctx.device)
+            if self._counts is not None:
+                new[:len(self._counts)] = self._counts
+            self._counts = new
+            self._device_sets = torch.empty(len(new) * lib.dressi_adamw_set_bytes(),
+                                            dtype=torch.uint8, device=self.ctx.device)
         self._grow(at)
         if self.master is not None:
             where = self.master.data_ptr()
@@ -216,9 +228,9 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("AdamW.step cannot be captured into a graph: its step count is "
-                               "the host's")
+        if not self.capturable and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW.step cannot be captured into a graph without "
+                               "capturable=True: its step count is the host's")
         dev = self.ctx.device.index
         kept = []  # copies that the launch reads
         live, params, grads = [], [], []
@@ -240,7 +252,12 @@ class AdamW(torch.optim.Optimizer):
             return loss
         every = len(live) == len(self._expect)
         steps = self._steps
-        if every and self._even:
+        if self.capturable:
+            if not (every and self._even):
+                raise RuntimeError("AdamW: a capturable step needs every parameter's gradient")
+            now, table, view = steps, self._table, self._view
+            sets = [(g, 0) for g, _ in self._sets]
+        elif every and self._even:
             # all in step: a set for each group, as the table has it
             now = [t + 1 for t in steps]
             sets = [(g, steps[at] + 1) for g, at in self._sets]
@@ -267,7 +284,8 @@ class AdamW(torch.optim.Optimizer):
                 ctx._ctx.handle, table, len(live), hyper, len(hyper), self.state_bits, self._total,
                 self._moments[0].data_ptr(), self._moments[1].data_ptr(),
                 _addr(self._scales[0]), _addr(self._scales[1]), self.seed, self.max_grad_norm or 0.0,
-                self._scratch.data_ptr(), _addr(self.grad_norm)))
+                self._scratch.data_ptr(), _addr(self.grad_norm), _addr(self._counts),
+                _addr(self._device_sets)))
         self._steps = now
         self._even = self._even and every
         return loss
@@ -315,7 +333,12 @@ class AdamW(torch.optim.Optimizer):
         "exp_avg_sq_scale" in 8 bits), "master" where there is one (the
         16-bit parameters' copies, laid out like the moments), and the groups'
         hyperparameters."""
-        out = {"step": list(self._steps), "seed": self.seed,
+        steps = list(self._steps)
+        if self.capturable:
+            ends = [at for _, at in self._sets[1:]] + [len(steps)]
+            for t, (_, a), b in zip(self._counts.tolist(), self._sets, ends):
+                steps[a:b] = [t] * (b - a)
+        out = {"step": steps, "seed": self.seed,
                "exp_avg": self._moments[0], "exp_avg_sq": self._moments[1],
                "param_groups": [{k: v for k, v in g.items() if k != "params"}
                                 for g in self.param_groups]}
@@ -350,11 +373,15 @@ class AdamW(torch.optim.Optimizer):
                 _check_hyper(g)
             for mine, g in zip(self.param_groups, groups):
                 mine.update({k: v for k, v in g.items() if k != "params"})
+        ends = [at for _, at in self._sets[1:]] + [len(steps)]
+        even = all(len(set(steps[a:b])) == 1 for (_, a), b in zip(self._sets, ends))
+        if self.capturable and not even:
+            raise ValueError("a capturable optimizer's groups have one step count each")
         for k, t in named.items():
             t.copy_(state_dict[k])
-        self._steps = steps
-        ends = [at for _, at in self._sets[1:]] + [len(steps)]
-        self._even = all(len(set(steps[a:b])) == 1 for (_, a), b in zip(self._sets, ends))
+        self._steps, self._even = steps, even
+        if self.capturable:
+            self._counts.copy_(torch.tensor([steps[a] for _, a in self._sets]))
         self.seed = int(state_dict.get("seed", self.seed)) & 0xffffffff
 
 

@@ -171,6 +171,29 @@ def test_steps_8(ctx, sizes, kind, size):
     assert any(not torch.equal(p, q) for p, q in zip(ps, start))
 
 
+@pytest.mark.parametrize("kind", TYPES, ids=str)
+def test_large_8_bit(ctx, kind):
+    """Enough elements for the larger share of a workgroup: the codes of a stretch in their midst
+    and of the ragged end, and the norm over all."""
+    import opendressi_amd.torch as dr
+    n, b1, b2 = 2 ** 23 + 4099, F32(0.9), F32(0.999)
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    p = torch.randn(n, generator=gen, device="cuda").to(kind)
+    p.grad = torch.randn(n, generator=gen, device="cuda").to(kind)
+    opt = dr.AdamW(ctx, [p], lr=1e-2, state_bits=8, max_grad_norm=1e9)
+    opt.step()
+    norm = math.sqrt(float(p.grad.double().square().sum()))
+    assert abs(float(opt.grad_norm) - norm) <= 2 * U * norm
+    m, v = opt.moments()
+    for a, b in ((0, 320), (2 ** 22 - 64, 2 ** 22 + 64), (2 ** 23 - 32, n)):
+        g = _np(p.grad[a:b])
+        r = _mix(range(a, b), 1)
+        want_m = _rounded(F32(0) * b1 + g * F32(1 - 0.9), 14, ((r & 0xffff) << 4) + 8)
+        want_v = _rounded(F32(0) * b2 + (g * g) * F32(1 - 0.999), 30, ((r >> 16) << 4) + 8)
+        assert np.array_equal(_np(m[a:b]), want_m[:b - a].astype(F32))
+        assert np.array_equal(_np(v[a:b]), want_v[:b - a].astype(F32))
+
+
 def test_8_bit_moments_follow(ctx):
     """The slow moment moves by 0.1 % a step, a fraction of its code's step. Under a constant
     gradient v = g^2 (1 - b2^t); the rounding being unbiased, the mean over 2^16 elements follows.
@@ -434,6 +457,53 @@ def test_mixed_types(ctx):
     for p, q in zip(ps, alone):
         assert torch.equal(p, q)
     assert torch.equal(opt.master[64:71], opts[3].master[:7])
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_captured_steps(ctx, bits):
+    """A step in a graph goes on counting: replays, with other work between, are the eager steps.
+    The rates' powers come from the device's pow there, a rounding of a double apart."""
+    import opendressi_amd.torch as dr
+    rng = np.random.default_rng(10)
+    sizes = (5000, 77)
+    ps = [torch.tensor(_values(rng, n)).cuda() for n in sizes]
+    qs = [p.clone() for p in ps]
+    kw = dict(lr=1e-2, state_bits=bits, max_grad_norm=1.0)
+    groups = lambda t: [dict(params=t[:1]), dict(params=t[1:], lr=3e-2)]  # noqa: E731
+    opt, ref = dr.AdamW(ctx, groups(ps), capturable=True, **kw), dr.AdamW(ctx, groups(qs), **kw)
+    for p, q in zip(ps, qs):
+        p.grad, q.grad = torch.zeros_like(p), torch.zeros_like(q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        opt.step()
+    torch.cuda.current_stream().wait_stream(side)
+    ref.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for t in range(5):
+        for p, q in zip(ps, qs):
+            g = torch.tensor(_values(rng, p.numel())).cuda()
+            p.grad.copy_(g)
+            q.grad.copy_(g)
+        graph.replay()
+        torch.cuda.synchronize()
+        ref.step()
+        for p, q in zip(ps, qs):
+            assert torch.allclose(p, q, rtol=4 * U, atol=1e-2 * 16 * U), t
+    assert opt.state_dict()["step"] == ref.state_dict()["step"] == [6, 6]
+    with pytest.raises(RuntimeError, match="captur"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            ref.step()
+    torch.cuda.synchronize()
+    ps[0].grad = None
+    with pytest.raises(RuntimeError, match="every"):
+        opt.step()
+    # the state goes from one to the other
+    ref.load_state_dict(opt.state_dict())
+    opt.load_state_dict(ref.state_dict())
+    assert opt._counts.tolist() == [6, 6]
 
 
 def test_hooks_closures_and_schedulers(ctx):

@@ -26,7 +26,7 @@ def test_entry_points_refuse():
     assert lib.dressi_group_norm_bwd(None, None, None, 0, 1, 1, 8, 8, 8, 1, None, None, 0, 0, None,
                                      None, None, 0, None, None, None) == -1
     assert lib.dressi_adamw_step(None, None, 0, None, 0, 32, 0, None, None, None, None, 0, 0.0,
-                                 None, None) == -1
+                                 None, None, None, None) == -1
     assert lib.dressi_adamw_values(None, 0, None, None, None, None, None, None) == -1
 
 
