@@ -33,8 +33,7 @@ namespace {
 
 constexpr uint32_t kMaxThreads = 512;
 constexpr uint32_t kMaxVecs = 256;  // of a workgroup
-constexpr uint32_t kBatch = 4;      // pixels of a thread in flight
-constexpr uint32_t kBatchBwd = 4;   // the same of two images
+constexpr uint32_t kMinPixels = 2;  // that a thread should have of a chunk
 constexpr uint32_t kTargetGroups = 512;  // workgroups that a launch should have
 // Pixels that a thread keeps in registers (one pass). A workgroup's reads are a
 // block's few channels of each pixel, a cache line each: from 4096 pixels on
@@ -122,7 +121,7 @@ Cut make_cut(uint32_t n_items, uint64_t n_px, uint32_t n_ch, uint32_t n_groups, 
     const uint64_t others = (uint64_t)n_items * c.n_blocks;
     // chunks of 2^30 pixels at most
     const uint64_t want = std::max((kTargetGroups + others - 1) / others, (n_px >> 30) + 1);
-    const uint64_t batch = (uint64_t)c.rows * kBatch;
+    const uint64_t batch = (uint64_t)c.rows * kMinPixels;
     const uint64_t chunks = std::max<uint64_t>(1, std::min(want, (n_px + batch - 1) / batch));
     c.chunk_px = (uint32_t)((n_px + chunks - 1) / chunks + c.rows - 1) / c.rows * c.rows;
     c.chunks = (uint32_t)((n_px + c.chunk_px - 1) / c.chunk_px);
@@ -159,6 +158,16 @@ Cut make_item_cut(uint32_t n_items, uint64_t n_px, uint32_t n_ch, uint32_t n_gro
     }
     return Cut{};
 }
+
+// Pixels of a thread in flight. Forward 4 of 16 bytes in one group (1024 x 1024 x
+// 64 bfloat16 in 8 groups: 73 us, 76 with 8), else 8 (8 x 1024 x 1024 x 64 in 16
+// groups: 585 us, 596 with 4; 2 x 512 x 512 x 66 in 6: 51 and 55). Backward 4, of
+// the widest vectors 2, whose registers leave too few waves else (4 x 1024 x 1024
+// x 64 bfloat16: 487 us, 497 with 4).
+template <typename T, int V, int S>
+constexpr uint32_t kBatchOf = S == 1 && sizeof(T) * V >= 16 ? 4 : 8;
+template <int V>
+constexpr uint32_t kBatchBwdOf = V == 8 ? 2 : 4;
 
 // A thread's place: its vector of the block and the row of pixels it walks.
 struct Place {
@@ -389,6 +398,7 @@ __device__ __forceinline__ uint32_t group_of(const Cut& c, uint32_t vec, int g) 
 // The first pass: each chunk's (mean less the pivot, squares) for each group.
 template <typename T, int V, int S>
 __global__ __launch_bounds__(kMaxThreads) void k_gn_stats(const T* x, const Cut c, float2* part) {
+    constexpr uint32_t kBatch = kBatchOf<T, V, S>;
     __shared__ float2 red[S][kMaxThreads];
     __shared__ float first[S * kMaxVecs];
     const Place at(c);
@@ -591,6 +601,7 @@ __global__ __launch_bounds__(kMaxThreads) void k_gn_apply(const T* x, const Cut 
                                                           const float2* part, const Affine aff,
                                                           float eps, uint32_t act, T* y,
                                                           float* mean_out, float* rstd_out) {
+    constexpr uint32_t kBatch = kBatchOf<T, V, S>;
     __shared__ float2 stat[S * kMaxVecs];
     const Place at(c);
     const uint32_t unit = backwards(blockIdx.x, gridDim.x);
@@ -845,6 +856,7 @@ __global__ __launch_bounds__(kMaxThreads) void k_gn_bwd_sums(const T* gy, const 
                                                              const float* mean, const float* rstd,
                                                              float2* group_part,
                                                              float2* ch_part) {
+    constexpr uint32_t kBatchBwd = kBatchBwdOf<V>;
     __shared__ float2 red[V][kMaxThreads];
     const Place at(c);
     const uint32_t vec = c.first_vec(blockIdx.y) + at.vec;
@@ -984,6 +996,7 @@ __global__ __launch_bounds__(kMaxThreads) void k_gn_bwd_apply(const T* gy, const
                                                               const float2* group_part, T* gx,
                                                               const ParamGrad params,
                                                               uint32_t extra) {
+    constexpr uint32_t kBatchBwd = kBatchBwdOf<V>;
     __shared__ float2 mean_of[S * kMaxVecs];
     const uint32_t units = gridDim.x - extra;
     if (blockIdx.x >= units) {

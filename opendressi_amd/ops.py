@@ -821,10 +821,10 @@ def group_norm(ctx: Context, x: torch.Tensor, groups: int, weight: torch.Tensor 
     n_px, item, px = at
     size = lib.dressi_group_norm_scratch(code, n, n_px, c, item, px, groups,
                                          x.data_ptr() | y.data_ptr(), 0)
-    scratch = torch.empty(size, dtype=torch.uint8, device=x.device)
+    scratch = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
     _prep(ctx)
     check(lib.dressi_group_norm(ctx.handle, x.data_ptr(), code, n, n_px, c, item, px, groups,
-                                _addr(weight), _addr(bias), aff, eps, act, scratch.data_ptr(),
+                                _addr(weight), _addr(bias), aff, eps, act, _addr(scratch),
                                 size, y.data_ptr(), mean.data_ptr(), rstd.data_ptr()))
     return y, mean, rstd
 
@@ -860,10 +860,10 @@ def group_norm_bwd(ctx: Context, gy: torch.Tensor, x: torch.Tensor, mean: torch.
     n_px, item, px = at if x.numel() else (0, 0, c)
     size = lib.dressi_group_norm_scratch(code, n, n_px, c, item, px, groups,
                                          gy.data_ptr() | x.data_ptr() | (_addr(gx) or 0), 1)
-    scratch = torch.empty(size, dtype=torch.uint8, device=x.device)
+    scratch = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
     _prep(ctx)
     check(lib.dressi_group_norm_bwd(ctx.handle, gy.data_ptr(), x.data_ptr(), code, n, n_px, c,
                                     item, px, groups, _addr(weight), _addr(bias), aff, act,
-                                    mean.data_ptr(), rstd.data_ptr(), scratch.data_ptr(), size,
+                                    mean.data_ptr(), rstd.data_ptr(), _addr(scratch), size,
                                     _addr(gx), _addr(gw), _addr(gb)))
     return gx, gw, gb
