@@ -8,12 +8,17 @@
 //   gz = gy act'(z), gb = sum gz, gw = sum gz xh (over items and pixels)
 //   gx = s (w gz - mean_g(w gz) - xh mean_g(w gz xh))
 //
-// Memory bounds it. A group's channels lie side by side in a pixel, so a
-// workgroup takes whole pixels of a run (a "chunk") of one item: a thread
-// keeps one vector of V channels and walks the pixels. Two passes: one leaves
-// each chunk's sums, the other begins by joining the chunks' sums of its item
-// (every workgroup for itself: a launch in between costs more) and then reads
-// the image again.
+// Memory bounds it: about 12 operations a value forward and 20 backward, 5 (with
+// gelu 20) of them an exponential's. A group's channels lie side by side in a
+// pixel, so a workgroup takes whole pixels of a run (a "chunk") of one item: a
+// thread keeps one vector of V channels and walks the pixels. Two passes: one
+// leaves each chunk's sums, the other begins by joining the chunks' sums of its
+// item (every workgroup for itself) and then reads the image again. Reading it
+// once would take a wait between the workgroups of one launch, which two such
+// launches side by side could spend for ever; a small image, or a group of few
+// pixels, is held by one workgroup and read once. What crosses the memory is
+// each pass's images and nothing else (counters: 4 x 1024 x 1024 x 64 bfloat16,
+// forward 537 MB read twice and written once).
 //
 // Statistics are those of x less a pivot, the group's first value: a batch of a
 // thread's values gives its mean and the squares about that mean, both from
@@ -34,7 +39,11 @@ namespace {
 constexpr uint32_t kMaxThreads = 512;
 constexpr uint32_t kMaxVecs = 256;  // of a workgroup
 constexpr uint32_t kMinPixels = 2;  // that a thread should have of a chunk
-constexpr uint32_t kTargetGroups = 512;  // workgroups that a launch should have
+// Workgroups that a launch should have: two a compute unit. Each joins the sums of
+// its item's chunks, so more of them cost one large item (512 x 512 x 64 bfloat16
+// forward: 25 us with 512, 31 with 1024) and fewer leave loads unissued (8 x 1024
+// x 1024 x 64: 602 us with 512, 647 with 256).
+constexpr uint32_t kTargetGroups = 512;
 // Pixels that a thread keeps in registers (one pass). A workgroup's reads are a
 // block's few channels of each pixel, a cache line each: from 4096 pixels on
 // (backward, with three images: 2048) two passes over whole pixels take less,
@@ -396,6 +405,8 @@ __device__ __forceinline__ uint32_t group_of(const Cut& c, uint32_t vec, int g) 
 }
 
 // The first pass: each chunk's (mean less the pivot, squares) for each group.
+// 4 x 1024 x 1024 x 64 bfloat16: 88 us, 6.1 TB/s. A small image's time is that
+// of a launch and of a few loads one after another: 512 x 512 x 64 9.4 us.
 template <typename T, int V, int S>
 __global__ __launch_bounds__(kMaxThreads) void k_gn_stats(const T* x, const Cut c, float2* part) {
     constexpr uint32_t kBatch = kBatchOf<T, V, S>;
@@ -594,8 +605,10 @@ __device__ __forceinline__ uint32_t backwards(uint32_t k, uint32_t n) {
     return k < rounds * 8 ? (rounds - 1 - k / 8) * 8 + k % 8 : k;
 }
 
-// The second pass. It walks the image backwards, each part on the die that
-// read it in the first pass: what was read last may still be in a cache.
+// The second pass; 4 x 1024 x 1024 x 64 bfloat16: 185 us, 5.8 TB/s; 512 x 512 x
+// 64: 14.5 us. It walks the image backwards, each part on the die that
+// read it in the first pass: what was read last may still be in a cache (4 x 256
+// x 256 x 64 float32, both passes: 34.0 us, 36.5 with the dies mixed).
 template <typename T, int V, int S>
 __global__ __launch_bounds__(kMaxThreads) void k_gn_apply(const T* x, const Cut c,
                                                           const float2* part, const Affine aff,
@@ -716,7 +729,8 @@ __device__ __forceinline__ N add_item(const Cut& c, const ItemPlace& at, N s, N 
 }
 
 // Both passes where a block's pixels fit its workgroup's registers: x is read
-// once, in one launch.
+// once, in one launch. 8 x 32 x 32 x 256 bfloat16: 7.5 us, 10.2 in two passes;
+// 16 x 16 x 32 float32: 4.3 and 7.6.
 template <typename T, int V>
 __global__ __launch_bounds__(kItemThreads) void k_gn_item(const T* x, const Cut c,
                                                           const Affine aff, float eps,
@@ -848,7 +862,8 @@ struct Channels {
 };
 
 // The first pass: per chunk the groups' sums of w gz and w gz xh, and for all
-// chunks of a workgroup the channels' sums of gz and gz xh. MANY: it takes every
+// chunks of a workgroup the channels' sums of gz and gz xh. 4 x 1024 x 1024 x 64
+// bfloat16: 177 us, 6.1 TB/s. MANY: it takes every
 // gridDim.x-th chunk of all items'; else it has one.
 template <typename T, int V, int S, bool MANY>
 __global__ __launch_bounds__(kMaxThreads) void k_gn_bwd_sums(const T* gy, const T* x, const Cut c,
@@ -987,8 +1002,8 @@ __global__ __launch_bounds__(kMaxThreads) void k_gn_param_grad(const ParamGrad a
     param_grad(a, blockIdx.x);
 }
 
-// The second pass, backwards like the forward one. The last `extra` workgroups
-// take gw and gb.
+// The second pass, backwards like the forward one; 4 x 1024 x 1024 x 64 bfloat16:
+// 295 us, 5.5 TB/s. The last `extra` workgroups take gw and gb.
 template <typename T, int V, int S>
 __global__ __launch_bounds__(kMaxThreads) void k_gn_bwd_apply(const T* gy, const T* x, const Cut c,
                                                               const Affine aff, uint32_t act,
@@ -1074,7 +1089,8 @@ __global__ __launch_bounds__(kMaxThreads) void k_gn_bwd_apply(const T* gy, const
 
 // Both passes where a block's pixels fit its workgroup's registers. A workgroup
 // takes every gridDim.x-th item; ch_part (null for one workgroup a block: gw
-// and gb are whole then) gets its items' channel sums.
+// and gb are whole then) gets its items' channel sums. 8 x 32 x 32 x 256
+// bfloat16: 11.9 us with the launch that adds them, 15.9 in two passes.
 template <typename T, int V>
 __global__ __launch_bounds__(kItemThreads) void k_gn_bwd_item(
         const T* gy, const T* x, const Cut c, const Affine aff, uint32_t act, const float* mean,

@@ -9,6 +9,7 @@ stream. PyTorch is only the memory/stream provider here.
 from __future__ import annotations
 
 import ctypes as C
+import math
 
 import torch
 
@@ -745,7 +746,11 @@ def _typed(ctx: Context, t: torch.Tensor, name: str) -> int:
 def _pixel_strides(x: torch.Tensor) -> tuple[int, int, int] | None:
     """(pixels of an item, item stride, pixel stride) of [N, ..., C], or None
     where its channels are not neighbours or its pixels not evenly spaced."""
-    shape, stride = x.shape, x.stride()
+    shape = x.shape
+    if x.is_contiguous():
+        n_px = math.prod(shape[1:-1])
+        return n_px, n_px * shape[-1], shape[-1]
+    stride = x.stride()
     if shape[-1] > 1 and stride[-1] != 1:
         return None
     n_px, px_stride = 1, shape[-1]
@@ -765,10 +770,12 @@ def _pixel_strides(x: torch.Tensor) -> tuple[int, int, int] | None:
 def _affine(ctx: Context, c: int, weight, bias) -> int:
     """Checks weight and bias of c channels; their type's code."""
     kind = None
+    if weight is bias is None:
+        return F32
     for t, name in ((weight, "weight"), (bias, "bias")):
         if t is None:
             continue
-        if t.dim() != 1 or t.shape[0] != c:
+        if t.shape != (c,):
             raise ValueError(f"{name} must be [{c}], got {tuple(t.shape)}")
         if not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous")
@@ -777,7 +784,7 @@ def _affine(ctx: Context, c: int, weight, bias) -> int:
             raise TypeError(f"weight is {weight.dtype}, bias {bias.dtype}: they must be of one "
                             "type")
         kind = code
-    return F32 if kind is None else kind
+    return kind
 
 
 def _norm_args(x: torch.Tensor, groups: int, activation: str) -> int:
@@ -841,13 +848,14 @@ def group_norm_bwd(ctx: Context, gy: torch.Tensor, x: torch.Tensor, mean: torch.
     act = _norm_args(x, groups, activation)
     code, aff = _typed(ctx, x, "x"), _affine(ctx, x.shape[-1], weight, bias)
     n, c = x.shape[0], x.shape[-1]
-    if gy.shape != x.shape or gy.dtype != x.dtype or gy.device != x.device:
+    if gy.shape != x.shape or gy.dtype is not x.dtype or gy.get_device() != ctx.device:
         raise ValueError(f"gy must be like x: {x.dtype} {tuple(x.shape)}, got {gy.dtype} "
                          f"{tuple(gy.shape)} on {gy.device}")
     for t, name in ((mean, "mean"), (rstd, "rstd")):
-        _ptr(t, name)
-        if t.shape != (n, groups) or t.device != x.device:
-            raise ValueError(f"{name} must be [{n}, {groups}], got {tuple(t.shape)}")
+        if t.dtype is not torch.float32 or t.shape != (n, groups) or not t.is_contiguous() \
+                or t.get_device() != ctx.device:
+            raise ValueError(f"{name} must be packed float32 [{n}, {groups}] on cuda:{ctx.device}, "
+                             f"got {t.dtype} {tuple(t.shape)} on {t.device}")
     gx = torch.empty_like(x, memory_format=torch.contiguous_format) if need[0] else None
     some = weight if weight is not None else bias
     gw, gb = (None if not wanted else torch.empty(c, dtype=torch.float32, device=x.device)
