@@ -45,10 +45,10 @@ constexpr uint32_t kMinPixels = 2;  // that a thread should have of a chunk
 // x 1024 x 64: 602 us with 512, 647 with 256).
 constexpr uint32_t kTargetGroups = 512;
 // Pixels that a thread keeps in registers (one pass). A workgroup's reads are a
-// block's few channels of each pixel, a cache line each: from 4096 pixels on
+// block's few channels of each pixel, a cache line each: past 4096 pixels
 // (backward, with three images: 2048) two passes over whole pixels take less,
-// 9.6 us against 10.8 for 64 x 64 x 32 float32 backward, 13 against 16 for
-// 64 x 64 x 64 bfloat16.
+// 9.3 us against 10.8 for 64 x 64 x 32 float32 backward, 10.9 against 16 for
+// 64 x 64 x 64 bfloat16; forward they take 8.5 and 9.9 there, one pass 8.0 and 9.1.
 constexpr uint32_t kHold = 8, kHoldBwd = 4;
 constexpr uint32_t kItemThreads = 512;  // of a workgroup that holds its pixels
 
@@ -137,10 +137,9 @@ Cut make_cut(uint32_t n_items, uint64_t n_px, uint32_t n_ch, uint32_t n_groups, 
     return c;
 }
 
-// For one pass: a workgroup holds all pixels of a block, at most kHold vectors a
-// thread; a row's vectors lie in one wave. chunks is 0 where
-// they are too many. Blocks take as many groups as leave 256 workgroups: their
-// reads are longer then.
+// For one pass: a workgroup holds all pixels of a block, at most `hold` vectors a
+// thread; a row's vectors lie in one wave. chunks is 0 where they are too many.
+// Blocks take as many groups as leave 256 workgroups: their reads are longer then.
 Cut make_item_cut(uint32_t n_items, uint64_t n_px, uint32_t n_ch, uint32_t n_groups,
                   uint32_t v, uint32_t hold) {
     const uint64_t most = std::max<uint64_t>(1, (uint64_t)n_items * n_groups / 256);
@@ -257,7 +256,8 @@ __device__ __forceinline__ float sigmoid(float z) {
 }
 // The normal distribution's Phi(z), given e = exp(-z^2 / 2): Abramowitz and
 // Stegun's 7.1.26, erf to 1.5e-7, which is Phi to the rounding of a float near 1.
-// It takes a fifth of a library erf's time and shares e with the density.
+// It shares e with the density (2 x 512 x 512 x 88 float16 backward: 108 us, 159
+// with a library erf beside the exponential).
 __device__ __forceinline__ float gauss_cdf(float z, float e) {
     const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.f));
     float q = fmaf(1.061405429f, t, -1.453152027f);
@@ -863,8 +863,8 @@ struct Channels {
 
 // The first pass: per chunk the groups' sums of w gz and w gz xh, and for all
 // chunks of a workgroup the channels' sums of gz and gz xh. 4 x 1024 x 1024 x 64
-// bfloat16: 177 us, 6.1 TB/s. MANY: it takes every
-// gridDim.x-th chunk of all items'; else it has one.
+// bfloat16: 177 us, 6.1 TB/s. MANY: it takes every gridDim.x-th chunk of all
+// items'; else it has one, and a set of sums less in its registers.
 template <typename T, int V, int S, bool MANY>
 __global__ __launch_bounds__(kMaxThreads) void k_gn_bwd_sums(const T* gy, const T* x, const Cut c,
                                                              const Affine aff, uint32_t act,
@@ -1182,8 +1182,11 @@ __global__ __launch_bounds__(kItemThreads) void k_gn_bwd_item(
 // host
 // ---------------------------------------------------------------------------
 
-// How wide a thread's vectors are: 16 bytes at most, as the channels, the
-// strides and the images' addresses (or-ed) allow. `whole`: a vector that no group's edge cuts.
+// How wide a thread's vectors are: 16 bytes at most, as the channels, the strides
+// and the images' addresses (or-ed) allow. `whole`: that no group's edge cuts. One
+// pass takes whole ones, two passes wider ones where there are (their channels
+// count apart then: 2 x 512 x 512 x 66 bfloat16 in 6 groups, forward: 55 us with
+// vectors of 2 cut by edges, 75 with single channels).
 struct Width {
     uint32_t any, whole;
 };
