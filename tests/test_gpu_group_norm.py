@@ -362,6 +362,29 @@ def test_refusals(ctx):
             K.group_norm_bwd(ctx, gy, x, m, rstd, 2)
 
 
+@pytest.mark.parametrize("c", [8, 520])
+def test_more_items_than_a_launch(ctx, c):
+    """Rows past the first launch's last are those of a call on them alone, and count in the
+    weight's gradients."""
+    from opendressi_amd import ops as K
+    n = 2 ** 22 + 5
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    x = torch.empty((n, c), dtype=torch.bfloat16, device="cuda").normal_(generator=gen)
+    w, b = torch.full((c,), 1.5, device="cuda"), torch.full((c,), 0.5, device="cuda")
+    at = torch.tensor([0, 2 ** 22 - 1, 2 ** 22, n - 1], device="cuda")
+    y, mean, rstd = K.group_norm(ctx, x, 2, w, b, 1e-5, "silu")
+    few = K.group_norm(ctx, x[at], 2, w, b, 1e-5, "silu")
+    for p, q in zip((y, mean, rstd), few):
+        assert torch.equal(p[at], q)
+    del y
+    gx, gw, gb = K.group_norm_bwd(ctx, x, x, mean, rstd, 2, w, b, "none")
+    want = K.group_norm_bwd(ctx, x[at], x[at], *few[1:], 2, w, b, "none")
+    assert torch.equal(gx[at], want[0])
+    # sums of gy, of unit variance: 2^22 roundings of sums of a few thousand in float32
+    col = sum(p.double().sum(0) for p in x.split(2 ** 19))
+    assert ((gb.double() - col).abs() <= 2.0 ** -24 * 2 ** 22).all()
+
+
 def test_past_32_bits(ctx):
     """An image of more than 2^32 values: its ends and the places around the powers of two, and
     the sums over all of it."""
