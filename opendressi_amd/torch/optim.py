@@ -147,6 +147,8 @@ class AdamW(torch.optim.Optimizer):
                     where += 4 * _share(p)
         self._expect = [(p, p.numel(), p.dtype) for p in self._params]
         self._table, self._view, self._total = table, view, at
+        self._fields = view["param"], view["grad"]
+        self._hyper = (AdamwSet * len(self._sets))()
 
     def _check_param(self, p) -> None:
         if not isinstance(p, torch.Tensor):
@@ -252,16 +254,17 @@ class AdamW(torch.optim.Optimizer):
             return loss
         every = len(live) == len(self._expect)
         steps = self._steps
-        if self.capturable:
-            if not (every and self._even):
-                raise RuntimeError("AdamW: a capturable step needs every parameter's gradient")
-            now, table, view = steps, self._table, self._view
-            sets = [(g, 0) for g, _ in self._sets]
-        elif every and self._even:
+        if every and self._even:
             # all in step: a set for each group, as the table has it
-            now = [t + 1 for t in steps]
-            sets = [(g, steps[at] + 1) for g, at in self._sets]
-            table, view = self._table, self._view
+            table, hyper = self._table, self._hyper
+            self._fields[0][:], self._fields[1][:] = params, grads
+            for e, (g, first) in zip(hyper, self._sets):
+                e.lr, e.eps, e.weight_decay = g["lr"], g["eps"], g["weight_decay"]
+                e.beta1, e.beta2 = g["betas"]
+                e.step = steps[first] + 1
+            now = steps if self.capturable else [t + 1 for t in steps]
+        elif self.capturable:
+            raise RuntimeError("AdamW: a capturable step needs every parameter's gradient")
         else:
             now = list(steps)
             index, sets, of = {}, [], []
@@ -272,11 +275,10 @@ class AdamW(torch.optim.Optimizer):
                     sets.append((self._groups[i], now[i]))
                 of.append(k)
             view = self._view[live].copy()
-            view["set"] = of
+            view["set"], view["param"], view["grad"] = of, params, grads
             table = (AdamwTensor * len(live)).from_buffer(view)
-        view["param"], view["grad"] = params, grads
-        hyper = (AdamwSet * len(sets))(*(
-            (g["lr"], *g["betas"], g["eps"], g["weight_decay"], t) for g, t in sets))
+            hyper = (AdamwSet * len(sets))(*(
+                (g["lr"], *g["betas"], g["eps"], g["weight_decay"], t) for g, t in sets))
         ctx = self.ctx
         with ctx.lock:
             ctx._ctx.use_torch_stream()
@@ -318,14 +320,15 @@ class AdamW(torch.optim.Optimizer):
         in bfloat16, which holds them exactly."""
         if self.state_bits == 32:
             return self._moments
-        out = torch.empty((2, self._total), dtype=torch.bfloat16, device=self.ctx.device)
+        m = torch.empty(self._total, dtype=torch.bfloat16, device=self.ctx.device)
+        v = torch.empty_like(m)
         with self.ctx.lock:
             self.ctx._ctx.use_torch_stream()
             check(lib.dressi_adamw_values(
                 self.ctx._ctx.handle, self._total, self._moments[0].data_ptr(),
                 self._moments[1].data_ptr(), _addr(self._scales[0]), _addr(self._scales[1]),
-                out[0].data_ptr(), out[1].data_ptr()))
-        return out[0], out[1]
+                m.data_ptr(), v.data_ptr()))
+        return m, v
 
     def state_dict(self) -> dict:
         """Flat state: "step" (one count a parameter), "exp_avg" and
