@@ -202,9 +202,10 @@ struct Moments {
 template <bool Q8>
 struct RawMoments {
     Pack<float, kLaneElems> m, v;
+    template <bool STREAM>
     __device__ __forceinline__ void load(const State& st, uint64_t i) {
-        m = load_pack<float, kLaneElems>((const float*)st.m + i);
-        v = load_pack<float, kLaneElems>((const float*)st.v + i);
+        m = load_pack<float, kLaneElems, STREAM>((const float*)st.m + i);
+        v = load_pack<float, kLaneElems, STREAM>((const float*)st.v + i);
     }
     __device__ __forceinline__ void clear() { m = v = {}; }
     __device__ __forceinline__ Moments values() const {
@@ -218,9 +219,10 @@ template <>
 struct RawMoments<true> {
     uint32_t m, v;  // four codes each
     uint8_t m_scale, v_scale;
+    template <bool STREAM>
     __device__ __forceinline__ void load(const State& st, uint64_t i) {
-        m = *(const uint32_t*)((const uint8_t*)st.m + i);
-        v = *(const uint32_t*)((const uint8_t*)st.v + i);
+        m = load_as<STREAM>((const uint32_t*)((const uint8_t*)st.m + i));
+        v = load_as<STREAM>((const uint32_t*)((const uint8_t*)st.v + i));
         m_scale = st.m_scale[i / kBlock];
         v_scale = st.v_scale[i / kBlock];
     }
@@ -240,7 +242,7 @@ struct RawMoments<true> {
 
 // All 64 lanes call this together (the block's maximum crosses lanes); `live`
 // says which hold elements.
-template <bool Q8>
+template <bool Q8, bool STREAM>
 __device__ __forceinline__ void store_moments(const State& st, uint64_t i, const Moments& o,
                                               uint32_t key, bool live) {
     if constexpr (Q8) {
@@ -265,16 +267,16 @@ __device__ __forceinline__ void store_moments(const State& st, uint64_t i, const
             cv |= b << (8 * j);
         }
         if (live) {
-            *(uint32_t*)((uint8_t*)st.m + i) = cm;
-            *(uint32_t*)((uint8_t*)st.v + i) = cv;
+            store_as<STREAM>((uint32_t*)((uint8_t*)st.m + i), cm);
+            store_as<STREAM>((uint32_t*)((uint8_t*)st.v + i), cv);
             if ((threadIdx.x & 7u) == 0) {
                 st.m_scale[i / kBlock] = (uint8_t)fm;
                 st.v_scale[i / kBlock] = (uint8_t)fv;
             }
         }
     } else if (live) {
-        store_vec<float, kLaneElems>((float*)st.m + i, o.m);
-        store_vec<float, kLaneElems>((float*)st.v + i, o.v);
+        store_vec<float, kLaneElems, STREAM>((float*)st.m + i, o.m);
+        store_vec<float, kLaneElems, STREAM>((float*)st.v + i, o.v);
     }
 }
 
@@ -303,8 +305,9 @@ __device__ __forceinline__ float newest(float param, float master) {
 }
 
 // A chunk of one tensor. FULL: all of its elements are there and aligned for
-// a lane's vector loads, which are all issued before the first is used.
-template <typename T, bool Q8, int ITER, bool FULL>
+// a lane's vector loads, which are all issued before the first is used. STREAM:
+// a FULL chunk's go past the caches.
+template <typename T, bool Q8, int ITER, bool FULL, bool STREAM>
 __device__ __forceinline__ void step_chunk(const TensorArg& t, const SetArg& h, const State& st,
                                            uint64_t at, float coef, bool clip) {
     constexpr uint32_t kStep = kThreads * kLaneElems;
@@ -319,12 +322,12 @@ __device__ __forceinline__ void step_chunk(const TensorArg& t, const SetArg& h, 
     for (int k = 0; k < ITER; k++) {
         const uint64_t i = at + (uint64_t)k * kStep + threadIdx.x * kLaneElems;
         if (FULL) {
-            gv[k] = load_pack<T, kLaneElems>(g + i);
-            pv[k] = load_pack<T, kLaneElems>(p + i);
+            gv[k] = load_pack<T, kLaneElems, STREAM>(g + i);
+            pv[k] = load_pack<T, kLaneElems, STREAM>(p + i);
             if (wide) {
-                mv[k] = load_pack<float, kLaneElems>(t.master + i);
+                mv[k] = load_pack<float, kLaneElems, STREAM>(t.master + i);
             }
-            raw[k].load(st, t.state + i);
+            raw[k].template load<STREAM>(st, t.state + i);
         } else {
 #pragma unroll
             for (uint32_t j = 0; j < kLaneElems; j++) {
@@ -335,7 +338,7 @@ __device__ __forceinline__ void step_chunk(const TensorArg& t, const SetArg& h, 
             }
             raw[k].clear();
             if (i < padded) {  // a share is padded with zeros to whole blocks
-                raw[k].load(st, t.state + i);
+                raw[k].template load<false>(st, t.state + i);
             }
         }
     }
@@ -359,11 +362,11 @@ __device__ __forceinline__ void step_chunk(const TensorArg& t, const SetArg& h, 
                 }
             }
         }
-        store_moments<Q8>(st, t.state + i, o, h.key, FULL || i < padded);
+        store_moments<Q8, STREAM>(st, t.state + i, o, h.key, FULL || i < padded);
         if (FULL) {
-            store_vec<T, kLaneElems>(p + i, px);
+            store_vec<T, kLaneElems, STREAM>(p + i, px);
             if (wide) {
-                store_vec<float, kLaneElems>(t.master + i, px);
+                store_vec<float, kLaneElems, STREAM>(t.master + i, px);
             }
         } else {
 #pragma unroll
@@ -379,24 +382,24 @@ __device__ __forceinline__ void step_chunk(const TensorArg& t, const SetArg& h, 
     }
 }
 
-template <typename T, bool Q8, int ITER>
+template <typename T, bool Q8, int ITER, bool STREAM>
 __device__ __forceinline__ void step_tensor(const TensorArg& t, const SetArg& h, const State& st,
                                             uint64_t at, float coef, bool clip) {
     constexpr uintptr_t kMask = kLaneElems * sizeof(T) - 1;
     const bool vec = (((uintptr_t)t.param | (uintptr_t)t.grad) & kMask) == 0;
     if (vec && at + (uint64_t)ITER * kThreads * kLaneElems <= t.n) {
-        step_chunk<T, Q8, ITER, true>(t, h, st, at, coef, clip);
+        step_chunk<T, Q8, ITER, true, STREAM>(t, h, st, at, coef, clip);
     } else {
-        step_chunk<T, Q8, ITER, false>(t, h, st, at, coef, clip);
+        step_chunk<T, Q8, ITER, false, false>(t, h, st, at, coef, clip);
     }
 }
 
 // A workgroup per chunk of 1024 ITER elements of one tensor: everything is
-// read and written once, so memory bounds it. 2^28 float32 elements take 1387 us
-// with moments in 32 bits (28 bytes each, 5.4 TB/s) and 785 in 8 (16.1 bytes, 5.5
+// read and written once, so memory bounds it. 2^28 float32 elements take 1315 us
+// with moments in 32 bits (28 bytes each, 5.7 TB/s) and 770 in 8 (16.1 bytes, 5.6
 // TB/s; counters: 2.72 GB read, 1.63 written, which is what there is); 2 million,
 // clipped, 5.6 us for the norm and 11 for the step; three small tensors 3.2.
-template <bool Q8, int ITER>
+template <bool Q8, int ITER, bool STREAM>
 __global__ __launch_bounds__(256) void k_adamw_step(const Table tb, const State st) {
     float coef = 1.f;
     const bool clip = st.partials != nullptr;
@@ -418,13 +421,13 @@ __global__ __launch_bounds__(256) void k_adamw_step(const Table tb, const State 
     const uint64_t at = (uint64_t)(blockIdx.x - t.first_chunk) * (ITER * kThreads * kLaneElems);
     switch (t.type) {
         case DRESSI_F32:
-            step_tensor<float, Q8, ITER>(t, h, st, at, coef, clip);
+            step_tensor<float, Q8, ITER, STREAM>(t, h, st, at, coef, clip);
             break;
         case DRESSI_BF16:
-            step_tensor<bf16, Q8, ITER>(t, h, st, at, coef, clip);
+            step_tensor<bf16, Q8, ITER, STREAM>(t, h, st, at, coef, clip);
             break;
         default:
-            step_tensor<f16, Q8, ITER>(t, h, st, at, coef, clip);
+            step_tensor<f16, Q8, ITER, STREAM>(t, h, st, at, coef, clip);
     }
 }
 
@@ -460,7 +463,7 @@ __global__ __launch_bounds__(256) void k_adamw_values(const State st, uint64_t n
     const uint64_t i = ((uint64_t)blockIdx.x * kThreads + threadIdx.x) * kLaneElems;
     if (i < n) {
         RawMoments<true> raw;
-        raw.load(st, i);
+        raw.load<false>(st, i);
         const Moments o = raw.values();
         store_vec<bf16, kLaneElems>(m + i, o.m);
         store_vec<bf16, kLaneElems>(v + i, o.v);
@@ -469,11 +472,17 @@ __global__ __launch_bounds__(256) void k_adamw_values(const State st, uint64_t n
 
 // Elements up to which a workgroup takes 1024 of them, else 4096 (8-bit moments,
 // which take more registers: 2048): more workgroups against more loads in flight
-// in each. 8-bit moments take 25.7 us so and 27.8 with 4096 at 2^23 elements, 802
-// and 779 at 2^28 (bfloat16 parameters, 2^27: 448 us with 2048, 451 with 4096);
-// 32-bit ones the same at 2^22, and 4096 leaves a quarter of the sums of a clipped
-// norm (61 and 54 us at 2^23).
+// in each. 8-bit moments take 25.7 us so and 27.8 with 4096 at 2^23 elements, and
+// the two are level at 2^28; 32-bit ones are at 2^22, and 4096 leaves a quarter
+// of the sums of a clipped norm (61 and 54 us at 2^23, both through the caches).
 constexpr uint64_t kSmallTotal = 1ull << 20, kSmallTotal8 = 1ull << 23;
+
+// Bytes of a step from which they go past the caches (256 MB the last), which hold
+// less and less of them for the next one. Past them and through them: 117 MB 21.8
+// and 19.4 us, 235 MB clipped 46.7 and 54.0, 940 MB 157 and 175, 7.5 GB 1315 and
+// 1396; bfloat16 with 2^27 elements, 32-bit moments and clipped 730 and 829, 8-bit
+// 422 and 446.
+constexpr uint64_t kStreamBytes = 160ull << 20;
 
 int check_tensors(const dressi_adamw_tensor* t, uint32_t n, uint32_t n_sets, uint64_t state_elems) {
     for (uint32_t i = 0; i < n; i++) {
@@ -597,9 +606,11 @@ int dressi_adamw_step(dressi_ctx* ctx, const dressi_adamw_tensor* tensors, uint3
     if (int rc = check_tensors(tensors, n_tensors, n_sets, state_elems)) {
         return rc;
     }
-    uint64_t total = 0;
+    uint64_t total = 0, bytes = 0;  // elements, and what is read and written of them
     for (uint32_t i = 0; i < n_tensors; i++) {
         total += tensors[i].n;
+        const bool wide = tensors[i].type != DRESSI_F32 && tensors[i].master;
+        bytes += tensors[i].n * (3 * type_bytes(tensors[i].type) + (wide ? 8 : 0) + (q8 ? 4 : 16));
     }
     for (uint32_t i = 0; i < n_sets; i++) {
         if (int rc = check_set(sets[i], i, steps != nullptr)) {
@@ -610,6 +621,7 @@ int dressi_adamw_step(dressi_ctx* ctx, const dressi_adamw_tensor* tensors, uint3
         return clip ? launch_zero(ctx->stream, norm, sizeof(float)) : DRESSI_OK;
     }
     const bool small = total <= (q8 ? kSmallTotal8 : kSmallTotal);
+    const bool stream = bytes >= kStreamBytes;
     const uint32_t iter = small ? 1 : q8 ? 2 : 4;
     const uint32_t chunk = kThreads * kLaneElems * iter;
     for (uint32_t i = 0; on_device && i < n_sets; i++) {
@@ -647,8 +659,11 @@ int dressi_adamw_step(dressi_ctx* ctx, const dressi_adamw_tensor* tensors, uint3
         st.n_partials = used;
     }
     return for_batches(tensors, n_tensors, sets, on_device, seed, chunk, [&](const Table& tb) -> int {
-        const auto step = q8 ? (small ? k_adamw_step<true, 1> : k_adamw_step<true, 2>)
-                             : (small ? k_adamw_step<false, 1> : k_adamw_step<false, 4>);
+        const auto step =
+            q8 ? (small ? k_adamw_step<true, 1, false>
+                  : stream ? k_adamw_step<true, 2, true> : k_adamw_step<true, 2, false>)
+               : (small ? k_adamw_step<false, 1, false>
+                  : stream ? k_adamw_step<false, 4, true> : k_adamw_step<false, 4, false>);
         hipLaunchKernelGGL(step, dim3(tb.n_chunks), dim3(kThreads), 0, ctx->stream, tb, st);
         DRESSI_CHECK_LAUNCH();
         return DRESSI_OK;

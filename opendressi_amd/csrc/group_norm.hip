@@ -73,6 +73,7 @@ struct Cut {
     uint32_t chunks;     // of an item
     uint32_t chunk_px;
     uint32_t stream;     // results go past the caches
+    uint32_t keep_px;    // of a chunk, its last: what the first pass leaves in a cache
 
     // vectors of a block, and its first
     __host__ __device__ uint32_t first_vec(uint32_t b) const {
@@ -383,11 +384,18 @@ __device__ __forceinline__ void add_batch(const Pack<T, V> (&v)[B], uint32_t cou
 
 // B of a thread's pixels, `stride` elements apart; past `count` the last again.
 template <typename T, int V, int B>
-__device__ __forceinline__ void load_batch(const T* p, size_t stride, uint32_t count,
+__device__ __forceinline__ void load_batch(const T* p, size_t stride, uint32_t count, bool stream,
                                            Pack<T, V> (&v)[B]) {
+    if (stream) {
 #pragma unroll
-    for (uint32_t k = 0; k < B; k++) {
-        v[k] = load_pack<T, V>(p + (k < count ? k : count - 1) * stride);
+        for (uint32_t k = 0; k < B; k++) {
+            v[k] = load_pack<T, V, true>(p + (k < count ? k : count - 1) * stride);
+        }
+    } else {
+#pragma unroll
+        for (uint32_t k = 0; k < B; k++) {
+            v[k] = load_pack<T, V>(p + (k < count ? k : count - 1) * stride);
+        }
     }
 }
 
@@ -405,8 +413,8 @@ __device__ __forceinline__ uint32_t group_of(const Cut& c, uint32_t vec, int g) 
 }
 
 // The first pass: each chunk's (mean less the pivot, squares) for each group.
-// 4 x 1024 x 1024 x 64 bfloat16: 88 us, 6.1 TB/s. A small image's time is that
-// of a launch and of a few loads one after another: 512 x 512 x 64 9.4 us.
+// 4 x 1024 x 1024 x 64 bfloat16: 82 us, 6.6 TB/s. A small image's time is that
+// of a launch and of a few loads one after another: 512 x 512 x 64 10 us.
 template <typename T, int V, int S>
 __global__ __launch_bounds__(kMaxThreads) void k_gn_stats(const T* x, const Cut c, float2* part) {
     constexpr uint32_t kBatch = kBatchOf<T, V, S>;
@@ -429,10 +437,11 @@ __global__ __launch_bounds__(kMaxThreads) void k_gn_stats(const T* x, const Cut 
         for (int g = 0; g < S; g++) {
             pivot[g] = pivot_of(x, c, item, group_of<V, S>(c, vec, g));
         }
+        const uint32_t keep = c.keep_px / c.rows;
         uint32_t count = left % kBatch ? left % kBatch : kBatch;
         while (left > 0) {
             Pack<T, V> v[kBatch];
-            load_batch<T, V, kBatch>(p, step, count, v);
+            load_batch<T, V, kBatch>(p, step, count, left > keep, v);
             add_batch<T, V, S, kBatch>(v, count, pivot, n, mean, m2);
             left -= count;
             p += count * step;
@@ -523,7 +532,7 @@ __device__ __forceinline__ void join_chunks(const T* x, const Cut& c, uint32_t i
     __syncthreads();
 }
 
-__device__ __forceinline__ void store_as(void* p, uint32_t type, size_t i, float x) {
+__device__ __forceinline__ void store_one(void* p, uint32_t type, size_t i, float x) {
     if (type == DRESSI_F32) {
         ((float*)p)[i] = x;
     } else if (type == DRESSI_BF16) {
@@ -577,7 +586,7 @@ __device__ __forceinline__ void load_affine(const Affine& a, uint32_t ch, float 
 template <typename T, int V>
 __device__ __forceinline__ void put(T* p, const float (&x)[V], uint32_t stream) {
     if (stream) {
-        stream_vec<T, V>(p, x);
+        store_vec<T, V, true>(p, x);
     } else {
         store_vec<T, V>(p, x);
     }
@@ -605,8 +614,8 @@ __device__ __forceinline__ uint32_t backwards(uint32_t k, uint32_t n) {
     return k < rounds * 8 ? (rounds - 1 - k / 8) * 8 + k % 8 : k;
 }
 
-// The second pass; 4 x 1024 x 1024 x 64 bfloat16: 185 us, 5.8 TB/s; 512 x 512 x
-// 64: 14.5 us. It walks the image backwards, each part on the die that
+// The second pass; 4 x 1024 x 1024 x 64 bfloat16: 191 us, 5.6 TB/s; 512 x 512 x
+// 64: 14.6 us. It walks the image backwards, each part on the die that
 // read it in the first pass: what was read last may still be in a cache (4 x 256
 // x 256 x 64 float32, both passes: 34.0 us, 36.5 with the dies mixed).
 template <typename T, int V, int S>
@@ -628,9 +637,10 @@ __global__ __launch_bounds__(kMaxThreads) void k_gn_apply(const T* x, const Cut 
     // the first batch and the weights are on their way while the chunks are joined
     Pack<T, V> v[kBatch];
     uint32_t count = left < kBatch ? left : kBatch;
+    const uint32_t all = left, keep = c.keep_px / c.rows;
     float w[V], b[V], mean[S];
     if (left > 0) {
-        load_batch<T, V, kBatch>(p + (left - count) * step, step, count, v);
+        load_batch<T, V, kBatch>(p + (left - count) * step, step, count, keep == 0, v);
         load_affine<V>(aff, vec * V, w, b);
     }
     join_chunks<T, V>(x, c, item, part, eps, stat);
@@ -664,7 +674,7 @@ __global__ __launch_bounds__(kMaxThreads) void k_gn_apply(const T* x, const Cut 
             break;
         }
         count = left < kBatch ? left : kBatch;
-        load_batch<T, V, kBatch>(p + (left - count) * step, step, count, v);
+        load_batch<T, V, kBatch>(p + (left - count) * step, step, count, all - left >= keep, v);
     }
 }
 
@@ -863,7 +873,7 @@ struct Channels {
 
 // The first pass: per chunk the groups' sums of w gz and w gz xh, and for all
 // chunks of a workgroup the channels' sums of gz and gz xh. 4 x 1024 x 1024 x 64
-// bfloat16: 177 us, 6.1 TB/s. MANY: it takes every gridDim.x-th chunk of all
+// bfloat16: 169 us, 6.4 TB/s. MANY: it takes every gridDim.x-th chunk of all
 // items'; else it has one, and a set of sums less in its registers.
 template <typename T, int V, int S, bool MANY>
 __global__ __launch_bounds__(kMaxThreads) void k_gn_bwd_sums(const T* gy, const T* x, const Cut c,
@@ -895,11 +905,12 @@ __global__ __launch_bounds__(kMaxThreads) void k_gn_bwd_sums(const T* gy, const 
             const size_t px0 = (size_t)chunk * c.chunk_px + at.row;
             const T* p = x + (size_t)item * c.item_stride + px0 * c.px_stride + (size_t)vec * V;
             const T* q = gy + ((size_t)item * c.n_px + px0) * c.n_ch + (size_t)vec * V;
+            const uint32_t keep = c.keep_px / c.rows;
             uint32_t count = left % kBatchBwd ? left % kBatchBwd : kBatchBwd;
             while (left > 0) {
                 Pack<T, V> xv[kBatchBwd], gv[kBatchBwd];
-                load_batch<T, V, kBatchBwd>(p, step, count, xv);
-                load_batch<T, V, kBatchBwd>(q, qstep, count, gv);
+                load_batch<T, V, kBatchBwd>(p, step, count, left > keep, xv);
+                load_batch<T, V, kBatchBwd>(q, qstep, count, left > keep, gv);
 #pragma unroll
                 for (uint32_t k = 0; k < kBatchBwd; k++) {
                     if (k < count) {
@@ -990,10 +1001,10 @@ __device__ __forceinline__ void param_grad(const ParamGrad& a, uint32_t block) {
             s.y += sum[r][lane].y;
         }
         if (a.gb) {
-            store_as(a.gb, a.type, ch, (float)s.x);
+            store_one(a.gb, a.type, ch, (float)s.x);
         }
         if (a.gw) {
-            store_as(a.gw, a.type, ch, (float)s.y);
+            store_one(a.gw, a.type, ch, (float)s.y);
         }
     }
 }
@@ -1003,7 +1014,7 @@ __global__ __launch_bounds__(kMaxThreads) void k_gn_param_grad(const ParamGrad a
 }
 
 // The second pass, backwards like the forward one; 4 x 1024 x 1024 x 64 bfloat16:
-// 295 us, 5.5 TB/s. The last `extra` workgroups take gw and gb.
+// 284 us, 5.7 TB/s. The last `extra` workgroups take gw and gb.
 template <typename T, int V, int S>
 __global__ __launch_bounds__(kMaxThreads) void k_gn_bwd_apply(const T* gy, const T* x, const Cut c,
                                                               const Affine aff, uint32_t act,
@@ -1033,10 +1044,11 @@ __global__ __launch_bounds__(kMaxThreads) void k_gn_bwd_apply(const T* gy, const
     const size_t step = (size_t)c.rows * c.px_stride, qstep = (size_t)c.rows * c.n_ch;
     Pack<T, V> xv[kBatchBwd], gv[kBatchBwd];
     uint32_t count = left < kBatchBwd ? left : kBatchBwd;
+    const uint32_t all = left, keep = c.keep_px / c.rows;
     Channels<V, S> ch;
     if (left > 0) {
-        load_batch<T, V, kBatchBwd>(p + (left - count) * step, step, count, xv);
-        load_batch<T, V, kBatchBwd>(q + (left - count) * qstep, qstep, count, gv);
+        load_batch<T, V, kBatchBwd>(p + (left - count) * step, step, count, keep == 0, xv);
+        load_batch<T, V, kBatchBwd>(q + (left - count) * qstep, qstep, count, keep == 0, gv);
         ch.load(c, aff, item, vec, mean, rstd);
     }
     {
@@ -1082,8 +1094,9 @@ __global__ __launch_bounds__(kMaxThreads) void k_gn_bwd_apply(const T* gy, const
             break;
         }
         count = left < kBatchBwd ? left : kBatchBwd;
-        load_batch<T, V, kBatchBwd>(p + (left - count) * step, step, count, xv);
-        load_batch<T, V, kBatchBwd>(q + (left - count) * qstep, qstep, count, gv);
+        const bool past = all - left >= keep;
+        load_batch<T, V, kBatchBwd>(p + (left - count) * step, step, count, past, xv);
+        load_batch<T, V, kBatchBwd>(q + (left - count) * qstep, qstep, count, past, gv);
     }
 }
 
@@ -1170,10 +1183,10 @@ __global__ __launch_bounds__(kItemThreads) void k_gn_bwd_item(
             return;
         }
         if (gb) {
-            store_as(gb, aff.type, ch0 + k, s.x);
+            store_one(gb, aff.type, ch0 + k, s.x);
         }
         if (gw) {
-            store_as(gw, aff.type, ch0 + k, s.y);
+            store_one(gw, aff.type, ch0 + k, s.y);
         }
     });
 }
@@ -1228,6 +1241,13 @@ Scratch scratch_of(const Cut& c, bool whole, bool backward) {
 // 512 x 512 x 64; with a pass after it that reads the result 125 and 127, 37 and 37.
 constexpr uint64_t kStreamBytes = 32ull << 20;
 
+// Bytes of the first pass's reads that the second may find in the last-level cache
+// (256 MB): the ends of the chunks. The rest goes past it both times: 8 x 1024 x
+// 1024 x 64 bfloat16 574 us forward and 894 backward, 586 and 983 with all of it
+// through the caches; all past them 1024 x 1024 x 64 takes 80 us forward, not 73.
+// 96 and 224 MB kept measure the same.
+constexpr uint64_t kKeepBytes = 160ull << 20;
+
 // How a call is cut: in one pass if it can be.
 struct Plan {
     Cut c;
@@ -1235,7 +1255,8 @@ struct Plan {
     bool whole, split;
 };
 Plan make_plan(uint32_t type, uint32_t n_items, uint64_t n_px, uint32_t n_ch, uint64_t item_stride,
-               uint64_t px_stride, uint32_t n_groups, uint64_t addresses, uint32_t hold) {
+               uint64_t px_stride, uint32_t n_groups, uint64_t addresses, uint32_t hold,
+               uint32_t images) {
     const Width w = vec_width(type, n_ch, n_groups, n_items > 1 ? item_stride : 0,
                               n_px > 1 ? px_stride : 0, addresses);
     Plan p;
@@ -1250,7 +1271,11 @@ Plan make_plan(uint32_t type, uint32_t n_items, uint64_t n_px, uint32_t n_ch, ui
     }
     p.c.item_stride = item_stride;
     p.c.px_stride = px_stride;
-    p.c.stream = (uint64_t)n_items * n_px * n_ch * type_bytes(type) >= kStreamBytes;
+    const uint64_t bytes = (uint64_t)n_items * n_px * n_ch * type_bytes(type);
+    p.c.stream = bytes >= kStreamBytes;
+    const uint64_t again = bytes * images;  // of the second pass's reads
+    p.c.keep_px = again <= kKeepBytes ? p.c.chunk_px
+                                      : (uint32_t)(p.c.chunk_px * ((double)kKeepBytes / again));
     return p;
 }
 
@@ -1390,7 +1415,7 @@ size_t dressi_group_norm_scratch(uint32_t type, uint32_t n_items, uint64_t n_px,
         return 0;
     }
     const Plan p = make_plan(type, n_items, n_px, n_ch, item_stride, px_stride, n_groups,
-                             addresses, backward ? kHoldBwd : kHold);
+                             addresses, backward ? kHoldBwd : kHold, backward ? 2 : 1);
     return scratch_of(p.c, p.whole, backward != 0).bytes;
 }
 
@@ -1413,7 +1438,7 @@ int dressi_group_norm(dressi_ctx* ctx, const void* x, uint32_t type, uint32_t n_
     const uint64_t addresses = (uintptr_t)x | (uintptr_t)y;
     DRESSI_REQUIRE(addresses % type_bytes(type) == 0, "group_norm: not aligned to its type");
     const Plan p = make_plan(type, n_items, n_px, n_ch, item_stride, px_stride, n_groups,
-                             addresses, kHold);
+                             addresses, kHold, 1);
     const size_t need = scratch_of(p.c, p.whole, false).bytes;
     DRESSI_REQUIRE(need == 0 || (scratch && scratch_bytes >= need), "group_norm: scratch too small");
     return for_width(type, p.v, [&](auto w) {
@@ -1454,7 +1479,7 @@ int dressi_group_norm_bwd(dressi_ctx* ctx, const void* gy, const void* x, uint32
     const uint64_t addresses = (uintptr_t)gy | (uintptr_t)x | (uintptr_t)gx;
     DRESSI_REQUIRE(addresses % type_bytes(type) == 0, "group_norm_bwd: not aligned to its type");
     const Plan p = make_plan(type, n_items, n_px, n_ch, item_stride, px_stride, n_groups,
-                             addresses, kHoldBwd);
+                             addresses, kHoldBwd, 2);
     DRESSI_REQUIRE(scratch && scratch_bytes >= scratch_of(p.c, p.whole, true).bytes,
                    "group_norm_bwd: scratch too small");
     return for_width(type, p.v, [&](auto w) {

@@ -29,11 +29,40 @@ struct alignas(sizeof(T) * V) Pack {
     T v[V];
 };
 
+// The widest words that make up N bytes.
+template <size_t N>
+using Words = std::conditional_t<N % 4 == 0, uint32_t, std::conditional_t<N % 2 == 0, uint16_t, uint8_t>>
+    __attribute__((ext_vector_type(N % 4 == 0 ? N / 4 : N % 2 == 0 ? N / 2 : N)));
+
+// Memory that is not used again soon (`STREAM`) goes past the caches, so that it
+// does not drive out what is.
+template <bool STREAM, typename P>
+__device__ __forceinline__ P load_as(const P* p) {
+    if constexpr (STREAM) {
+        const Words<sizeof(P)> w = __builtin_nontemporal_load((const Words<sizeof(P)>*)p);
+        P a;
+        __builtin_memcpy(&a, &w, sizeof(P));
+        return a;
+    } else {
+        return *p;
+    }
+}
+template <bool STREAM, typename P>
+__device__ __forceinline__ void store_as(P* p, const P& a) {
+    if constexpr (STREAM) {
+        Words<sizeof(P)> w;
+        __builtin_memcpy(&w, &a, sizeof(P));
+        __builtin_nontemporal_store(w, (Words<sizeof(P)>*)p);
+    } else {
+        *p = a;
+    }
+}
+
 // V neighbours in one load, as they lie in memory: held so, 16 bytes take four
 // registers where floats take eight. `p` aligned to all of them.
-template <typename T, int V>
+template <typename T, int V, bool STREAM = false>
 __device__ __forceinline__ Pack<T, V> load_pack(const T* p) {
-    return *(const Pack<T, V>*)p;
+    return load_as<STREAM>((const Pack<T, V>*)p);
 }
 template <typename T, int V>
 __device__ __forceinline__ void unpack(const Pack<T, V>& a, float (&x)[V]) {
@@ -46,36 +75,20 @@ __device__ __forceinline__ void unpack(const Pack<T, V>& a, float (&x)[V]) {
 // V neighbours in one load or store; `p` aligned to all of them.
 template <typename T, int V>
 __device__ __forceinline__ void load_vec(const T* p, float* x) {
-    const Pack<T, V> a = *(const Pack<T, V>*)p;
+    const Pack<T, V> a = load_pack<T, V>(p);
 #pragma unroll
     for (int i = 0; i < V; i++) {
         x[i] = to_float(a.v[i]);
     }
 }
-template <typename T, int V>
+template <typename T, int V, bool STREAM = false>
 __device__ __forceinline__ void store_vec(T* p, const float* x) {
     Pack<T, V> a;
 #pragma unroll
     for (int i = 0; i < V; i++) {
         a.v[i] = from_float<T>(x[i]);
     }
-    *(Pack<T, V>*)p = a;
-}
-
-// The same for what is not read again soon: it goes past the caches.
-template <typename T, int V>
-__device__ __forceinline__ void stream_vec(T* p, const float* x) {
-    Pack<T, V> a;
-#pragma unroll
-    for (int i = 0; i < V; i++) {
-        a.v[i] = from_float<T>(x[i]);
-    }
-    using Word = std::conditional_t<sizeof(a) % 4 == 0, uint32_t, uint16_t>;
-    constexpr int kWords = sizeof(a) / sizeof(Word);
-    typedef Word Words __attribute__((ext_vector_type(kWords)));
-    Words w;
-    __builtin_memcpy(&w, &a, sizeof(a));
-    __builtin_nontemporal_store(w, (Words*)p);
+    store_as<STREAM>((Pack<T, V>*)p, a);
 }
 
 inline size_t type_bytes(uint32_t type) { return type == DRESSI_F32 ? 4 : 2; }

@@ -194,6 +194,51 @@ def test_large_8_bit(ctx, kind):
         assert np.array_equal(_np(v[a:b]), want_v[:b - a].astype(F32))
 
 
+@pytest.mark.parametrize("kind", TYPES, ids=str)
+def test_larger_than_a_cache(ctx, kind):
+    """A step of several hundred MB does to each stretch what a step on that stretch alone does."""
+    import opendressi_amd.torch as dr
+    n, cut = 12 * 2 ** 20 + 1029, 3 * 2 ** 20
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    p = torch.randn(n, generator=gen, device="cuda").to(kind)
+    parts = [torch.nn.Parameter(q.clone()) for q in p.split(cut)]
+    opt = dr.AdamW(ctx, [p], lr=1e-2)
+    opts = [dr.AdamW(ctx, [q], lr=1e-2) for q in parts]
+    for _ in range(2):
+        g = torch.randn(n, generator=gen, device="cuda").to(kind)
+        p.grad = g
+        opt.step()
+        for q, h, o in zip(parts, g.split(cut), opts):
+            q.grad = h.clone()
+            o.step()
+    assert torch.equal(p, torch.cat([q.detach() for q in parts]))
+    for i, m in enumerate(opt.moments()):
+        assert torch.equal(m, torch.cat([o.moments()[i] for o in opts]))
+
+
+def test_larger_than_a_cache_8_bit(ctx):
+    """The codes of a second step over several hundred MB, against the rounding in numpy."""
+    import opendressi_amd.torch as dr
+    n, b1, b2 = 12 * 2 ** 20 + 1029, F32(0.9), F32(0.999)
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    p = torch.randn(n, generator=gen, device="cuda")
+    opt = dr.AdamW(ctx, [p], lr=1e-2, state_bits=8)
+    was = [torch.zeros(n, device="cuda")] * 2
+    for t in (1, 2):
+        p.grad = torch.randn(n, generator=gen, device="cuda")
+        opt.step()
+        m, v = opt.moments()
+        for a, b in ((0, 320), (2 ** 23 - 64, 2 ** 23 + 64), (n - 1029, n)):
+            g = _np(p.grad[a:b])
+            r = _mix(range(a, b), t)
+            want_m = _rounded(_np(was[0][a:b]) * b1 + g * F32(1 - 0.9), 14, ((r & 0xffff) << 4) + 8)
+            want_v = _rounded(_np(was[1][a:b]) * b2 + (g * g) * F32(1 - 0.999), 30,
+                              ((r >> 16) << 4) + 8)
+            assert np.array_equal(_np(m[a:b]), want_m[:b - a].astype(F32))
+            assert np.array_equal(_np(v[a:b]), want_v[:b - a].astype(F32))
+        was = [m.clone(), v.clone()]
+
+
 def test_8_bit_moments_follow(ctx):
     """The slow moment moves by 0.1 % a step, a fraction of its code's step. Under a constant
     gradient v = g^2 (1 - b2^t); the rounding being unbiased, the mean over 2^16 elements follows.

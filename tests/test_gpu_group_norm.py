@@ -157,6 +157,16 @@ def test_many_items(ctx, shape, groups, kind):
     _check(x, gy, w, b, groups, 1e-5, "silu", _run(ctx, x, gy, w, b, groups, 1e-5, "silu"))
 
 
+@pytest.mark.parametrize("shape,groups,kind", [((1, 1111, 1200, 64), 8, torch.bfloat16),
+                                               ((2, 700, 1031, 66), 6, torch.float16),
+                                               ((3, 401, 1031, 41), 41, torch.float32)], ids=str)
+def test_larger_than_a_cache(ctx, shape, groups, kind):
+    """Images of which the second pass finds only the last part where the first left it."""
+    print(f"[group_norm large] {shape} {groups} {kind}", flush=True)
+    x, gy, w, b = _inputs(shape, kind, 14)
+    _check(x, gy, w, b, groups, 1e-5, "silu", _run(ctx, x, gy, w, b, groups, 1e-5, "silu"))
+
+
 @pytest.mark.parametrize("offset", [0.0, 300.0, -3e4])
 @pytest.mark.parametrize("shape,groups", [((2, 64, 65, 32), 4), ((1, 30, 30, 5), 1),
                                           ((1, 300, 300, 8), 1)], ids=str)
