@@ -457,16 +457,32 @@ __global__ __launch_bounds__(64) void k_adamw_tick(const dressi_adamw_set set, u
 }
 
 // The values that 8-bit moments stand for, as bfloat16 (which holds them all:
-// three mantissa bits). 4 elements a lane.
+// three mantissa bits). Two times 4 elements a lane; the values go past the caches
+// (2^23 elements and a sum of both after them: 19.5 us, 20 through the caches), and
+// so do the codes if they are too many for one (`STREAM`): 2^28 elements take 254
+// us so (6.4 TB/s), 289 through them and 331 with 4 elements a lane; 2^26, whose
+// codes a cache holds, 64 us past it and 59 through it.
+constexpr uint32_t kValuesIter = 2;
+template <bool STREAM>
 __global__ __launch_bounds__(256) void k_adamw_values(const State st, uint64_t n, bf16* m,
                                                       bf16* v) {
-    const uint64_t i = ((uint64_t)blockIdx.x * kThreads + threadIdx.x) * kLaneElems;
-    if (i < n) {
-        RawMoments<true> raw;
-        raw.load<false>(st, i);
-        const Moments o = raw.values();
-        store_vec<bf16, kLaneElems>(m + i, o.m);
-        store_vec<bf16, kLaneElems>(v + i, o.v);
+    constexpr uint32_t kStep = kThreads * kLaneElems;
+    const uint64_t at = (uint64_t)blockIdx.x * (kStep * kValuesIter) + threadIdx.x * kLaneElems;
+    RawMoments<true> raw[kValuesIter];
+#pragma unroll
+    for (uint32_t k = 0; k < kValuesIter; k++) {
+        if (at + k * kStep < n) {
+            raw[k].load<STREAM>(st, at + k * kStep);
+        }
+    }
+#pragma unroll
+    for (uint32_t k = 0; k < kValuesIter; k++) {
+        const uint64_t i = at + k * kStep;
+        if (i < n) {
+            const Moments o = raw[k].values();
+            store_vec<bf16, kLaneElems, true>(m + i, o.m);
+            store_vec<bf16, kLaneElems, true>(v + i, o.v);
+        }
     }
 }
 
@@ -687,8 +703,10 @@ int dressi_adamw_values(dressi_ctx* ctx, uint64_t n, const void* exp_avg, const 
                    "adamw: the buffers are not aligned");
     State st{nullptr, (void*)exp_avg, (void*)exp_avg_sq, (uint8_t*)exp_avg_scale,
              (uint8_t*)exp_avg_sq_scale, nullptr, 0, 0.f, nullptr};
+    const auto values = 2 * n >= kStreamBytes ? k_adamw_values<true> : k_adamw_values<false>;
     // within the launch limit, in whole blocks
-    constexpr uint64_t kPiece = kLaunchThreads * kLaneElems;
+    constexpr uint64_t kShare = kThreads * kLaneElems * kValuesIter;
+    constexpr uint64_t kPiece = kLaunchThreads / kThreads * kShare;
     for (uint64_t at = 0; at < n; at += kPiece) {
         const uint64_t take = std::min(kPiece, n - at);
         State s = st;
@@ -696,8 +714,8 @@ int dressi_adamw_values(dressi_ctx* ctx, uint64_t n, const void* exp_avg, const 
         s.v = (uint8_t*)st.v + at;
         s.m_scale = st.m_scale + at / kBlock;
         s.v_scale = st.v_scale + at / kBlock;
-        const uint32_t blocks = (uint32_t)((take + kThreads * kLaneElems - 1) / (kThreads * kLaneElems));
-        hipLaunchKernelGGL(k_adamw_values, dim3(blocks), dim3(kThreads), 0, ctx->stream, s, take,
+        const uint32_t blocks = (uint32_t)((take + kShare - 1) / kShare);
+        hipLaunchKernelGGL(values, dim3(blocks), dim3(kThreads), 0, ctx->stream, s, take,
                            (bf16*)exp_avg_bf16 + at, (bf16*)exp_avg_sq_bf16 + at);
         DRESSI_CHECK_LAUNCH();
     }

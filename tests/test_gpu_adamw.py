@@ -239,6 +239,26 @@ def test_larger_than_a_cache_8_bit(ctx):
         was = [m.clone(), v.clone()]
 
 
+def test_values_larger_than_a_cache(ctx):
+    """The values of more codes than a cache holds: each stretch's as numpy rounds them."""
+    import opendressi_amd.torch as dr
+    n, b1, b2 = 84 * 2 ** 20 + 1029, F32(0.9), F32(0.999)
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    p = torch.zeros(n, device="cuda")
+    p.grad = torch.randn(n, generator=gen, device="cuda")
+    opt = dr.AdamW(ctx, [p], state_bits=8)
+    opt.step()
+    m, v = opt.moments()
+    assert m.isfinite().all() and v.isfinite().all()
+    for a, b in ((0, 2080), (2 ** 26 - 64, 2 ** 26 + 2048), (n - 1029, n)):
+        g = _np(p.grad[a:b])
+        r = _mix(range(a, b), 1)
+        want_m = _rounded(F32(0) * b1 + g * F32(1 - 0.9), 14, ((r & 0xffff) << 4) + 8)
+        want_v = _rounded(F32(0) * b2 + (g * g) * F32(1 - 0.999), 30, ((r >> 16) << 4) + 8)
+        assert np.array_equal(_np(m[a:b]), want_m[:b - a].astype(F32))
+        assert np.array_equal(_np(v[a:b]), want_v[:b - a].astype(F32))
+
+
 def test_8_bit_moments_follow(ctx):
     """The slow moment moves by 0.1 % a step, a fraction of its code's step. Under a constant
     gradient v = g^2 (1 - b2^t); the rounding being unbiased, the mean over 2^16 elements follows.
