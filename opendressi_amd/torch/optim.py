@@ -10,6 +10,7 @@ from collections import OrderedDict
 
 import numpy as np
 import torch
+from torch.autograd.graph import increment_version
 
 from .._lib import AdamwSet, AdamwTensor, check, lib
 from ..ops import TYPE_CODES, _addr
@@ -69,8 +70,10 @@ class AdamW(torch.optim.Optimizer):
 
     capturable keeps the step counts on the device, so that a step can be
     captured into a graph (at the learning rates of the capture); every
-    parameter then needs a gradient in every step. Hooks registered on the optimizer run; torch's global optimizer
-    hooks do not."""
+    parameter then needs a gradient in every step.
+
+    Hooks registered on the optimizer run; torch's global optimizer hooks do
+    not."""
 
     def __init__(self, ctx: RasterizeHipContext, params, lr: float = 1e-3, betas=(0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float = 1e-2, state_bits: int = 32,
@@ -288,6 +291,8 @@ class AdamW(torch.optim.Optimizer):
                 _addr(self._scales[0]), _addr(self._scales[1]), self.seed, self.max_grad_norm or 0.0,
                 self._scratch.data_ptr(), _addr(self.grad_norm), _addr(self._counts),
                 _addr(self._device_sets)))
+        # written in place: a backward pass over the values before the step has to refuse them
+        increment_version(self._params if every else [self._params[i] for i in live])
         self._steps = now
         self._even = self._even and every
         return loss

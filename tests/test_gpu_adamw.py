@@ -595,6 +595,24 @@ def test_hooks_closures_and_schedulers(ctx):
     assert torch.allclose(p.detach(), torch.full_like(p, -0.75))
 
 
+def test_marks_what_it_writes(ctx):
+    """A backward pass that needs a parameter's values of before the step is refused, as after
+    any write in place; one that needs no written parameter's is not."""
+    import opendressi_amd.torch as dr
+    p, q = (torch.nn.Parameter(torch.full((40,), x, device="cuda")) for x in (2.0, 3.0))
+    opt = dr.AdamW(ctx, [p, q], lr=0.1)
+    p.grad = torch.ones(40, device="cuda")  # q has none
+    one, other = (p * p).sum(), (q * q).sum()
+    opt.step()
+    assert (p._version, q._version) == (1, 0)
+    other.backward()
+    assert (q.grad == 6.0).all()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        one.backward()
+    opt.step()
+    assert (p._version, q._version) == (2, 1)
+
+
 def test_state_is_freed(ctx):
     """Nothing but the optimizer holds its state."""
     import gc
