@@ -41,8 +41,9 @@ constexpr uint32_t kMaxVecs = 256;  // of a workgroup
 constexpr uint32_t kMinPixels = 2;  // that a thread should have of a chunk
 // Workgroups that a launch should have: two a compute unit. Each joins the sums of
 // its item's chunks, so more of them cost one large item (512 x 512 x 64 bfloat16
-// forward: 25 us with 512, 31 with 1024) and fewer leave loads unissued (8 x 1024
-// x 1024 x 64: 602 us with 512, 647 with 256).
+// forward: 23 us with 512, 30 with 1024 of half the threads) and fewer leave loads
+// unissued (2 x 512 x 512 x 66: forward 50 and backward 77 us with 512, 55 and 96
+// with 256).
 constexpr uint32_t kTargetGroups = 512;
 // Pixels that a thread keeps in registers (one pass). A workgroup's reads are a
 // block's few channels of each pixel, a cache line each: past 4096 pixels
@@ -169,10 +170,10 @@ Cut make_item_cut(uint32_t n_items, uint64_t n_px, uint32_t n_ch, uint32_t n_gro
 }
 
 // Pixels of a thread in flight. Forward 4 of 16 bytes in one group (1024 x 1024 x
-// 64 bfloat16 in 8 groups: 73 us, 76 with 8), else 8 (8 x 1024 x 1024 x 64 in 16
-// groups: 585 us, 596 with 4; 2 x 512 x 512 x 66 in 6: 51 and 55). Backward 4, of
-// the widest vectors 2, whose registers leave too few waves else (4 x 1024 x 1024
-// x 64 bfloat16: 487 us, 497 with 4).
+// 64 bfloat16 in 8 groups: 73 us, 78 with 8), else 8 (2 x 512 x 512 x 66 in 6: 50
+// us, 54 with 4). Backward 4, of the widest vectors 2, whose registers leave too
+// few waves else (1024 x 1024 x 64 bfloat16: 123 us, 127 with 4; eight of them in
+// 16 groups: 895 and 905).
 template <typename T, int V, int S>
 constexpr uint32_t kBatchOf = S == 1 && sizeof(T) * V >= 16 ? 4 : 8;
 template <int V>
@@ -1198,7 +1199,7 @@ __global__ __launch_bounds__(kItemThreads) void k_gn_bwd_item(
 // How wide a thread's vectors are: 16 bytes at most, as the channels, the strides
 // and the images' addresses (or-ed) allow. `whole`: that no group's edge cuts. One
 // pass takes whole ones, two passes wider ones where there are (their channels
-// count apart then: 2 x 512 x 512 x 66 bfloat16 in 6 groups, forward: 55 us with
+// count apart then: 2 x 512 x 512 x 66 bfloat16 in 6 groups, forward: 50 us with
 // vectors of 2 cut by edges, 75 with single channels).
 struct Width {
     uint32_t any, whole;
@@ -1237,13 +1238,13 @@ Scratch scratch_of(const Cut& c, bool whole, bool backward) {
 }
 
 // Bytes of an image from which results go past the caches. Forward with them and
-// without takes 73 and 87 us for 1024 x 1024 x 64 bfloat16, 25.3 and 26.1 for
+// without takes 73 and 88 us for 1024 x 1024 x 64 bfloat16, 22.9 and 24.8 for
 // 512 x 512 x 64; with a pass after it that reads the result 125 and 127, 37 and 37.
 constexpr uint64_t kStreamBytes = 32ull << 20;
 
 // Bytes of the first pass's reads that the second may find in the last-level cache
 // (256 MB): the ends of the chunks. The rest goes past it both times: 8 x 1024 x
-// 1024 x 64 bfloat16 574 us forward and 894 backward, 586 and 983 with all of it
+// 1024 x 64 bfloat16 574 us forward and 895 backward, 596 and 1054 with all of it
 // through the caches; all past them 1024 x 1024 x 64 takes 80 us forward, not 73.
 // 96 and 224 MB kept measure the same.
 constexpr uint64_t kKeepBytes = 160ull << 20;
