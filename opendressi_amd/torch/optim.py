@@ -35,6 +35,21 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
+def _layout(t: torch.Tensor) -> tuple[tuple, tuple]:
+    """(shape, stride): the order in which t's elements lie."""
+    return tuple(t.shape), t.stride()
+
+
+def _same_order(p: torch.Tensor, layout: tuple, packed: bool) -> bool:
+    """Whether p's elements lie in the order of `layout`; packed: that order is
+    row-major, in which another shape changes nothing."""
+    if packed and p.is_contiguous():
+        return True
+    shape, stride = layout
+    return p.shape == shape and all(
+        n == 1 or a == b for n, a, b in zip(shape, p.stride(), stride))
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW (decoupled weight decay) in one launch for up to 64 tensors.
 
@@ -61,6 +76,10 @@ class AdamW(torch.optim.Optimizer):
     are roundings; without it a small update of a 16-bit parameter is lost.
     Where such a parameter is written by others between steps (clamped,
     loaded), the copy takes the new value.
+
+    The state of a parameter lies in the order its elements have in memory at
+    its first step. Where that order changes later (channels_last), its steps
+    go through copies in the old one.
 
     max_grad_norm multiplies the gradients by
     min(1, max_grad_norm / (norm + 1e-6)), norm the 2-norm over all of them,
@@ -95,7 +114,9 @@ class AdamW(torch.optim.Optimizer):
         self._groups: list[dict] = []  # each parameter's
         self._pre_hooks: OrderedDict = OrderedDict()
         self._post_hooks: OrderedDict = OrderedDict()
-        self._expect: list[tuple] = []  # each parameter with its size and type
+        self._layouts: list[tuple] = []  # shape and stride of the order its share is in
+        self._fresh: set[int] = set()  # those whose share no step or state has touched
+        self._expect: list[tuple] = []  # each parameter with its size, type and if it is packed
         self._sets: list[tuple[dict, int]] = []  # each group with the place of its first parameter
         self._even = True  # every group's parameters have taken the same steps
         self._total = 0
@@ -123,6 +144,8 @@ class AdamW(torch.optim.Optimizer):
         if group["params"]:
             self._sets.append((group, len(self._params)))
         for p in group["params"]:
+            self._fresh.add(len(self._params))
+            self._layouts.append(_layout(p))
             self._params.append(p)
             self._steps.append(0)
             self._groups.append(group)
@@ -148,10 +171,16 @@ class AdamW(torch.optim.Optimizer):
                 if p.dtype != torch.float32:
                     view["master"][i] = where
                     where += 4 * _share(p)
-        self._expect = [(p, p.numel(), p.dtype) for p in self._params]
+        self._expect_layouts()
         self._table, self._view, self._total = table, view, at
         self._fields = view["param"], view["grad"]
         self._hyper = (AdamwSet * len(self._sets))()
+
+    def _expect_layouts(self) -> None:
+        """What a step looks for; packed: the share is in row-major order."""
+        self._expect = [(p, p.numel(), p.dtype,
+                         torch.empty_strided(*at, device="meta").is_contiguous())
+                        for p, at in zip(self._params, self._layouts)]
 
     def _check_param(self, p) -> None:
         if not isinstance(p, torch.Tensor):
@@ -238,18 +267,22 @@ class AdamW(torch.optim.Optimizer):
                                "capturable=True: its step count is the host's")
         dev = self.ctx.device.index
         kept = []  # copies that the launch reads
+        moved = []  # parameters in another order than their state, with their copies
         live, params, grads = [], [], []
-        for i, (p, n, kind) in enumerate(self._expect):
+        for i, (p, n, kind, packed) in enumerate(self._expect):
             g = p.grad
             if g is None:
                 continue
-            # a parameter's and its gradient's storage may have been replaced
+            # a parameter's and its gradient's storage may have been replaced or reordered
             if (g.dtype is not kind or p.dtype is not kind or g.numel() != n or p.numel() != n
                     or g.get_device() != dev or p.get_device() != dev
                     or g.layout is not torch.strided
-                    or not (g.is_contiguous() and p.is_contiguous())):
-                g = self._reorder(i, p, g, n, kind)
+                    or not (packed and g.is_contiguous() and p.is_contiguous())):
+                q, g = self._reorder(i, p, g, n, kind)
                 kept.append(g)
+                if q is not p:
+                    moved.append((p, q))
+                    p = q
             live.append(i)
             params.append(p.data_ptr())
             grads.append(g.data_ptr())
@@ -291,15 +324,21 @@ class AdamW(torch.optim.Optimizer):
                 _addr(self._scales[0]), _addr(self._scales[1]), self.seed, self.max_grad_norm or 0.0,
                 self._scratch.data_ptr(), _addr(self.grad_norm), _addr(self._counts),
                 _addr(self._device_sets)))
+        with torch.no_grad():
+            for p, q in moved:
+                p.copy_(q)
         # written in place: a backward pass over the values before the step has to refuse them
         increment_version(self._params if every else [self._params[i] for i in live])
         self._steps = now
         self._even = self._even and every
+        if self._fresh:
+            self._fresh.difference_update(live)
         return loss
 
-    def _reorder(self, i: int, p, g, n: int, kind) -> torch.Tensor:
-        """The gradient in its parameter's memory order; refuses what the
-        kernel cannot take."""
+    def _reorder(self, i: int, p, g, n: int, kind) -> tuple[torch.Tensor, torch.Tensor]:
+        """The parameter (a copy, where its order is not its state's) and the
+        gradient, both in the state's order; refuses what the kernel cannot
+        take."""
         if g.layout is not torch.strided:
             raise RuntimeError("AdamW: sparse gradients are not supported")
         if g.numel() != n or p.numel() != n or g.dtype is not kind or p.dtype is not kind \
@@ -309,17 +348,30 @@ class AdamW(torch.optim.Optimizer):
                              f"{tuple(g.shape)} on {g.device}")
         if not _dense(p):
             raise ValueError(f"parameter {i} is no longer densely stored")
-        if g.stride() == p.stride():
-            return g
+        layout, packed = self._layouts[i], self._expect[i][3]
+        if _same_order(p, layout, packed):
+            layout = _layout(p)
+        elif i in self._fresh:
+            # zeros, and a master copy of which the kernel takes what is still the parameter's
+            layout = self._layouts[i] = _layout(p)
+            self._expect[i] = (p, n, kind, p.is_contiguous())
+        elif tuple(p.shape) != layout[0]:
+            raise ValueError(f"parameter {i} changed its shape from {layout[0]} to "
+                             f"{tuple(p.shape)}, and its order")
+
+        def ordered(t):
+            if t.stride() == layout[1]:
+                return t
+            return torch.empty_strided(*layout, dtype=kind, device=t.device).copy_(t)
+
         with torch.no_grad():
-            return torch.empty_strided(p.shape, p.stride(), dtype=g.dtype,
-                                       device=g.device).copy_(g)
+            return p if _same_order(p, layout, False) else ordered(p), ordered(g)
 
     # ---- state ----
 
     def moments(self) -> tuple[torch.Tensor, torch.Tensor]:
         """(m, v) of all parameters, flat, in the parameters' order, each
-        parameter's share in its memory order and padded with zeros to a
+        parameter's share in its memory order (of its first step) and padded with zeros to a
         multiple of 32. With 32-bit state they are the optimizer's own
         float32 buffers, with 8-bit state the values that the codes stand for,
         in bfloat16, which holds them exactly."""
@@ -339,14 +391,17 @@ class AdamW(torch.optim.Optimizer):
         """Flat state: "step" (one count a parameter), "exp_avg" and
         "exp_avg_sq" as they are kept (with "exp_avg_scale" and
         "exp_avg_sq_scale" in 8 bits), "master" where there is one (the
-        16-bit parameters' copies, laid out like the moments), and the groups'
+        16-bit parameters' copies, laid out like the moments), "layout" (the
+        shape and stride of each parameter's share), and the groups'
         hyperparameters."""
         steps = list(self._steps)
         if self.capturable:
             ends = [at for _, at in self._sets[1:]] + [len(steps)]
             for t, (_, a), b in zip(self._counts.tolist(), self._sets, ends):
                 steps[a:b] = [t] * (b - a)
-        out = {"step": steps, "seed": self.seed,
+        layout = [_layout(p) if p.numel() == n and _same_order(p, at, packed) else at
+                  for (p, n, _, packed), at in zip(self._expect, self._layouts)]
+        out = {"step": steps, "seed": self.seed, "layout": layout,
                "exp_avg": self._moments[0], "exp_avg_sq": self._moments[1],
                "param_groups": [{k: v for k, v in g.items() if k != "params"}
                                 for g in self.param_groups]}
@@ -359,7 +414,9 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict: dict) -> None:
         """Takes over the state of an optimizer of the same parameters and
         state_bits. "seed", "master" and "param_groups" may be missing: then
-        they stay as they are."""
+        they stay as they are; without "layout" the state is taken to be in
+        the parameters' present order. Where a parameter lies in another order
+        than its state, its steps go through copies in the state's."""
         steps = [int(t) for t in state_dict["step"]]
         if len(steps) != len(self._params) or min(steps, default=0) < 0:
             raise ValueError(f"state of {len(steps)} parameters for {len(self._params)}")
@@ -373,6 +430,7 @@ class AdamW(torch.optim.Optimizer):
             if src.dtype != t.dtype or src.shape != t.shape:
                 raise ValueError(f"{k} must be {t.dtype} {tuple(t.shape)}, got {src.dtype} "
                                  f"{tuple(src.shape)}")
+        layouts = self._check_layouts(state_dict.get("layout"))
         groups = state_dict.get("param_groups")
         if groups is not None:
             if len(groups) != len(self.param_groups):
@@ -388,9 +446,32 @@ class AdamW(torch.optim.Optimizer):
         for k, t in named.items():
             t.copy_(state_dict[k])
         self._steps, self._even = steps, even
+        self._fresh.clear()
+        self._layouts = layouts
+        self._expect_layouts()
         if self.capturable:
             self._counts.copy_(torch.tensor([steps[a] for _, a in self._sets]))
         self.seed = int(state_dict.get("seed", self.seed)) & 0xffffffff
+
+    def _check_layouts(self, layouts) -> list[tuple]:
+        """A state dict's, one for each parameter and of its shape; None: the
+        parameters' own."""
+        if layouts is None:
+            return [_layout(p) if _dense(p) else at
+                    for p, at in zip(self._params, self._layouts)]
+        if len(layouts) != len(self._params):
+            raise ValueError(f"layouts of {len(layouts)} parameters for {len(self._params)}")
+        out = []
+        for i, (p, (shape, stride)) in enumerate(zip(self._params, layouts)):
+            shape, stride = tuple(shape), tuple(stride)
+            if shape != tuple(p.shape):
+                raise ValueError(f"state of a parameter {i} of shape {shape}, not "
+                                 f"{tuple(p.shape)}")
+            if len(stride) != len(shape) or min(stride, default=0) < 0 or \
+                    not _dense(torch.empty_strided(shape, stride, device="meta")):
+                raise ValueError(f"parameter {i}'s share has strides {stride}")
+            out.append((shape, stride))
+        return out
 
 
 def _share(p: torch.Tensor) -> int:

@@ -1,0 +1,61 @@
+"""What AdamW keeps between steps (opendressi_amd.torch.AdamW): its order."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    import opendressi_amd.torch as dr
+    return dr.RasterizeHipContext()
+
+
+def _values(shapes, seed, kind=torch.float32):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return [torch.randn(s, generator=gen, device="cuda").to(kind) for s in shapes]
+
+
+def _steps(opt, params, shapes, seeds):
+    for s in seeds:
+        for p, g in zip(params, _values(shapes, s, params[0].dtype)):
+            p.grad = g
+        opt.step()
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("kind", TYPES, ids=str)
+@pytest.mark.parametrize("resumed", [False, True])
+def test_channels_last_after_some_steps(ctx, bits, kind, resumed):
+    """Weights that become channels-last after two steps, in the same run or in one that goes on
+    from its state, take the steps of weights that stay as they are, bit for bit."""
+    import opendressi_amd.torch as dr
+    shapes = [(20, 12, 3, 3), (33,), (7, 5, 2, 4)]
+    kw = dict(lr=0.05, state_bits=bits, seed=5, max_grad_norm=1.0)
+    print(f"[adamw order] {bits} {kind} resumed {resumed}", flush=True)
+    want = _values(shapes, 0, kind)
+    ref = dr.AdamW(ctx, want, **kw)
+    _steps(ref, want, shapes, range(1, 6))
+    got = _values(shapes, 0, kind)
+    opt = dr.AdamW(ctx, got, **kw)
+    _steps(opt, got, shapes, (1, 2))
+    if resumed:
+        kept = opt.state_dict()
+        got = [p.clone(memory_format=torch.channels_last) if p.dim() == 4 else p.clone()
+               for p in got]
+        opt = dr.AdamW(ctx, got, **kw)
+        opt.load_state_dict(kept)
+    else:
+        for p in got:
+            if p.dim() == 4:
+                p.data = p.data.to(memory_format=torch.channels_last)
+    _steps(opt, got, shapes, (3, 4))
+    assert not got[0].is_contiguous()
+    got[0].data = got[0].data.contiguous()
+    _steps(opt, got, shapes, (5,))
+    for p, q in zip(got, want):
+        assert torch.equal(p, q)
+    for a, b in zip(opt.moments(), ref.moments()):
+        assert torch.equal(a, b)

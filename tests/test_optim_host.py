@@ -1,0 +1,171 @@
+"""AdamW's bookkeeping (opendressi_amd.torch.AdamW) without a GPU: parameters on the host, the
+step's entry point replaced by the formula in numpy."""
+import ctypes as C
+import threading
+import types
+
+import numpy as np
+import pytest
+import torch
+
+from opendressi_amd.torch import optim
+
+
+def _array(address, n):
+    return np.ctypeslib.as_array((C.c_float * n).from_address(address))
+
+
+class _Lib:
+    """dressi_adamw_step over host memory, float32 with 32-bit moments."""
+
+    def __init__(self, real):
+        self.dressi_adamw_scratch = real.dressi_adamw_scratch
+        self.dressi_adamw_set_bytes = real.dressi_adamw_set_bytes
+        self.calls = 0
+
+    def dressi_adamw_step(self, handle, table, n, sets, n_sets, bits, total, m, v, m_scale, v_scale,
+                          seed, max_norm, scratch, norm, counts, device_sets):
+        self.calls += 1
+        if bits != 32:
+            return 0
+        for e in table[:n]:
+            s = sets[e.set]
+            g, p = _array(e.grad, e.n), _array(e.param, e.n)
+            em, ev = (_array(a + 4 * e.state, e.n) for a in (m, v))
+            em[:] = em * s.beta1 + g * (1 - s.beta1)
+            ev[:] = ev * s.beta2 + g * g * (1 - s.beta2)
+            den = np.sqrt(ev / (1 - s.beta2 ** s.step)) + s.eps
+            p[:] = p * (1 - s.lr * s.weight_decay) - em / den * (s.lr / (1 - s.beta1 ** s.step))
+        return 0
+
+
+@pytest.fixture
+def lib(monkeypatch):
+    fake = _Lib(optim.lib)
+    monkeypatch.setattr(optim, "lib", fake)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    return fake
+
+
+CTX = types.SimpleNamespace(device=torch.device("cpu"), lock=threading.RLock(),
+                            _ctx=types.SimpleNamespace(use_torch_stream=lambda: None, handle=None))
+SHAPES = [(4, 3, 2, 5), (7,), (6, 5)]
+
+
+def _values(seed):
+    gen = torch.Generator().manual_seed(seed)
+    return [torch.randn(s, generator=gen) for s in SHAPES]
+
+
+def _another_order(t):
+    """t's values in another order of memory (channels last, or columns first)."""
+    if t.dim() == 4:
+        return t.contiguous(memory_format=torch.channels_last)
+    return t.t().contiguous().t() if t.dim() == 2 else t
+
+
+def _steps(opt, params, seeds):
+    for s in seeds:
+        for p, g in zip(params, _values(s)):
+            p.grad = g
+        opt.step()
+
+
+@pytest.mark.parametrize("when", [0, 2])
+@pytest.mark.parametrize("back", [False, True])
+def test_another_order_between_steps(lib, when, back):
+    """A parameter that is laid out anew before or after its first step, and back, takes the steps
+    of one that is not: the same values at the same indices."""
+    want = _values(0)
+    _steps(optim.AdamW(CTX, want, lr=0.1), want, range(1, 7))
+    got = _values(0)
+    opt = optim.AdamW(CTX, got, lr=0.1)
+    _steps(opt, got, range(1, 1 + when))
+    for p in got:
+        p.data = _another_order(p.data)
+    assert not got[0].is_contiguous() and not got[2].is_contiguous()
+    _steps(opt, got, range(1 + when, 5))
+    if back:
+        for p in got:
+            p.data = p.data.contiguous()
+    _steps(opt, got, range(5, 7))
+    for p, q in zip(got, want):
+        assert torch.equal(p, q)
+    assert got[0].is_contiguous() == got[2].is_contiguous() == back
+
+
+@pytest.mark.parametrize("first", [False, True])
+@pytest.mark.parametrize("then", [False, True])
+def test_resume_in_another_order(lib, first, then):
+    """State goes from parameters in one order to ones in another."""
+    want = _values(0)
+    _steps(optim.AdamW(CTX, want, lr=0.1), want, range(1, 6))
+    a = [_another_order(t) if first else t for t in _values(0)]
+    opt = optim.AdamW(CTX, a, lr=0.1)
+    _steps(opt, a, range(1, 4))
+    kept = opt.state_dict()
+    b = [_another_order(t) if then else t.contiguous() for t in a]
+    b = [t.clone(memory_format=torch.preserve_format) for t in b]
+    other = optim.AdamW(CTX, b)
+    other.load_state_dict(kept)
+    _steps(other, b, range(4, 6))
+    for p, q in zip(b, want):
+        assert torch.equal(p, q)
+    assert [s for s, _ in other.state_dict()["layout"]] == SHAPES
+
+
+def test_resume_without_a_layout(lib):
+    """A dict that does not say so is in the order that the parameters have when it is loaded."""
+    want = [_another_order(t) for t in _values(0)]
+    opt = optim.AdamW(CTX, want, lr=0.1)
+    _steps(opt, want, range(1, 3))
+    kept = {k: v for k, v in opt.state_dict().items() if k != "layout"}
+    got = [t.contiguous() for t in want]
+    other = optim.AdamW(CTX, got)
+    for p in got:
+        p.data = _another_order(p.data).clone(memory_format=torch.preserve_format)
+    other.load_state_dict(dict(kept, exp_avg=kept["exp_avg"].clone(),
+                               exp_avg_sq=kept["exp_avg_sq"].clone()))
+    _steps(opt, want, range(3, 5))
+    _steps(other, got, range(3, 5))
+    for p, q in zip(got, want):
+        assert torch.equal(p, q)
+
+
+def test_state_of_other_shapes_is_refused(lib):
+    """Shapes of the same padded sizes, or transposed, are not the same parameters."""
+    opt = optim.AdamW(CTX, _values(0))
+    kept = opt.state_dict()
+    for shapes in ([(4, 3, 2, 5), (9,), (6, 5)], [(4, 3, 2, 5), (7,), (5, 6)]):
+        other = optim.AdamW(CTX, [torch.zeros(s) for s in shapes])
+        with pytest.raises(ValueError, match="shape"):
+            other.load_state_dict(kept)
+    for bad in (kept["layout"][:2], [((4, 3, 2, 5), (30, 10, 5, 2))] + kept["layout"][1:],
+                [((4, 3, 2, 5), (30, 10, 5))] + kept["layout"][1:]):
+        with pytest.raises(ValueError, match="layouts|strides"):
+            opt.load_state_dict(dict(kept, layout=bad))
+    assert opt.state_dict()["layout"] == kept["layout"]
+
+
+def test_another_shape_between_steps(lib):
+    """The same elements in the same order under another shape go on; in another order they are
+    refused, for which of the old ones is which nobody says."""
+    p, q = torch.zeros(6), torch.zeros(6)
+    opt, ref = optim.AdamW(CTX, [p], lr=0.1), optim.AdamW(CTX, [q], lr=0.1)
+    g = torch.arange(6.0) - 2
+    for o, t in ((opt, p), (ref, q)):
+        t.grad = g
+        o.step()
+    p.grad = None
+    p.data = p.data.view(2, 3)
+    p.grad, q.grad = g.view(2, 3), g
+    opt.step(), ref.step()
+    assert torch.equal(p.flatten(), q)
+    assert opt.state_dict()["layout"] == [((2, 3), (3, 1))]
+    p.grad = None
+    p.data = p.data.reshape(3, 2).t().contiguous().t()
+    p.grad = torch.ones(3, 2)
+    before, calls = p.clone(), lib.calls
+    with pytest.raises(ValueError, match="shape"):
+        opt.step()
+    assert torch.equal(p, before) and lib.calls == calls
