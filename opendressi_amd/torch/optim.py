@@ -62,7 +62,8 @@ class AdamW(torch.optim.Optimizer):
 
     `params` is an iterable of parameters or of groups with their own lr,
     betas, eps and weight_decay. Parameters are float32, bfloat16 or float16
-    on the context's device, densely stored; they are updated in place, in
+    on the context's device, densely stored, no two in the same memory (a step
+    takes them all at once); they are updated in place, in
     float32, on torch's current stream.
 
     state_bits 32 keeps the moments in float32; 8 keeps them in a byte each,
@@ -136,6 +137,7 @@ class AdamW(torch.optim.Optimizer):
             else list(group["params"])
         for p in group["params"]:
             self._check_param(p)
+        _check_apart(self._params + group["params"])
         for k, v in self.defaults.items():
             group.setdefault(k, v)
         _check_hyper(group)
@@ -482,6 +484,17 @@ def _share(p: torch.Tensor) -> int:
 def _flat(t: torch.Tensor) -> torch.Tensor:
     """A densely stored tensor's elements in memory order."""
     return torch.as_strided(t, (t.numel(),), (1,))
+
+
+def _check_apart(params) -> None:
+    """Refuses a parameter that is there twice, or two that share memory."""
+    spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size(), i)
+                   for i, p in enumerate(params) if p.numel())
+    for (_, end, i), (begin, _, k) in zip(spans, spans[1:]):
+        if begin < end:
+            raise ValueError(f"parameters {min(i, k)} and {max(i, k)} are the same or share memory")
+    if len(set(map(id, params))) != len(params):
+        raise ValueError("an empty parameter is there twice")
 
 
 def _check_hyper(g: dict) -> None:

@@ -169,3 +169,18 @@ def test_another_shape_between_steps(lib):
     with pytest.raises(ValueError, match="shape"):
         opt.step()
     assert torch.equal(p, before) and lib.calls == calls
+
+
+def test_parameters_that_share_memory_are_refused(lib):
+    """All tensors are stepped at once: one of them twice, or two over the same elements, would be
+    read and written by two workgroups."""
+    p, flat, none = torch.zeros(8), torch.zeros(20), torch.zeros(0)
+    for params in ([p, p], [p, torch.ones(3), p.view(2, 4)], [flat[:11], flat[10:]],
+                   [flat[4:6], flat], [none, none],
+                   [dict(params=[p, p])], [dict(params=p), dict(params=p)]):
+        with pytest.raises(ValueError, match="share|twice|more than one"):
+            optim.AdamW(CTX, params)
+    opt = optim.AdamW(CTX, [flat[:10], flat[10:], none, torch.zeros(0)])
+    with pytest.raises(ValueError, match="share"):
+        opt.add_param_group({"params": [flat[9:11]]})
+    assert len(opt.param_groups) == 1 and len(opt.state_dict()["step"]) == 4
