@@ -90,7 +90,9 @@ class AdamW(torch.optim.Optimizer):
 
     capturable keeps the step counts on the device, so that a step can be
     captured into a graph (at the learning rates of the capture); every
-    parameter then needs a gradient in every step.
+    parameter then needs a gradient in every step. A graph holds the state by
+    its address: once a step has been captured, groups cannot be added, and
+    loaded state has to lie in the order of the present one.
 
     Hooks registered on the optimizer run; torch's global optimizer hooks do
     not."""
@@ -109,6 +111,7 @@ class AdamW(torch.optim.Optimizer):
         self.master_weights = bool(master_weights)
         self.seed = int(seed) & 0xffffffff
         self.capturable = bool(capturable)
+        self._captured = False  # a graph holds the state's addresses
         self.grad_norm = None
         self._params: list[torch.Tensor] = []  # in the order of their shares
         self._steps: list[int] = []
@@ -132,6 +135,9 @@ class AdamW(torch.optim.Optimizer):
 
     def add_param_group(self, param_group) -> None:
         """Adds a group; its parameters' state follows the others', at zero."""
+        if self._captured:
+            raise RuntimeError("AdamW: a step has been captured into a graph, whose replays write "
+                               "the state where it is: no group can be added")
         group = dict(param_group)
         group["params"] = [group["params"]] if isinstance(group["params"], torch.Tensor) \
             else list(group["params"])
@@ -264,7 +270,8 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        if not self.capturable and torch.cuda.is_current_stream_capturing():
+        capturing = torch.cuda.is_current_stream_capturing()
+        if capturing and not self.capturable:
             raise RuntimeError("AdamW.step cannot be captured into a graph without "
                                "capturable=True: its step count is the host's")
         dev = self.ctx.device.index
@@ -317,6 +324,8 @@ class AdamW(torch.optim.Optimizer):
             table = (AdamwTensor * len(live)).from_buffer(view)
             hyper = (AdamwSet * len(sets))(*(
                 (g["lr"], *g["betas"], g["eps"], g["weight_decay"], t) for g, t in sets))
+        if capturing:
+            self._captured = True
         ctx = self.ctx
         with ctx.lock:
             ctx._ctx.use_torch_stream()
@@ -433,6 +442,11 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"{k} must be {t.dtype} {tuple(t.shape)}, got {src.dtype} "
                                  f"{tuple(src.shape)}")
         layouts = self._check_layouts(state_dict.get("layout"))
+        if self._captured and not all(
+                a == b or torch.empty_strided(*a, device="meta").is_contiguous() and packed
+                for a, b, (_, _, _, packed) in zip(layouts, self._layouts, self._expect)):
+            raise ValueError("a step has been captured into a graph, which takes the state in "
+                             "the order that it had then")
         groups = state_dict.get("param_groups")
         if groups is not None:
             if len(groups) != len(self.param_groups):

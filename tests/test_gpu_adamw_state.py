@@ -59,3 +59,34 @@ def test_channels_last_after_some_steps(ctx, bits, kind, resumed):
         assert torch.equal(p, q)
     for a, b in zip(opt.moments(), ref.moments()):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_after_a_capture(ctx, bits):
+    """Once a graph holds the state, a group is refused, and the graph goes on as the eager steps
+    do."""
+    import opendressi_amd.torch as dr
+    shapes = [(40, 3), (65,)]
+    ps, qs = _values(shapes, 0), _values(shapes, 0)
+    opt = dr.AdamW(ctx, ps, lr=0.05, state_bits=bits, capturable=True)
+    ref = dr.AdamW(ctx, qs, lr=0.05, state_bits=bits, capturable=True)
+    _steps(ref, qs, shapes, (1, 2, 3))
+    for p, g in zip(ps, _values(shapes, 1)):
+        p.grad = g
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        opt.step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for t in (2, 3):
+        with pytest.raises(RuntimeError, match="captured"):
+            opt.add_param_group({"params": torch.zeros(9, device="cuda")})
+        for p, g in zip(ps, _values(shapes, t)):
+            p.grad.copy_(g)
+        graph.replay()
+        torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(ps, qs))
+    assert all(torch.equal(a, b) for a, b in zip(opt.moments(), ref.moments()))

@@ -184,3 +184,27 @@ def test_parameters_that_share_memory_are_refused(lib):
     with pytest.raises(ValueError, match="share"):
         opt.add_param_group({"params": [flat[9:11]]})
     assert len(opt.param_groups) == 1 and len(opt.state_dict()["step"]) == 4
+
+
+def test_state_stays_where_a_graph_has_it(lib, monkeypatch):
+    """Replays write the state that the capture saw: after one, no call replaces it or changes
+    its order."""
+    params = _values(0)
+    opt = optim.AdamW(CTX, params, capturable=True)
+    _steps(opt, params, (1,))
+    opt.add_param_group({"params": torch.zeros(3)})
+    opt.param_groups[1]["params"][0].grad = torch.ones(3)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    _steps(opt, params, (2,))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    held = [t.data_ptr() for t in (*opt.moments(), opt._counts, opt._device_sets)]
+    with pytest.raises(RuntimeError, match="captured"):
+        opt.add_param_group({"params": torch.zeros(4)})
+    kept = opt.state_dict()
+    other = [(s, tuple(torch.zeros(s).t().contiguous().t().stride())) if len(s) == 2 else (s, t)
+             for s, t in kept["layout"]]
+    with pytest.raises(ValueError, match="captured"):
+        opt.load_state_dict(dict(kept, layout=other))
+    opt.load_state_dict(kept)
+    assert len(opt.param_groups) == 2 and opt.state_dict()["layout"] == kept["layout"]
+    assert held == [t.data_ptr() for t in (*opt.moments(), opt._counts, opt._device_sets)]
