@@ -422,6 +422,10 @@ class AdamW(torch.optim.Optimizer):
             out["master"] = self.master
         return out
 
+    def __getstate__(self):
+        raise TypeError("an AdamW is not copied or pickled: its context and its flat state are "
+                        "its own; take its state_dict to another one")
+
     def load_state_dict(self, state_dict: dict) -> None:
         """Takes over the state of an optimizer of the same parameters and
         state_bits. "seed", "master" and "param_groups" may be missing: then

@@ -1,6 +1,8 @@
 """AdamW's bookkeeping (opendressi_amd.torch.AdamW) without a GPU: parameters on the host, the
 step's entry point replaced by the formula in numpy."""
+import copy
 import ctypes as C
+import pickle
 import threading
 import types
 
@@ -208,3 +210,11 @@ def test_state_stays_where_a_graph_has_it(lib, monkeypatch):
     opt.load_state_dict(kept)
     assert len(opt.param_groups) == 2 and opt.state_dict()["layout"] == kept["layout"]
     assert held == [t.data_ptr() for t in (*opt.moments(), opt._counts, opt._device_sets)]
+
+
+def test_copies_are_refused(lib):
+    """A copy would have had no parameters and no state."""
+    opt = optim.AdamW(CTX, _values(0))
+    for make in (copy.copy, copy.deepcopy, pickle.dumps):
+        with pytest.raises(TypeError, match="state_dict"):
+            make(opt)
