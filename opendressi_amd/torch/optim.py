@@ -118,6 +118,9 @@ class AdamW(torch.optim.Optimizer):
         self._groups: list[dict] = []  # each parameter's
         self._pre_hooks: OrderedDict = OrderedDict()
         self._post_hooks: OrderedDict = OrderedDict()
+        # of state_dict and load_state_dict, before and after
+        self._save_hooks = OrderedDict(), OrderedDict()
+        self._load_hooks = OrderedDict(), OrderedDict()
         self._layouts: list[tuple] = []  # shape and stride of the order its share is in
         self._fresh: set[int] = set()  # those whose share no step or state has touched
         self._expect: list[tuple] = []  # each parameter with its size, type and if it is packed
@@ -255,15 +258,29 @@ class AdamW(torch.optim.Optimizer):
     def register_step_pre_hook(self, hook):
         """hook(optimizer, args, kwargs) before each step; it may return new
         (args, kwargs). Returns a handle whose remove() takes it out."""
-        handle = torch.utils.hooks.RemovableHandle(self._pre_hooks)
-        self._pre_hooks[handle.id] = hook
-        return handle
+        return _register(self._pre_hooks, hook)
 
     def register_step_post_hook(self, hook):
         """hook(optimizer, args, kwargs) after each step."""
-        handle = torch.utils.hooks.RemovableHandle(self._post_hooks)
-        self._post_hooks[handle.id] = hook
-        return handle
+        return _register(self._post_hooks, hook)
+
+    def register_state_dict_pre_hook(self, hook, prepend: bool = False):
+        """hook(optimizer) before each state_dict."""
+        return _register(self._save_hooks[0], hook, prepend)
+
+    def register_state_dict_post_hook(self, hook, prepend: bool = False):
+        """hook(optimizer, state_dict) after each state_dict; it may return
+        another dict."""
+        return _register(self._save_hooks[1], hook, prepend)
+
+    def register_load_state_dict_pre_hook(self, hook, prepend: bool = False):
+        """hook(optimizer, state_dict) before each load_state_dict, with a
+        shallow copy of the dict; it may return another."""
+        return _register(self._load_hooks[0], hook, prepend)
+
+    def register_load_state_dict_post_hook(self, hook, prepend: bool = False):
+        """hook(optimizer) after each load_state_dict."""
+        return _register(self._load_hooks[1], hook, prepend)
 
     def _step(self, closure=None):
         loss = None
@@ -405,6 +422,8 @@ class AdamW(torch.optim.Optimizer):
         16-bit parameters' copies, laid out like the moments), "layout" (the
         shape and stride of each parameter's share), and the groups'
         hyperparameters."""
+        for hook in list(self._save_hooks[0].values()):
+            hook(self)
         steps = list(self._steps)
         if self.capturable:
             ends = [at for _, at in self._sets[1:]] + [len(steps)]
@@ -420,6 +439,9 @@ class AdamW(torch.optim.Optimizer):
             out["exp_avg_scale"], out["exp_avg_sq_scale"] = self._scales
         if self.master is not None:
             out["master"] = self.master
+        for hook in list(self._save_hooks[1].values()):
+            new = hook(self, out)
+            out = out if new is None else new
         return out
 
     def __getstate__(self):
@@ -432,6 +454,10 @@ class AdamW(torch.optim.Optimizer):
         they stay as they are; without "layout" the state is taken to be in
         the parameters' present order. Where a parameter lies in another order
         than its state, its steps go through copies in the state's."""
+        state_dict = dict(state_dict)
+        for hook in list(self._load_hooks[0].values()):
+            new = hook(self, state_dict)
+            state_dict = state_dict if new is None else new
         steps = [int(t) for t in state_dict["step"]]
         if len(steps) != len(self._params) or min(steps, default=0) < 0:
             raise ValueError(f"state of {len(steps)} parameters for {len(self._params)}")
@@ -472,6 +498,8 @@ class AdamW(torch.optim.Optimizer):
         if self.capturable:
             self._counts.copy_(torch.tensor([steps[a] for _, a in self._sets]))
         self.seed = int(state_dict.get("seed", self.seed)) & 0xffffffff
+        for hook in list(self._load_hooks[1].values()):
+            hook(self)
 
     def _check_layouts(self, layouts) -> list[tuple]:
         """A state dict's, one for each parameter and of its shape; None: the
@@ -492,6 +520,15 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"parameter {i}'s share has strides {stride}")
             out.append((shape, stride))
         return out
+
+
+def _register(hooks: OrderedDict, hook, prepend: bool = False):
+    """Adds a hook; the handle's remove() takes it out."""
+    handle = torch.utils.hooks.RemovableHandle(hooks)
+    hooks[handle.id] = hook
+    if prepend:
+        hooks.move_to_end(handle.id, last=False)
+    return handle
 
 
 def _share(p: torch.Tensor) -> int:

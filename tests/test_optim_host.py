@@ -218,3 +218,22 @@ def test_copies_are_refused(lib):
     for make in (copy.copy, copy.deepcopy, pickle.dumps):
         with pytest.raises(TypeError, match="state_dict"):
             make(opt)
+
+
+def test_state_dict_hooks(lib):
+    """Before and after, in their order, with the dict they are given or give back."""
+    opt, seen = optim.AdamW(CTX, _values(0), seed=3), []
+    opt.register_state_dict_pre_hook(lambda o: seen.append("save"))
+    opt.register_state_dict_post_hook(lambda o, d: d.update(mark=1))
+    opt.register_state_dict_post_hook(lambda o, d: dict(d, more=o is opt))
+    first = opt.register_state_dict_pre_hook(lambda o: seen.append("first"), prepend=True)
+    kept = opt.state_dict()
+    assert kept["mark"] == 1 and kept["more"] is True and seen == ["first", "save"]
+    first.remove()
+    opt = optim.AdamW(CTX, _values(0))
+    opt.register_load_state_dict_pre_hook(lambda o, d: seen.append(d.pop("mark")))
+    opt.register_load_state_dict_pre_hook(lambda o, d: dict(d, seed=9))
+    opt.register_load_state_dict_post_hook(lambda o: seen.append(o.seed))
+    opt.load_state_dict(kept)
+    assert opt.seed == 9 and seen[-2:] == [1, 9]
+    assert kept["seed"] == 3 and kept["mark"] == 1
