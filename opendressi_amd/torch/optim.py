@@ -483,12 +483,14 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"{len(groups)} groups for {len(self.param_groups)}")
             for g in groups:
                 _check_hyper(g)
-            for mine, g in zip(self.param_groups, groups):
-                mine.update({k: v for k, v in g.items() if k != "params"})
         ends = [at for _, at in self._sets[1:]] + [len(steps)]
         even = all(len(set(steps[a:b])) == 1 for (_, a), b in zip(self._sets, ends))
         if self.capturable and not even:
             raise ValueError("a capturable optimizer's groups have one step count each")
+        seed = int(state_dict.get("seed", self.seed)) & 0xffffffff
+        # nothing is refused from here on
+        for mine, g in zip(self.param_groups, groups or ()):
+            mine.update({k: v for k, v in g.items() if k != "params"})
         for k, t in named.items():
             t.copy_(state_dict[k])
         self._steps, self._even = steps, even
@@ -497,7 +499,7 @@ class AdamW(torch.optim.Optimizer):
         self._expect_layouts()
         if self.capturable:
             self._counts.copy_(torch.tensor([steps[a] for _, a in self._sets]))
-        self.seed = int(state_dict.get("seed", self.seed)) & 0xffffffff
+        self.seed = seed
         for hook in list(self._load_hooks[1].values()):
             hook(self)
 

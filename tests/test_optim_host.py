@@ -237,3 +237,25 @@ def test_state_dict_hooks(lib):
     opt.load_state_dict(kept)
     assert opt.seed == 9 and seen[-2:] == [1, 9]
     assert kept["seed"] == 3 and kept["mark"] == 1
+
+
+def test_a_refused_state_changes_nothing(lib):
+    """Whatever a state dict is refused for, the optimizer is as it was, its rates too."""
+    params = _values(0)
+    opt = optim.AdamW(CTX, params, lr=0.25, capturable=True, seed=4)
+    _steps(opt, params, (1, 2))
+    moments = [t.clone() for t in opt.moments()]
+    good = dict(opt.state_dict(), seed=5, exp_avg=torch.ones_like(moments[0]))
+    good["param_groups"] = [dict(good["param_groups"][0], lr=0.5)]
+    bad = [dict(good, step=[1, 2, 3]), dict(good, step=[1, 1]), dict(good, step=["x", 1, 1]),
+           dict(good, exp_avg_sq=torch.zeros(3)), dict(good, param_groups=[]),
+           dict(good, param_groups=[dict(lr=-1.0)]), dict(good, layout=[]), dict(good, seed="x"),
+           dict(good, param_groups=[dict(lr=0.5)]),
+           {k: v for k, v in good.items() if k != "exp_avg"}]
+    for state in bad:
+        with pytest.raises((ValueError, KeyError, TypeError)):
+            opt.load_state_dict(state)
+        assert opt.param_groups[0]["lr"] == 0.25 and opt.seed == 4
+        assert all(torch.equal(a, b) for a, b in zip(opt.moments(), moments))
+    opt.load_state_dict(good)
+    assert opt.param_groups[0]["lr"] == 0.5 and opt.seed == 5 and (opt.moments()[0] == 1).all()
