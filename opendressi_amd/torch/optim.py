@@ -313,6 +313,8 @@ class AdamW(torch.optim.Optimizer):
             params.append(p.data_ptr())
             grads.append(g.data_ptr())
         if not live:
+            if self.grad_norm is not None:
+                self.grad_norm.zero_()  # the norm of nothing
             return loss
         every = len(live) == len(self._expect)
         steps = self._steps

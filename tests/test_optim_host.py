@@ -259,3 +259,11 @@ def test_a_refused_state_changes_nothing(lib):
         assert all(torch.equal(a, b) for a, b in zip(opt.moments(), moments))
     opt.load_state_dict(good)
     assert opt.param_groups[0]["lr"] == 0.5 and opt.seed == 5 and (opt.moments()[0] == 1).all()
+
+
+def test_the_norm_of_no_gradients(lib):
+    """A step without gradients leaves no older step's norm behind."""
+    opt = optim.AdamW(CTX, _values(0), max_grad_norm=1.0)
+    opt.grad_norm.fill_(7.0)
+    opt.step()
+    assert float(opt.grad_norm) == 0.0 and lib.calls == 0
