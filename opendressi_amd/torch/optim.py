@@ -5,6 +5,7 @@ surface, whose optimizer is part of its graph.
 """
 from __future__ import annotations
 
+import ctypes as C
 import math
 from collections import OrderedDict
 
@@ -103,7 +104,9 @@ class AdamW(torch.optim.Optimizer):
                  capturable: bool = False):
         if state_bits not in (8, 32):
             raise ValueError(f"state_bits must be 8 or 32, got {state_bits}")
-        if max_grad_norm is not None and not 0.0 < max_grad_norm < math.inf:
+        if max_grad_norm is not None and (not 0.0 < max_grad_norm < math.inf or
+                                          C.c_float(max_grad_norm).value == 0.0):
+            # the step takes it in 32 bits, where zero says not to clip
             raise ValueError(f"max_grad_norm must be above 0, got {max_grad_norm}")
         self.ctx = ctx
         self.state_bits = state_bits

@@ -267,3 +267,11 @@ def test_the_norm_of_no_gradients(lib):
     opt.grad_norm.fill_(7.0)
     opt.step()
     assert float(opt.grad_norm) == 0.0 and lib.calls == 0
+
+
+def test_a_norm_that_is_zero_in_32_bits_is_refused(lib):
+    for bad in (0.0, -1.0, float("nan"), float("inf"), 1e-46, 1e-300):
+        with pytest.raises(ValueError, match="max_grad_norm"):
+            optim.AdamW(CTX, _values(0), max_grad_norm=bad)
+    for good in (1e-40, 1e-6, 1e30, 1e39):
+        optim.AdamW(CTX, _values(0), max_grad_norm=good)
