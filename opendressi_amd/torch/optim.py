@@ -108,6 +108,8 @@ class AdamW(torch.optim.Optimizer):
                                           C.c_float(max_grad_norm).value == 0.0):
             # the step takes it in 32 bits, where zero says not to clip
             raise ValueError(f"max_grad_norm must be above 0, got {max_grad_norm}")
+        if isinstance(params, (set, frozenset)):
+            raise TypeError("parameters need an order, in which their state lies: not a set")
         self.ctx = ctx
         self.state_bits = state_bits
         self.max_grad_norm = max_grad_norm
@@ -145,6 +147,9 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError("AdamW: a step has been captured into a graph, whose replays write "
                                "the state where it is: no group can be added")
         group = dict(param_group)
+        if isinstance(group["params"], (set, frozenset)):
+            raise TypeError("a group's parameters need an order, in which their state lies: "
+                            "not a set")
         group["params"] = [group["params"]] if isinstance(group["params"], torch.Tensor) \
             else list(group["params"])
         for p in group["params"]:

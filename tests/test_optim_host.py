@@ -275,3 +275,12 @@ def test_a_norm_that_is_zero_in_32_bits_is_refused(lib):
             optim.AdamW(CTX, _values(0), max_grad_norm=bad)
     for good in (1e-40, 1e-6, 1e30, 1e39):
         optim.AdamW(CTX, _values(0), max_grad_norm=good)
+
+
+def test_sets_of_parameters_are_refused(lib):
+    """Their order is another in every run, and state lies in it."""
+    for params in (set(_values(0)), [dict(params=set(_values(0)))],
+                   [dict(params=frozenset(_values(0)))]):
+        with pytest.raises(TypeError, match="order"):
+            optim.AdamW(CTX, params)
+    assert len(optim.AdamW(CTX, (t for t in _values(0))).state_dict()["step"]) == 3
