@@ -640,11 +640,6 @@ int dressi_adamw_step(dressi_ctx* ctx, const dressi_adamw_tensor* tensors, uint3
     const bool stream = bytes >= kStreamBytes;
     const uint32_t iter = small ? 1 : q8 ? 2 : 4;
     const uint32_t chunk = kThreads * kLaneElems * iter;
-    for (uint32_t i = 0; on_device && i < n_sets; i++) {
-        hipLaunchKernelGGL(k_adamw_tick, dim3(1), dim3(64), 0, ctx->stream, sets[i], seed,
-                           steps + i, (SetArg*)device_sets + i);
-        DRESSI_CHECK_LAUNCH();
-    }
     State st{(const SetArg*)device_sets, exp_avg, exp_avg_sq, exp_avg_scale, exp_avg_sq_scale, nullptr, 0, max_norm, norm};
     if (clip) {
         uint32_t launches = 0;
@@ -673,6 +668,12 @@ int dressi_adamw_step(dressi_ctx* ctx, const dressi_adamw_tensor* tensors, uint3
         }
         st.partials = (const double*)scratch;
         st.n_partials = used;
+    }
+    // after all that may be refused: a step that is not taken does not count
+    for (uint32_t i = 0; on_device && i < n_sets; i++) {
+        hipLaunchKernelGGL(k_adamw_tick, dim3(1), dim3(64), 0, ctx->stream, sets[i], seed,
+                           steps + i, (SetArg*)device_sets + i);
+        DRESSI_CHECK_LAUNCH();
     }
     return for_batches(tensors, n_tensors, sets, on_device, seed, chunk, [&](const Table& tb) -> int {
         const auto step =

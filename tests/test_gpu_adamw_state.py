@@ -90,3 +90,21 @@ def test_after_a_capture(ctx, bits):
         torch.cuda.synchronize()
     assert all(torch.equal(p, q) for p, q in zip(ps, qs))
     assert all(torch.equal(a, b) for a, b in zip(opt.moments(), ref.moments()))
+
+
+def test_a_refused_step_does_not_count(ctx):
+    """More tensors than a clipped step takes: refused before its counts on the device move."""
+    from opendressi_amd._lib import AdamwSet, AdamwTensor, lib
+    n = 1024 * 64 + 1
+    p, state = torch.zeros(32, device="cuda"), torch.zeros(2, 32, device="cuda")
+    table = (AdamwTensor * n)(*[(p.data_ptr(), p.data_ptr(), None, 1, 0, 0, 0)] * n)
+    sets = (AdamwSet * 1)((1e-3, 0.9, 0.999, 1e-8, 0.0, 0))
+    scratch = torch.empty(lib.dressi_adamw_scratch(), dtype=torch.uint8, device="cuda")
+    norm, steps = torch.zeros((), device="cuda"), torch.zeros(1, dtype=torch.int64, device="cuda")
+    rates = torch.empty(lib.dressi_adamw_set_bytes(), dtype=torch.uint8, device="cuda")
+    ctx._ctx.use_torch_stream()
+    rc = lib.dressi_adamw_step(ctx._ctx.handle, table, n, sets, 1, 32, 32, state[0].data_ptr(),
+                               state[1].data_ptr(), None, None, 0, 1.0, scratch.data_ptr(),
+                               norm.data_ptr(), steps.data_ptr(), rates.data_ptr())
+    assert rc == -1 and b"too many tensors" in lib.dressi_last_error()
+    assert int(steps) == 0 and not p.any() and not state.any()
