@@ -1,6 +1,12 @@
-"""What AdamW keeps between steps (opendressi_amd.torch.AdamW): its order."""
+"""What AdamW keeps between steps (opendressi_amd.torch.AdamW): its order, its counts, and the
+codes of clipped steps."""
+import math
+
+import numpy as np
 import pytest
 import torch
+from test_gpu_adamw import F32, U, _mix, _np, _rounded
+from test_gpu_adamw import _values as _mixed
 
 pytestmark = pytest.mark.gpu
 
@@ -108,3 +114,41 @@ def test_a_refused_step_does_not_count(ctx):
                                norm.data_ptr(), steps.data_ptr(), rates.data_ptr())
     assert rc == -1 and b"too many tensors" in lib.dressi_last_error()
     assert int(steps) == 0 and not p.any() and not state.any()
+
+
+@pytest.mark.parametrize("kind", TYPES, ids=str)
+@pytest.mark.parametrize("sizes", [[33, 1000], [2 ** 23 + 4099]], ids=str)
+def test_clipped_8_bit_codes(ctx, sizes, kind):
+    """Three steps whose clip is active, from the norm on the device (a double sum, its root
+    rounded once): the factor in float32, and every code as the definition gives it."""
+    import opendressi_amd.torch as dr
+    print(f"[adamw clipped 8] {sizes} {kind}", flush=True)
+    rng = np.random.default_rng(11)
+    b1, b2 = F32(0.9), F32(0.999)
+    ps = [torch.tensor(_mixed(rng, n)).to(kind).cuda() for n in sizes]
+    opt = dr.AdamW(ctx, ps, state_bits=8, max_grad_norm=0.25, seed=2)
+    # of a large tensor its first elements, those around a workgroup's share, and the ragged end
+    spans = [[(0, n)] if n < 5000 else [(0, 96), (2 ** 22 - 32, 2 ** 22 + 32), (2 ** 23 - 32, n)]
+             for n in sizes]
+    m, v = [[[np.zeros(b - a, F32) for a, b in s] for s in spans] for _ in range(2)]
+    for t in (1, 2, 3):
+        for p, n in zip(ps, sizes):
+            p.grad = torch.tensor(_mixed(rng, n)).to(kind).cuda()
+        opt.step()
+        norm = math.sqrt(sum(float(p.grad.double().square().sum()) for p in ps))
+        assert abs(float(opt.grad_norm) - norm) <= 2 * U * norm
+        c = F32(0.25) / (F32(float(opt.grad_norm)) + F32(1e-6))
+        assert c < 1
+        gm, gv = opt.moments()
+        at = 0
+        for i, n in enumerate(sizes):
+            for k, (a, b) in enumerate(spans[i]):
+                g = _np(ps[i].grad[a:b]) * c
+                r = _mix(range(at + a, at + b), t, 2)
+                x = m[i][k] * b1 + g * F32(1 - 0.9)
+                y = v[i][k] * b2 + (g * g) * F32(1 - 0.999)
+                m[i][k] = _rounded(x, 14, ((r & 0xffff) << 4) + 8)[:b - a].astype(F32)
+                v[i][k] = _rounded(y, 30, ((r >> 16) << 4) + 8)[:b - a].astype(F32)
+                assert np.array_equal(_np(gm[at + a:at + b]), m[i][k]), (t, i, k)
+                assert np.array_equal(_np(gv[at + a:at + b]), v[i][k]), (t, i, k)
+            at += -(-n // 32) * 32
