@@ -303,7 +303,7 @@ __device__ __forceinline__ void act_slopes(uint32_t act, const float (&z)[V], fl
         case DRESSI_ACT_RELU:
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                g[j] *= z[j] > 0.f ? 1.f : 0.f;
+                g[j] = z[j] > 0.f ? g[j] : 0.f;  // an infinity or a NaN is masked too
             }
             break;
         case DRESSI_ACT_SILU:

@@ -1,0 +1,46 @@
+"""Group norm (opendressi_amd.ops.group_norm, group_norm_bwd) where values or gradients are
+unusual."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+# one pass; two passes; two passes whose vectors are cut by groups' edges; many items in one pass
+# and in two
+SHAPES = [((2, 8, 9, 32), 4), ((1, 90, 91, 64), 8), ((2, 70, 71, 66), 6), ((300, 4, 16), 2),
+          ((700, 9, 520), 1)]
+
+
+@pytest.fixture(scope="module")
+def ctx():
+    import opendressi_amd as od
+    c = od.Context(0)
+    yield c
+    c.close()
+
+
+def _inputs(shape, kind, seed):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    r = lambda *s: torch.randn(s, generator=gen, device="cuda")  # noqa: E731
+    c = shape[-1]
+    return r(*shape).to(kind), r(*shape).to(kind), 1 + 0.2 * r(c), 0.3 * r(c)
+
+
+@pytest.mark.parametrize("shape,groups", SHAPES, ids=str)
+@pytest.mark.parametrize("kind", TYPES, ids=str)
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_relu_masks_any_gradient(ctx, shape, groups, kind, bad):
+    """Where relu's slope is zero, no gradient passes, whatever it is: the bits of a zero there."""
+    from opendressi_amd import ops as K
+    print(f"[group_norm relu] {shape} {groups} {kind} {bad}", flush=True)
+    x, gy, w, b = _inputs(shape, kind, 1)
+    z, mean, rstd = K.group_norm(ctx, x, groups, w, b)
+    off = z < -0.1
+    assert off.any()
+    want = K.group_norm_bwd(ctx, gy.masked_fill(off, 0.0), x, mean, rstd, groups, w, b, "relu")
+    got = K.group_norm_bwd(ctx, gy.masked_fill(off, bad), x, mean, rstd, groups, w, b, "relu")
+    for p, q in zip(got, want):
+        assert q.isfinite().all() and torch.equal(p, q)
