@@ -817,19 +817,25 @@ __global__ __launch_bounds__(kItemThreads) void k_gn_item(const T* x, const Cut 
 // backward
 // ---------------------------------------------------------------------------
 
-// What a thread of the backward pass knows of its channels.
+// What a thread of the backward pass knows of its channels; ws = rstd w. With it
+// z is rounded as in the forward pass, so that relu's mask is that of its y, and
+// gx = ws gz - mean_g(ws gz) - xh mean_g(ws gz xh) takes two operations.
 template <int V, int S>
 struct Channels {
-    float mu[S], rstd[S], w[V], b[V];
+    float mu[S], rstd[S], ws[V], b[V];
 
     __device__ __forceinline__ void load(const Cut& c, const Affine& aff, uint32_t item,
                                          uint32_t vec, const float* mean, const float* rs) {
-        load_affine<V>(aff, vec * V, w, b);
+        load_affine<V>(aff, vec * V, ws, b);
 #pragma unroll
         for (int g = 0; g < S; g++) {
             const size_t at = (size_t)item * c.n_groups + group_of<V, S>(c, vec, g);
             mu[g] = mean[at];
             rstd[g] = rs[at];
+        }
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            ws[j] *= rstd[j / (V / S)];
         }
     }
     // xh and gz of a vector
@@ -841,8 +847,9 @@ struct Channels {
         unpack(gy, gz);
 #pragma unroll
         for (int j = 0; j < V; j++) {
-            xh[j] = (xh[j] - mu[j / (V / S)]) * rstd[j / (V / S)];
-            z[j] = fmaf(xh[j], w[j], b[j]);
+            const float d = xh[j] - mu[j / (V / S)];
+            xh[j] = d * rstd[j / (V / S)];
+            z[j] = fmaf(d, ws[j], b[j]);
         }
         act_slopes<V>(act, z, gz);
     }
@@ -857,7 +864,7 @@ struct Channels {
             sb[j] = fmaf(gz[j], xh[j], sb[j]);
         }
     }
-    // gx from the groups' means of w gz and w gz xh
+    // gx from the groups' means of ws gz and ws gz xh
     template <typename T>
     __device__ __forceinline__ void finish(const Pack<T, V>& x, const Pack<T, V>& gy, uint32_t act,
                                            const float2 (&m)[S], T* gx, uint32_t stream) const {
@@ -866,13 +873,13 @@ struct Channels {
 #pragma unroll
         for (int j = 0; j < V; j++) {
             const int g = j / (V / S);
-            gz[j] = rstd[g] * (fmaf(gz[j], w[j], -m[g].x) - xh[j] * m[g].y);
+            gz[j] = fmaf(-xh[j], m[g].y, fmaf(gz[j], ws[j], -m[g].x));
         }
         put<T, V>(gx, gz, stream);
     }
 };
 
-// The first pass: per chunk the groups' sums of w gz and w gz xh, and for all
+// The first pass: per chunk the groups' sums of ws gz and ws gz xh, and for all
 // chunks of a workgroup the channels' sums of gz and gz xh. 4 x 1024 x 1024 x 64
 // bfloat16: 169 us, 6.4 TB/s. MANY: it takes every gridDim.x-th chunk of all
 // items'; else it has one, and a set of sums less in its registers.
@@ -931,8 +938,8 @@ __global__ __launch_bounds__(kMaxThreads) void k_gn_bwd_sums(const T* gy, const 
                 if (at.pixels(c, chunk) > 0) {
 #pragma unroll
                     for (int j = g * (V / S); j < (g + 1) * (V / S); j++) {
-                        s.x = fmaf(ch.w[j], a[j], s.x);
-                        s.y = fmaf(ch.w[j], b[j], s.y);
+                        s.x = fmaf(ch.ws[j], a[j], s.x);
+                        s.y = fmaf(ch.ws[j], b[j], s.y);
                     }
                 }
                 red[g][threadIdx.x] = s;
@@ -1151,8 +1158,8 @@ __global__ __launch_bounds__(kItemThreads) void k_gn_bwd_item(
             }
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                g.x = fmaf(ch.w[j], a[j], g.x);
-                g.y = fmaf(ch.w[j], b[j], g.y);
+                g.x = fmaf(ch.ws[j], a[j], g.x);
+                g.y = fmaf(ch.ws[j], b[j], g.y);
                 sa[j] += a[j];
                 sb[j] += b[j];
             }

@@ -44,3 +44,21 @@ def test_relu_masks_any_gradient(ctx, shape, groups, kind, bad):
     got = K.group_norm_bwd(ctx, gy.masked_fill(off, bad), x, mean, rstd, groups, w, b, "relu")
     for p, q in zip(got, want):
         assert q.isfinite().all() and torch.equal(p, q)
+
+
+@pytest.mark.parametrize("shape,groups", SHAPES, ids=str)
+def test_relu_masks_what_it_gave_as_zero(ctx, shape, groups):
+    """Each channel's bias puts one pixel of each item as near to relu's kink as float32 goes: the
+    gradient passes where the output is above zero and nowhere else."""
+    from opendressi_amd import ops as K
+    print(f"[group_norm kink] {shape} {groups}", flush=True)
+    x, _, w, _ = _inputs(shape, torch.float32, 2)
+    n, c = shape[0], shape[-1]
+    z, mean, rstd = K.group_norm(ctx, x, groups, w)
+    # one pixel's z for each channel, with its sign turned
+    at = torch.arange(c, device="cuda") % (x.numel() // (n * c))
+    b = -z.view(n, -1, c)[0].gather(0, at[None])[0].contiguous()
+    y = K.group_norm(ctx, x, groups, w, b, activation="relu")[0]
+    _, _, gb = K.group_norm_bwd(ctx, torch.ones_like(x), x, mean, rstd, groups, w, b, "relu",
+                                (False, False, True))
+    assert torch.equal(gb.double(), (y > 0).view(-1, c).double().sum(0))
