@@ -20,10 +20,14 @@
 // each pass's images and nothing else (counters: 4 x 1024 x 1024 x 64 bfloat16,
 // forward 537 MB read twice and written once).
 //
-// Statistics are those of x less a pivot, the group's first value: a batch of a
-// thread's values gives its mean and the squares about that mean, both from
-// registers, and (count, mean, squares) of two sets are joined. So values far
-// from zero lose nothing to cancellation, nor does a pivot far from the rest.
+// Statistics are those of x less a pivot, a thread's first value: a batch of its
+// values gives its mean and the squares about that mean, both from registers, and
+// (count, mean, squares) of two sets are joined; sets of several threads and chunks
+// are added in double. So values far from zero lose nothing to cancellation. What
+// passes between workgroups is a float less a pivot of the whole group. One far
+// from the rest would round it to the distance (one pixel of 1024 x 1024 off by
+// 10^4 deviations, as the pivot: the mean off by 4e-5 deviations), so that pivot is
+// the middle one of three values.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -199,7 +203,17 @@ struct Place {
 __device__ __forceinline__ float2 shfl_xor(float2 x, uint32_t o) {
     return make_float2(__shfl_xor(x.x, o), __shfl_xor(x.y, o));
 }
+__device__ __forceinline__ double2 shfl_xor(double2 x, uint32_t o) {
+    return make_double2(__shfl_xor(x.x, o), __shfl_xor(x.y, o));
+}
 __device__ __forceinline__ float shfl_xor(float x, uint32_t o) { return __shfl_xor(x, o); }
+
+__device__ __forceinline__ void accumulate(float& a, float b) { a += b; }
+template <typename N>
+__device__ __forceinline__ void accumulate(N& a, N b) {
+    a.x += b.x;
+    a.y += b.y;
+}
 
 // (n, mean, squares about it) of two sets joined.
 __device__ __forceinline__ void join(float& n, float& mean, float& m2, float nb, float meanb,
@@ -209,44 +223,55 @@ __device__ __forceinline__ void join(float& n, float& mean, float& m2, float nb,
     m2 += m2b + d * d * (n * share);
 }
 
-// Sums over a workgroup. Each thread has left S pairs, its vector's channels or
-// groups, in red[s][thread]; sum k is that of the rows and of the `per`
-// entries k per .. of a row, counted through its vectors. use(k, sum) is
-// called by one thread for each of the n sums. A power of two of lanes take
-// one sum; all threads call this.
-template <int S, uint32_t THREADS, typename Use>
-__device__ __forceinline__ void add_all(const float2 (*red)[THREADS], uint32_t rows, uint32_t nv,
-                                        uint32_t per, uint32_t n, Use&& use) {
-    uint32_t lanes = 64;
-    while (lanes > 1 && lanes * n > blockDim.x) {
-        lanes >>= 1;
+// Lanes that share one of n sums or groups, as a power of two: so many that the
+// workgroup takes all of them at once if it can.
+__device__ __forceinline__ uint32_t lanes_of(uint32_t n) {
+    uint32_t shift = 6;
+    while (shift > 0 && (n << shift) > blockDim.x) {
+        shift--;
     }
-    uint32_t lr = lanes;  // of them, side by side over the rows
-    while (lr > 1 && lr >= 2 * rows) {
-        lr >>= 1;
+    return shift;
+}
+
+// Sums over a workgroup. Each thread has left S entries, of its vector's channels
+// or groups; sum k is that of terms(k)(s, thread, row), entry s of a thread, over
+// the rows and the `per` entries k per .. of a row, counted through its vectors.
+// use(k, sum) is called by the first of the lanes that take a sum; all threads
+// call this.
+template <int S, typename N, typename Terms, typename Use>
+__device__ __forceinline__ void add_terms(uint32_t rows, uint32_t nv, uint32_t per, uint32_t n,
+                                          Terms&& terms, Use&& use) {
+    const uint32_t shift = lanes_of(n), lanes = 1u << shift, k0 = threadIdx.x >> shift;
+    uint32_t side = shift;  // of the lanes, side by side over the rows
+    while (side > 0 && (1u << side) >= 2 * rows) {
+        side--;
     }
-    const uint32_t lq = lanes / lr, lane = threadIdx.x & (lanes - 1);
-    for (uint32_t k = threadIdx.x / lanes; k - threadIdx.x / lanes < n; k += blockDim.x / lanes) {
-        float2 s = make_float2(0.f, 0.f);
+    const uint32_t lane = threadIdx.x & (lanes - 1), lr = 1u << side;
+    for (uint32_t k = k0; k - k0 < n; k += blockDim.x >> shift) {
+        N s{};
         if (k < n) {
-            for (uint32_t q = lane / lr; q < per; q += lq) {
+            const auto term = terms(k);
+            for (uint32_t q = lane >> side; q < per; q += lanes >> side) {
                 const uint32_t entry = k * per + q, at = entry / S;
                 for (uint32_t r = lane & (lr - 1); r < rows; r += lr) {
-                    const float2 x = red[entry - at * S][r * nv + at];
-                    s.x += x.x;
-                    s.y += x.y;
+                    accumulate(s, term(entry - at * S, r * nv + at, r));
                 }
             }
         }
         for (uint32_t o = 1; o < lanes; o <<= 1) {
-            const float2 x = shfl_xor(s, o);
-            s.x += x.x;
-            s.y += x.y;
+            accumulate(s, shfl_xor(s, o));
         }
         if (k < n && lane == 0) {
             use(k, s);
         }
     }
+}
+// Of pairs in red[s][thread].
+template <int S, uint32_t THREADS, typename Use>
+__device__ __forceinline__ void add_all(const float2 (*red)[THREADS], uint32_t rows, uint32_t nv,
+                                        uint32_t per, uint32_t n, Use&& use) {
+    const auto term = [&](uint32_t s, uint32_t i, uint32_t) { return red[s][i]; };
+    add_terms<S, float2>(rows, nv, per, n, [&](uint32_t) { return term; }, use);
 }
 
 // ---------------------------------------------------------------------------
@@ -400,12 +425,23 @@ __device__ __forceinline__ void load_batch(const T* p, size_t stride, uint32_t c
     }
 }
 
-// The value of a group's first channel at the item's first pixel.
+// What a group's values are taken less: the middle one of its first channel's
+// values at three of the item's pixels, about a quarter of it apart and in no
+// common column. What is far from the rest (a few pixels, a patch of them, a
+// border) does not have two of the three. Loaded early and looked at late.
 template <typename T>
-__device__ __forceinline__ float pivot_of(const T* x, const Cut& c, uint32_t item,
-                                          uint32_t group) {
-    return to_float(x[(size_t)item * c.item_stride + (size_t)group * c.group_ch]);
-}
+struct Pivot {
+    T v[3];
+    __device__ __forceinline__ void load(const T* x, const Cut& c, uint32_t item, uint32_t group) {
+        const T* p = x + (size_t)item * c.item_stride + (size_t)group * c.group_ch;
+        v[0] = p[((c.n_px * 15467) >> 16) * c.px_stride];
+        v[1] = p[((c.n_px * 33461) >> 16) * c.px_stride];
+        v[2] = p[((c.n_px * 50159) >> 16) * c.px_stride];
+    }
+    __device__ __forceinline__ float value() const {
+        return __builtin_amdgcn_fmed3f(to_float(v[0]), to_float(v[1]), to_float(v[2]));
+    }
+};
 
 // Group (of the image) of set g of vector `vec`.
 template <int V, int S>
@@ -420,7 +456,7 @@ template <typename T, int V, int S>
 __global__ __launch_bounds__(kMaxThreads) void k_gn_stats(const T* x, const Cut c, float2* part) {
     constexpr uint32_t kBatch = kBatchOf<T, V, S>;
     __shared__ float2 red[S][kMaxThreads];
-    __shared__ float first[S * kMaxVecs];
+    __shared__ float about[S][kMaxThreads];
     const Place at(c);
     const uint32_t item = blockIdx.x / c.chunks, chunk = blockIdx.x - item * c.chunks;
     const uint32_t vec = c.first_vec(blockIdx.y) + at.vec, group0 = c.first_group(blockIdx.y);
@@ -429,66 +465,66 @@ __global__ __launch_bounds__(kMaxThreads) void k_gn_stats(const T* x, const Cut 
     for (int g = 0; g < S; g++) {
         mean[g] = m2[g] = pivot[g] = 0.f;
     }
+    const uint32_t groups = c.groups(blockIdx.y), mine = threadIdx.x >> lanes_of(groups);
+    Pivot<T> base;
+    base.load(x, c, item, group0 + std::min(mine, groups - 1));
     uint32_t left = at.pixels(c, chunk);
     if (left > 0) {
         const T* p = x + (size_t)item * c.item_stride +
                      ((size_t)chunk * c.chunk_px + at.row) * c.px_stride + (size_t)vec * V;
         const size_t step = (size_t)c.rows * c.px_stride;
-#pragma unroll
-        for (int g = 0; g < S; g++) {
-            pivot[g] = pivot_of(x, c, item, group_of<V, S>(c, vec, g));
-        }
         const uint32_t keep = c.keep_px / c.rows;
         uint32_t count = left % kBatch ? left % kBatch : kBatch;
         while (left > 0) {
             Pack<T, V> v[kBatch];
             load_batch<T, V, kBatch>(p, step, count, left > keep, v);
+#pragma unroll
+            for (int g = 0; g < S; g++) {
+                pivot[g] = n > 0.f ? pivot[g] : to_float(v[0].v[g * (V / S)]);
+            }
             add_batch<T, V, S, kBatch>(v, count, pivot, n, mean, m2);
             left -= count;
             p += count * step;
             count = kBatch;
         }
     }
-    // sums and squares about the mean of one of the group's threads: small, so
-    // that they can be added as they are
-    const uint32_t groups = c.groups(blockIdx.y);
-    if (at.row == 0) {
-#pragma unroll
-        for (int g = 0; g < S; g++) {
-            const uint32_t k = group_of<V, S>(c, vec, g) - group0;
-            if (at.vec == 0 || (vec * V + g * (V / S)) % c.group_ch == 0) {
-                first[k] = mean[g];
-            }
-        }
-    }
-    __syncthreads();
+    const uint32_t len = c.px_of(chunk), entries = at.nv * S / groups;
     if (at.live) {
 #pragma unroll
         for (int g = 0; g < S; g++) {
-            const float d = mean[g] - first[group_of<V, S>(c, vec, g) - group0];
-            red[g][threadIdx.x] = n > 0.f ? make_float2(n * d, fmaf(n * d, d, m2[g]))
-                                          : make_float2(0.f, 0.f);
+            red[g][threadIdx.x] = make_float2(mean[g], m2[g]);
+            about[g][threadIdx.x] = pivot[g];
         }
     }
     __syncthreads();
-    const uint32_t entries = at.nv * S / groups;
-    const float values = (float)c.px_of(chunk) * (float)(entries * (V / S));
-    add_all<S, kMaxThreads>(red, c.rows, at.nv, entries, groups, [&](uint32_t k, float2 s) {
-        const float d = s.x / values;
-        const uint32_t slot = c.parts == 1 ? group0 + k : blockIdx.y;
-        part[((size_t)item * c.n_groups * c.parts + slot) * c.chunks + chunk] =
-            make_float2(first[k] + d, fmaf(-s.x, d, s.y));
-    });
-}
-
-// Lanes that share the joining of one group's chunks: a power of two, so that
-// the workgroup takes all of its groups at once if it can.
-__device__ __forceinline__ uint32_t lanes_of_group(uint32_t groups) {
-    uint32_t l = 64;
-    while (l > 1 && l * groups > blockDim.x) {
-        l >>= 1;
-    }
-    return l;
+    // the chunk's sums and squares about one of its pivots in double, where their
+    // difference loses nothing to a thread's values far from the others'
+    const auto pivot_of_group = [&](uint32_t k) {
+        return (double)about[k * entries % S][k * entries / S];
+    };
+    const double values = (double)len * (double)(entries * (V / S));
+    // of a thread: of the first len % rows rows, and of the others
+    const uint32_t over = len % c.rows;
+    const double most = (double)((len / c.rows + 1) * (V / S)), least = most - (double)(V / S);
+    add_terms<S, double2>(
+        c.rows, at.nv, entries, groups,
+        [&](uint32_t k) {
+            return [&, p = pivot_of_group(k)](uint32_t set, uint32_t i, uint32_t row) {
+                const float2 x = red[set][i];
+                const double m = ((double)about[set][i] - p) + (double)x.x;
+                const double n = row < over ? most : least, s = n * m;
+                return make_double2(s, fma(s, m, (double)x.y));
+            };
+        },
+        [&](uint32_t k, double2 s) {
+            const double d = s.x / values;
+            if (k != mine) {
+                base.load(x, c, item, group0 + k);
+            }
+            const uint32_t slot = c.parts == 1 ? group0 + k : blockIdx.y;
+            part[((size_t)item * c.n_groups * c.parts + slot) * c.chunks + chunk] = make_float2(
+                (float)(pivot_of_group(k) - (double)base.value() + d), (float)fma(-s.x, d, s.y));
+        });
 }
 
 // (mean, 1 / sqrt(var + eps)) of the block's groups into `stat`: sums and
@@ -497,12 +533,14 @@ template <typename T, int V>
 __device__ __forceinline__ void join_chunks(const T* x, const Cut& c, uint32_t item,
                                             const float2* part, float eps, float2* stat) {
     const uint32_t groups = c.groups(blockIdx.y), group0 = c.first_group(blockIdx.y);
-    const uint32_t lanes = lanes_of_group(groups), lane = threadIdx.x & (lanes - 1);
+    const uint32_t shift = lanes_of(groups), lanes = 1u << shift, g0 = threadIdx.x >> shift;
+    const uint32_t lane = threadIdx.x & (lanes - 1);
     const double last = (double)c.px_of(c.chunks - 1);
-    for (uint32_t g = threadIdx.x / lanes; g - threadIdx.x / lanes < groups;
-         g += blockDim.x / lanes) {
+    for (uint32_t g = g0; g - g0 < groups; g += blockDim.x >> shift) {
         double s = 0.0, q = 0.0;
+        Pivot<T> pivot;
         if (g < groups) {
+            pivot.load(x, c, item, group0 + g);
             const float2* p =
                 part + ((size_t)item * c.n_groups + group0 + g) * c.parts * c.chunks;
             for (uint32_t k = 0; k < c.parts; k++, p += c.chunks) {
@@ -526,8 +564,7 @@ __device__ __forceinline__ void join_chunks(const T* x, const Cut& c, uint32_t i
             const double n = (double)c.n_px * c.group_ch, mean = s / n;
             const double m2 = q - s * mean;
             const float var = m2 < 0.0 ? 0.f : (float)(m2 / n);  // a NaN stays one
-            stat[g] = make_float2(pivot_of(x, c, item, group0 + g) + (float)mean,
-                                  1.f / sqrtf(var + eps));
+            stat[g] = make_float2((float)((double)pivot.value() + mean), 1.f / sqrtf(var + eps));
         }
     }
     __syncthreads();
@@ -691,12 +728,6 @@ struct ItemPlace {
     }
 };
 
-__device__ __forceinline__ void accumulate(float& a, float b) { a += b; }
-__device__ __forceinline__ void accumulate(float2& a, float2 b) {
-    a.x += b.x;
-    a.y += b.y;
-}
-
 // The sum of `s` over the thread's group; every thread calls it, those without
 // pixels with 0. `part` is not reused before the next barrier but one.
 template <typename N>
@@ -763,8 +794,10 @@ __global__ __launch_bounds__(kItemThreads) void k_gn_item(const T* x, const Cut 
     }
     float w[V], b[V], pivot = 0.f;
     if (at.mine > 0) {
+        Pivot<T> p3;
+        p3.load(x, c, item, group);
         load_affine<V>(aff, vec * V, w, b);
-        pivot = pivot_of(x, c, item, group);
+        pivot = p3.value();
     }
     const float values = (float)c.n_px * (float)c.group_ch;
     float s = 0.f, q = 0.f;
@@ -1061,10 +1094,10 @@ __global__ __launch_bounds__(kMaxThreads) void k_gn_bwd_apply(const T* gy, const
     }
     {
         const uint32_t groups = c.groups(blockIdx.y), entries = c.parts * c.chunks;
-        const uint32_t lanes = lanes_of_group(groups), lane = threadIdx.x & (lanes - 1);
+        const uint32_t shift = lanes_of(groups), lanes = 1u << shift, g0 = threadIdx.x >> shift;
+        const uint32_t lane = threadIdx.x & (lanes - 1);
         const float inv = 1.f / ((float)c.n_px * (float)c.group_ch);
-        for (uint32_t g = threadIdx.x / lanes; g - threadIdx.x / lanes < groups;
-             g += blockDim.x / lanes) {
+        for (uint32_t g = g0; g - g0 < groups; g += blockDim.x >> shift) {
             float2 s = make_float2(0.f, 0.f);
             if (g < groups) {
                 const float2* e0 = group_part + ((size_t)item * c.n_groups + group0 + g) * entries;

@@ -62,3 +62,51 @@ def test_relu_masks_what_it_gave_as_zero(ctx, shape, groups):
     _, _, gb = K.group_norm_bwd(ctx, torch.ones_like(x), x, mean, rstd, groups, w, b, "relu",
                                 (False, False, True))
     assert torch.equal(gb.double(), (y > 0).view(-1, c).double().sum(0))
+
+
+@pytest.mark.parametrize("hw", [32, 256, 1024])
+@pytest.mark.parametrize("kind", TYPES, ids=str)
+@pytest.mark.parametrize("where", [0.0, 0.25, 0.5, 0.75, 1.0])
+def test_one_pixel_far_from_the_rest(ctx, hw, kind, where):
+    """One pixel 10^4 deviations off, wherever it is, costs the others nothing: the mean within 64
+    roundings of a value's usual size (not of the far one's), the deviation and the outputs within
+    64 of their own."""
+    print(f"[group_norm far] {hw} {kind} {where}", flush=True)
+    x, _, _, _ = _inputs((1, hw, hw, 8), kind, 3)
+    x.view(-1, 8)[min(hw * hw - 1, int(hw * hw * where))] = 1e4
+    _check_far(ctx, x)
+
+
+@pytest.mark.parametrize("hw", [64, 256, 1024])
+@pytest.mark.parametrize("kind", TYPES, ids=str)
+@pytest.mark.parametrize("side", ["left", "top", "frame", "corner"])
+def test_a_border_far_from_the_rest(ctx, hw, kind, side):
+    """The same for a column, a row, a frame or a patch."""
+    print(f"[group_norm border] {hw} {kind} {side}", flush=True)
+    x, _, _, _ = _inputs((1, hw, hw, 8), kind, 3)
+    if side == "corner":
+        x[:, :hw // 8, :hw // 8] = -1e4
+    if side in ("left", "frame"):
+        x[:, :, 0] = 1e4
+    if side in ("top", "frame"):
+        x[:, 0] = 1e4
+    if side == "frame":
+        x[:, -1] = x[:, :, -1] = 1e4
+    _check_far(ctx, x)
+
+
+def _check_far(ctx, x):
+    from opendressi_amd import ops as K
+    y, mean, rstd = K.group_norm(ctx, x, 2)
+    xd = x.double().view(-1, 2, 4)
+    exact = xd.mean((0, 2))
+    dev = torch.sqrt((xd - exact[:, None]).square().mean((0, 2)) + 1e-5)
+    u = 2.0 ** -24
+    # E|x| of the rest is 0.8, and the far value adds its share
+    tol = 64 * u * (0.8 + exact.abs())
+    assert ((mean[0].double() - exact).abs() <= tol).all(), (mean[0].double() - exact).abs().max()
+    assert ((rstd[0].double() * dev - 1).abs() <= 64 * u).all()
+    want = (xd - exact[:, None]) / dev[:, None]
+    half = torch.finfo(x.dtype).eps / 2 if x.dtype != torch.float32 else 0.0
+    err = (y.double().view(-1, 2, 4) - want).abs()
+    assert (err <= (tol / dev)[:, None] + (72 * u + half) * want.abs() + 2.0 ** -25).all()
