@@ -281,21 +281,46 @@ __device__ __forceinline__ void add_all(const float2 (*red)[THREADS], uint32_t r
 __device__ __forceinline__ float sigmoid(float z) {
     return __builtin_amdgcn_rcpf(1.f + __expf(-z));  // an ulp of each
 }
-// The normal distribution's Phi(z), given e = exp(-z^2 / 2): Abramowitz and
-// Stegun's 7.1.26, erf to 1.5e-7, which is Phi to the rounding of a float near 1.
-// It shares e with the density (2 x 512 x 512 x 88 float16 backward: 108 us, 159
-// with a library erf beside the exponential).
-__device__ __forceinline__ float gauss_cdf(float z, float e) {
+// The normal distribution's Phi(z) and e = exp(-z^2 / 2), its tail beyond |z| being
+// e times a smooth function of |z|, for 16-bit images Abramowitz and Stegun's
+// 7.1.26: erf to 1.5e-7, a rounding of a float near 1 (2 x 512 x 512 x 88 float16
+// backward: 108 us, 159 with a library erf beside the exponential).
+template <typename T>
+__device__ __forceinline__ void gauss(float z, float& cdf, float& e) {
+    e = __expf(-0.5f * z * z);
     const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f * 0.70710678f, fabsf(z), 1.f));
     float q = fmaf(1.061405429f, t, -1.453152027f);
     q = fmaf(q, t, 1.421413741f);
     q = fmaf(q, t, -0.284496736f);
     q = fmaf(q, t, 0.254829592f);
-    q *= 0.5f * t * e;  // of the tail beyond |z|
-    return z < 0.f ? q : 1.f - q;
+    q *= 0.5f * t * e;
+    cdf = z < 0.f ? q : 1.f - q;
+}
+// For float images 1/2 + s P(s), s = a / (1 + a), a = 0.26 |z|: P fitted to the least
+// relative error over |z| < 14 (7e-9; past it e is zero), its coefficients rounded
+// one after the other. Near z = 0, where a function of t = 1 / (1 + a) takes every
+// rounding of t, little is added to the 1/2. The error of z Phi(z) over normal z is
+// 2.2e-8 (7.1.26: 5.6e-8; 0.5 (1 + erf) in floats: 2.5e-8), of its slope 2.6e-8
+// (6.6e-8, 2.7e-8). 2 x 512 x 512 x 88 takes 109 and 183 us with it and 104 and 181
+// with 7.1.26; with it float16 images would take 78 and 130, not 70 and 118.
+template <>
+__device__ __forceinline__ void gauss<float>(float z, float& cdf, float& e) {
+    e = __expf(-0.5f * z * z);
+    const float a = 0.26f * fminf(fabsf(z), 14.f);
+    const float s = a * __builtin_amdgcn_rcpf(1.f + a);
+    float q = fmaf(-0.0338316262f, s, 0.134448603f);
+    q = fmaf(q, s, -0.147560731f);
+    q = fmaf(q, s, -0.0892333016f);
+    q = fmaf(q, s, 0.168799251f);
+    q = fmaf(q, s, 0.542275906f);
+    q = fmaf(q, s, -1.70436502f);
+    q = fmaf(q, s, 2.16385388f);
+    q = fmaf(q, s, -1.53439391f);
+    q = fmaf(q, s, 0.5f);
+    cdf = z < 0.f ? q * e : fmaf(-q, e, 1.f);
 }
 
-template <int V>
+template <typename T, int V>
 __device__ __forceinline__ void act_values(uint32_t act, float (&z)[V]) {
     switch (act) {
         case DRESSI_ACT_RELU:
@@ -313,7 +338,9 @@ __device__ __forceinline__ void act_values(uint32_t act, float (&z)[V]) {
         case DRESSI_ACT_GELU:
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                z[j] *= gauss_cdf(z[j], __expf(-0.5f * z[j] * z[j]));
+                float cdf, e;
+                gauss<T>(z[j], cdf, e);
+                z[j] *= cdf;
             }
             break;
         default:
@@ -322,7 +349,7 @@ __device__ __forceinline__ void act_values(uint32_t act, float (&z)[V]) {
 }
 
 // g times the activation's slope at z
-template <int V>
+template <typename T, int V>
 __device__ __forceinline__ void act_slopes(uint32_t act, const float (&z)[V], float (&g)[V]) {
     switch (act) {
         case DRESSI_ACT_RELU:
@@ -341,8 +368,9 @@ __device__ __forceinline__ void act_slopes(uint32_t act, const float (&z)[V], fl
         case DRESSI_ACT_GELU:
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                const float e = __expf(-0.5f * z[j] * z[j]);
-                g[j] *= fmaf(z[j] * 0.39894228f, e, gauss_cdf(z[j], e));
+                float cdf, e;
+                gauss<T>(z[j], cdf, e);
+                g[j] *= fmaf(z[j] * 0.39894228f, e, cdf);
             }
             break;
         default:
@@ -641,7 +669,7 @@ __device__ __forceinline__ void normalise(const Pack<T, V>& x, const float (&mea
     for (int j = 0; j < V; j++) {
         v[j] = fmaf(v[j] - mean[j / (V / S)], ws[j], b[j]);
     }
-    act_values<V>(act, v);
+    act_values<T, V>(act, v);
     put<T, V>(y, v, stream);
 }
 
@@ -884,7 +912,7 @@ struct Channels {
             xh[j] = d * rstd[j / (V / S)];
             z[j] = fmaf(d, ws[j], b[j]);
         }
-        act_slopes<V>(act, z, gz);
+        act_slopes<T, V>(act, z, gz);
     }
     template <typename T>
     __device__ __forceinline__ void add(const Pack<T, V>& x, const Pack<T, V>& gy, uint32_t act,

@@ -110,3 +110,48 @@ def _check_far(ctx, x):
     half = torch.finfo(x.dtype).eps / 2 if x.dtype != torch.float32 else 0.0
     err = (y.double().view(-1, 2, 4) - want).abs()
     assert (err <= (tol / dev)[:, None] + (72 * u + half) * want.abs() + 2.0 ** -25).all()
+
+
+def _rms(t):
+    return float(t.double().square().mean().sqrt())
+
+
+def test_gelu_is_as_good_as_its_formula_in_floats(ctx):
+    """float32 images: the error of z Phi(z) and of its slope over normal z, against those of
+    z 0.5 (1 + erf(z / sqrt 2)) and of its derivative in float32, whose roundings are as many (a
+    quarter more for their other order)."""
+    from opendressi_amd import ops as K
+    x = _inputs((1, 512, 512, 8), torch.float32, 4)[0]
+    z, mean, rstd = K.group_norm(ctx, x, 1)
+    y = K.group_norm(ctx, x, 1, activation="gelu")[0]
+    plain = z * (0.5 * (1 + torch.erf(z * 0.5 ** 0.5)))
+    want = z.double() * torch.special.ndtr(z.double())
+    assert _rms(y - want) <= 1.25 * _rms(plain - want)
+    # z is the bias where x has no variance; two pixels' slopes add up to twice one's
+    b = _inputs((1, 2 ** 16), torch.float32, 5)[0][0]
+    x = torch.zeros((1, 2, 2 ** 16), device="cuda")
+    _, mean, rstd = K.group_norm(ctx, x, 1, None, b, activation="gelu")
+    slope = K.group_norm_bwd(ctx, torch.ones_like(x), x, mean, rstd, 1, None, b, "gelu")[2] / 2
+    d, pdf = b.double(), 1 / math.sqrt(2 * math.pi)
+    want = torch.special.ndtr(d) + d * torch.exp(-0.5 * d * d) * pdf
+    plain = 0.5 * (1 + torch.erf(b * 0.5 ** 0.5)) + b * torch.exp(-0.5 * b * b) * pdf
+    assert _rms(slope - want) <= 1.25 * _rms(plain - want)
+
+
+def test_gelu_tail(ctx):
+    """z Phi(z) of float32 images below zero, relative to itself: 2^-24 (z^2 + 6 |z| + 16), of the
+    exponent's two roundings, of the tail's factor (0.4 / |z| as a difference from a half) and of
+    the rest."""
+    from opendressi_amd import ops as K
+    b = torch.linspace(-12.0, -1e-3, 2 ** 16, device="cuda")
+    x = torch.zeros((1, 2, 2 ** 16), device="cuda")
+    y = K.group_norm(ctx, x, 1, None, b, activation="gelu")[0][0]
+    d = b.double()
+    want = d * 0.5 * torch.special.erfc(-d * math.sqrt(0.5))
+    tol = 2.0 ** -24 * (d * d + 6 * d.abs() + 16)
+    assert ((y.double() / want - 1).abs() <= tol).all()
+    far = torch.tensor([-math.inf, -1e30, -40.0, 0.0, 40.0, 1e30, math.inf, math.nan],
+                       device="cuda")
+    y = K.group_norm(ctx, torch.zeros((1, 2, 8), device="cuda"), 1, None, far,
+                     activation="gelu")[0][0, 0]
+    assert y[0].isnan() and not y[1:4].any() and torch.equal(y[4:7], far[4:7]) and y[7].isnan()
