@@ -146,6 +146,8 @@ Cut make_cut(uint32_t n_items, uint64_t n_px, uint32_t n_ch, uint32_t n_groups, 
 // For one pass: a workgroup holds all pixels of a block, at most `hold` vectors a
 // thread; a row's vectors lie in one wave. chunks is 0 where they are too many.
 // Blocks take as many groups as leave 256 workgroups: their reads are longer then.
+// They are the launch's y, which ends at kMaxBatchItems; two passes, whose blocks
+// hold 129 vectors at least or all groups, stay far below it.
 Cut make_item_cut(uint32_t n_items, uint64_t n_px, uint32_t n_ch, uint32_t n_groups,
                   uint32_t v, uint32_t hold) {
     const uint64_t most = std::max<uint64_t>(1, (uint64_t)n_items * n_groups / 256);
@@ -159,7 +161,7 @@ Cut make_item_cut(uint32_t n_items, uint64_t n_px, uint32_t n_ch, uint32_t n_gro
             lanes *= 2;
         }
         c.rows = kItemThreads / lanes;
-        if (n_px <= (uint64_t)c.rows * hold) {
+        if (n_px <= (uint64_t)c.rows * hold && c.n_blocks <= kMaxBatchItems) {
             // no more rows than pixels, in whole waves
             const uint64_t need = (n_px * lanes + 63) / 64 * 64;
             c.threads = (uint32_t)std::min<uint64_t>(kItemThreads, need);

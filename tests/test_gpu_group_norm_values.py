@@ -155,3 +155,41 @@ def test_gelu_tail(ctx):
     y = K.group_norm(ctx, torch.zeros((1, 2, 8), device="cuda"), 1, None, far,
                      activation="gelu")[0][0, 0]
     assert y[0].isnan() and not y[1:4].any() and torch.equal(y[4:7], far[4:7]) and y[7].isnan()
+
+
+@pytest.mark.parametrize("shape,groups", [((1, 64, 64, 131072), 131072),
+                                          ((2, 48, 48, 69632), 69632)], ids=str)
+def test_more_groups_than_a_launch_has_rows(ctx, shape, groups):
+    """One channel a group, more of them than a launch's y dimension goes: statistics, outputs and
+    gradients of a stretch of channels at each end and in the midst, against float64."""
+    from opendressi_amd import ops as K
+    print(f"[group_norm groups] {shape} {groups}", flush=True)
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    x = torch.empty(shape, device="cuda").normal_(generator=gen)
+    gy = torch.empty(shape, device="cuda").normal_(generator=gen)
+    w = torch.rand(groups, generator=gen, device="cuda") + 0.5
+    y, mean, rstd = K.group_norm(ctx, x, groups, w, None, 1e-5, "none")
+    gx, gw, _ = K.group_norm_bwd(ctx, gy, x, mean, rstd, groups, w, None, "none",
+                                 (True, True, False))
+    u, n = 2.0 ** -24, shape[1] * shape[2]
+    for a in (0, 65530, groups - 64):
+        part = (slice(None),) * 3 + (slice(a, a + 64),)
+        d, g = x[part].double(), gy[part].double()
+        m, v = d.mean((1, 2)), d.var((1, 2), correction=0)
+        r = 1 / torch.sqrt(v + 1e-5)
+        assert ((mean[:, a:a + 64] - m).abs() <= 64 * u).all()
+        assert ((rstd[:, a:a + 64] / r - 1).abs() <= 64 * u).all()
+        at = lambda t: t[:, None, None]  # noqa: E731
+        xh, ww = (d - at(m)) * at(r), w[a:a + 64].double()
+        # 64 roundings of the mean and of the deviation, 8 of the arithmetic
+        assert ((y[part] - xh * ww).abs() <= u * ww * (72 * xh.abs() + 72 * at(r))).all()
+        # sums of n products in float32, in sequences of up to 2^11 and then by halves
+        length = 2 * u * (math.sqrt(min(n * shape[0], 2 ** 11)) + 24)
+        want = (g * xh).sum((0, 1, 2))
+        assert ((gw[a:a + 64] - want).abs() <= (length + 144 * u) * (g.abs() * (xh.abs() + 1)).sum(
+            (0, 1, 2))).all()
+        mg, mgx = (at(t.mean((1, 2))) for t in (g, g * xh))
+        want = at(r) * ww * (g - mg - xh * mgx)
+        size = at(r) * ww * (g.abs() + at(g.abs().mean((1, 2))) +
+                             xh.abs() * at((g * xh).abs().mean((1, 2))))
+        assert ((gx[part] - want).abs() <= (length + 160 * u) * (size + at(r) * ww)).all()
