@@ -1085,7 +1085,7 @@ __global__ __launch_bounds__(kMaxThreads) void k_gn_param_grad(const ParamGrad a
 }
 
 // The second pass, backwards like the forward one; 4 x 1024 x 1024 x 64 bfloat16:
-// 284 us, 5.7 TB/s. The last `extra` workgroups take gw and gb.
+// 284 us, 5.7 TB/s. The last `extra` columns of workgroups take gw and gb.
 template <typename T, int V, int S>
 __global__ __launch_bounds__(kMaxThreads) void k_gn_bwd_apply(const T* gy, const T* x, const Cut c,
                                                               const Affine aff, uint32_t act,
@@ -1097,9 +1097,7 @@ __global__ __launch_bounds__(kMaxThreads) void k_gn_bwd_apply(const T* gy, const
     __shared__ float2 mean_of[S * kMaxVecs];
     const uint32_t units = gridDim.x - extra;
     if (blockIdx.x >= units) {
-        if (blockIdx.y == 0) {
-            param_grad(params, blockIdx.x - units);
-        }
+        param_grad(params, (blockIdx.x - units) * gridDim.y + blockIdx.y);
         return;
     }
     const Place at(c);
@@ -1459,7 +1457,7 @@ int launch_backward(hipStream_t s, const Cut& c, const void* gy, const void* x, 
     const uint32_t most = items_at_once(c);
     for (uint32_t i = 0; i < c.n_items; i += most) {
         const uint32_t items = std::min(most, c.n_items - i);
-        const uint32_t extra = i + items == c.n_items && (gw || gb) ? div_up(c.n_ch, kParamCh) : 0;
+        const uint32_t extra = i + items == c.n_items && (gw || gb) ? div_up(div_up(c.n_ch, kParamCh), c.n_blocks) : 0;
         const size_t at = (size_t)i * c.n_px * c.n_ch, g = (size_t)i * c.n_groups;
         hipLaunchKernelGGL((k_gn_bwd_apply<T, V, S>), dim3(items * c.chunks + extra, c.n_blocks),
                            block, 0, s, (const T*)gy + at,
