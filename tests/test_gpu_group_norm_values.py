@@ -193,3 +193,70 @@ def test_more_groups_than_a_launch_has_rows(ctx, shape, groups):
         size = at(r) * ww * (g.abs() + at(g.abs().mean((1, 2))) +
                              xh.abs() * at((g * xh).abs().mean((1, 2))))
         assert ((gx[part] - want).abs() <= (length + 160 * u) * (size + at(r) * ww)).all()
+
+
+def _check_sparse(x, gy, mean, rstd, groups, at, got):
+    """Gradients where gy is zero but at the pixels `at` of x [N, P, C] (item, pixel), from the
+    formula in float64 with the forward pass's statistics: what a call leaves out, or takes twice,
+    is as large as the sums themselves."""
+    gx, gw, gb = got
+    n, px, c = x.shape
+    per = c // groups
+    i, p = (torch.tensor(t, device="cuda") for t in zip(*at))
+    g, d = gy[i, p].double(), x[i, p].double()
+    m, r = (t[i].double().repeat_interleave(per, 1) for t in (mean, rstd))
+    xh = (d - m) * r
+    u = 2.0 ** -24
+    # a few terms each: a rounding of the sum, 4 of xh
+    assert ((gb - g.sum(0)).abs() <= 8 * u * g.abs().sum(0)).all()
+    assert ((gw - (g * xh).sum(0)).abs() <= 16 * u * (g * (xh.abs() + m.abs() * r)).abs().sum(0)).all()
+    # gx = rstd (gy - A - xh B), A and B the item's sums over its values
+    sums = torch.zeros((2, n, groups), dtype=torch.float64, device="cuda")
+    sums[0].index_add_(0, i, g.view(-1, groups, per).sum(2))
+    sums[1].index_add_(0, i, (g * xh).view(-1, groups, per).sum(2))
+    a, b = (t[i].repeat_interleave(per, 1) / (px * per) for t in sums)
+    want = r * (g - a - xh * b)
+    half = torch.finfo(x.dtype).eps / 2
+    assert ((gx[i, p] - want).abs() <= (half + 32 * u) * r * (g.abs() + a.abs() + (xh * b).abs())
+            ).all()
+
+
+def test_gradients_past_32_bits(ctx):
+    """Gradients at a few pixels of an image of more than 2^32 values, before and behind the powers
+    of two; everywhere else gx is the means' share alone."""
+    from opendressi_amd import ops as K
+    n_px, c = 2 ** 29 + 1031, 8
+    gen = torch.Generator(device="cuda").manual_seed(15)
+    x = torch.empty((1, n_px, c), dtype=torch.bfloat16, device="cuda").normal_(generator=gen)
+    mean, rstd = K.group_norm(ctx, x, 2)[1:]
+    at = [(0, p) for p in (0, 5, 2 ** 28, 2 ** 29 - 1, 2 ** 29, 2 ** 29 + 517, n_px - 1)]
+    gy = torch.zeros_like(x)
+    for _, p in at:
+        gy[0, p].normal_(generator=gen)
+    gx, gw, gb = K.group_norm_bwd(ctx, gy, x, mean, rstd, 2)
+    _check_sparse(x, gy, mean, rstd, 2, at, (gx, gw, gb))
+    for _, p in at:
+        gx[0, p] = 0
+    # seven pixels' sums over 2^31 values, times |xh| of at most 10
+    for part in gx[0].split(2 ** 27):
+        assert part.isfinite().all() and float(part.abs().max()) <= 1e-6
+
+
+@pytest.mark.parametrize("c", [8, 520])
+def test_gradients_of_more_items_than_a_launch(ctx, c):
+    """Gradients of a few rows, before and behind the first launch's last: gw and gb have each of
+    them once, and gx is theirs."""
+    from opendressi_amd import ops as K
+    n = 2 ** 22 + 5
+    gen = torch.Generator(device="cuda").manual_seed(16)
+    x = torch.empty((n, 1, c), dtype=torch.bfloat16, device="cuda").normal_(generator=gen)
+    mean, rstd = K.group_norm(ctx, x, 2)[1:]
+    at = [(i, 0) for i in (0, 7, 2 ** 21, 2 ** 22 - 1, 2 ** 22, 2 ** 22 + 2, n - 1)]
+    gy = torch.zeros_like(x)
+    for i, _ in at:
+        gy[i].normal_(generator=gen)
+    gx, gw, gb = K.group_norm_bwd(ctx, gy, x, mean, rstd, 2)
+    _check_sparse(x, gy, mean, rstd, 2, at, (gx, gw, gb))
+    rest = torch.ones(n, dtype=torch.bool, device="cuda")
+    rest[[i for i, _ in at]] = False
+    assert not gx[rest].any()
