@@ -362,9 +362,10 @@ class AdamW(torch.optim.Optimizer):
                 _addr(self._scales[0]), _addr(self._scales[1]), self.seed, self.max_grad_norm or 0.0,
                 self._scratch.data_ptr(), _addr(self.grad_norm), _addr(self._counts),
                 _addr(self._device_sets)))
-        with torch.no_grad():
-            for p, q in moved:
-                p.copy_(q)
+        if moved:
+            with torch.no_grad():
+                for p, q in moved:
+                    p.copy_(q)
         # written in place: a backward pass over the values before the step has to refuse them
         increment_version(self._params if every else [self._params[i] for i in live])
         self._steps = now
