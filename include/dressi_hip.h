@@ -856,7 +856,8 @@ int dressi_group_norm_bwd(dressi_ctx* ctx, const void* gy, const void* x,
  * (n floats, 16-byte aligned, or NULL; not looked at for DRESSI_F32): the
  * float copy of which a 16-bit parameter is the rounding. Where it is not,
  * the parameter has been written since, and the copy takes its value. `set`
- * names its dressi_adamw_set. */
+ * names its dressi_adamw_set. All tensors of a step are written at once: neither
+ * they nor their shares of the state overlap. */
 typedef struct dressi_adamw_tensor {
     void* param;
     const void* grad;

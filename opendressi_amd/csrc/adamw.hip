@@ -186,7 +186,10 @@ __device__ __forceinline__ uint32_t encode(float x, int up, uint32_t r) {
     return (__float_as_uint(__builtin_ldexpf(__uint_as_float(abs_bits(x)), -up)) + r) >> 20;
 }
 
-// 32 bits of element i at a step, by two rounds of multiplying and folding.
+// 32 bits of element i at a step. Folds of 16, 15 and 16 bits around products with
+// 0x7feb352d and 0x846ca68b are the 32-bit hash that C. Wellons found and published
+// (2018, by a search for the least bias); the factor of the high word is the first
+// of A. Appleby's published 32-bit finalizer (2008).
 __device__ __forceinline__ uint32_t noise(uint64_t i, uint32_t key) {
     uint32_t x = (uint32_t)i ^ key ^ ((uint32_t)(i >> 32) * 0x85ebca6bu);
     x = (x ^ (x >> 16)) * 0x7feb352du;
