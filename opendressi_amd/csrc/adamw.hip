@@ -398,10 +398,10 @@ __device__ __forceinline__ void step_tensor(const TensorArg& t, const SetArg& h,
 }
 
 // A workgroup per chunk of 1024 ITER elements of one tensor: everything is
-// read and written once, so memory bounds it. 2^28 float32 elements take 1315 us
-// with moments in 32 bits (28 bytes each, 5.7 TB/s) and 770 in 8 (16.1 bytes, 5.6
+// read and written once, so memory bounds it. 2^28 float32 elements take 1302 us
+// with moments in 32 bits (28 bytes each, 5.8 TB/s) and 734 in 8 (16.1 bytes, 5.9
 // TB/s; counters: 2.72 GB read, 1.63 written, which is what there is); 2 million,
-// clipped, 5.6 us for the norm and 11 for the step; three small tensors 3.2.
+// clipped, 5.4 us for the norm and 11.2 for the step; three small tensors 3.2.
 template <bool Q8, int ITER, bool STREAM>
 __global__ __launch_bounds__(256) void k_adamw_step(const Table tb, const State st) {
     float coef = 1.f;

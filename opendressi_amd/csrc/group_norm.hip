@@ -20,14 +20,18 @@
 // each pass's images and nothing else (counters: 4 x 1024 x 1024 x 64 bfloat16,
 // forward 537 MB read twice and written once).
 //
-// Statistics are those of x less a pivot, a thread's first value: a batch of its
-// values gives its mean and the squares about that mean, both from registers, and
-// (count, mean, squares) of two sets are joined; sets of several threads and chunks
-// are added in double. So values far from zero lose nothing to cancellation. What
-// passes between workgroups is a float less a pivot of the whole group. One far
+// Statistics are those of x less a pivot, in two passes a thread's first value: a
+// batch of its values gives its mean and the squares about that mean, both from
+// registers, and (count, mean, squares) of two sets are joined; sets of several
+// threads and chunks are added in double. So values far from zero lose nothing to cancellation. What
+// passes between workgroups, and what one pass adds up, is less a pivot of the whole
+// group. One far
 // from the rest would round it to the distance (one pixel of 1024 x 1024 off by
 // 10^4 deviations, as the pivot: the mean off by 4e-5 deviations), so that pivot is
 // the middle one of three values.
+//
+// The times beside the choices below are those of graphs of 30 calls, replayed, both
+// sides in turn; a kernel's own under the profiler are up to a microsecond longer.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -45,15 +49,15 @@ constexpr uint32_t kMaxVecs = 256;  // of a workgroup
 constexpr uint32_t kMinPixels = 2;  // that a thread should have of a chunk
 // Workgroups that a launch should have: two a compute unit. Each joins the sums of
 // its item's chunks, so more of them cost one large item (512 x 512 x 64 bfloat16
-// forward: 23 us with 512, 30 with 1024 of half the threads) and fewer leave loads
-// unissued (2 x 512 x 512 x 66: forward 50 and backward 77 us with 512, 55 and 96
-// with 256).
+// forward: 23 us with 512, 31 with 1024 of half the threads) and fewer leave loads
+// unissued (2 x 512 x 512 x 66: forward 49 and backward 77 us with 512, 53 and 94
+// with 256; 512 x 512 x 64 is level).
 constexpr uint32_t kTargetGroups = 512;
 // Pixels that a thread keeps in registers (one pass). A workgroup's reads are a
 // block's few channels of each pixel, a cache line each: past 4096 pixels
 // (backward, with three images: 2048) two passes over whole pixels take less,
-// 9.3 us against 10.8 for 64 x 64 x 32 float32 backward, 10.9 against 16 for
-// 64 x 64 x 64 bfloat16; forward they take 8.5 and 9.9 there, one pass 8.0 and 9.1.
+// 9.3 us against 11.2 for 64 x 64 x 32 float32 backward, 10.8 against 16.5 for
+// 64 x 64 x 64 bfloat16; forward they take 8.4 and 9.2 there, one pass 8.1 and 9.1.
 constexpr uint32_t kHold = 8, kHoldBwd = 4;
 constexpr uint32_t kItemThreads = 512;  // of a workgroup that holds its pixels
 
@@ -176,10 +180,10 @@ Cut make_item_cut(uint32_t n_items, uint64_t n_px, uint32_t n_ch, uint32_t n_gro
 }
 
 // Pixels of a thread in flight. Forward 4 of 16 bytes in one group (1024 x 1024 x
-// 64 bfloat16 in 8 groups: 73 us, 78 with 8), else 8 (2 x 512 x 512 x 66 in 6: 50
-// us, 54 with 4). Backward 4, of the widest vectors 2, whose registers leave too
-// few waves else (1024 x 1024 x 64 bfloat16: 123 us, 127 with 4; eight of them in
-// 16 groups: 895 and 905).
+// 64 bfloat16 in 8 groups: 71 us, 78 with 8), else 8 (2 x 512 x 512 x 66 in 6: 50
+// us, 51 with 4). Backward 4, of the widest vectors 2, whose registers leave too
+// few waves else (1024 x 1024 x 64 bfloat16: 122 us, 126 with 4; eight of them in
+// 16 groups: 903 and 918).
 template <typename T, int V, int S>
 constexpr uint32_t kBatchOf = S == 1 && sizeof(T) * V >= 16 ? 4 : 8;
 template <int V>
@@ -286,7 +290,7 @@ __device__ __forceinline__ float sigmoid(float z) {
 // The normal distribution's Phi(z) and e = exp(-z^2 / 2), its tail beyond |z| being
 // e times a smooth function of |z|, for 16-bit images Abramowitz and Stegun's
 // 7.1.26: erf to 1.5e-7, a rounding of a float near 1 (2 x 512 x 512 x 88 float16
-// backward: 108 us, 159 with a library erf beside the exponential).
+// backward: 116 us, 153 with a library erf beside the exponential).
 template <typename T>
 __device__ __forceinline__ void gauss(float z, float& cdf, float& e) {
     e = __expf(-0.5f * z * z);
@@ -480,7 +484,7 @@ __device__ __forceinline__ uint32_t group_of(const Cut& c, uint32_t vec, int g) 
 }
 
 // The first pass: each chunk's (mean less the pivot, squares) for each group.
-// 4 x 1024 x 1024 x 64 bfloat16: 82 us, 6.6 TB/s. A small image's time is that
+// 4 x 1024 x 1024 x 64 bfloat16: 84 us, 6.4 TB/s. A small image's time is that
 // of a launch and of a few loads one after another: 512 x 512 x 64 10 us.
 template <typename T, int V, int S>
 __global__ __launch_bounds__(kMaxThreads) void k_gn_stats(const T* x, const Cut c, float2* part) {
@@ -682,10 +686,10 @@ __device__ __forceinline__ uint32_t backwards(uint32_t k, uint32_t n) {
     return k < rounds * 8 ? (rounds - 1 - k / 8) * 8 + k % 8 : k;
 }
 
-// The second pass; 4 x 1024 x 1024 x 64 bfloat16: 191 us, 5.6 TB/s; 512 x 512 x
-// 64: 14.6 us. It walks the image backwards, each part on the die that
+// The second pass; 4 x 1024 x 1024 x 64 bfloat16: 192 us, 5.6 TB/s; 512 x 512 x
+// 64: 14.9 us. It walks the image backwards, each part on the die that
 // read it in the first pass: what was read last may still be in a cache (4 x 256
-// x 256 x 64 float32, both passes: 34.0 us, 36.5 with the dies mixed).
+// x 256 x 64 float32, both passes: 34.2 us, 37.3 with the dies mixed).
 template <typename T, int V, int S>
 __global__ __launch_bounds__(kMaxThreads) void k_gn_apply(const T* x, const Cut c,
                                                           const float2* part, const Affine aff,
@@ -801,8 +805,8 @@ __device__ __forceinline__ N add_item(const Cut& c, const ItemPlace& at, N s, N 
 }
 
 // Both passes where a block's pixels fit its workgroup's registers: x is read
-// once, in one launch. 8 x 32 x 32 x 256 bfloat16: 7.5 us, 10.2 in two passes;
-// 16 x 16 x 32 float32: 4.3 and 7.6.
+// once, in one launch. 8 x 32 x 32 x 256 bfloat16: 7.6 us, 10.1 in two passes;
+// 16 x 16 x 32 float32: 4.3 and 7.9.
 template <typename T, int V>
 __global__ __launch_bounds__(kItemThreads) void k_gn_item(const T* x, const Cut c,
                                                           const Affine aff, float eps,
@@ -944,7 +948,7 @@ struct Channels {
 
 // The first pass: per chunk the groups' sums of ws gz and ws gz xh, and for all
 // chunks of a workgroup the channels' sums of gz and gz xh. 4 x 1024 x 1024 x 64
-// bfloat16: 169 us, 6.4 TB/s. MANY: it takes every gridDim.x-th chunk of all
+// bfloat16: 170 us, 6.3 TB/s. MANY: it takes every gridDim.x-th chunk of all
 // items'; else it has one, and a set of sums less in its registers.
 template <typename T, int V, int S, bool MANY>
 __global__ __launch_bounds__(kMaxThreads) void k_gn_bwd_sums(const T* gy, const T* x, const Cut c,
@@ -1085,7 +1089,7 @@ __global__ __launch_bounds__(kMaxThreads) void k_gn_param_grad(const ParamGrad a
 }
 
 // The second pass, backwards like the forward one; 4 x 1024 x 1024 x 64 bfloat16:
-// 284 us, 5.7 TB/s. The last `extra` columns of workgroups take gw and gb.
+// 287 us, 5.6 TB/s. The last `extra` columns of workgroups take gw and gb.
 template <typename T, int V, int S>
 __global__ __launch_bounds__(kMaxThreads) void k_gn_bwd_apply(const T* gy, const T* x, const Cut c,
                                                               const Affine aff, uint32_t act,
@@ -1172,7 +1176,7 @@ __global__ __launch_bounds__(kMaxThreads) void k_gn_bwd_apply(const T* gy, const
 // Both passes where a block's pixels fit its workgroup's registers. A workgroup
 // takes every gridDim.x-th item; ch_part (null for one workgroup a block: gw
 // and gb are whole then) gets its items' channel sums. 8 x 32 x 32 x 256
-// bfloat16: 11.9 us with the launch that adds them, 15.9 in two passes.
+// bfloat16: 11.8 us with the launch that adds them, 12.6 in two passes.
 template <typename T, int V>
 __global__ __launch_bounds__(kItemThreads) void k_gn_bwd_item(
         const T* gy, const T* x, const Cut c, const Affine aff, uint32_t act, const float* mean,
@@ -1268,7 +1272,7 @@ __global__ __launch_bounds__(kItemThreads) void k_gn_bwd_item(
 // and the images' addresses (or-ed) allow. `whole`: that no group's edge cuts. One
 // pass takes whole ones, two passes wider ones where there are (their channels
 // count apart then: 2 x 512 x 512 x 66 bfloat16 in 6 groups, forward: 50 us with
-// vectors of 2 cut by edges, 75 with single channels).
+// vectors of 2 cut by edges, 73 with single channels).
 struct Width {
     uint32_t any, whole;
 };
@@ -1306,14 +1310,14 @@ Scratch scratch_of(const Cut& c, bool whole, bool backward) {
 }
 
 // Bytes of an image from which results go past the caches. Forward with them and
-// without takes 73 and 88 us for 1024 x 1024 x 64 bfloat16, 22.9 and 24.8 for
+// without takes 70 and 88 us for 1024 x 1024 x 64 bfloat16, 23.3 and 24.8 for
 // 512 x 512 x 64; with a pass after it that reads the result 125 and 127, 37 and 37.
 constexpr uint64_t kStreamBytes = 32ull << 20;
 
 // Bytes of the first pass's reads that the second may find in the last-level cache
 // (256 MB): the ends of the chunks. The rest goes past it both times: 8 x 1024 x
-// 1024 x 64 bfloat16 574 us forward and 895 backward, 596 and 1054 with all of it
-// through the caches; all past them 1024 x 1024 x 64 takes 80 us forward, not 73.
+// 1024 x 64 bfloat16 560 us forward and 904 backward, 573 and 1063 with all of it
+// through the caches; all past them 1024 x 1024 x 64 takes 80 us forward, not 72.
 // 96 and 224 MB kept measure the same.
 constexpr uint64_t kKeepBytes = 160ull << 20;
 
