@@ -41,14 +41,18 @@ def _layout(t: torch.Tensor) -> tuple[tuple, tuple]:
     return tuple(t.shape), t.stride()
 
 
+def _row_major(layout: tuple) -> bool:
+    return torch.empty_strided(*layout, device="meta").is_contiguous()
+
+
 def _same_order(p: torch.Tensor, layout: tuple, packed: bool) -> bool:
     """Whether p's elements lie in the order of `layout`; packed: that order is
     row-major, in which another shape changes nothing."""
     if packed and p.is_contiguous():
         return True
     shape, stride = layout
-    return p.shape == shape and all(
-        n == 1 or a == b for n, a, b in zip(shape, p.stride(), stride))
+    return p.shape == shape and (p.stride() == stride or all(
+        n == 1 or a == b for n, a, b in zip(shape, p.stride(), stride)))
 
 
 class AdamW(torch.optim.Optimizer):
@@ -128,7 +132,7 @@ class AdamW(torch.optim.Optimizer):
         self._load_hooks = OrderedDict(), OrderedDict()
         self._layouts: list[tuple] = []  # shape and stride of the order its share is in
         self._fresh: set[int] = set()  # those whose share no step or state has touched
-        self._expect: list[tuple] = []  # each parameter with its size, type and if it is packed
+        self._expect: list[tuple] = []  # each parameter with its size, type and (unpacked) layout
         self._sets: list[tuple[dict, int]] = []  # each group with the place of its first parameter
         self._even = True  # every group's parameters have taken the same steps
         self._total = 0
@@ -196,9 +200,8 @@ class AdamW(torch.optim.Optimizer):
         self._hyper = (AdamwSet * len(self._sets))()
 
     def _expect_layouts(self) -> None:
-        """What a step looks for; packed: the share is in row-major order."""
-        self._expect = [(p, p.numel(), p.dtype,
-                         torch.empty_strided(*at, device="meta").is_contiguous())
+        """What a step looks for; the layout is None for row-major order."""
+        self._expect = [(p, p.numel(), p.dtype, None if _row_major(at) else at)
                         for p, at in zip(self._params, self._layouts)]
 
     def _check_param(self, p) -> None:
@@ -303,7 +306,7 @@ class AdamW(torch.optim.Optimizer):
         kept = []  # copies that the launch reads
         moved = []  # parameters in another order than their state, with their copies
         live, params, grads = [], [], []
-        for i, (p, n, kind, packed) in enumerate(self._expect):
+        for i, (p, n, kind, order) in enumerate(self._expect):
             g = p.grad
             if g is None:
                 continue
@@ -311,7 +314,8 @@ class AdamW(torch.optim.Optimizer):
             if (g.dtype is not kind or p.dtype is not kind or g.numel() != n or p.numel() != n
                     or g.get_device() != dev or p.get_device() != dev
                     or g.layout is not torch.strided
-                    or not (packed and g.is_contiguous() and p.is_contiguous())):
+                    or not (g.is_contiguous() and p.is_contiguous() if order is None else
+                            (p.shape, p.stride()) == order and g.stride() == order[1])):
                 q, g = self._reorder(i, p, g, n, kind)
                 kept.append(g)
                 if q is not p:
@@ -385,18 +389,20 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"parameter {i} or its gradient changed its size, type or device: "
                              f"{p.dtype} {tuple(p.shape)} on {p.device}, {g.dtype} "
                              f"{tuple(g.shape)} on {g.device}")
-        if not _dense(p):
-            raise ValueError(f"parameter {i} is no longer densely stored")
-        layout, packed = self._layouts[i], self._expect[i][3]
-        if _same_order(p, layout, packed):
+        layout, there = self._layouts[i], True
+        if _same_order(p, layout, self._expect[i][3] is None):
             layout = _layout(p)
+        elif not _dense(p):
+            raise ValueError(f"parameter {i} is no longer densely stored")
         elif i in self._fresh:
             # zeros, and a master copy of which the kernel takes what is still the parameter's
             layout = self._layouts[i] = _layout(p)
-            self._expect[i] = (p, n, kind, p.is_contiguous())
+            self._expect[i] = (p, n, kind, None if p.is_contiguous() else layout)
         elif tuple(p.shape) != layout[0]:
             raise ValueError(f"parameter {i} changed its shape from {layout[0]} to "
                              f"{tuple(p.shape)}, and its order")
+        else:
+            there = False
 
         def ordered(t):
             if t.stride() == layout[1]:
@@ -404,7 +410,7 @@ class AdamW(torch.optim.Optimizer):
             return torch.empty_strided(*layout, dtype=kind, device=t.device).copy_(t)
 
         with torch.no_grad():
-            return p if _same_order(p, layout, False) else ordered(p), ordered(g)
+            return p if there else ordered(p), ordered(g)
 
     # ---- state ----
 
@@ -440,8 +446,8 @@ class AdamW(torch.optim.Optimizer):
             ends = [at for _, at in self._sets[1:]] + [len(steps)]
             for t, (_, a), b in zip(self._counts.tolist(), self._sets, ends):
                 steps[a:b] = [t] * (b - a)
-        layout = [_layout(p) if p.numel() == n and _same_order(p, at, packed) else at
-                  for (p, n, _, packed), at in zip(self._expect, self._layouts)]
+        layout = [_layout(p) if p.numel() == n and _same_order(p, at, order is None) else at
+                  for (p, n, _, order), at in zip(self._expect, self._layouts)]
         out = {"step": steps, "seed": self.seed, "layout": layout,
                "exp_avg": self._moments[0], "exp_avg_sq": self._moments[1],
                "param_groups": [{k: v for k, v in g.items() if k != "params"}
@@ -484,8 +490,8 @@ class AdamW(torch.optim.Optimizer):
                                  f"{tuple(src.shape)}")
         layouts = self._check_layouts(state_dict.get("layout"))
         if self._captured and not all(
-                a == b or torch.empty_strided(*a, device="meta").is_contiguous() and packed
-                for a, b, (_, _, _, packed) in zip(layouts, self._layouts, self._expect)):
+                a == b or _row_major(a) and order is None
+                for a, b, (_, _, _, order) in zip(layouts, self._layouts, self._expect)):
             raise ValueError("a step has been captured into a graph, which takes the state in "
                              "the order that it had then")
         groups = state_dict.get("param_groups")
