@@ -801,8 +801,9 @@ int dressi_tex_profile(dressi_tex_plan* plan, uint32_t iters, char* names,
                        uint32_t* n);
 
 /* ------------------------------------------------------------------------ */
-/* Training a neural shader: group norm and AdamW (no counterpart in the    */
-/* reference, whose graph has its optimizer and no normalisation).          */
+/* Training a neural shader: group norm, layer norm, AdamW and clipping (no */
+/* counterpart in the reference, whose graph has its optimizer, no          */
+/* normalisation and no norm of its gradients).                             */
 /* ------------------------------------------------------------------------ */
 
 /* Element types of the entry points below. */
@@ -848,6 +849,35 @@ int dressi_group_norm_bwd(dressi_ctx* ctx, const void* gy, const void* x,
                           const void* weight, const void* bias,
                           uint32_t affine_type, uint32_t activation,
                           const float* mean, const float* rstd, void* scratch,
+                          size_t scratch_bytes, void* gx, void* gw, void* gb);
+
+/* Layer normalisation of the channels of each pixel (of each row) with an
+ * activation: y = act((x - mean) rstd w + b), mean and rstd = 1 / sqrt(var +
+ * eps) over the n_ch channels of one pixel. x is [n_items][n_px][n_ch] of
+ * `type` with the channels next to each other, item_stride and px_stride
+ * elements apart; y is packed. weight / bias [n_ch] of `affine_type`, or
+ * NULL for 1 / 0. mean, rstd [n_items][n_px]: what the backward pass needs;
+ * both may be NULL. Sums and statistics are held in 32 bits. scratch: device
+ * memory of at least dressi_layer_norm_scratch bytes, aligned to 16 (NULL
+ * where that is 0), used by this call only. */
+size_t dressi_layer_norm_scratch(uint32_t type, uint64_t n_items,
+                                 uint64_t n_px, uint32_t n_ch, int backward);
+int dressi_layer_norm(dressi_ctx* ctx, const void* x, uint32_t type,
+                      uint64_t n_items, uint64_t n_px, uint32_t n_ch,
+                      uint64_t item_stride, uint64_t px_stride,
+                      const void* weight, const void* bias,
+                      uint32_t affine_type, float eps, uint32_t activation,
+                      void* scratch, size_t scratch_bytes, void* y,
+                      float* mean, float* rstd);
+/* Its gradients: gy packed -> gx packed (of `type`), gw, gb [n_ch] (of
+ * affine_type); any of the three may be NULL. Sums run in a fixed order. */
+int dressi_layer_norm_bwd(dressi_ctx* ctx, const void* gy, const void* x,
+                          uint32_t type, uint64_t n_items, uint64_t n_px,
+                          uint32_t n_ch, uint64_t item_stride,
+                          uint64_t px_stride, const void* weight,
+                          const void* bias, uint32_t affine_type,
+                          uint32_t activation, const float* mean,
+                          const float* rstd, void* scratch,
                           size_t scratch_bytes, void* gx, void* gw, void* gb);
 
 /* One tensor of an AdamW step: n elements of `type`, packed, updated in
@@ -906,6 +936,30 @@ int dressi_adamw_values(dressi_ctx* ctx, uint64_t n, const void* exp_avg,
                         const void* exp_avg_sq, const uint8_t* exp_avg_scale,
                         const uint8_t* exp_avg_sq_scale, void* exp_avg_bf16,
                         void* exp_avg_sq_bf16);
+
+/* One tensor of a norm: n elements of `type`, packed. */
+typedef struct dressi_clip_tensor {
+    void* data;
+    uint64_t n;
+    uint32_t type;
+    uint32_t unused;
+} dressi_clip_tensor;
+
+/* The square root of the sum of squares, and the largest magnitude. */
+#define DRESSI_NORM_2 0u
+#define DRESSI_NORM_LARGEST 1u
+
+/* The norm of all elements of all tensors together, to `norm` on the device,
+ * and each element multiplied by min(1, max_norm / (norm + 1e-6)) in place.
+ * max_norm INFINITY: the norm alone, nothing is written. Where the norm is
+ * not finite, the elements become what the formula gives (zero or NaN). Squares are added in
+ * double, in a fixed order. No two tensors overlap where elements are
+ * written. scratch: device memory of dressi_clip_norm_scratch bytes, aligned
+ * to 8, used by this call only. */
+size_t dressi_clip_norm_scratch(void);
+int dressi_clip_norm(dressi_ctx* ctx, const dressi_clip_tensor* tensors,
+                     uint32_t n_tensors, uint32_t kind, double max_norm,
+                     void* scratch, float* norm);
 
 #ifdef __cplusplus
 }

@@ -56,6 +56,7 @@ class AdamwSet(C.Structure):
 
 F32, BF16, F16 = range(3)
 ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU = range(4)
+NORM_2, NORM_LARGEST = range(2)
 
 PBR_KEEP_PRED = 1
 PBR_KEEP_GRAD = 2
@@ -200,11 +201,18 @@ _SIGS = {
                                _U, _F, _U, _P, _S, _P, _P, _P]),
     "dressi_group_norm_bwd": (_I, [_P, _P, _P, _U, _U, C.c_uint64, _U, C.c_uint64, C.c_uint64, _U,
                                    _P, _P, _U, _U, _P, _P, _P, _S, _P, _P, _P]),
+    "dressi_layer_norm_scratch": (_S, [_U, C.c_uint64, C.c_uint64, _U, _I]),
+    "dressi_layer_norm": (_I, [_P, _P, _U, C.c_uint64, C.c_uint64, _U, C.c_uint64, C.c_uint64, _P,
+                               _P, _U, _F, _U, _P, _S, _P, _P, _P]),
+    "dressi_layer_norm_bwd": (_I, [_P, _P, _P, _U, C.c_uint64, C.c_uint64, _U, C.c_uint64,
+                                   C.c_uint64, _P, _P, _U, _U, _P, _P, _P, _S, _P, _P, _P]),
     "dressi_adamw_scratch": (_S, []),
     "dressi_adamw_set_bytes": (_S, []),
     "dressi_adamw_step": (_I, [_P, _P, _U, _P, _U, _U, C.c_uint64, _P, _P, _P, _P, _U, _F, _P,
                                _P, _P, _P]),
     "dressi_adamw_values": (_I, [_P, C.c_uint64, _P, _P, _P, _P, _P, _P]),
+    "dressi_clip_norm_scratch": (_S, []),
+    "dressi_clip_norm": (_I, [_P, _P, _U, _U, C.c_double, _P, _P]),
 }
 
 EXPORTED = tuple(_SIGS)

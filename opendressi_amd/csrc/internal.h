@@ -103,6 +103,31 @@ int ctx_workspace_zeroed(dressi_ctx* ctx, int slot, size_t bytes, void** out);
 
 inline uint32_t div_up(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
 
+// Makes `device` the calling thread's current one for a call, whose null stream
+// is then that device's, and gives the thread its own back.
+class DeviceScope {
+public:
+    explicit DeviceScope(int device) {
+        if (hipGetDevice(&before_) != hipSuccess || before_ == device) {
+            before_ = -1;
+        } else {
+            error_ = hipSetDevice(device);
+        }
+    }
+    ~DeviceScope() {
+        if (before_ >= 0) {
+            hipSetDevice(before_);
+        }
+    }
+    DeviceScope(const DeviceScope&) = delete;
+    DeviceScope& operator=(const DeviceScope&) = delete;
+    hipError_t error() const { return error_; }
+
+private:
+    int before_ = -1;
+    hipError_t error_ = hipSuccess;
+};
+
 // Fills `bytes` (a multiple of 4) at `p` with zero by a kernel on stream `s`
 // (not hipMemsetAsync: memset nodes of captured graphs have given wrong
 // results on replays, and per-op entry points may be captured).

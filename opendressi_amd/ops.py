@@ -875,3 +875,97 @@ def group_norm_bwd(ctx: Context, gy: torch.Tensor, x: torch.Tensor, mean: torch.
                                     mean.data_ptr(), rstd.data_ptr(), _addr(scratch), size,
                                     _addr(gx), _addr(gw), _addr(gb)))
     return gx, gw, gb
+
+
+# ---- layer norm with an activation (any rows) --------------------------------
+
+def _row_strides(x: torch.Tensor) -> tuple[torch.Tensor, int, int, int, int]:
+    """x (..., C), packed where its rows are not evenly spaced; its items, an item's rows, item
+    and row strides."""
+    if x.dim() == 1:
+        x = x.unsqueeze(0)
+    at = _pixel_strides(x)
+    if at is None:
+        x = x.contiguous()
+        at = _pixel_strides(x)
+    return x, x.shape[0], *at
+
+
+def _layer_args(x: torch.Tensor, activation: str) -> int:
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"x must be [..., C], got {tuple(x.shape)}")
+    act = ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError(f"unknown activation {activation!r}; one of {', '.join(ACTIVATIONS)}")
+    return act
+
+
+def layer_norm(ctx: Context, x: torch.Tensor, weight: torch.Tensor | None = None,
+               bias: torch.Tensor | None = None, eps: float = 1e-5, activation: str = "none",
+               stats: bool = True
+               ) -> tuple[torch.Tensor, torch.Tensor | None, torch.Tensor | None]:
+    """Layer normalisation of the channels of each pixel of x (..., C), or of
+    any rows, and an activation ("none", "relu", "silu", "gelu"):
+    act((x - mean) rstd w + b), mean and rstd over the C channels. float32,
+    bfloat16 or float16, computed in float32; weight and bias (C,) of one type
+    of the three. Returns y (packed), mean and rstd (...) float32, which the
+    backward pass takes (None where `stats` is false). x may have any even
+    pixel stride (a slice of the channels of a wider image); others are packed
+    first."""
+    act = _layer_args(x, activation)
+    c = x.shape[-1]
+    code, aff = _typed(ctx, x, "x"), _affine(ctx, c, weight, bias)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = rstd = None
+    if stats:
+        mean, rstd = torch.empty((2, *x.shape[:-1]), dtype=torch.float32, device=x.device)
+    if x.numel() == 0:
+        return y, mean, rstd
+    x, n, n_px, item, px = _row_strides(x)
+    size = lib.dressi_layer_norm_scratch(code, n, n_px, c, 0)
+    scratch = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+    _prep(ctx)
+    check(lib.dressi_layer_norm(ctx.handle, x.data_ptr(), code, n, n_px, c, item, px,
+                                _addr(weight), _addr(bias), aff, eps, act, _addr(scratch), size,
+                                y.data_ptr(), _addr(mean), _addr(rstd)))
+    return y, mean, rstd
+
+
+def layer_norm_bwd(ctx: Context, gy: torch.Tensor, x: torch.Tensor, mean: torch.Tensor,
+                   rstd: torch.Tensor, weight: torch.Tensor | None = None,
+                   bias: torch.Tensor | None = None, activation: str = "none",
+                   need: tuple[bool, bool, bool] = (True, True, True)
+                   ) -> tuple[torch.Tensor | None, torch.Tensor | None, torch.Tensor | None]:
+    """Gradients of layer_norm: gy (..., C), and x, mean, rstd of the forward
+    pass -> gx (like x, packed), gw, gb (C,) in the weight's and bias's type
+    (float32 where there is none). `need` says which of the three are wanted;
+    the others are None."""
+    act = _layer_args(x, activation)
+    c = x.shape[-1]
+    code, aff = _typed(ctx, x, "x"), _affine(ctx, c, weight, bias)
+    if gy.shape != x.shape or gy.dtype is not x.dtype or gy.get_device() != ctx.device:
+        raise ValueError(f"gy must be like x: {x.dtype} {tuple(x.shape)}, got {gy.dtype} "
+                         f"{tuple(gy.shape)} on {gy.device}")
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        if t.dtype is not torch.float32 or t.shape != x.shape[:-1] or not t.is_contiguous() \
+                or t.get_device() != ctx.device:
+            raise ValueError(f"{name} must be packed float32 {list(x.shape[:-1])} on "
+                             f"cuda:{ctx.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    gx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
+    some = weight if weight is not None else bias
+    kind = torch.float32 if some is None else some.dtype
+    gw, gb = (torch.empty(c, dtype=kind, device=x.device) if wanted else None
+              for wanted in need[1:])
+    n = n_px = 0
+    item = px = c
+    if x.numel():
+        x, n, n_px, item, px = _row_strides(x)
+        gy = gy.contiguous()
+    size = lib.dressi_layer_norm_scratch(code, n, n_px, c, 1)
+    scratch = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+    _prep(ctx)
+    check(lib.dressi_layer_norm_bwd(ctx.handle, gy.data_ptr(), x.data_ptr(), code, n, n_px, c,
+                                    item, px, _addr(weight), _addr(bias), aff, act,
+                                    mean.data_ptr(), rstd.data_ptr(), _addr(scratch), size,
+                                    _addr(gx), _addr(gw), _addr(gb)))
+    return gx, gw, gb

@@ -13,7 +13,9 @@
 and, for a neural shader trained through them,
 
     y   = dr.group_norm(ctx, x, groups=8, weight=w, bias=b, activation="silu")
+    y   = dr.layer_norm(ctx, x, weight=w, bias=b, activation="gelu")
     opt = dr.AdamW(ctx, params, lr=1e-3, state_bits=8, max_grad_norm=1.0)
+    n   = dr.clip_grad_norm_(ctx, params, 1.0)  # for other optimizers
 
 Coordinate conventions follow nvdiffrast (OpenGL clip space, z in [-w, w]);
 the remap to the [0, w] depth range of the reference's rasterizers happens
@@ -24,8 +26,9 @@ returned on the input's device. `RasterizeVulkanContext` is kept as an alias
 so reference code runs unchanged.
 """
 
+from .clip import clip_grad_norm_, grad_norm
 from .context import RasterizeHipContext, RasterizeVulkanContext
-from .norm import group_norm
+from .norm import group_norm, layer_norm
 from .optim import AdamW
 from .ops import antialias, interpolate, rasterize, rasterize_soft, texture
 
@@ -38,5 +41,8 @@ __all__ = [
     "antialias",
     "rasterize_soft",
     "group_norm",
+    "layer_norm",
     "AdamW",
+    "clip_grad_norm_",
+    "grad_norm",
 ]

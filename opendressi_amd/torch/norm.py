@@ -1,5 +1,5 @@
-"""group_norm: the normalisation layer of a neural shader over the surface's
-channels-last images. No counterpart in the reference's surface.
+"""group_norm and layer_norm: the normalisation layers of a neural shader over
+the surface's channels-last images. No counterpart in the reference's surface.
 """
 from __future__ import annotations
 
@@ -7,6 +7,12 @@ import torch
 
 from .. import ops as K
 from .context import RasterizeHipContext
+
+
+def _check_tensors(x, weight, bias) -> None:
+    for t, name in ((x, "x"), (weight, "weight"), (bias, "bias")):
+        if not isinstance(t, torch.Tensor) and (t is not None or name == "x"):
+            raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
 
 
 class _GroupNormFn(torch.autograd.Function):
@@ -47,7 +53,54 @@ def group_norm(ctx: RasterizeHipContext, x: torch.Tensor, groups: int, weight=No
     with the mean and variance over the pixels and the C / groups channels of
     each group of each item, computed in float32; activation is "none",
     "relu", "silu" or "gelu". Differentiable w.r.t. x, weight and bias."""
-    for t, name in ((x, "x"), (weight, "weight"), (bias, "bias")):
-        if not isinstance(t, torch.Tensor) and (t is not None or name == "x"):
-            raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    _check_tensors(x, weight, bias)
     return _GroupNormFn.apply(x, weight, bias, ctx, int(groups), float(eps), activation)
+
+
+def _moved(dev, x, weight, bias):
+    """The three on the context's device, the last two packed."""
+    x, weight, bias = (None if t is None else t.detach().to(dev) for t in (x, weight, bias))
+    return (x, *(None if t is None else t.contiguous() for t in (weight, bias)))
+
+
+class _LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(fctx, x, weight, bias, vctx, eps, activation):
+        with vctx.lock:
+            x_d, w_d, b_d = _moved(vctx.device, x, weight, bias)
+            y, mean, rstd = K.layer_norm(vctx._ctx, x_d, w_d, b_d, eps, activation)
+        fctx.dressi = (vctx, activation)
+        fctx.save_for_backward(x, weight, bias, mean, rstd)
+        return y.to(x.device)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(fctx, grad_out):
+        vctx, activation = fctx.dressi
+        x, weight, bias, mean, rstd = fctx.saved_tensors
+        with vctx.lock:
+            x_d, w_d, b_d = _moved(vctx.device, x, weight, bias)
+            grads = K.layer_norm_bwd(vctx._ctx, grad_out.detach().to(vctx.device), x_d, mean, rstd,
+                                     w_d, b_d, activation, fctx.needs_input_grad[:3])
+        grads = [None if g is None else g.to(t.device) for g, t in zip(grads, (x, weight, bias))]
+        return (*grads, None, None, None)
+
+
+def layer_norm(ctx: RasterizeHipContext, x: torch.Tensor, weight=None, bias=None,
+               eps: float = 1e-5, activation: str = "none") -> torch.Tensor:
+    """Layer normalisation of the channels of each pixel and an activation.
+
+    x is [..., C] (an image batch [N, H, W, C], vertices' or rays' features
+    [V, C], one row [C]) in float32, bfloat16 or float16; weight and bias are
+    [C], of one type of the three, or None. Returns
+    act((x - mean) / sqrt(var + eps) * weight + bias), with the mean and
+    variance over the C channels of each pixel, computed in float32;
+    activation is "none", "relu", "silu" or "gelu". Differentiable w.r.t. x,
+    weight and bias."""
+    _check_tensors(x, weight, bias)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
+                                       for t in (x, weight, bias)):
+        return _LayerNormFn.apply(x, weight, bias, ctx, float(eps), activation)
+    with ctx.lock:
+        return K.layer_norm(ctx._ctx, *_moved(ctx.device, x, weight, bias), float(eps), activation,
+                            stats=False)[0].to(x.device)

@@ -1,0 +1,114 @@
+"""Layer norm's and clipping's refusals, without a GPU."""
+import ctypes as C
+import math
+import threading
+import types
+
+import numpy as np
+import pytest
+import torch
+
+from opendressi_amd import _lib as L
+from opendressi_amd.torch import clip
+
+# never read: every call here is refused before the context is used
+CTX = C.cast(C.create_string_buffer(4096), C.c_void_p)
+X, Y, W = (0x1000 * k for k in (1, 2, 3))  # addresses, not memory
+
+
+def _refused(rc, *words):
+    text = L.lib.dressi_last_error().decode()
+    assert rc != 0 and all(w in text for w in words), text
+
+
+def _forward(ctx=CTX, x=X, type=0, items=2, px=3, c=8, item=24, step=8, aff=0, eps=1e-5, act=0,
+             scratch=None, size=0, y=Y, mean=X, rstd=X):
+    return L.lib.dressi_layer_norm(ctx, x, type, items, px, c, item, step, W, W, aff, eps, act,
+                                   scratch, size, y, mean, rstd)
+
+
+def _backward(ctx=CTX, gy=X, x=X, type=0, items=2, px=3, c=8, step=8, aff=0, act=0, mean=X, rstd=X,
+              scratch=X, size=1 << 30, gx=Y, gw=W, gb=W):
+    return L.lib.dressi_layer_norm_bwd(ctx, gy, x, type, items, px, c, 24, step, W, W, aff, act,
+                                       mean, rstd, scratch, size, gx, gw, gb)
+
+
+def test_layer_norm_refuses():
+    for bad, word in ((dict(ctx=None), "context"), (dict(type=3), "type"), (dict(aff=9), "type"),
+                      (dict(act=4), "activation"), (dict(c=0), "channels"),
+                      (dict(c=(1 << 24) + 1, step=1 << 25), "channels"),
+                      (dict(items=1 << 30, px=1 << 30), "rows"), (dict(step=7), "overlap"),
+                      (dict(x=X + 2), "aligned"), (dict(x=None), "arguments")):
+        _refused(_forward(**bad), word)
+        _refused(_backward(**bad), word)
+    for bad, word in ((dict(eps=-1.0), "eps"), (dict(eps=math.nan), "eps"),
+                      (dict(eps=math.inf), "eps"), (dict(y=None), "arguments"),
+                      (dict(mean=None), "arguments"), (dict(rstd=None), "arguments"),
+                      (dict(y=Y + 1), "aligned")):
+        _refused(_forward(**bad), word)
+    for bad, word in ((dict(gy=None), "arguments"), (dict(mean=None), "arguments"),
+                      (dict(rstd=None), "arguments"), (dict(gx=Y + 2), "aligned"),
+                      (dict(size=0), "scratch"), (dict(scratch=None), "scratch")):
+        _refused(_backward(**bad), word)
+
+
+def test_nothing_to_do():
+    assert _forward(items=0) == 0 and _forward(px=0) == 0
+    assert _backward(gx=None, gw=None, gb=None) == 0
+    assert L.lib.dressi_layer_norm_scratch(0, 0, 5, 8, 1) == 0
+
+
+def _table(*rows):
+    t = np.zeros(len(rows), clip._ENTRY)
+    for e, (data, n, kind) in zip(t, rows):
+        e["data"], e["n"], e["type"] = data, n, kind
+    return t
+
+
+def _clip(table, kind=0, max_norm=1.0, ctx=CTX, scratch=X, norm=X):
+    return L.lib.dressi_clip_norm(ctx, table.ctypes.data, len(table), kind, max_norm, scratch, norm)
+
+
+def test_clip_norm_refuses():
+    good = _table((0x10000, 100, 0), (0x20000, 100, 1))
+    for bad, word in ((dict(ctx=None), "context"), (dict(norm=None), "arguments"),
+                      (dict(kind=2), "norm"), (dict(max_norm=-1.0), "max_norm"),
+                      (dict(max_norm=math.nan), "max_norm"), (dict(scratch=X + 4), "scratch"),
+                      (dict(scratch=None), "scratch")):
+        _refused(_clip(good, **bad), word)
+    for rows, word in (([(0x10000, 100, 3)], "type"), ([(0, 100, 0)], "NULL"),
+                       ([(0x10002, 100, 0)], "aligned"), ([(0x10001, 100, 1)], "aligned"),
+                       ([(0x10000, (1 << 40) + 1, 0)], "large"),
+                       ([(0x10000, 100, 0), (0x10000, 100, 0)], "share"),
+                       ([(0x10000, 100, 0), (0x20000, 1, 0), (0x10000 + 396, 2, 1)], "0 and 2"),
+                       ([(0x10000 + 198, 1, 2), (0x10000, 100, 1)], "0 and 1")):
+        _refused(_clip(_table(*rows)), word)
+
+
+HOST = types.SimpleNamespace(device=torch.device("cuda", 0), lock=threading.RLock())
+
+
+def _param(grad, shape=(3,)):
+    p = torch.zeros(shape, dtype=grad.dtype)
+    p.grad = grad
+    return p
+
+
+def test_clip_grad_norm_refuses():
+    p = _param(torch.ones(3))
+    for args, error in (((-1.0,), ValueError), ((math.nan,), ValueError), ((1.0, 1.0), ValueError),
+                        ((1.0, 0.0), ValueError), ((1.0, 2.0), ValueError)):
+        with pytest.raises(error):  # the last for its device
+            clip.clip_grad_norm_(HOST, [p], *args)
+    with pytest.raises(TypeError):
+        clip.clip_grad_norm_(HOST, [_param(torch.ones(3, dtype=torch.float64))], 1.0)
+    with pytest.raises(RuntimeError):
+        clip.grad_norm(HOST, [_param(torch.ones(3).to_sparse())])
+    with pytest.raises(ValueError):
+        clip.grad_norm(HOST, [p], 3.0)
+
+
+def test_elements_that_share_memory():
+    base = torch.zeros(40)
+    assert clip._apart(base[::2]) and clip._apart(base.view(4, 10)[:, 3:7].t())
+    assert not clip._apart(base[:1].expand(5)) and not clip._apart(base.as_strided((5, 5), (2, 1)))
