@@ -91,6 +91,37 @@ __device__ __forceinline__ void store_vec(T* p, const float* x) {
     store_as<STREAM>((Pack<T, V>*)p, a);
 }
 
+// V neighbours at any address that one of them may have: vector memory takes 16
+// bytes from there in one instruction too.
+template <typename T, int V>
+struct LooseOf {
+    typedef Words<sizeof(T) * V> type __attribute__((aligned(alignof(T))));
+};
+template <typename T, int V, bool STREAM = false>
+__device__ __forceinline__ Pack<T, V> load_loose(const T* p) {
+    using L = typename LooseOf<T, V>::type;
+    const L w = STREAM ? __builtin_nontemporal_load((const L*)p) : *(const L*)p;
+    Pack<T, V> a;
+    __builtin_memcpy(&a, &w, sizeof(a));
+    return a;
+}
+template <typename T, int V, bool STREAM = false>
+__device__ __forceinline__ void store_loose(T* p, const float* x) {
+    using L = typename LooseOf<T, V>::type;
+    Pack<T, V> a;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        a.v[i] = from_float<T>(x[i]);
+    }
+    L w;
+    __builtin_memcpy(&w, &a, sizeof(a));
+    if (STREAM) {
+        __builtin_nontemporal_store(w, (L*)p);
+    } else {
+        *(L*)p = w;
+    }
+}
+
 inline size_t type_bytes(uint32_t type) { return type == DRESSI_F32 ? 4 : 2; }
 
 }  // namespace dressi
