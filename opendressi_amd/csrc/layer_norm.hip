@@ -19,9 +19,8 @@
 // vector's before, count once in the sums, and are written twice with the same
 // bits.
 //
-// The mean is taken twice: of x, then of x less that, whose sum comes with that
-// of the squares. So a mean many deviations from zero is as exact as a float can
-// be, and the variance is that about it.
+// The squares are those of x less the mean, from registers, so values far from
+// zero lose no more than the mean's own rounding.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -42,15 +41,27 @@ struct Rows {
     uint64_t n, n_px;
     uint64_t item_stride, px_stride;  // of x, in elements
     uint32_t n_ch;
-    float inv;  // 1 / n_ch
+    uint32_t flat;  // rows are evenly spaced, and a workgroup's within 2^32 bytes
+    float inv;      // 1 / n_ch
     __device__ __forceinline__ size_t at(uint64_t row) const {
         if (n_px == n) {
             return (size_t)(row * px_stride);
         }
-        const uint64_t item = row / n_px;
+        const uint64_t item = n <= 0xffffffffu ? (uint32_t)row / (uint32_t)n_px : row / n_px;
         return (size_t)(item * item_stride + (row - item * n_px) * px_stride);
     }
 };
+constexpr uint64_t kMaxPxStride = 1ull << 22;  // elements, of up to 256 rows
+
+// The element at a distance in bytes.
+template <typename T>
+__device__ __forceinline__ T* at_byte(T* p, uint32_t bytes) {
+    return (T*)((char*)p + bytes);
+}
+template <typename T>
+__device__ __forceinline__ const T* at_byte(const T* p, uint32_t bytes) {
+    return (const T*)((const char*)p + bytes);
+}
 
 // Vector `vec` of a row: where it begins, and how many of its values count in
 // the vector before (all, past the end).
@@ -70,20 +81,30 @@ __device__ __forceinline__ float counted(float x, uint32_t j, uint32_t skip) {
     return WHOLE || j >= skip ? x : 0.f;
 }
 
+template <typename T, int V>
+__device__ __forceinline__ void load_floats(const void* p, uint32_t ch, float* w) {
+    float x[V];
+    unpack(load_loose<T, V>((const T*)p + ch), x);
+#pragma unroll
+    for (int j = 0; j < V; j++) {
+        w[j] = x[j];
+    }
+}
+// V of the weight's or bias's values.
 template <int V>
 __device__ __forceinline__ void load_params(const void* p, uint32_t type, uint32_t ch, float absent,
-                                            float (&w)[V]) {
+                                            float* w) {
     if (!p) {
 #pragma unroll
         for (int j = 0; j < V; j++) {
             w[j] = absent;
         }
     } else if (type == DRESSI_F32) {
-        unpack(load_loose<float, V>((const float*)p + ch), w);
+        load_floats<float, V>(p, ch, w);
     } else if (type == DRESSI_BF16) {
-        unpack(load_loose<bf16, V>((const bf16*)p + ch), w);
+        load_floats<bf16, V>(p, ch, w);
     } else {
-        unpack(load_loose<f16, V>((const f16*)p + ch), w);
+        load_floats<f16, V>(p, ch, w);
     }
 }
 
@@ -149,28 +170,27 @@ __device__ __forceinline__ float2 wide_sum(float2 x, float2* part) {
     return x;
 }
 
-// 1 / deviation from the sums s of x - m and q of its squares, and the mean.
-__device__ __forceinline__ float finish(float m, float s, float q, float inv, float eps,
-                                        float& mean) {
-    const float off = s * inv;
-    mean = m + off;
-    const float var = fmaf(-off, off, q * inv);
-    return 1.f / sqrtf((var < 0.f ? 0.f : var) + eps);  // a NaN stays one
+// 1 / sqrt(v) to less than a step of a float: the hardware's, refined once.
+__device__ __forceinline__ float inv_sqrt(float v) {
+    if (!(v >= 0x1p-100f && v <= 0x1p100f)) {
+        return 1.f / sqrtf(v);  // zero, an infinity, a NaN, and what the steps below lose
+    }
+    const float r = __builtin_amdgcn_rsqf(v);
+    return fmaf(0.5f * r, fmaf(-v * r, r, 1.f), r);
 }
 
-// y of a vector.
-template <typename T, int V, bool STREAM>
-__device__ __forceinline__ void write_y(const Pack<T, V>& x, float mean, float rstd,
-                                        const float (&w)[V], const float (&b)[V], uint32_t act,
-                                        T* y) {
-    float z[V];
-    unpack(x, z);
-#pragma unroll
-    for (int j = 0; j < V; j++) {
-        z[j] = fmaf((z[j] - mean) * rstd, w[j], b[j]);
+// f(whether past the caches), in two branches that the compiler keeps apart: it
+// would make one of them, through the caches, out of loads or stores that differ
+// in that alone.
+template <typename F>
+__device__ __forceinline__ void by_stream(bool stream, F&& f) {
+    if (stream) {
+        asm volatile("");
+        f(std::true_type());
+        asm volatile("");
+    } else {
+        f(std::false_type());
     }
-    act_values<T, V>(act, z);
-    store_loose<T, V, STREAM>(y, z);
 }
 
 struct Forward {
@@ -182,91 +202,117 @@ struct Forward {
     Affine aff;
     float eps;
     uint32_t act;
+    bool stream, stream_in;
 };
 
 // ---------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------
 
-// Rows that a lane has in flight, of K vectors each.
-template <int V, int K>
-constexpr int kInFlight = K == 1 ? 4 : K == 2 ? 2 : 1;
+// Lanes of a row from which its loads may go past the caches: fewer take less than
+// a whole line with each.
+constexpr int kStreamLanes = 32;
+
+// Rows that a lane has in flight, of E values each: 64 bytes.
+template <typename T, int E>
+constexpr int kInFlight = E * sizeof(T) >= 48 ? 1 : E * sizeof(T) >= 32 ? 2 : 4;
 
 // L lanes hold a row, K vectors each.
-template <typename T, int V, int L, int K, bool WHOLE, bool STREAM>
+template <typename T, int V, int L, int K, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void k_ln_rows(const Forward a) {
-    constexpr int R = kInFlight<V, K>;
-    constexpr uint32_t kSlots = kThreads / L;
+    constexpr int E = K * V, R = kInFlight<T, E>;
+    constexpr uint32_t kSlots = kThreads / L, kTake = kSlots * R;
     const uint32_t lane = threadIdx.x % L, slot = threadIdx.x / L;
     const Rows& rows = a.rows;
-    uint32_t first[K], skip[K];
-    float w[K][V], b[K][V];
+    const uint32_t px_bytes = (uint32_t)(rows.px_stride * sizeof(T));
+    uint32_t first[K], skip[K];  // first: in bytes
+    float w[E], b[E];
 #pragma unroll
     for (int k = 0; k < K; k++) {
         const Span<V> sp(k * L + lane, rows.n_ch);
-        first[k] = sp.first;
+        first[k] = sp.first * sizeof(T);
         skip[k] = sp.skip;
-        load_params<V>(a.aff.weight, a.aff.type, sp.first, 1.f, w[k]);
-        load_params<V>(a.aff.bias, a.aff.type, sp.first, 0.f, b[k]);
+        load_params<V>(a.aff.weight, a.aff.type, sp.first, 1.f, w + k * V);
+        load_params<V>(a.aff.bias, a.aff.type, sp.first, 0.f, b + k * V);
     }
-    const T* x = (const T*)a.x;
-    T* y = (T*)a.y;
-    for (uint64_t r0 = (uint64_t)blockIdx.x * (kSlots * R); r0 < rows.n;
-         r0 += (uint64_t)gridDim.x * (kSlots * R)) {
+    const uint32_t in = slot * px_bytes, out = slot * rows.n_ch * sizeof(T);
+    for (uint64_t r0 = (uint64_t)blockIdx.x * kTake; r0 < rows.n; r0 += (uint64_t)gridDim.x * kTake) {
+        const T* x = (const T*)a.x;
         Pack<T, V> v[R][K];
+        if (rows.flat && r0 + kTake <= rows.n) {
+            x += r0 * rows.px_stride;
+            by_stream(L >= kStreamLanes && a.stream_in, [&](auto past) {
 #pragma unroll
-        for (int i = 0; i < R; i++) {
-            const uint64_t row = r0 + i * kSlots + slot;
-            const T* p = x + rows.at(row < rows.n ? row : rows.n - 1);
+                for (int i = 0; i < R; i++) {
 #pragma unroll
-            for (int k = 0; k < K; k++) {
-                v[i][k] = load_loose<T, V, STREAM>(p + first[k]);
+                    for (int k = 0; k < K; k++) {
+                        v[i][k] = load_loose<T, V, decltype(past)::value>(
+                            at_byte(x + (size_t)(i * kSlots) * rows.px_stride, in + first[k]));
+                    }
+                }
+            });
+        } else {  // past the end the last row again
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                const T* p = x + rows.at(std::min(r0 + i * kSlots + slot, rows.n - 1));
+#pragma unroll
+                for (int k = 0; k < K; k++) {
+                    v[i][k] = load_loose<T, V>(at_byte(p, first[k]));
+                }
             }
         }
-        float m[R], s[R], q[R];
+        float z[R][E], m[R], q[R];
 #pragma unroll
         for (int i = 0; i < R; i++) {
             m[i] = 0.f;
 #pragma unroll
-            for (int k = 0; k < K; k++) {
-#pragma unroll
-                for (int j = 0; j < V; j++) {
-                    m[i] += counted<WHOLE>(to_float(v[i][k].v[j]), j, skip[k]);
-                }
+            for (int e = 0; e < E; e++) {
+                z[i][e] = to_float(v[i][e / V].v[e % V]);
+                m[i] += counted<WHOLE>(z[i][e], e % V, skip[e / V]);
             }
         }
 #pragma unroll
         for (int i = 0; i < R; i++) {
             m[i] = lane_sum<L>(m[i]) * rows.inv;
-            s[i] = q[i] = 0.f;
+            q[i] = 0.f;
 #pragma unroll
-            for (int k = 0; k < K; k++) {
-#pragma unroll
-                for (int j = 0; j < V; j++) {
-                    const float d = counted<WHOLE>(to_float(v[i][k].v[j]) - m[i], j, skip[k]);
-                    s[i] += d;
-                    q[i] = fmaf(d, d, q[i]);
-                }
+            for (int e = 0; e < E; e++) {
+                z[i][e] -= m[i];
+                const float d = counted<WHOLE>(z[i][e], e % V, skip[e / V]);
+                q[i] = fmaf(d, d, q[i]);
             }
         }
 #pragma unroll
         for (int i = 0; i < R; i++) {
-            const uint64_t row = r0 + i * kSlots + slot;
-            float mean;
-            const float rstd = finish(m[i], lane_sum<L>(s[i]), lane_sum<L>(q[i]), rows.inv, a.eps,
-                                      mean);
-            if (row < rows.n) {
-                T* out = y + row * rows.n_ch;
+            q[i] = inv_sqrt(fmaf(lane_sum<L>(q[i]), rows.inv, a.eps));
 #pragma unroll
-                for (int k = 0; k < K; k++) {
-                    if (WHOLE || skip[k] < V) {
-                        write_y<T, V, STREAM>(v[i][k], mean, rstd, w[k], b[k], a.act,
-                                              out + first[k]);
+            for (int e = 0; e < E; e++) {
+                z[i][e] = fmaf(z[i][e] * q[i], w[e], b[e]);
+            }
+        }
+        act_values<T, R * E>(a.act, *(float (*)[R * E])&z[0][0]);
+        T* y = (T*)a.y + r0 * rows.n_ch;
+        by_stream(a.stream, [&](auto past) {
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                if (r0 + i * kSlots + slot < rows.n) {
+                    T* yi = y + (size_t)(i * kSlots) * rows.n_ch;
+#pragma unroll
+                    for (int k = 0; k < K; k++) {
+                        if (WHOLE || skip[k] < V) {
+                            store_loose<T, V, decltype(past)::value>(at_byte(yi, out + first[k]),
+                                                                     z[i] + k * V);
+                        }
                     }
                 }
-                if (lane == 0 && a.mean) {
-                    a.mean[row] = mean;
-                    a.rstd[row] = rstd;
+            }
+        });
+        if (lane == 0 && a.mean) {
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                if (r0 + i * kSlots + slot < rows.n) {
+                    (a.mean + r0 + i * kSlots)[slot] = m[i];
+                    (a.rstd + r0 + i * kSlots)[slot] = q[i];
                 }
             }
         }
@@ -275,174 +321,160 @@ __global__ __launch_bounds__(kThreads) void k_ln_rows(const Forward a) {
 
 // A workgroup holds a row, K vectors a thread. HOLD: weight and bias stay in
 // registers between rows.
-template <typename T, int V, int K, uint32_t THREADS, bool HOLD, bool WHOLE, bool STREAM>
+template <typename T, int V, int K, uint32_t THREADS, bool HOLD, bool WHOLE>
 __global__ __launch_bounds__(THREADS) void k_ln_wide(const Forward a) {
-    __shared__ float part1[THREADS / 64];
-    __shared__ float2 part2[THREADS / 64];
+    __shared__ float part[2][THREADS / 64];
+    constexpr int E = K * V;
     const Rows& rows = a.rows;
     uint32_t first[K], skip[K];
-    float w[K][V], b[K][V];
+    float w[E], b[E];
 #pragma unroll
     for (int k = 0; k < K; k++) {
         const Span<V> sp(k * blockDim.x + threadIdx.x, rows.n_ch);
         first[k] = sp.first;
         skip[k] = sp.skip;
         if (HOLD) {
-            load_params<V>(a.aff.weight, a.aff.type, sp.first, 1.f, w[k]);
-            load_params<V>(a.aff.bias, a.aff.type, sp.first, 0.f, b[k]);
+            load_params<V>(a.aff.weight, a.aff.type, sp.first, 1.f, w + k * V);
+            load_params<V>(a.aff.bias, a.aff.type, sp.first, 0.f, b + k * V);
         }
     }
     for (uint64_t row = blockIdx.x; row < rows.n; row += gridDim.x) {
         const T* p = (const T*)a.x + rows.at(row);
         Pack<T, V> v[K];
+        by_stream(a.stream_in, [&](auto past) {
 #pragma unroll
-        for (int k = 0; k < K; k++) {
-            v[k] = load_loose<T, V, STREAM>(p + first[k]);
+            for (int k = 0; k < K; k++) {
+                v[k] = load_loose<T, V, decltype(past)::value>(p + first[k]);
+            }
+        });
+        float m = 0.f, q = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            m += counted<WHOLE>(to_float(v[e / V].v[e % V]), e % V, skip[e / V]);
         }
-        float m = 0.f;
+        m = wide_sum(m, part[0]) * rows.inv;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const float d = counted<WHOLE>(to_float(v[e / V].v[e % V]) - m, e % V, skip[e / V]);
+            q = fmaf(d, d, q);
+        }
+        q = inv_sqrt(fmaf(wide_sum(q, part[1]), rows.inv, a.eps));
+        T* y = (T*)a.y + row * rows.n_ch;
 #pragma unroll
         for (int k = 0; k < K; k++) {
+            if (!HOLD) {
+                load_params<V>(a.aff.weight, a.aff.type, first[k], 1.f, w + k * V);
+                load_params<V>(a.aff.bias, a.aff.type, first[k], 0.f, b + k * V);
+            }
+            float z[V];
+            unpack(v[k], z);
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                m += counted<WHOLE>(to_float(v[k].v[j]), j, skip[k]);
+                z[j] = fmaf((z[j] - m) * q, w[k * V + j], b[k * V + j]);
             }
-        }
-        m = wide_sum(m, part1) * rows.inv;
-        float2 s = make_float2(0.f, 0.f);
-#pragma unroll
-        for (int k = 0; k < K; k++) {
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                const float d = counted<WHOLE>(to_float(v[k].v[j]) - m, j, skip[k]);
-                s.x += d;
-                s.y = fmaf(d, d, s.y);
-            }
-        }
-        s = wide_sum(s, part2);
-        float mean;
-        const float rstd = finish(m, s.x, s.y, rows.inv, a.eps, mean);
-        T* out = (T*)a.y + row * rows.n_ch;
-#pragma unroll
-        for (int k = 0; k < K; k++) {
+            act_values<T, V>(a.act, z);
             if (WHOLE || skip[k] < V) {
-                if (!HOLD) {
-                    load_params<V>(a.aff.weight, a.aff.type, first[k], 1.f, w[k]);
-                    load_params<V>(a.aff.bias, a.aff.type, first[k], 0.f, b[k]);
-                }
-                write_y<T, V, STREAM>(v[k], mean, rstd, w[k], b[k], a.act, out + first[k]);
+                by_stream(a.stream, [&](auto past) {
+                    store_loose<T, V, decltype(past)::value>(y + first[k], z);
+                });
             }
         }
         if (threadIdx.x == 0 && a.mean) {
-            a.mean[row] = mean;
-            a.rstd[row] = rstd;
+            a.mean[row] = m;
+            a.rstd[row] = q;
         }
     }
 }
 
-// Rows beyond a workgroup's registers go in chunks of kChunkVecs vectors, a
-// workgroup each, in two passes: one leaves every chunk's (mean, squares about
-// it), the other joins those of its row, every workgroup for itself.
-constexpr uint32_t kChunkIter = 4;
-constexpr uint32_t kChunkVecs = kChunkIter * kThreads;
+// Rows beyond a workgroup's registers go in chunks of a workgroup's E values a
+// thread, in two passes: one leaves every chunk's (mean, squares about it), the
+// other joins those of its row, every wave for itself. A workgroup keeps to one
+// chunk, whose weight and bias it holds, and takes every gridDim.x-th row.
+constexpr int kChunkElems = 32, kChunkElemsBwd = 16;  // a thread's
 
 // A thread's vectors of a chunk.
-template <int V>
+template <int V, int K>
 struct ChunkSpan {
-    uint32_t first[kChunkIter], skip[kChunkIter], count;  // count: of the chunk
+    uint32_t first[K], skip[K], count;  // count: of the chunk
     __device__ __forceinline__ ChunkSpan(uint32_t chunk, uint32_t n_ch) {
+        constexpr uint32_t kVecs = K * kThreads;
 #pragma unroll
-        for (uint32_t k = 0; k < kChunkIter; k++) {
-            const Span<V> sp(chunk * kChunkVecs + k * kThreads + threadIdx.x, n_ch);
+        for (uint32_t k = 0; k < K; k++) {
+            const Span<V> sp(chunk * kVecs + k * kThreads + threadIdx.x, n_ch);
             first[k] = sp.first;
             skip[k] = sp.skip;
         }
-        count = std::min(n_ch - chunk * (kChunkVecs * V), kChunkVecs * V);
+        count = std::min(n_ch - chunk * (kVecs * V), kVecs * V);
     }
 };
 
 template <typename T, int V>
-__global__ __launch_bounds__(kThreads) void k_ln_chunk_stats(const Forward a, uint32_t chunks,
-                                                             float2* part) {
-    __shared__ float part1[kThreads / 64];
-    __shared__ float2 part2[kThreads / 64];
-    for (uint64_t u = blockIdx.x; u < a.rows.n * chunks; u += gridDim.x) {
-        const uint64_t row = u / chunks;
-        const ChunkSpan<V> sp((uint32_t)(u - row * chunks), a.rows.n_ch);
+__global__ __launch_bounds__(kThreads) void k_ln_chunk_stats(const Forward a, float2* row_part) {
+    __shared__ float part[2][kThreads / 64];
+    constexpr int K = kChunkElems / V;
+    const ChunkSpan<V, K> sp(blockIdx.y, a.rows.n_ch);
+    const float inv = 1.f / (float)sp.count;
+    for (uint64_t row = blockIdx.x; row < a.rows.n; row += gridDim.x) {
         const T* p = (const T*)a.x + a.rows.at(row);
-        Pack<T, V> v[kChunkIter];
+        Pack<T, V> v[K];
 #pragma unroll
-        for (uint32_t k = 0; k < kChunkIter; k++) {
+        for (int k = 0; k < K; k++) {
             v[k] = load_loose<T, V>(p + sp.first[k]);
         }
-        float m = 0.f;
+        float m = 0.f, q = 0.f;
 #pragma unroll
-        for (uint32_t k = 0; k < kChunkIter; k++) {
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                m += counted<false>(to_float(v[k].v[j]), j, sp.skip[k]);
-            }
+        for (int e = 0; e < kChunkElems; e++) {
+            m += counted<false>(to_float(v[e / V].v[e % V]), e % V, sp.skip[e / V]);
         }
-        const float inv = 1.f / (float)sp.count;
-        m = wide_sum(m, part1) * inv;
-        float2 s = make_float2(0.f, 0.f);
+        m = wide_sum(m, part[0]) * inv;
 #pragma unroll
-        for (uint32_t k = 0; k < kChunkIter; k++) {
-#pragma unroll
-            for (int j = 0; j < V; j++) {
-                const float d = counted<false>(to_float(v[k].v[j]) - m, j, sp.skip[k]);
-                s.x += d;
-                s.y = fmaf(d, d, s.y);
-            }
+        for (int e = 0; e < kChunkElems; e++) {
+            const float d = counted<false>(to_float(v[e / V].v[e % V]) - m, e % V, sp.skip[e / V]);
+            q = fmaf(d, d, q);
         }
-        s = wide_sum(s, part2);
+        q = wide_sum(q, part[1]);
         if (threadIdx.x == 0) {
-            const float off = s.x * inv;
-            part[u] = make_float2(m + off, fmaf(-off, s.x, s.y));
+            row_part[row * gridDim.y + blockIdx.y] = make_float2(m, q);
         }
     }
 }
 
-// A row's sums over its chunks' entries, in double, in all threads.
+// A row's sums over its chunks' entries, in double, in all lanes.
 template <typename F>
 __device__ __forceinline__ double2 join_chunks(const float2* part, uint32_t chunks, F&& f) {
-    __shared__ double2 sums[kThreads / 64];
     double2 s = make_double2(0.0, 0.0);
-    for (uint32_t i = threadIdx.x; i < chunks; i += kThreads) {
+    for (uint32_t i = threadIdx.x & 63u; i < chunks; i += 64) {
         f(i, part[i], s);
     }
     for (int o = 1; o < 64; o <<= 1) {
         s.x += __shfl_xor(s.x, o);
         s.y += __shfl_xor(s.y, o);
     }
-    __syncthreads();  // those of before have been read
-    if ((threadIdx.x & 63u) == 0) {
-        sums[threadIdx.x >> 6] = s;
-    }
-    __syncthreads();
-    s = sums[0];
-    for (uint32_t i = 1; i < kThreads / 64; i++) {
-        s.x += sums[i].x;
-        s.y += sums[i].y;
-    }
     return s;
 }
 
 template <typename T, int V>
-__global__ __launch_bounds__(kThreads) void k_ln_chunk_apply(const Forward a, uint32_t chunks,
-                                                             const float2* part) {
-    const uint32_t n_ch = a.rows.n_ch;
-    const double full = kChunkVecs * V, last = n_ch - (chunks - 1) * full;
-    for (uint64_t u = blockIdx.x; u < a.rows.n * chunks; u += gridDim.x) {
-        const uint64_t row = u / chunks;
-        const ChunkSpan<V> sp((uint32_t)(u - row * chunks), n_ch);
-        const T* p = (const T*)a.x + a.rows.at(row);
-        Pack<T, V> v[kChunkIter];
+__global__ __launch_bounds__(kThreads) void k_ln_chunk_apply(const Forward a,
+                                                             const float2* row_part) {
+    constexpr int K = kChunkElems / V;
+    const uint32_t n_ch = a.rows.n_ch, chunks = gridDim.y;
+    const ChunkSpan<V, K> sp(blockIdx.y, n_ch);
+    const double full = kChunkElems * kThreads, last = n_ch - (chunks - 1) * full;
+    float w[kChunkElems], b[kChunkElems];
 #pragma unroll
-        for (uint32_t k = 0; k < kChunkIter; k++) {
+    for (int k = 0; k < K; k++) {
+        load_params<V>(a.aff.weight, a.aff.type, sp.first[k], 1.f, w + k * V);
+        load_params<V>(a.aff.bias, a.aff.type, sp.first[k], 0.f, b + k * V);
+    }
+    for (uint64_t row = blockIdx.x; row < a.rows.n; row += gridDim.x) {
+        const T* p = (const T*)a.x + a.rows.at(row);
+        Pack<T, V> v[K];
+#pragma unroll
+        for (int k = 0; k < K; k++) {
             v[k] = load_loose<T, V>(p + sp.first[k]);
         }
         // about the first chunk's mean: their difference loses nothing
-        const float2* entries = part + row * chunks;
+        const float2* entries = row_part + row * chunks;
         const double pivot = (double)entries[0].x;
         const double2 s = join_chunks(entries, chunks, [&](uint32_t i, float2 e, double2& t) {
             const double n = i + 1 == chunks ? last : full, d = (double)e.x - pivot;
@@ -451,18 +483,24 @@ __global__ __launch_bounds__(kThreads) void k_ln_chunk_apply(const Forward a, ui
         });
         const double d = s.x / n_ch, var = s.y / n_ch - d * d;
         const float mean = (float)(pivot + d);
-        const float rstd = 1.f / sqrtf((float)(var < 0.0 ? 0.0 : var) + a.eps);
-        T* out = (T*)a.y + row * n_ch;
+        const float rstd = inv_sqrt((float)(var < 0.0 ? 0.0 : var) + a.eps);
+        T* y = (T*)a.y + row * n_ch;
 #pragma unroll
-        for (uint32_t k = 0; k < kChunkIter; k++) {
+        for (int k = 0; k < K; k++) {
+            float z[V];
+            unpack(v[k], z);
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                z[j] = fmaf((z[j] - mean) * rstd, w[k * V + j], b[k * V + j]);
+            }
+            act_values<T, V>(a.act, z);
             if (sp.skip[k] < V) {
-                float w[V], b[V];
-                load_params<V>(a.aff.weight, a.aff.type, sp.first[k], 1.f, w);
-                load_params<V>(a.aff.bias, a.aff.type, sp.first[k], 0.f, b);
-                write_y<T, V, false>(v[k], mean, rstd, w, b, a.act, out + sp.first[k]);
+                by_stream(a.stream, [&](auto past) {
+                    store_loose<T, V, decltype(past)::value>(y + sp.first[k], z);
+                });
             }
         }
-        if (u == row * chunks && threadIdx.x == 0 && a.mean) {
+        if (blockIdx.y == 0 && threadIdx.x == 0 && a.mean) {
             a.mean[row] = mean;
             a.rstd[row] = rstd;
         }
@@ -488,138 +526,189 @@ struct Backward {
     Rows rows;
     Affine aff;
     uint32_t act;
+    bool stream, stream_in;
 };
 
-// xh and t = w gz of a vector, and gz added to the sums of a column.
-template <typename T, int V>
-__device__ __forceinline__ void slopes(const Pack<T, V>& xv, const Pack<T, V>& gv, float mean,
-                                       float rstd, const float (&w)[V], const float (&b)[V],
-                                       uint32_t act, float (&xh)[V], float (&t)[V], float (&gw)[V],
-                                       float (&gb)[V]) {
-    float z[V];
-    unpack(xv, xh);
-    unpack(gv, t);
+// Of E values: xh in place of x and t = w gz in place of gy, gz added to the sums
+// of its columns, and t to those of the row.
+template <typename T, int V, int E, bool WHOLE>
+__device__ __forceinline__ float2 slopes(float mean, float rstd, const float (&w)[E],
+                                         const float (&b)[E], uint32_t act, const uint32_t* skip,
+                                         float (&xh)[E], float (&t)[E], float (&gw)[E],
+                                         float (&gb)[E]) {
+    float z[E];
 #pragma unroll
-    for (int j = 0; j < V; j++) {
-        xh[j] = (xh[j] - mean) * rstd;
-        z[j] = fmaf(xh[j], w[j], b[j]);
+    for (int e = 0; e < E; e++) {
+        xh[e] = (xh[e] - mean) * rstd;
+        z[e] = fmaf(xh[e], w[e], b[e]);
     }
-    act_slopes<T, V>(act, z, t);
+    act_slopes<T, E>(act, z, t);
+    float2 s = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int j = 0; j < V; j++) {
-        gb[j] += t[j];
-        gw[j] = fmaf(t[j], xh[j], gw[j]);
-        t[j] *= w[j];
-    }
-}
-
-template <int V, bool WHOLE>
-__device__ __forceinline__ void add_row(const float (&xh)[V], const float (&t)[V], uint32_t skip,
-                                        float2& s) {
-#pragma unroll
-    for (int j = 0; j < V; j++) {
-        const float c = counted<WHOLE>(t[j], j, skip);
+    for (int e = 0; e < E; e++) {
+        gb[e] += t[e];
+        gw[e] = fmaf(t[e], xh[e], gw[e]);
+        t[e] *= w[e];
+        const float c = counted<WHOLE>(t[e], e % V, skip[e / V]);
         s.x += c;
-        s.y += counted<WHOLE>(t[j] * xh[j], j, skip);
+        s.y += WHOLE ? t[e] * xh[e] : counted<false>(t[e] * xh[e], e % V, skip[e / V]);
     }
+    return s;
 }
 
-// gx of a vector, a and c the means of t and t xh.
-template <typename T, int V, bool STREAM>
-__device__ __forceinline__ void write_gx(const float (&xh)[V], const float (&t)[V], float rstd,
-                                         float a, float c, T* gx) {
+// gx of a vector, a and c the row's means of t and t xh.
+template <typename T, int V>
+__device__ __forceinline__ void write_gx(const float* xh, const float* t, float rstd, float a,
+                                         float c, T* gx, bool stream) {
     float g[V];
 #pragma unroll
     for (int j = 0; j < V; j++) {
-        g[j] = rstd * ((t[j] - a) - xh[j] * c);
+        g[j] = rstd * fmaf(-xh[j], c, t[j] - a);
     }
-    store_loose<T, V, STREAM>(gx, g);
+    by_stream(stream, [&](auto past) { store_loose<T, V, decltype(past)::value>(gx, g); });
 }
 
-__device__ __forceinline__ void write_sums(const Backward& a, uint32_t ch, float gw, float gb) {
-    if (a.part) {
-        float* p = a.part + blockIdx.x * a.part_stride;
-        p[ch] = gw;
-        p[a.rows.n_ch + ch] = gb;
+// A workgroup's sums of the columns `ch` on, of which the first `skip` are
+// another's.
+template <int V>
+__device__ __forceinline__ void write_sums(const Backward& a, uint32_t ch, uint32_t skip,
+                                           const float* gw, const float* gb) {
+    float* p = a.part ? a.part + blockIdx.x * a.part_stride + ch : nullptr;
+    if (p && skip == 0) {
+        store_loose<float, V>(p, gw);
+        store_loose<float, V>(p + a.rows.n_ch, gb);
         return;
     }
-    if (a.gw) {
-        store_one(a.gw, a.aff.type, ch, gw);
-    }
-    if (a.gb) {
-        store_one(a.gb, a.aff.type, ch, gb);
+#pragma unroll
+    for (uint32_t j = 0; j < V; j++) {
+        if (j < skip) {
+            continue;
+        }
+        if (p) {
+            p[j] = gw[j];
+            p[a.rows.n_ch + j] = gb[j];
+            continue;
+        }
+        if (a.gw) {
+            store_one(a.gw, a.aff.type, ch + j, gw[j]);
+        }
+        if (a.gb) {
+            store_one(a.gb, a.aff.type, ch + j, gb[j]);
+        }
     }
 }
 
-template <int V, int K>
-constexpr int kInFlightBwd = K == 1 ? 2 : 1;
+// Whether a lane reads its next row while it works on one, or else two at a time.
+template <int L, bool WHOLE>
+constexpr bool kAhead = WHOLE || L >= 32;
 
-template <typename T, int V, int L, int K, bool WHOLE, bool STREAM>
+// L lanes hold a row, K vectors each.
+template <typename T, int V, int L, int K, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void k_ln_bwd_rows(const Backward a) {
-    constexpr int R = kInFlightBwd<V, K>;
-    constexpr uint32_t kSlots = kThreads / L, kWaves = kThreads / 64;
-    __shared__ float2 red[kWaves][L * K * V];
+    constexpr int E = K * V, R = kAhead<L, WHOLE> ? 1 : 2;
+    constexpr uint32_t kSlots = kThreads / L, kTake = kSlots * R, kWaves = kThreads / 64;
+    __shared__ float red[kWaves][2][L * E];
     const uint32_t lane = threadIdx.x % L, slot = threadIdx.x / L;
     const Rows& rows = a.rows;
-    uint32_t first[K], skip[K];
-    float w[K][V], b[K][V], gw[K][V], gb[K][V];
+    const uint32_t px_bytes = (uint32_t)(rows.px_stride * sizeof(T));
+    const uint32_t row_bytes = rows.n_ch * sizeof(T);
+    uint32_t first[K], skip[K];  // first: in bytes
+    float w[E], b[E], gw[E], gb[E];
 #pragma unroll
     for (int k = 0; k < K; k++) {
         const Span<V> sp(k * L + lane, rows.n_ch);
-        first[k] = sp.first;
+        first[k] = sp.first * sizeof(T);
         skip[k] = sp.skip;
-        load_params<V>(a.aff.weight, a.aff.type, sp.first, 1.f, w[k]);
-        load_params<V>(a.aff.bias, a.aff.type, sp.first, 0.f, b[k]);
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-            gw[k][j] = gb[k][j] = 0.f;
-        }
+        load_params<V>(a.aff.weight, a.aff.type, sp.first, 1.f, w + k * V);
+        load_params<V>(a.aff.bias, a.aff.type, sp.first, 0.f, b + k * V);
     }
-    const T* x = (const T*)a.x;
-    const T* gy = (const T*)a.gy;
-    T* gx = (T*)a.gx;
-    for (uint64_t r0 = (uint64_t)blockIdx.x * (kSlots * R); r0 < rows.n;
-         r0 += (uint64_t)gridDim.x * (kSlots * R)) {
-        Pack<T, V> xv[R][K], gv[R][K];
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        gw[e] = gb[e] = 0.f;
+    }
+    struct Raw {
+        Pack<T, V> x[R][K], g[R][K];
         float mean[R], rstd[R];
+    };
+    const uint32_t in = slot * px_bytes, out = slot * row_bytes;
+    const auto load = [&](uint64_t r0, Raw& r) {
+        const T* x = (const T*)a.x;
+        const T* g = (const T*)a.gy;
+        if (rows.flat && r0 + kTake <= rows.n) {
+            x += r0 * rows.px_stride;
+            g += r0 * rows.n_ch;
+            by_stream(L >= kStreamLanes && a.stream_in, [&](auto past) {
 #pragma unroll
-        for (int i = 0; i < R; i++) {
-            const uint64_t at = r0 + i * kSlots + slot, row = at < rows.n ? at : rows.n - 1;
-            const T* p = x + rows.at(row);
-            const T* q = gy + row * rows.n_ch;
-            mean[i] = a.mean[row];
-            rstd[i] = a.rstd[row];
+                for (int i = 0; i < R; i++) {
+                    r.mean[i] = (a.mean + r0 + i * kSlots)[slot];
+                    r.rstd[i] = (a.rstd + r0 + i * kSlots)[slot];
 #pragma unroll
-            for (int k = 0; k < K; k++) {
-                xv[i][k] = load_loose<T, V, STREAM>(p + first[k]);
-                gv[i][k] = load_loose<T, V, STREAM>(q + first[k]);
+                    for (int k = 0; k < K; k++) {
+                        r.x[i][k] = load_loose<T, V, decltype(past)::value>(
+                            at_byte(x + (size_t)(i * kSlots) * rows.px_stride, in + first[k]));
+                        r.g[i][k] = load_loose<T, V, decltype(past)::value>(
+                            at_byte(g + (size_t)(i * kSlots) * rows.n_ch, out + first[k]));
+                    }
+                }
+            });
+        } else {  // past the end the last row again
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                const uint64_t row = std::min(r0 + i * kSlots + slot, rows.n - 1);
+                const T* p = x + rows.at(row);
+                const T* q = g + row * rows.n_ch;
+                r.mean[i] = a.mean[row];
+                r.rstd[i] = a.rstd[row];
+#pragma unroll
+                for (int k = 0; k < K; k++) {
+                    r.x[i][k] = load_loose<T, V>(at_byte(p, first[k]));
+                    r.g[i][k] = load_loose<T, V>(at_byte(q, first[k]));
+                }
             }
         }
+    };
+    const uint64_t step = (uint64_t)gridDim.x * kTake;
+    uint64_t r0 = (uint64_t)blockIdx.x * kTake;  // there are no more workgroups than rows for them
+    Raw raw;
+    if (kAhead<L, WHOLE>) {
+        load(r0, raw);
+    }
+    for (; r0 < rows.n; r0 += step) {
+        Raw ahead;
+        if (!kAhead<L, WHOLE>) {
+            load(r0, raw);
+        } else if (r0 + step < rows.n) {
+            load(r0 + step, ahead);
+        }
 #pragma unroll
         for (int i = 0; i < R; i++) {
-            const uint64_t row = r0 + i * kSlots + slot;
-            const bool live = row < rows.n;
-            float xh[K][V], t[K][V];
+            const bool live = r0 + i * kSlots + slot < rows.n;
+            float xh[E], t[E];
             float2 s = make_float2(0.f, 0.f);
             if (live) {
 #pragma unroll
-                for (int k = 0; k < K; k++) {
-                    slopes<T, V>(xv[i][k], gv[i][k], mean[i], rstd[i], w[k], b[k], a.act, xh[k],
-                                 t[k], gw[k], gb[k]);
-                    add_row<V, WHOLE>(xh[k], t[k], skip[k], s);
+                for (int e = 0; e < E; e++) {
+                    xh[e] = to_float(raw.x[i][e / V].v[e % V]);
+                    t[e] = to_float(raw.g[i][e / V].v[e % V]);
                 }
+                s = slopes<T, V, E, WHOLE>(raw.mean[i], raw.rstd[i], w, b, a.act, skip, xh, t, gw,
+                                           gb);
             }
             s.x = lane_sum<L>(s.x) * rows.inv;
             s.y = lane_sum<L>(s.y) * rows.inv;
-            if (live && gx) {
+            if (live && a.gx) {
+                T* gx = (T*)a.gx + (r0 + i * kSlots) * rows.n_ch;
 #pragma unroll
                 for (int k = 0; k < K; k++) {
                     if (WHOLE || skip[k] < V) {
-                        write_gx<T, V, STREAM>(xh[k], t[k], rstd[i], s.x, s.y,
-                                               gx + row * rows.n_ch + first[k]);
+                        write_gx<T, V>(xh + k * V, t + k * V, raw.rstd[i], s.x, s.y,
+                                       at_byte(gx, out + first[k]), a.stream);
                     }
                 }
             }
+        }
+        if (kAhead<L, WHOLE>) {
+            raw = ahead;
         }
     }
     if (!a.part && !a.gw && !a.gb) {
@@ -628,53 +717,162 @@ __global__ __launch_bounds__(kThreads) void k_ln_bwd_rows(const Backward a) {
     // a column's sums over the slots: of a wave, then of the waves
     const uint32_t wave = threadIdx.x >> 6;
 #pragma unroll
-    for (int k = 0; k < K; k++) {
+    for (int e = 0; e < E; e++) {
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-            for (int o = L; o < 64; o <<= 1) {
-                gw[k][j] += __shfl_xor(gw[k][j], o);
-                gb[k][j] += __shfl_xor(gb[k][j], o);
-            }
-            if ((threadIdx.x & 63u) < L) {
-                red[wave][(k * V + j) * L + lane] = make_float2(gw[k][j], gb[k][j]);
-            }
+        for (int o = L; o < 64; o <<= 1) {
+            gw[e] += __shfl_xor(gw[e], o);
+            gb[e] += __shfl_xor(gb[e], o);
+        }
+        if ((threadIdx.x & 63u) < L) {
+            // a vector's values side by side
+            const uint32_t at = ((e / V) * L + lane) * V + e % V;
+            red[wave][0][at] = gw[e];
+            red[wave][1][at] = gb[e];
         }
     }
     __syncthreads();
-    for (uint32_t e = threadIdx.x; e < L * K * V; e += kThreads) {
-        const uint32_t vec = e / (L * V) * L + e % L, j = e / L % V;
-        const Span<V> sp(vec, rows.n_ch);
-        if (j >= sp.skip) {
-            float2 s = red[0][e];
+    for (uint32_t e = threadIdx.x; e < L * E; e += kThreads) {
+        const Span<V> sp(e / V, rows.n_ch);
+        if (e % V >= sp.skip) {
+            float sw = red[0][0][e], sb = red[0][1][e];
 #pragma unroll
             for (uint32_t i = 1; i < kWaves; i++) {
-                s.x += red[i][e].x;
-                s.y += red[i][e].y;
+                sw += red[i][0][e];
+                sb += red[i][1][e];
             }
-            write_sums(a, sp.first + j, s.x, s.y);
+            write_sums<1>(a, sp.first + e % V, 0, &sw, &sb);
         }
     }
 }
 
-template <typename T, int V, int K, uint32_t THREADS, bool HOLD, bool WHOLE, bool STREAM>
+// A workgroup holds a row, K vectors a thread, and reads the next one meanwhile,
+// unless there are 1024 threads: those have too few registers each for that, and
+// keep weight and bias in LDS.
+template <typename T, int V, int K, uint32_t THREADS, bool WHOLE>
 __global__ __launch_bounds__(THREADS) void k_ln_bwd_wide(const Backward a) {
     __shared__ float2 part[2][THREADS / 64];
+    constexpr int E = K * V;
+    constexpr bool kFew = THREADS == 1024;
+    __shared__ Pack<float, V> affine[kFew ? 2 : 1][kFew ? K * THREADS : 1];
     const Rows& rows = a.rows;
     uint32_t first[K], skip[K];
-    float w[K][V], b[K][V], gw[K][V], gb[K][V];
+    float w[E], b[E], gw[E], gb[E];
 #pragma unroll
     for (int k = 0; k < K; k++) {
         const Span<V> sp(k * blockDim.x + threadIdx.x, rows.n_ch);
         first[k] = sp.first;
         skip[k] = sp.skip;
-        if (HOLD) {
-            load_params<V>(a.aff.weight, a.aff.type, sp.first, 1.f, w[k]);
-            load_params<V>(a.aff.bias, a.aff.type, sp.first, 0.f, b[k]);
-        }
+        load_params<V>(a.aff.weight, a.aff.type, sp.first, 1.f, w + k * V);
+        load_params<V>(a.aff.bias, a.aff.type, sp.first, 0.f, b + k * V);
+        if (kFew) {  // each thread's own: no barrier
 #pragma unroll
-        for (int j = 0; j < V; j++) {
-            gw[k][j] = gb[k][j] = 0.f;
+            for (int j = 0; j < V; j++) {
+                affine[0][k * THREADS + threadIdx.x].v[j] = w[k * V + j];
+                affine[1][k * THREADS + threadIdx.x].v[j] = b[k * V + j];
+            }
         }
+    }
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        gw[e] = gb[e] = 0.f;
+    }
+    struct Raw {
+        Pack<T, V> x[K], g[K];
+        float mean, rstd;
+    };
+    const auto load = [&](uint64_t row, Raw& r) {
+        const T* p = (const T*)a.x + rows.at(row);
+        const T* q = (const T*)a.gy + row * rows.n_ch;
+        r.mean = a.mean[row];
+        r.rstd = a.rstd[row];
+        by_stream(!kFew && a.stream_in, [&](auto past) {
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                r.x[k] = load_loose<T, V, decltype(past)::value>(p + first[k]);
+                r.g[k] = load_loose<T, V, decltype(past)::value>(q + first[k]);
+            }
+        });
+    };
+    uint32_t turn = 0;
+    Raw raw;
+    if (!kFew) {
+        load(blockIdx.x, raw);  // there are no more workgroups than rows
+    }
+    for (uint64_t row = blockIdx.x; row < rows.n; row += gridDim.x, turn ^= 1) {
+        Raw ahead;
+        if (kFew) {
+            load(row, raw);
+        } else if (row + gridDim.x < rows.n) {
+            load(row + gridDim.x, ahead);
+        }
+        float xh[E], t[E];
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            xh[e] = to_float(raw.x[e / V].v[e % V]);
+            t[e] = to_float(raw.g[e / V].v[e % V]);
+        }
+        const float rstd = raw.rstd;
+        float2 s = make_float2(0.f, 0.f);
+        if constexpr (kFew) {
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                float wk[V], bk[V];
+                unpack(affine[0][k * THREADS + threadIdx.x], wk);
+                unpack(affine[1][k * THREADS + threadIdx.x], bk);
+                const auto part_of = [&](float* p) -> float (&)[V] {
+                    return *(float (*)[V])(p + k * V);
+                };
+                const float2 sk = slopes<T, V, V, WHOLE>(
+                    raw.mean, rstd, wk, bk, a.act, skip + k, part_of(xh), part_of(t), part_of(gw),
+                    part_of(gb));
+                s.x += sk.x;
+                s.y += sk.y;
+            }
+        } else {
+            s = slopes<T, V, E, WHOLE>(raw.mean, rstd, w, b, a.act, skip, xh, t, gw, gb);
+        }
+        s = wide_sum(s, part[turn]);
+        if (a.gx) {
+            T* gx = (T*)a.gx + row * rows.n_ch;
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                if (WHOLE || skip[k] < V) {
+                    write_gx<T, V>(xh + k * V, t + k * V, rstd, s.x * rows.inv, s.y * rows.inv,
+                                   gx + first[k], a.stream);
+                }
+            }
+        }
+        if (!kFew) {
+            raw = ahead;
+        }
+    }
+    if (!a.part && !a.gw && !a.gb) {
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        write_sums<V>(a, first[k], skip[k], gw + k * V, gb + k * V);
+    }
+}
+
+// Longer rows, in chunks like the forward pass's. The first pass leaves a chunk's
+// sums of t and t xh of each row, and the columns' over its rows.
+template <typename T, int V, bool APPLY>
+__global__ __launch_bounds__(kThreads) void k_ln_bwd_chunk(const Backward a, float2* row_part) {
+    __shared__ float2 part[2][kThreads / 64];
+    constexpr int E = kChunkElemsBwd, K = E / V;
+    const Rows& rows = a.rows;
+    const uint32_t chunk = blockIdx.y, chunks = gridDim.y;
+    const ChunkSpan<V, K> sp(chunk, rows.n_ch);
+    float w[E], b[E], gw[E], gb[E];
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        load_params<V>(a.aff.weight, a.aff.type, sp.first[k], 1.f, w + k * V);
+        load_params<V>(a.aff.bias, a.aff.type, sp.first[k], 0.f, b + k * V);
+    }
+#pragma unroll
+    for (int e = 0; e < E; e++) {
+        gw[e] = gb[e] = 0.f;
     }
     uint32_t turn = 0;
     for (uint64_t row = blockIdx.x; row < rows.n; row += gridDim.x, turn ^= 1) {
@@ -684,125 +882,43 @@ __global__ __launch_bounds__(THREADS) void k_ln_bwd_wide(const Backward a) {
         Pack<T, V> xv[K], gv[K];
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            xv[k] = load_loose<T, V, STREAM>(p + first[k]);
-            gv[k] = load_loose<T, V, STREAM>(q + first[k]);
+            xv[k] = load_loose<T, V>(p + sp.first[k]);
+            gv[k] = load_loose<T, V>(q + sp.first[k]);
         }
-        float xh[K][V], t[K][V];
-        float2 s = make_float2(0.f, 0.f);
+        float xh[E], t[E];
 #pragma unroll
-        for (int k = 0; k < K; k++) {
-            if (!HOLD) {
-                load_params<V>(a.aff.weight, a.aff.type, first[k], 1.f, w[k]);
-                load_params<V>(a.aff.bias, a.aff.type, first[k], 0.f, b[k]);
-            }
-            slopes<T, V>(xv[k], gv[k], mean, rstd, w[k], b[k], a.act, xh[k], t[k], gw[k], gb[k]);
-            add_row<V, WHOLE>(xh[k], t[k], skip[k], s);
+        for (int e = 0; e < E; e++) {
+            xh[e] = to_float(xv[e / V].v[e % V]);
+            t[e] = to_float(gv[e / V].v[e % V]);
         }
-        s = wide_sum(s, part[turn]);
-        if (a.gx) {
-            T* out = (T*)a.gx + row * rows.n_ch;
+        const float2 s = slopes<T, V, E, false>(mean, rstd, w, b, a.act, sp.skip, xh, t, gw, gb);
+        if constexpr (APPLY) {
+            const double2 sum = join_chunks(row_part + row * chunks, chunks,
+                                            [](uint32_t, float2 e, double2& d) {
+                                                d.x += (double)e.x;
+                                                d.y += (double)e.y;
+                                            });
+            const float ma = (float)(sum.x / rows.n_ch), mc = (float)(sum.y / rows.n_ch);
+            T* gx = (T*)a.gx + row * rows.n_ch;
 #pragma unroll
             for (int k = 0; k < K; k++) {
-                if (WHOLE || skip[k] < V) {
-                    write_gx<T, V, STREAM>(xh[k], t[k], rstd, s.x * rows.inv, s.y * rows.inv,
-                                           out + first[k]);
+                if (sp.skip[k] < V) {
+                    write_gx<T, V>(xh + k * V, t + k * V, rstd, ma, mc, gx + sp.first[k], a.stream);
                 }
+            }
+        } else {
+            const float2 sum = wide_sum(s, part[turn]);
+            if (threadIdx.x == 0) {
+                row_part[row * chunks + chunk] = sum;
             }
         }
     }
-    if (!a.part && !a.gw && !a.gb) {
+    if (APPLY || (!a.part && !a.gw && !a.gb)) {
         return;
     }
 #pragma unroll
     for (int k = 0; k < K; k++) {
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-            if (j >= skip[k]) {
-                write_sums(a, first[k] + j, gw[k][j], gb[k][j]);
-            }
-        }
-    }
-}
-
-// Longer rows, in chunks: a workgroup takes one chunk of every gridDim.x-th row.
-// The first pass leaves the chunk's sums of t and t xh of each row, and the
-// columns' over its rows.
-template <typename T, int V>
-__global__ __launch_bounds__(kThreads) void k_ln_bwd_chunk_sums(const Backward a, uint32_t chunks,
-                                                                float2* row_part) {
-    __shared__ float2 part[2][kThreads / 64];
-    const Rows& rows = a.rows;
-    const uint32_t chunk = blockIdx.y;
-    const ChunkSpan<V> sp(chunk, rows.n_ch);
-    float gw[kChunkIter][V], gb[kChunkIter][V];
-#pragma unroll
-    for (uint32_t k = 0; k < kChunkIter; k++) {
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-            gw[k][j] = gb[k][j] = 0.f;
-        }
-    }
-    uint32_t turn = 0;
-    for (uint64_t row = blockIdx.x; row < rows.n; row += gridDim.x, turn ^= 1) {
-        const T* p = (const T*)a.x + rows.at(row);
-        const T* q = (const T*)a.gy + row * rows.n_ch;
-        const float mean = a.mean[row], rstd = a.rstd[row];
-        float2 s = make_float2(0.f, 0.f);
-#pragma unroll
-        for (uint32_t k = 0; k < kChunkIter; k++) {
-            float w[V], b[V], xh[V], t[V];
-            load_params<V>(a.aff.weight, a.aff.type, sp.first[k], 1.f, w);
-            load_params<V>(a.aff.bias, a.aff.type, sp.first[k], 0.f, b);
-            slopes<T, V>(load_loose<T, V>(p + sp.first[k]), load_loose<T, V>(q + sp.first[k]), mean,
-                         rstd, w, b, a.act, xh, t, gw[k], gb[k]);
-            add_row<V, false>(xh, t, sp.skip[k], s);
-        }
-        s = wide_sum(s, part[turn]);
-        if (threadIdx.x == 0) {
-            row_part[row * chunks + chunk] = s;
-        }
-    }
-    if (!a.part && !a.gw && !a.gb) {
-        return;
-    }
-#pragma unroll
-    for (uint32_t k = 0; k < kChunkIter; k++) {
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-            if (j >= sp.skip[k]) {
-                write_sums(a, sp.first[k] + j, gw[k][j], gb[k][j]);
-            }
-        }
-    }
-}
-
-template <typename T, int V>
-__global__ __launch_bounds__(kThreads) void k_ln_bwd_chunk_apply(const Backward a, uint32_t chunks,
-                                                                 const float2* row_part) {
-    const uint32_t n_ch = a.rows.n_ch;
-    for (uint64_t u = blockIdx.x; u < a.rows.n * chunks; u += gridDim.x) {
-        const uint64_t row = u / chunks;
-        const ChunkSpan<V> sp((uint32_t)(u - row * chunks), n_ch);
-        const T* p = (const T*)a.x + a.rows.at(row);
-        const T* q = (const T*)a.gy + row * n_ch;
-        const float mean = a.mean[row], rstd = a.rstd[row];
-        const double2 s = join_chunks(row_part + row * chunks, chunks,
-                                      [](uint32_t, float2 e, double2& t) {
-                                          t.x += (double)e.x;
-                                          t.y += (double)e.y;
-                                      });
-        const float ma = (float)(s.x / n_ch), mc = (float)(s.y / n_ch);
-#pragma unroll
-        for (uint32_t k = 0; k < kChunkIter; k++) {
-            if (sp.skip[k] < V) {
-                float w[V], b[V], xh[V], t[V], gw[V] = {}, gb[V] = {};
-                load_params<V>(a.aff.weight, a.aff.type, sp.first[k], 1.f, w);
-                load_params<V>(a.aff.bias, a.aff.type, sp.first[k], 0.f, b);
-                slopes<T, V>(load_loose<T, V>(p + sp.first[k]), load_loose<T, V>(q + sp.first[k]),
-                             mean, rstd, w, b, a.act, xh, t, gw, gb);
-                write_gx<T, V, false>(xh, t, rstd, ma, mc, (T*)a.gx + row * n_ch + sp.first[k]);
-            }
-        }
+        write_sums<V>(a, sp.first[k], sp.skip[k], gw + k * V, gb + k * V);
     }
 }
 
@@ -857,60 +973,87 @@ __global__ __launch_bounds__(kParamThreads) void k_ln_params(const float* part, 
 // how a call is cut
 // ---------------------------------------------------------------------------
 
-// A type's vectors, and a single value where a row is shorter.
+// A type's vectors, and single values where a row is shorter.
 constexpr uint32_t vec_of(uint32_t type, uint32_t n_ch) {
     const uint32_t v = type == DRESSI_F32 ? 4 : 8;
     return n_ch >= v ? v : 1;
 }
 
-// Vectors of a row up to which a wave, then a workgroup of 1024, holds it, forward and backward.
-constexpr uint32_t kWaveVecs = 256, kWaveVecsBwd = 128;
-constexpr uint32_t kHoldElems = 32768, kHoldElemsBwd = 16384;
+// Values of a row up to which a wave, then a workgroup, holds it.
+constexpr uint32_t kWaveElems = 64 * 32, kWaveElemsBwd = 64 * 16;
+constexpr uint32_t kHoldElems = 1024 * 32, kHoldElemsBwd = 1024 * 16;
 
-// Bytes of results from which they go past the caches.
-constexpr uint64_t kStreamBytes = 32ull << 20;
+// Bytes of results, and of inputs, from which they go past the caches.
+constexpr uint64_t kStreamBytes = 32ull << 20, kStreamInBytes = 256ull << 20;
 
 struct Plan {
-    uint32_t v, vecs;  // of a row
-    bool chunked, wide, whole, stream;
-    uint32_t lanes, iter;  // of a row; wide: lanes = the workgroup's threads
-    uint32_t chunks;       // of a row
-    uint32_t groups;       // workgroups whose sums of gw and gb are added
+    uint32_t v;
+    bool wide, whole, stream, stream_in;
+    uint32_t lanes;   // of a row; wide: the workgroup's threads
+    uint32_t elems;   // of a lane
+    uint32_t chunks;  // of a row, where there are some
+    uint32_t groups;  // workgroups whose sums of gw and gb are added
 };
 
+// Lanes and values of each for a row that a wave holds: the fewest values held
+// in all, in lanes of 8 to 24 (backward 8 or 16) where they suffice.
+void cut_row(Plan& p, uint32_t n_ch, bool backward) {
+    const uint32_t vecs = div_up(n_ch, p.v);
+    if (p.v == 1) {  // a lane a row
+        p.lanes = p.elems = 1;
+        while (p.elems < n_ch) {
+            p.elems *= 2;
+        }
+        return;
+    }
+    uint32_t best = ~0u;
+    const uint32_t any[] = {16, 24, 8, 4, 32}, bwd[] = {8, 4, 16};
+    const uint32_t* list = backward ? bwd : any;
+    for (uint32_t i = 0; i < (backward ? 3u : 5u); i++) {
+        const uint32_t elems = list[i];
+        uint32_t lanes = 1;
+        while (lanes < 64 && lanes * elems < n_ch) {
+            lanes *= 2;
+        }
+        if (elems < p.v || lanes * elems < vecs * p.v || (elems == 32 && lanes < 64)) {
+            continue;
+        }
+        if (lanes * elems < best || (n_ch <= 16 && elems == p.v && lanes * elems == best)) {
+            best = lanes * elems;
+            p.lanes = lanes;
+            p.elems = elems;
+        }
+    }
+}
+
+// By the number of rows and not by where they lie: so is the scratch.
 Plan make_plan(uint32_t type, uint64_t rows, uint32_t n_ch, bool backward) {
     Plan p{};
     p.v = vec_of(type, n_ch);
-    p.vecs = div_up(n_ch, p.v);
-    p.stream = rows * n_ch * type_bytes(type) >= kStreamBytes;
-    const uint32_t most = backward ? kWaveVecsBwd : kWaveVecs;
+    const uint64_t bytes = rows * n_ch * type_bytes(type);
+    p.stream = bytes >= kStreamBytes;
+    p.stream_in = bytes * (backward ? 2 : 1) >= kStreamInBytes;
     if (n_ch > (backward ? kHoldElemsBwd : kHoldElems)) {
-        p.chunked = true;
-        p.chunks = div_up(p.vecs, kChunkVecs);
+        p.elems = backward ? kChunkElemsBwd : kChunkElems;
+        p.chunks = div_up(n_ch, p.elems * kThreads);
         p.groups = (uint32_t)std::min<uint64_t>(rows, std::max(1u, 1024 / p.chunks));
-    } else if (p.vecs > most) {
+    } else if (n_ch > (backward ? kWaveElemsBwd : kWaveElems)) {
         p.wide = true;
-        const uint32_t elems = backward ? 16 : 32;  // a thread's at most
-        p.iter = 1;
-        while (p.iter * p.v < elems && p.vecs > p.iter * 256) {
-            p.iter *= 2;
+        p.elems = p.v;
+        while (p.elems < (backward ? 16 : 32) && n_ch > p.elems * 256) {
+            p.elems *= 2;
         }
-        p.lanes = div_up(div_up(p.vecs, p.iter), 64) * 64;
-        p.whole = n_ch == p.lanes * p.iter * p.v;
-        p.groups = (uint32_t)std::min<uint64_t>(rows, 512);
+        p.lanes = div_up(div_up(n_ch, p.elems), 64) * 64;
+        const uint32_t most = p.lanes > 512 ? 256 : 512 * 256 / std::max(256u, p.lanes);
+        p.groups = (uint32_t)std::min<uint64_t>(
+            {rows, most, std::max<uint64_t>(128, rows / 4)});
     } else {
-        p.lanes = 1;
-        while (p.lanes < 64 && p.lanes < p.vecs) {
-            p.lanes *= 2;
-        }
-        p.iter = 1;
-        while (p.iter * p.lanes < p.vecs) {
-            p.iter *= 2;
-        }
-        p.whole = n_ch == p.lanes * p.iter * p.v;
-        const uint64_t slots = kThreads / p.lanes * (p.iter == 1 ? 2 : 1);
-        p.groups = (uint32_t)std::min<uint64_t>((rows + slots - 1) / slots, 1024);
+        cut_row(p, n_ch, backward);
+        const bool one = n_ch == p.lanes * p.elems || p.lanes >= 32;  // kAhead
+        const uint64_t take = kThreads / p.lanes * (one ? 1 : 2);
+        p.groups = (uint32_t)std::min<uint64_t>((rows + take - 1) / take, 1024);
     }
+    p.whole = n_ch == p.lanes * p.elems;
     return p;
 }
 
@@ -918,120 +1061,147 @@ size_t part_stride(uint32_t n_ch) { return (2 * (size_t)n_ch + 3) / 4 * 4; }
 
 // Bytes of the chunks' sums, and of the workgroups' of gw and gb after them.
 size_t row_bytes(const Plan& p, uint64_t rows) {
-    return p.chunked ? (rows * p.chunks * sizeof(float2) + 15) / 16 * 16 : 0;
+    return (rows * p.chunks * sizeof(float2) + 15) / 16 * 16;
 }
 size_t scratch_bytes_of(const Plan& p, uint64_t rows, uint32_t n_ch, bool backward) {
-    const size_t sums = backward && p.groups > 1 ? p.groups * part_stride(n_ch) * sizeof(float) : 0;
-    return row_bytes(p, rows) + sums;
+    const bool sums = backward && p.groups > 1;
+    return row_bytes(p, rows) + (sums ? p.groups * part_stride(n_ch) * sizeof(float) : 0);
 }
 
 template <typename A>
-int launch(void (*kernel)(A), uint32_t grid, uint32_t threads, hipStream_t s, const A& a) {
-    hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), 0, s, a);
+int launch(void (*kernel)(A), uint64_t most, uint32_t limit, uint32_t threads, hipStream_t s,
+           const A& a) {
+    hipLaunchKernelGGL(kernel, dim3((uint32_t)std::min<uint64_t>(most, limit)), dim3(threads), 0, s,
+                       a);
     DRESSI_CHECK_LAUNCH();
     return DRESSI_OK;
 }
 
-// f(integral_constant)s of a truth value, and of a power of two up to MOST.
 template <typename F>
 auto for_bool(bool x, F&& f) {
     return x ? f(std::true_type()) : f(std::false_type());
 }
-template <int MOST, int LEAST = 1, typename F>
-int for_power(uint32_t x, F&& f) {
-    if constexpr (LEAST < MOST) {
-        if (x > LEAST) {
-            return for_power<MOST, LEAST * 2>(x, f);
+// f(x as a constant) of the values in the list.
+template <uint32_t FIRST, uint32_t... MORE, typename F>
+int for_value(uint32_t x, F&& f) {
+    if constexpr (sizeof...(MORE) > 0) {
+        if (x != FIRST) {
+            return for_value<MORE...>(x, f);
         }
     }
-    return f(std::integral_constant<int, LEAST>());
+    return f(std::integral_constant<uint32_t, FIRST>());
+}
+
+// f(a lane's values as a constant): 4 (in vectors of 4), 8, 16 and MOST.
+template <int V, uint32_t MOST, typename F>
+int for_elems(uint32_t x, F&& f) {
+    if constexpr (V == 4) {
+        return for_value<4, 8, 16, MOST>(x, f);
+    } else {
+        return for_value<8, 16, MOST>(x, f);
+    }
 }
 
 template <typename T, int V>
 int forward(hipStream_t s, const Plan& p, const Forward& a, void* scratch) {
-    const uint64_t n = a.rows.n;
-    if (p.chunked) {
-        const uint32_t grid = (uint32_t)std::min<uint64_t>(n * p.chunks, 1u << 20);
-        hipLaunchKernelGGL((k_ln_chunk_stats<T, V>), dim3(grid), dim3(kThreads), 0, s, a, p.chunks,
-                           (float2*)scratch);
-        DRESSI_CHECK_LAUNCH();
-        hipLaunchKernelGGL((k_ln_chunk_apply<T, V>), dim3(grid), dim3(kThreads), 0, s, a, p.chunks,
-                           (const float2*)scratch);
-        DRESSI_CHECK_LAUNCH();
-        return DRESSI_OK;
-    }
-    return for_bool(p.whole, [&](auto whole) {
-        return for_bool(p.stream, [&](auto stream) {
-            constexpr bool W = decltype(whole)::value, S = decltype(stream)::value;
-            if constexpr (V > 1) {
-                if (p.wide) {
-                    const uint32_t grid = (uint32_t)std::min<uint64_t>(n, 256 * (2048 / p.lanes));
-                    return for_power<32 / V, 2>(p.iter, [&](auto iter) {
-                        constexpr int K = decltype(iter)::value;
-                        return p.lanes <= 256
-                                   ? launch(k_ln_wide<T, V, K, 256, true, W, S>, grid, p.lanes, s, a)
-                                   : launch(k_ln_wide<T, V, K, 1024, false, W, S>, grid, p.lanes, s, a);
-                    });
-                }
-                if (p.lanes == 64 && p.iter > 1) {
-                    return for_power<4, 2>(p.iter, [&](auto iter) {
-                        constexpr int K = decltype(iter)::value;
-                        const uint64_t take = kThreads / 64 * kInFlight<V, K>;
-                        return launch(k_ln_rows<T, V, 64, K, W, S>,
-                                      (uint32_t)std::min<uint64_t>((n + take - 1) / take, 2048),
-                                      kThreads, s, a);
-                    });
-                }
-            }
-            return for_power<(V > 1 ? 64 : 8)>(p.lanes, [&](auto lanes) {
-                constexpr int L = decltype(lanes)::value;
-                const uint64_t take = kThreads / L * kInFlight<V, 1>;
-                return launch(k_ln_rows<T, V, L, 1, W, S>,
-                              (uint32_t)std::min<uint64_t>((n + take - 1) / take, 2048), kThreads,
-                              s, a);
-            });
-        });
-    });
-}
-
-template <typename T, int V>
-int backward(hipStream_t s, const Plan& p, const Backward& a, float2* row_part) {
-    const uint64_t n = a.rows.n;
-    if (p.chunked) {
-        hipLaunchKernelGGL((k_ln_bwd_chunk_sums<T, V>), dim3(p.groups, p.chunks), dim3(kThreads), 0,
-                           s, a, p.chunks, row_part);
-        DRESSI_CHECK_LAUNCH();
-        if (a.gx) {
-            hipLaunchKernelGGL((k_ln_bwd_chunk_apply<T, V>),
-                               dim3((uint32_t)std::min<uint64_t>(n * p.chunks, 1u << 20)),
-                               dim3(kThreads), 0, s, a, p.chunks, (const float2*)row_part);
+    if (p.chunks) {
+        const uint32_t most = std::max(1u, 2048 / p.chunks);
+        const dim3 grid((uint32_t)std::min<uint64_t>(a.rows.n, most), p.chunks);
+        if constexpr (V > 1) {
+            hipLaunchKernelGGL((k_ln_chunk_stats<T, V>), grid, dim3(kThreads), 0, s, a,
+                               (float2*)scratch);
+            DRESSI_CHECK_LAUNCH();
+            hipLaunchKernelGGL((k_ln_chunk_apply<T, V>), grid, dim3(kThreads), 0, s, a,
+                               (const float2*)scratch);
             DRESSI_CHECK_LAUNCH();
         }
         return DRESSI_OK;
     }
     return for_bool(p.whole, [&](auto whole) {
-        return for_bool(p.stream, [&](auto stream) {
-            constexpr bool W = decltype(whole)::value, S = decltype(stream)::value;
-            if constexpr (V > 1) {
-                if (p.wide) {
-                    return for_power<16 / V>(p.iter, [&](auto iter) {
-                        constexpr int K = decltype(iter)::value;
-                        return p.lanes <= 256
-                                   ? launch(k_ln_bwd_wide<T, V, K, 256, true, W, S>, p.groups,
-                                            p.lanes, s, a)
-                                   : launch(k_ln_bwd_wide<T, V, K, 1024, false, W, S>, p.groups,
-                                            p.lanes, s, a);
-                    });
-                }
-                if (p.lanes == 64 && p.iter == 2) {
-                    return launch(k_ln_bwd_rows<T, V, 64, 2, W, S>, p.groups, kThreads, s, a);
-                }
+        constexpr bool W = decltype(whole)::value;
+        const auto rows = [&](auto lanes, auto elems) {
+            constexpr int L = decltype(lanes)::value, K = decltype(elems)::value / V;
+            constexpr uint32_t kTake = kThreads / L * kInFlight<T, K * V>;
+            return launch(k_ln_rows<T, V, L, K, W>, (a.rows.n + kTake - 1) / kTake, 16384, kThreads, s,
+                          a);
+        };
+        if constexpr (V == 1) {
+            return for_value<1, 2, 4, 8>(p.elems, [&](auto elems) {
+                return rows(std::integral_constant<int, 1>(), elems);
+            });
+        } else {
+            if (p.wide) {
+                return for_value<16, 32>(p.elems, [&](auto elems) {
+                    constexpr int K = decltype(elems)::value / V;
+                    const uint32_t limit = 256 * (2048 / p.lanes);
+                    if constexpr (K * V == 32) {
+                        if (p.lanes > 256) {
+                            return launch(k_ln_wide<T, V, K, 1024, false, W>, a.rows.n, limit,
+                                          p.lanes, s, a);
+                        }
+                    }
+                    return launch(k_ln_wide<T, V, K, 256, true, W>, a.rows.n, limit, p.lanes, s,
+                                  a);
+                });
             }
-            return for_power<(V > 1 ? 64 : 8)>(p.lanes, [&](auto lanes) {
-                return launch(k_ln_bwd_rows<T, V, decltype(lanes)::value, 1, W, S>, p.groups,
+            if (p.elems == 32) {
+                return rows(std::integral_constant<int, 64>(), std::integral_constant<int, 32>());
+            }
+            return for_value<1, 2, 4, 8, 16, 32, 64>(p.lanes, [&](auto lanes) {
+                return for_elems<V, 24>(p.elems, [&](auto elems) { return rows(lanes, elems); });
+            });
+        }
+    });
+}
+
+template <typename T, int V>
+int backward(hipStream_t s, const Plan& p, const Backward& a, float2* row_part) {
+    if (p.chunks) {
+        if constexpr (V > 1) {
+            const dim3 grid(p.groups, p.chunks);
+            hipLaunchKernelGGL((k_ln_bwd_chunk<T, V, false>), grid, dim3(kThreads), 0, s, a,
+                               row_part);
+            DRESSI_CHECK_LAUNCH();
+            if (a.gx) {
+                hipLaunchKernelGGL((k_ln_bwd_chunk<T, V, true>), grid, dim3(kThreads), 0, s, a,
+                                   row_part);
+                DRESSI_CHECK_LAUNCH();
+            }
+        }
+        return DRESSI_OK;
+    }
+    return for_bool(p.whole, [&](auto whole) {
+        constexpr bool W = decltype(whole)::value;
+        if constexpr (V == 1) {
+            return for_value<1, 2, 4, 8>(p.elems, [&](auto elems) {
+                return launch(k_ln_bwd_rows<T, V, 1, decltype(elems)::value, W>, p.groups, ~0u,
                               kThreads, s, a);
             });
-        });
+        } else {
+            if (p.wide) {
+                return for_value<8, 16>(p.elems, [&](auto elems) {
+                    constexpr int K = decltype(elems)::value / V;
+                    if constexpr (K * V == 16) {
+                        if (p.lanes > 512) {
+                            return launch(k_ln_bwd_wide<T, V, K, 1024, W>, p.groups, ~0u, p.lanes,
+                                          s, a);
+                        }
+                        if (p.lanes > 256) {
+                            return launch(k_ln_bwd_wide<T, V, K, 512, W>, p.groups, ~0u, p.lanes,
+                                          s, a);
+                        }
+                    }
+                    return launch(k_ln_bwd_wide<T, V, K, 256, W>, p.groups, ~0u, p.lanes, s, a);
+                });
+            }
+            return for_value<1, 2, 4, 8, 16, 32, 64>(p.lanes, [&](auto lanes) {
+                return for_elems<V, 16>(p.elems, [&](auto elems) {
+                    return launch(k_ln_bwd_rows<T, V, decltype(lanes)::value,
+                                                decltype(elems)::value / V, W>,
+                                  p.groups, ~0u, kThreads, s, a);
+                });
+            });
+        }
     });
 }
 
@@ -1050,13 +1220,14 @@ int check_shape(const char* what, uint32_t type, uint64_t n_items, uint64_t n_px
 
 Rows make_rows(uint64_t n_items, uint64_t n_px, uint32_t n_ch, uint64_t item_stride,
                uint64_t px_stride) {
-    Rows r{n_items * n_px, n_px, item_stride, px_stride, n_ch, 1.f / (float)n_ch};
+    Rows r{n_items * n_px, n_px, item_stride, px_stride, n_ch, 0, 1.f / (float)n_ch};
     if (n_px == 1) {
         r.px_stride = item_stride;
     }
     if (n_items == 1 || n_px == 1 || item_stride == n_px * px_stride) {
         r.n_px = r.n;
     }
+    r.flat = r.n_px == r.n && r.px_stride <= kMaxPxStride;
     return r;
 }
 
@@ -1113,7 +1284,7 @@ int dressi_layer_norm(dressi_ctx* ctx, const void* x, uint32_t type, uint64_t n_
                    "layer_norm: scratch too small or not aligned");
     const DeviceScope scope(ctx->device);
     DRESSI_TRY_HIP(scope.error());
-    const Forward a{x, y, mean, rstd, rows, aff, eps, activation};
+    const Forward a{x, y, mean, rstd, rows, aff, eps, activation, p.stream, p.stream_in};
     return for_vec(type, p.v, [&](auto w) {
         using T = std::remove_reference_t<decltype(w.v[0])>;
         return forward<T, sizeof(w) / sizeof(T)>(ctx->stream, p, a, scratch);
@@ -1150,7 +1321,8 @@ int dressi_layer_norm_bwd(dressi_ctx* ctx, const void* gy, const void* x, uint32
             "layer_norm_bwd: scratch too small or not aligned");
         DRESSI_TRY_HIP(scope.error());
         const Backward a{gy, x, mean, rstd, gx, part, part_stride(n_ch),
-                         join ? nullptr : gw, join ? nullptr : gb, rows, aff, activation};
+                         join ? nullptr : gw, join ? nullptr : gb, rows, aff, activation,
+                         p.stream, p.stream_in};
         const int rc = for_vec(type, p.v, [&](auto w) {
             using T = std::remove_reference_t<decltype(w.v[0])>;
             return backward<T, sizeof(w) / sizeof(T)>(ctx->stream, p, a, (float2*)scratch);
