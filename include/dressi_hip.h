@@ -954,9 +954,11 @@ typedef struct dressi_clip_tensor {
  * max_norm INFINITY: the norm alone, nothing is written. Where the norm is
  * not finite, the elements become what the formula gives (zero or NaN). Squares are added in
  * double, in a fixed order. No two tensors overlap where elements are
- * written. scratch: device memory of dressi_clip_norm_scratch bytes, aligned
- * to 8, used by this call only. */
-size_t dressi_clip_norm_scratch(void);
+ * written. scratch: device memory of dressi_clip_norm_scratch bytes (of the
+ * tensors' numbers of elements and types), aligned to 8, or NULL where that
+ * is 0, used by this call only. */
+size_t dressi_clip_norm_scratch(const dressi_clip_tensor* tensors,
+                                uint32_t n_tensors);
 int dressi_clip_norm(dressi_ctx* ctx, const dressi_clip_tensor* tensors,
                      uint32_t n_tensors, uint32_t kind, double max_norm,
                      void* scratch, float* norm);

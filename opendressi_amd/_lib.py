@@ -211,7 +211,7 @@ _SIGS = {
     "dressi_adamw_step": (_I, [_P, _P, _U, _P, _U, _U, C.c_uint64, _P, _P, _P, _P, _U, _F, _P,
                                _P, _P, _P]),
     "dressi_adamw_values": (_I, [_P, C.c_uint64, _P, _P, _P, _P, _P, _P]),
-    "dressi_clip_norm_scratch": (_S, []),
+    "dressi_clip_norm_scratch": (_S, [_P, _U]),
     "dressi_clip_norm": (_I, [_P, _P, _U, _U, C.c_double, _P, _P]),
 }
 

@@ -915,15 +915,16 @@ def layer_norm(ctx: Context, x: torch.Tensor, weight: torch.Tensor | None = None
     act = _layer_args(x, activation)
     c = x.shape[-1]
     code, aff = _typed(ctx, x, "x"), _affine(ctx, c, weight, bias)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     mean = rstd = None
     if stats:
-        mean, rstd = torch.empty((2, *x.shape[:-1]), dtype=torch.float32, device=x.device)
+        mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
+        rstd = torch.empty_like(mean)
     if x.numel() == 0:
         return y, mean, rstd
     x, n, n_px, item, px = _row_strides(x)
     size = lib.dressi_layer_norm_scratch(code, n, n_px, c, 0)
-    scratch = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+    scratch = x.new_empty(size, dtype=torch.uint8) if size else None
     _prep(ctx)
     check(lib.dressi_layer_norm(ctx.handle, x.data_ptr(), code, n, n_px, c, item, px,
                                 _addr(weight), _addr(bias), aff, eps, act, _addr(scratch), size,
@@ -951,18 +952,17 @@ def layer_norm_bwd(ctx: Context, gy: torch.Tensor, x: torch.Tensor, mean: torch.
                 or t.get_device() != ctx.device:
             raise ValueError(f"{name} must be packed float32 {list(x.shape[:-1])} on "
                              f"cuda:{ctx.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    gx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need[0] else None
+    gx = torch.empty_like(x, memory_format=torch.contiguous_format) if need[0] else None
     some = weight if weight is not None else bias
-    kind = torch.float32 if some is None else some.dtype
-    gw, gb = (torch.empty(c, dtype=kind, device=x.device) if wanted else None
-              for wanted in need[1:])
+    gw, gb = (None if not wanted else x.new_empty(c, dtype=torch.float32) if some is None else
+              torch.empty_like(some) for wanted in need[1:])
     n = n_px = 0
     item = px = c
     if x.numel():
         x, n, n_px, item, px = _row_strides(x)
         gy = gy.contiguous()
     size = lib.dressi_layer_norm_scratch(code, n, n_px, c, 1)
-    scratch = torch.empty(size, dtype=torch.uint8, device=x.device) if size else None
+    scratch = x.new_empty(size, dtype=torch.uint8) if size else None
     _prep(ctx)
     check(lib.dressi_layer_norm_bwd(ctx.handle, gy.data_ptr(), x.data_ptr(), code, n, n_px, c,
                                     item, px, _addr(weight), _addr(bias), aff, act,

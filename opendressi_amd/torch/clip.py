@@ -5,35 +5,18 @@ inside its own step). No counterpart in the reference's surface.
 from __future__ import annotations
 
 import math
+from array import array
+from itertools import chain
 
-import numpy as np
 import torch
 from torch.autograd.graph import increment_version
 
 from .._lib import NORM_2, NORM_LARGEST, check, lib
-from ..ops import TYPE_CODES
+from ..ops import TYPE_CODES, _addr
 from .context import RasterizeHipContext
 from .optim import _dense
 
-# an entry of the table of tensors (dressi_clip_tensor)
-_ENTRY = np.dtype([("data", "<u8"), ("n", "<u8"), ("type", "<u4"), ("unused", "<u4")])
 _KINDS = {2.0: NORM_2, math.inf: NORM_LARGEST}
-
-
-def _clip(ctx: RasterizeHipContext, grads: list[torch.Tensor], kind: int,
-          max_norm: float) -> torch.Tensor:
-    """Dense gradients' norm, and what is above max_norm scaled."""
-    table = np.zeros(len(grads), _ENTRY)
-    table["data"] = [g.data_ptr() for g in grads]
-    table["n"] = [g.numel() for g in grads]
-    table["type"] = [TYPE_CODES[g.dtype] for g in grads]
-    with ctx.lock:
-        norm = torch.empty((), device=ctx.device)
-        scratch = torch.empty(lib.dressi_clip_norm_scratch(), dtype=torch.uint8, device=ctx.device)
-        ctx._ctx.use_torch_stream()
-        check(lib.dressi_clip_norm(ctx._ctx.handle, table.ctypes.data, len(grads), kind, max_norm,
-                                   scratch.data_ptr(), norm.data_ptr()))
-    return norm
 
 
 def _apart(t: torch.Tensor) -> bool:
@@ -47,20 +30,61 @@ def _apart(t: torch.Tensor) -> bool:
     return True
 
 
-def _gradients(ctx: RasterizeHipContext, parameters) -> list[torch.Tensor]:
-    """Those that there are, checked."""
-    if isinstance(parameters, torch.Tensor):
-        parameters = [parameters]
-    grads = [p.grad for p in parameters if p.grad is not None]
-    dev = ctx.device.index
-    for g in grads:
-        if g.layout is not torch.strided:
-            raise RuntimeError("clip_grad_norm_: sparse gradients are not supported")
-        if g.dtype not in TYPE_CODES:
-            raise TypeError(f"a gradient must be float32, bfloat16 or float16, got {g.dtype}")
-        if g.get_device() != dev:
-            raise ValueError(f"a gradient is on {g.device}, the context on {ctx.device}")
-    return grads
+def _all_contiguous(grads) -> bool:
+    try:
+        return all(map(torch.Tensor.is_contiguous, grads))
+    except RuntimeError:  # some sparse layouts raise
+        return False
+
+
+def _refuse(ctx, g) -> None:
+    """Raises for a gradient that a call does not take."""
+    if g.layout is not torch.strided:
+        raise RuntimeError("clip_grad_norm_: sparse gradients are not supported")
+    if g.dtype not in TYPE_CODES:
+        raise TypeError(f"a gradient must be float32, bfloat16 or float16, got {g.dtype}")
+    if g.get_device() != ctx.device.index:
+        raise ValueError(f"a gradient is on {g.device}, the context on {ctx.device}")
+
+
+class _Gradients:
+    """The parameters' gradients, checked, and the table of them that a call
+    takes: an address, a count and a type for each."""
+
+    def __init__(self, ctx: RasterizeHipContext, parameters):
+        if isinstance(parameters, torch.Tensor):
+            parameters = [parameters]
+        self.grads = grads = [g for p in parameters if (g := p.grad) is not None]
+        kinds = [g.dtype for g in grads]
+        for g in grads if not set(kinds) <= TYPE_CODES.keys() or \
+                not set(map(torch.Tensor.get_device, grads)) <= {ctx.device.index} else ():
+            _refuse(ctx, g)
+        self.views = views = []  # those not densely stored, with their packed copies
+        packed = grads
+        if not _all_contiguous(grads):
+            packed = []
+            for g in grads:
+                _refuse(ctx, g)
+                if not _dense(g):
+                    views.append((g, g.contiguous()))
+                    g = views[-1][1]
+                packed.append(g)
+        # three words an entry, as in dressi_clip_tensor
+        self.table = array("Q", chain.from_iterable(zip(
+            map(torch.Tensor.data_ptr, packed), map(torch.Tensor.numel, packed),
+            map(TYPE_CODES.__getitem__, kinds))))
+
+    def clip(self, ctx: RasterizeHipContext, kind: int, max_norm: float) -> torch.Tensor:
+        """Their norm; those above max_norm are scaled."""
+        at, n = self.table.buffer_info()[0], len(self.grads)
+        norm = torch.empty((), device=ctx.device)
+        size = lib.dressi_clip_norm_scratch(at, n)
+        scratch = norm.new_empty(size, dtype=torch.uint8) if size else None
+        with ctx.lock:
+            ctx._ctx.use_torch_stream()
+            check(lib.dressi_clip_norm(ctx._ctx.handle, at, n, kind, max_norm, _addr(scratch),
+                                       norm.data_ptr()))
+        return norm
 
 
 def _kind(norm_type) -> int:
@@ -75,9 +99,7 @@ def grad_norm(ctx: RasterizeHipContext, parameters, norm_type: float = 2.0) -> t
     on the context's device: the square root of their sum of squares, added in
     float64, or (norm_type inf) their largest magnitude. Without gradients it
     is zero; a NaN among them makes it NaN."""
-    kind = _kind(norm_type)
-    grads = [g if _dense(g) else g.contiguous() for g in _gradients(ctx, parameters)]
-    return _clip(ctx, grads, kind, math.inf)
+    return _Gradients(ctx, parameters).clip(ctx, _kind(norm_type), math.inf)
 
 
 def clip_grad_norm_(ctx: RasterizeHipContext, parameters, max_norm: float,
@@ -97,23 +119,21 @@ def clip_grad_norm_(ctx: RasterizeHipContext, parameters, max_norm: float,
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
-    grads = _gradients(ctx, parameters)
-    packed = [g if _dense(g) else g.contiguous() for g in grads]
-    views = [g for g, q in zip(grads, packed) if q is not g]
-    if views and (not all(map(_apart, views)) or
-                  len({g.data_ptr() for g in grads if g.numel()}) < sum(g.numel() > 0 for g in grads)):
+    g = _Gradients(ctx, parameters)
+    if g.views and (not all(_apart(v) for v, _ in g.views) or
+                    len({v.data_ptr() for v in g.grads if v.numel()}) <
+                    sum(v.numel() > 0 for v in g.grads)):
         raise ValueError("gradients are the same or share memory")
     if error_if_nonfinite:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("error_if_nonfinite waits for the norm, which a captured call cannot")
-        norm = _clip(ctx, packed, kind, math.inf)
+        norm = g.clip(ctx, kind, math.inf)
         if not math.isfinite(float(norm)):
             raise RuntimeError(f"the gradients' norm is {float(norm)}: they are not clipped")
-    norm = _clip(ctx, packed, kind, max_norm)
+    norm = g.clip(ctx, kind, max_norm)
     if max_norm < math.inf:
         with torch.no_grad():
-            for g, q in zip(grads, packed):
-                if q is not g:
-                    g.copy_(q)
-        increment_version(grads)  # written in place
+            for v, packed in g.views:
+                v.copy_(packed)
+        increment_version(g.grads)  # written in place
     return norm

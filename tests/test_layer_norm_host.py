@@ -48,7 +48,8 @@ def test_layer_norm_refuses():
         _refused(_forward(**bad), word)
     for bad, word in ((dict(gy=None), "arguments"), (dict(mean=None), "arguments"),
                       (dict(rstd=None), "arguments"), (dict(gx=Y + 2), "aligned"),
-                      (dict(size=0), "scratch"), (dict(scratch=None), "scratch")):
+                      (dict(px=5000, size=16), "scratch"), (dict(px=5000, scratch=None), "scratch"),
+                      (dict(px=5000, scratch=X + 8), "scratch")):
         _refused(_backward(**bad), word)
 
 
@@ -58,8 +59,17 @@ def test_nothing_to_do():
     assert L.lib.dressi_layer_norm_scratch(0, 0, 5, 8, 1) == 0
 
 
+def test_layer_norm_scratch():
+    """Forward for rows beyond a workgroup alone, backward where several workgroups add to the
+    weight's gradient; by the number of rows, however they are given."""
+    scratch = L.lib.dressi_layer_norm_scratch
+    assert scratch(0, 5, 1000, 32768, 0) == 0 and scratch(1, 5, 1000, 32769, 0) > 0
+    assert scratch(0, 1, 1, 64, 1) == 0 and scratch(0, 1, 10000, 64, 1) > 0
+    assert scratch(1, 1, 6000, 24, 1) == scratch(1, 6000, 1, 24, 1) == scratch(1, 20, 300, 24, 1)
+
+
 def _table(*rows):
-    t = np.zeros(len(rows), clip._ENTRY)
+    t = np.zeros(len(rows), [("data", "<u8"), ("n", "<u8"), ("type", "<u4"), ("unused", "<u4")])
     for e, (data, n, kind) in zip(t, rows):
         e["data"], e["n"], e["type"] = data, n, kind
     return t
@@ -69,8 +79,18 @@ def _clip(table, kind=0, max_norm=1.0, ctx=CTX, scratch=X, norm=X):
     return L.lib.dressi_clip_norm(ctx, table.ctypes.data, len(table), kind, max_norm, scratch, norm)
 
 
+def test_clip_norm_scratch():
+    """None where one workgroup holds all vectors of 16 bytes (8192) of at most 128 tensors."""
+    def bytes_of(*sizes, kind=0):
+        t = _table(*((0x1000, n, kind) for n in sizes))
+        return L.lib.dressi_clip_norm_scratch(t.ctypes.data, len(t))
+    assert bytes_of() == bytes_of(1, 0, 5) == bytes_of(32768) == bytes_of(65536, kind=1) == 0
+    assert bytes_of(*[1] * 128) == bytes_of(*[1] * 128 + [0] * 50) == 0
+    assert bytes_of(32769) > 0 and bytes_of(65537, kind=2) > 0 and bytes_of(*[1] * 129) > 0
+
+
 def test_clip_norm_refuses():
-    good = _table((0x10000, 100, 0), (0x20000, 100, 1))
+    good = _table((0x10000, 100, 0), (0x100000, 100000, 1))
     for bad, word in ((dict(ctx=None), "context"), (dict(norm=None), "arguments"),
                       (dict(kind=2), "norm"), (dict(max_norm=-1.0), "max_norm"),
                       (dict(max_norm=math.nan), "max_norm"), (dict(scratch=X + 4), "scratch"),
@@ -102,8 +122,9 @@ def test_clip_grad_norm_refuses():
             clip.clip_grad_norm_(HOST, [p], *args)
     with pytest.raises(TypeError):
         clip.clip_grad_norm_(HOST, [_param(torch.ones(3, dtype=torch.float64))], 1.0)
-    with pytest.raises(RuntimeError):
-        clip.grad_norm(HOST, [_param(torch.ones(3).to_sparse())])
+    for sparse in (torch.eye(3).to_sparse(), torch.eye(3).to_sparse_csr()):
+        with pytest.raises(RuntimeError, match="sparse"):
+            clip.grad_norm(HOST, [types.SimpleNamespace(grad=sparse)])
     with pytest.raises(ValueError):
         clip.grad_norm(HOST, [p], 3.0)
 
