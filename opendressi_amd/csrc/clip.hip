@@ -352,14 +352,18 @@ __global__ __launch_bounds__(kSmallThreads) void k_clip_small(const Table tb, do
     }
 }
 
-// Bytes of all tensors up to which a chunk is 4 KB and not 16: more workgroups.
+// Bytes of all tensors up to which a chunk is 4 KB and not 16: more workgroups
+// (2^22 bfloat16 8.3 us, 9.5 with chunks of 16 KB turned round; 2^22 float32 10.4
+// and 11.9 the other way).
 constexpr uint64_t kFewBytes = 4ull << 20;
 
 // Bytes that the second pass may find in the last-level cache (256 MB); the rest
-// goes past it both times.
-constexpr uint64_t kKeepBytes = 160ull << 20;
+// goes past it both times. 2^28 float32: 505 us, 516 with 160 MB kept and 524 with
+// 96.
+constexpr uint64_t kKeepBytes = 224ull << 20;
 
-// Workgroups of a launch: four a compute unit.
+// Workgroups of a launch: four a compute unit (2^28 float32 538 us with half of
+// them, 507 with twice as many, but 2^24 35 where these take 30).
 constexpr uint32_t kGroups = 1024;
 
 int check_tensors(const dressi_clip_tensor* t, uint32_t n, bool written) {
