@@ -140,30 +140,28 @@ __device__ __forceinline__ float lane_sum(float x) {
     return x;
 }
 
-// The sum over a workgroup, in all threads, through part[waves]: one barrier, so
-// that the next sum goes through another part.
-__device__ __forceinline__ float wide_sum(float x, float* part) {
+// The sum over `waves` waves of a workgroup from `first` on, in all threads,
+// through part[]: one barrier, so that the next sum goes through another part.
+__device__ __forceinline__ float wide_sum(float x, float* part, uint32_t waves) {
     x = lane_sum<64>(x);
     if ((threadIdx.x & 63u) == 0) {
         part[threadIdx.x >> 6] = x;
     }
     __syncthreads();
-    const uint32_t waves = blockDim.x >> 6;
     x = part[0];
     for (uint32_t i = 1; i < waves; i++) {
         x += part[i];
     }
     return x;
 }
-__device__ __forceinline__ float2 wide_sum(float2 x, float2* part) {
+__device__ __forceinline__ float2 wide_sum(float2 x, float2* part, uint32_t first, uint32_t waves) {
     x = make_float2(lane_sum<64>(x.x), lane_sum<64>(x.y));
     if ((threadIdx.x & 63u) == 0) {
         part[threadIdx.x >> 6] = x;
     }
     __syncthreads();
-    const uint32_t waves = blockDim.x >> 6;
-    x = part[0];
-    for (uint32_t i = 1; i < waves; i++) {
+    x = part[first];
+    for (uint32_t i = first + 1; i < first + waves; i++) {
         x.x += part[i].x;
         x.y += part[i].y;
     }
@@ -352,13 +350,13 @@ __global__ __launch_bounds__(THREADS) void k_ln_wide(const Forward a) {
         for (int e = 0; e < E; e++) {
             m += counted<WHOLE>(to_float(v[e / V].v[e % V]), e % V, skip[e / V]);
         }
-        m = wide_sum(m, part[0]) * rows.inv;
+        m = wide_sum(m, part[0], blockDim.x >> 6) * rows.inv;
 #pragma unroll
         for (int e = 0; e < E; e++) {
             const float d = counted<WHOLE>(to_float(v[e / V].v[e % V]) - m, e % V, skip[e / V]);
             q = fmaf(d, d, q);
         }
-        q = inv_sqrt(fmaf(wide_sum(q, part[1]), rows.inv, a.eps));
+        q = inv_sqrt(fmaf(wide_sum(q, part[1], blockDim.x >> 6), rows.inv, a.eps));
         T* y = (T*)a.y + row * rows.n_ch;
 #pragma unroll
         for (int k = 0; k < K; k++) {
@@ -426,13 +424,13 @@ __global__ __launch_bounds__(kThreads) void k_ln_chunk_stats(const Forward a, fl
         for (int e = 0; e < kChunkElems; e++) {
             m += counted<false>(to_float(v[e / V].v[e % V]), e % V, sp.skip[e / V]);
         }
-        m = wide_sum(m, part[0]) * inv;
+        m = wide_sum(m, part[0], blockDim.x >> 6) * inv;
 #pragma unroll
         for (int e = 0; e < kChunkElems; e++) {
             const float d = counted<false>(to_float(v[e / V].v[e % V]) - m, e % V, sp.skip[e / V]);
             q = fmaf(d, d, q);
         }
-        q = wide_sum(q, part[1]);
+        q = wide_sum(q, part[1], blockDim.x >> 6);
         if (threadIdx.x == 0) {
             row_part[row * gridDim.y + blockIdx.y] = make_float2(m, q);
         }
@@ -745,21 +743,23 @@ __global__ __launch_bounds__(kThreads) void k_ln_bwd_rows(const Backward a) {
     }
 }
 
-// A workgroup holds a row, K vectors a thread, and reads the next one meanwhile,
-// unless there are 1024 threads: those have too few registers each for that, and
-// keep weight and bias in LDS.
-template <typename T, int V, int K, uint32_t THREADS, bool WHOLE>
+// A workgroup holds a row, or two in a half each, K vectors a thread, and reads
+// the next meanwhile, unless there are 1024 threads: those have too few registers
+// each for that, and keep weight and bias in LDS.
+template <typename T, int V, int K, uint32_t THREADS, uint32_t HALVES, bool WHOLE>
 __global__ __launch_bounds__(THREADS) void k_ln_bwd_wide(const Backward a) {
     __shared__ float2 part[2][THREADS / 64];
     constexpr int E = K * V;
     constexpr bool kFew = THREADS == 1024;
     __shared__ Pack<float, V> affine[kFew ? 2 : 1][kFew ? K * THREADS : 1];
     const Rows& rows = a.rows;
+    const uint32_t lanes = blockDim.x / HALVES, half = threadIdx.x / lanes;
+    const uint32_t lane = threadIdx.x - half * lanes;
     uint32_t first[K], skip[K];
     float w[E], b[E], gw[E], gb[E];
 #pragma unroll
     for (int k = 0; k < K; k++) {
-        const Span<V> sp(k * blockDim.x + threadIdx.x, rows.n_ch);
+        const Span<V> sp(k * lanes + lane, rows.n_ch);
         first[k] = sp.first;
         skip[k] = sp.skip;
         load_params<V>(a.aff.weight, a.aff.type, sp.first, 1.f, w + k * V);
@@ -795,15 +795,20 @@ __global__ __launch_bounds__(THREADS) void k_ln_bwd_wide(const Backward a) {
     };
     uint32_t turn = 0;
     Raw raw;
+    const uint64_t step = (uint64_t)gridDim.x * HALVES;
+    const auto mine = [&](uint64_t row0) { return std::min(row0 + half, rows.n - 1); };
+    uint64_t row0 = (uint64_t)blockIdx.x * HALVES;  // there are no more workgroups than rows
     if (!kFew) {
-        load(blockIdx.x, raw);  // there are no more workgroups than rows
+        load(mine(row0), raw);
     }
-    for (uint64_t row = blockIdx.x; row < rows.n; row += gridDim.x, turn ^= 1) {
+    for (; row0 < rows.n; row0 += step, turn ^= 1) {
+        const uint64_t row = row0 + half;
+        const bool live = HALVES == 1 || row < rows.n;
         Raw ahead;
         if (kFew) {
             load(row, raw);
-        } else if (row + gridDim.x < rows.n) {
-            load(row + gridDim.x, ahead);
+        } else if (row0 + step < rows.n) {
+            load(mine(row0 + step), ahead);
         }
         float xh[E], t[E];
 #pragma unroll
@@ -828,11 +833,11 @@ __global__ __launch_bounds__(THREADS) void k_ln_bwd_wide(const Backward a) {
                 s.x += sk.x;
                 s.y += sk.y;
             }
-        } else {
+        } else if (live) {
             s = slopes<T, V, E, WHOLE>(raw.mean, rstd, w, b, a.act, skip, xh, t, gw, gb);
         }
-        s = wide_sum(s, part[turn]);
-        if (a.gx) {
+        s = wide_sum(s, part[turn], half * (lanes >> 6), lanes >> 6);
+        if (live && a.gx) {
             T* gx = (T*)a.gx + row * rows.n_ch;
 #pragma unroll
             for (int k = 0; k < K; k++) {
@@ -848,6 +853,25 @@ __global__ __launch_bounds__(THREADS) void k_ln_bwd_wide(const Backward a) {
     }
     if (!a.part && !a.gw && !a.gb) {
         return;
+    }
+    if constexpr (HALVES == 2) {
+        __shared__ float red[2][E][THREADS / 2];
+        if (half == 1) {
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                red[0][e][lane] = gw[e];
+                red[1][e][lane] = gb[e];
+            }
+        }
+        __syncthreads();
+        if (half == 1) {
+            return;
+        }
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            gw[e] += red[0][e][lane];
+            gb[e] += red[1][e][lane];
+        }
     }
 #pragma unroll
     for (int k = 0; k < K; k++) {
@@ -907,7 +931,7 @@ __global__ __launch_bounds__(kThreads) void k_ln_bwd_chunk(const Backward a, flo
                 }
             }
         } else {
-            const float2 sum = wide_sum(s, part[turn]);
+            const float2 sum = wide_sum(s, part[turn], 0, kThreads / 64);
             if (threadIdx.x == 0) {
                 row_part[row * chunks + chunk] = sum;
             }
@@ -1044,9 +1068,10 @@ Plan make_plan(uint32_t type, uint64_t rows, uint32_t n_ch, bool backward) {
             p.elems *= 2;
         }
         p.lanes = div_up(div_up(n_ch, p.elems), 64) * 64;
-        const uint32_t most = p.lanes > 512 ? 256 : 512 * 256 / std::max(256u, p.lanes);
-        p.groups = (uint32_t)std::min<uint64_t>(
-            {rows, most, std::max<uint64_t>(128, rows / 4)});
+        // 512 threads for each of 256 compute units, or twice that where they hold 8 values
+        const uint32_t most = p.elems == 16 ? 256 : 512;
+        const uint64_t pairs = p.lanes > 256 ? rows : (rows + 1) / 2;
+        p.groups = (uint32_t)std::min<uint64_t>({pairs, most, std::max<uint64_t>(128, pairs / 2)});
     } else {
         cut_row(p, n_ch, backward);
         const bool one = n_ch == p.lanes * p.elems || p.lanes >= 32;  // kAhead
@@ -1183,15 +1208,16 @@ int backward(hipStream_t s, const Plan& p, const Backward& a, float2* row_part) 
                     constexpr int K = decltype(elems)::value / V;
                     if constexpr (K * V == 16) {
                         if (p.lanes > 512) {
-                            return launch(k_ln_bwd_wide<T, V, K, 1024, W>, p.groups, ~0u, p.lanes,
-                                          s, a);
+                            return launch(k_ln_bwd_wide<T, V, K, 1024, 1, W>, p.groups, ~0u,
+                                          p.lanes, s, a);
                         }
                         if (p.lanes > 256) {
-                            return launch(k_ln_bwd_wide<T, V, K, 512, W>, p.groups, ~0u, p.lanes,
-                                          s, a);
+                            return launch(k_ln_bwd_wide<T, V, K, 512, 1, W>, p.groups, ~0u,
+                                          p.lanes, s, a);
                         }
                     }
-                    return launch(k_ln_bwd_wide<T, V, K, 256, W>, p.groups, ~0u, p.lanes, s, a);
+                    return launch(k_ln_bwd_wide<T, V, K, 512, 2, W>, p.groups, ~0u, 2 * p.lanes, s,
+                                  a);
                 });
             }
             return for_value<1, 2, 4, 8, 16, 32, 64>(p.lanes, [&](auto lanes) {

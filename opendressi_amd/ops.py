@@ -879,25 +879,30 @@ def group_norm_bwd(ctx: Context, gy: torch.Tensor, x: torch.Tensor, mean: torch.
 
 # ---- layer norm with an activation (any rows) --------------------------------
 
-def _row_strides(x: torch.Tensor) -> tuple[torch.Tensor, int, int, int, int]:
+def _row_strides(x: torch.Tensor, c: int) -> tuple[torch.Tensor, int, int, int, int]:
     """x (..., C), packed where its rows are not evenly spaced; its items, an item's rows, item
     and row strides."""
+    if x.is_contiguous():
+        return x, 1, x.numel() // c, 0, c
     if x.dim() == 1:
-        x = x.unsqueeze(0)
+        return x.contiguous(), 1, 1, c, c
     at = _pixel_strides(x)
     if at is None:
-        x = x.contiguous()
-        at = _pixel_strides(x)
+        return x.contiguous(), 1, x.numel() // c, 0, c
     return x, x.shape[0], *at
 
 
-def _layer_args(x: torch.Tensor, activation: str) -> int:
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"x must be [..., C], got {tuple(x.shape)}")
+def _layer_args(ctx: Context, x: torch.Tensor, weight, bias,
+                activation: str) -> tuple[int, int, int, int]:
+    """Checks the arguments that both passes share: channels, the types of x and of weight and
+    bias, the activation."""
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"unknown activation {activation!r}; one of {', '.join(ACTIVATIONS)}")
-    return act
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"x must be [..., C], got {tuple(x.shape)}")
+    c = x.shape[-1]
+    return c, _typed(ctx, x, "x"), _affine(ctx, c, weight, bias), act
 
 
 def layer_norm(ctx: Context, x: torch.Tensor, weight: torch.Tensor | None = None,
@@ -912,9 +917,7 @@ def layer_norm(ctx: Context, x: torch.Tensor, weight: torch.Tensor | None = None
     backward pass takes (None where `stats` is false). x may have any even
     pixel stride (a slice of the channels of a wider image); others are packed
     first."""
-    act = _layer_args(x, activation)
-    c = x.shape[-1]
-    code, aff = _typed(ctx, x, "x"), _affine(ctx, c, weight, bias)
+    c, code, aff, act = _layer_args(ctx, x, weight, bias, activation)
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
     mean = rstd = None
     if stats:
@@ -922,7 +925,7 @@ def layer_norm(ctx: Context, x: torch.Tensor, weight: torch.Tensor | None = None
         rstd = torch.empty_like(mean)
     if x.numel() == 0:
         return y, mean, rstd
-    x, n, n_px, item, px = _row_strides(x)
+    x, n, n_px, item, px = _row_strides(x, c)
     size = lib.dressi_layer_norm_scratch(code, n, n_px, c, 0)
     scratch = x.new_empty(size, dtype=torch.uint8) if size else None
     _prep(ctx)
@@ -941,9 +944,7 @@ def layer_norm_bwd(ctx: Context, gy: torch.Tensor, x: torch.Tensor, mean: torch.
     pass -> gx (like x, packed), gw, gb (C,) in the weight's and bias's type
     (float32 where there is none). `need` says which of the three are wanted;
     the others are None."""
-    act = _layer_args(x, activation)
-    c = x.shape[-1]
-    code, aff = _typed(ctx, x, "x"), _affine(ctx, c, weight, bias)
+    c, code, aff, act = _layer_args(ctx, x, weight, bias, activation)
     if gy.shape != x.shape or gy.dtype is not x.dtype or gy.get_device() != ctx.device:
         raise ValueError(f"gy must be like x: {x.dtype} {tuple(x.shape)}, got {gy.dtype} "
                          f"{tuple(gy.shape)} on {gy.device}")
@@ -959,7 +960,7 @@ def layer_norm_bwd(ctx: Context, gy: torch.Tensor, x: torch.Tensor, mean: torch.
     n = n_px = 0
     item = px = c
     if x.numel():
-        x, n, n_px, item, px = _row_strides(x)
+        x, n, n_px, item, px = _row_strides(x, c)
         gy = gy.contiguous()
     size = lib.dressi_layer_norm_scratch(code, n, n_px, c, 1)
     scratch = x.new_empty(size, dtype=torch.uint8) if size else None

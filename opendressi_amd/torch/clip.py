@@ -77,7 +77,8 @@ class _Gradients:
     def clip(self, ctx: RasterizeHipContext, kind: int, max_norm: float) -> torch.Tensor:
         """Their norm; those above max_norm are scaled."""
         at, n = self.table.buffer_info()[0], len(self.grads)
-        norm = torch.empty((), device=ctx.device)
+        norm = self.grads[0].new_empty((), dtype=torch.float32) if n else \
+            torch.empty((), device=ctx.device)
         size = lib.dressi_clip_norm_scratch(at, n)
         scratch = norm.new_empty(size, dtype=torch.uint8) if size else None
         with ctx.lock:
