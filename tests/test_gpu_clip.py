@@ -173,6 +173,41 @@ def test_not_finite(vctx, kind, n):
                 assert not params[1].grad.any() and int(params[0].grad.isnan().sum()) == 1
 
 
+def test_refused(vctx):
+    """A parameter that is there twice, gradients that share memory: nothing is written."""
+    import opendressi_amd as od
+    import opendressi_amd.torch as dr
+    for n in (10, 100000):
+        a, b = _params([n, n], [torch.float32], 10)
+        before = a.grad.clone()
+        with pytest.raises(od.DressiError, match="share memory"):
+            dr.clip_grad_norm_(vctx, [a, b, a], 1.0)
+        parts = a.grad[n // 2:], a.grad[:n // 2 + 1]
+        p = [torch.zeros(len(t), device="cuda") for t in parts]
+        p[0].grad, p[1].grad = parts
+        with pytest.raises(od.DressiError, match="share memory"):
+            dr.clip_grad_norm_(vctx, p, 1.0)
+        dr.grad_norm(vctx, p)
+        assert torch.equal(a.grad, before)
+    p = torch.zeros(4, 6, device="cuda")
+    p.grad = torch.ones(1, 6, device="cuda").expand(4, 6)
+    with pytest.raises(ValueError):
+        dr.clip_grad_norm_(vctx, [p], 1.0)
+    assert abs(float(dr.grad_norm(vctx, [p])) - 24 ** 0.5) < 1e-6
+    wide = torch.ones(4, 12, device="cuda")
+    p, q = torch.zeros(4, 6, device="cuda"), torch.zeros(4, 6, device="cuda")
+    p.grad = q.grad = wide[:, :6]
+    with pytest.raises(ValueError):
+        dr.clip_grad_norm_(vctx, [p, q], 1.0)
+    assert (wide == 1).all()
+    with pytest.raises(ValueError):
+        dr.clip_grad_norm_(vctx, [torch.zeros(3)], -1.0)
+    host = torch.zeros(3)
+    host.grad = torch.ones(3)
+    with pytest.raises(ValueError):
+        dr.clip_grad_norm_(vctx, [p, host], 1.0)
+
+
 def test_extreme_sizes(vctx):
     """Squares that are no float32: the sum is taken in float64. A norm of zero scales nothing."""
     import opendressi_amd.torch as dr
