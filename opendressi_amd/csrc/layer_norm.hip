@@ -1003,8 +1003,11 @@ constexpr uint32_t vec_of(uint32_t type, uint32_t n_ch) {
     return n_ch >= v ? v : 1;
 }
 
-// Values of a row up to which a wave, then a workgroup, holds it.
-constexpr uint32_t kWaveElems = 64 * 32, kWaveElemsBwd = 64 * 16;
+// Values of a row up to which a wave, then a workgroup, holds it. Backward a wave
+// with two vectors of 16 bits a lane holds so many registers that there are two a
+// SIMD (65536 x 1024 bfloat16 81 us, 75 with 128 lanes a row; float32 142 and 148).
+constexpr uint32_t kWaveElems = 64 * 32;
+constexpr uint32_t wave_elems_bwd(uint32_t v) { return 64 * (v == 4 ? 16 : 8); }
 constexpr uint32_t kHoldElems = 1024 * 32, kHoldElemsBwd = 1024 * 16;
 
 // Bytes of results, and of inputs, from which they go past the caches.
@@ -1019,35 +1022,31 @@ struct Plan {
     uint32_t groups;  // workgroups whose sums of gw and gb are added
 };
 
-// Lanes and values of each for a row that a wave holds: the fewest values held
-// in all, in lanes of 8 to 24 (backward 8 or 16) where they suffice.
+// Lanes and values of each for a row that a wave holds. One vector a lane, where
+// a wave's load or store is one piece of memory (2000000 x 24 float32 forward 58
+// us, 87 with six vectors a lane); forward three, where fewer than 9 of 16 lanes
+// had one (800000 x 130 bfloat16 75 us and 84; backward the registers of three
+// cost more than the lanes: 186 us, 226 with three). Longer rows take a whole wave.
 void cut_row(Plan& p, uint32_t n_ch, bool backward) {
     const uint32_t vecs = div_up(n_ch, p.v);
+    p.lanes = p.elems = 1;
     if (p.v == 1) {  // a lane a row
-        p.lanes = p.elems = 1;
         while (p.elems < n_ch) {
             p.elems *= 2;
         }
         return;
     }
-    uint32_t best = ~0u;
-    const uint32_t any[] = {16, 24, 8, 4, 32}, bwd[] = {8, 4, 16};
-    const uint32_t* list = backward ? bwd : any;
-    for (uint32_t i = 0; i < (backward ? 3u : 5u); i++) {
-        const uint32_t elems = list[i];
-        uint32_t lanes = 1;
-        while (lanes < 64 && lanes * elems < n_ch) {
-            lanes *= 2;
-        }
-        if (elems < p.v || lanes * elems < vecs * p.v || (elems == 32 && lanes < 64)) {
-            continue;
-        }
-        if (lanes * elems < best || (n_ch <= 16 && elems == p.v && lanes * elems == best)) {
-            best = lanes * elems;
-            p.lanes = lanes;
-            p.elems = elems;
-        }
+    while (p.lanes < 64 && p.lanes < vecs) {
+        p.lanes *= 2;
     }
+    uint32_t iter = div_up(vecs, p.lanes);
+    if (iter == 1 && !backward && 16 * vecs < 9 * p.lanes) {
+        p.lanes /= 4;
+        iter = 3;
+    } else if (iter > 4 || (backward && iter > 2)) {
+        iter = iter > 6 ? 8 : backward ? 4 : 6;
+    }
+    p.elems = iter * p.v;
 }
 
 // By the number of rows and not by where they lie: so is the scratch.
@@ -1061,7 +1060,7 @@ Plan make_plan(uint32_t type, uint64_t rows, uint32_t n_ch, bool backward) {
         p.elems = backward ? kChunkElemsBwd : kChunkElems;
         p.chunks = div_up(n_ch, p.elems * kThreads);
         p.groups = (uint32_t)std::min<uint64_t>(rows, std::max(1u, 1024 / p.chunks));
-    } else if (n_ch > (backward ? kWaveElemsBwd : kWaveElems)) {
+    } else if (n_ch > (backward ? wave_elems_bwd(p.v) : kWaveElems)) {
         p.wide = true;
         p.elems = p.v;
         while (p.elems < (backward ? 16 : 32) && n_ch > p.elems * 256) {
@@ -1069,9 +1068,9 @@ Plan make_plan(uint32_t type, uint64_t rows, uint32_t n_ch, bool backward) {
         }
         p.lanes = div_up(div_up(n_ch, p.elems), 64) * 64;
         // 512 threads for each of 256 compute units, or twice that where they hold 8 values
-        const uint32_t most = p.elems == 16 ? 256 : 512;
+        const uint32_t most = (p.elems == 16 ? 256 : 512) * 256 / std::min(256u, p.lanes);
         const uint64_t pairs = p.lanes > 256 ? rows : (rows + 1) / 2;
-        p.groups = (uint32_t)std::min<uint64_t>({pairs, most, std::max<uint64_t>(128, pairs / 2)});
+        p.groups = (uint32_t)std::min<uint64_t>({pairs, most, std::max<uint64_t>(256, pairs / 8)});
     } else {
         cut_row(p, n_ch, backward);
         const bool one = n_ch == p.lanes * p.elems || p.lanes >= 32;  // kAhead
@@ -1079,6 +1078,9 @@ Plan make_plan(uint32_t type, uint64_t rows, uint32_t n_ch, bool backward) {
         p.groups = (uint32_t)std::min<uint64_t>((rows + take - 1) / take, 1024);
     }
     p.whole = n_ch == p.lanes * p.elems;
+    // a store that does not fill lines is slower past the caches, which would have
+    // filled them (1500000 x 35 float32 in pieces of 32 bytes: 300 and 98 us)
+    p.stream = p.stream && (p.chunks > 0 || p.elems == p.v || p.lanes >= 8);
     return p;
 }
 
@@ -1115,16 +1117,6 @@ int for_value(uint32_t x, F&& f) {
         }
     }
     return f(std::integral_constant<uint32_t, FIRST>());
-}
-
-// f(a lane's values as a constant): 4 (in vectors of 4), 8, 16 and MOST.
-template <int V, uint32_t MOST, typename F>
-int for_elems(uint32_t x, F&& f) {
-    if constexpr (V == 4) {
-        return for_value<4, 8, 16, MOST>(x, f);
-    } else {
-        return for_value<8, 16, MOST>(x, f);
-    }
 }
 
 template <typename T, int V>
@@ -1169,11 +1161,24 @@ int forward(hipStream_t s, const Plan& p, const Forward& a, void* scratch) {
                                   a);
                 });
             }
-            if (p.elems == 32) {
-                return rows(std::integral_constant<int, 64>(), std::integral_constant<int, 32>());
+            if (p.lanes == 64 && p.elems > V) {
+                const auto wave = [&](auto iter) {
+                    return rows(std::integral_constant<int, 64>(),
+                                std::integral_constant<int, decltype(iter)::value * V>());
+                };
+                if constexpr (V == 4) {
+                    return for_value<2, 3, 4, 6, 8>(p.elems / V, wave);
+                } else {
+                    return for_value<2, 3, 4>(p.elems / V, wave);
+                }
+            }
+            if (p.elems > V) {
+                return for_value<8, 16>(p.lanes, [&](auto lanes) {
+                    return rows(lanes, std::integral_constant<int, 3 * V>());
+                });
             }
             return for_value<1, 2, 4, 8, 16, 32, 64>(p.lanes, [&](auto lanes) {
-                return for_elems<V, 24>(p.elems, [&](auto elems) { return rows(lanes, elems); });
+                return rows(lanes, std::integral_constant<int, V>());
             });
         }
     });
@@ -1220,12 +1225,17 @@ int backward(hipStream_t s, const Plan& p, const Backward& a, float2* row_part) 
                                   a);
                 });
             }
+            if constexpr (V == 4) {
+                if (p.elems > V) {
+                    return for_value<8, 16>(p.elems, [&](auto elems) {
+                        return launch(k_ln_bwd_rows<T, V, 64, decltype(elems)::value / V, W>,
+                                      p.groups, ~0u, kThreads, s, a);
+                    });
+                }
+            }
             return for_value<1, 2, 4, 8, 16, 32, 64>(p.lanes, [&](auto lanes) {
-                return for_elems<V, 16>(p.elems, [&](auto elems) {
-                    return launch(k_ln_bwd_rows<T, V, decltype(lanes)::value,
-                                                decltype(elems)::value / V, W>,
-                                  p.groups, ~0u, kThreads, s, a);
-                });
+                return launch(k_ln_bwd_rows<T, V, decltype(lanes)::value, 1, W>, p.groups, ~0u,
+                              kThreads, s, a);
             });
         }
     });
