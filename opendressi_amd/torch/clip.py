@@ -111,9 +111,9 @@ def clip_grad_norm_(ctx: RasterizeHipContext, parameters, max_norm: float,
 
     `parameters` is an iterable of tensors, or one; those whose grad is None
     are passed over. Gradients are float32, bfloat16 or float16, mixed as they
-    come, on the context's device; no two share memory (a parameter must not be there
-    twice). max_norm inf leaves all gradients as they are. Where the norm is not
-    finite, the gradients become NaN or zero, as the formula says;
+    come, on the context's device; no two share memory (a parameter must not
+    be there twice). max_norm inf leaves all gradients as they are. Where the
+    norm is not finite, the gradients become NaN or zero, as the formula says;
     error_if_nonfinite waits for the norm and raises instead, with the
     gradients as they were."""
     kind = _kind(norm_type)
@@ -127,7 +127,7 @@ def clip_grad_norm_(ctx: RasterizeHipContext, parameters, max_norm: float,
         raise ValueError("gradients are the same or share memory")
     if error_if_nonfinite:
         if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("error_if_nonfinite waits for the norm, which a captured call cannot")
+            raise RuntimeError("error_if_nonfinite waits for the norm: not in a captured call")
         norm = g.clip(ctx, kind, math.inf)
         if not math.isfinite(float(norm)):
             raise RuntimeError(f"the gradients' norm is {float(norm)}: they are not clipped")

@@ -230,6 +230,35 @@ def test_strides(ctx, kind):
         assert all(torch.equal(p, q) for p, q in zip(want, got))
 
 
+@pytest.mark.parametrize("kind", TYPES, ids=str)
+def test_crops_and_far_pixels(ctx, kind):
+    """Many rows that are not evenly spaced, and rows more than 2^22 elements apart: the packed
+    rows' bits."""
+    from opendressi_amd import ops as K
+    wide, _, w, b = _inputs((3, 301, 203, 40), kind, 31)
+    far = torch.randn(2 ** 23 + 5000, device="cuda").to(kind)
+    for x in (wide[:, 5:300, 7:200, 3:36], wide[1:, ::2, :, :33],
+              far.as_strided((2, 33), (2 ** 22 + 77, 1)),
+              far.as_strided((2, 4, 33), (50, 2 ** 21 + 3, 1))):
+        g = torch.randn(x.shape, device="cuda").to(kind)
+        packed, args = x.contiguous(), (w[:33].contiguous(), b[:33].contiguous())
+        want = K.layer_norm(ctx, packed, *args, 1e-5, "gelu")
+        got = K.layer_norm(ctx, x, *args, 1e-5, "gelu")
+        assert all(torch.equal(p, q) for p, q in zip(want, got))
+        want = K.layer_norm_bwd(ctx, g, packed, *want[1:], *args, "gelu")
+        got = K.layer_norm_bwd(ctx, g, x, *got[1:], *args, "gelu")
+        assert all(torch.equal(p, q) for p, q in zip(want, got))
+
+
+@pytest.mark.parametrize("shape", [(7, 256), (5, 512), (9, 768), (300, 1536), (600, 3000),
+                                   (513, 640), (2, 10240)], ids=str)
+@pytest.mark.parametrize("kind", TYPES, ids=str)
+def test_whole_waves(ctx, shape, kind):
+    print(f"[layer_norm whole] {shape} {kind}", flush=True)
+    x, gy, w, b = _inputs(shape, kind, 32)
+    _check(x, gy, w, b, 1e-5, "gelu", _run(ctx, x, gy, w, b, 1e-5, "gelu"))
+
+
 @pytest.mark.parametrize("c", [16, 33, 1100, 20000, 40000])
 def test_only_what_is_wanted(ctx, c):
     """Each gradient alone has the bits that it has beside the others; two runs have the same."""
