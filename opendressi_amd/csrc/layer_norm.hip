@@ -212,10 +212,11 @@ struct Forward {
 // forward
 // ---------------------------------------------------------------------------
 
-// Lanes of a row from which its loads may go past the caches: fewer take a line
-// or less with each, and in pieces would read it again (4194304 x 64 bfloat16 by
-// four lanes 237 us, through the caches 219).
-constexpr int kStreamLanes = 32;
+// Whether a wave's load is one piece of memory, or long pieces, and may go past
+// the caches: in short ones it would read lines again (4194304 x 64 bfloat16 by
+// four lanes 237 us, through the caches 219; by eight 180 and 189).
+template <int L, int K>
+constexpr bool kLongPieces = K == 1 || L >= 32;
 
 // Rows that a lane has in flight, of E values each: 64 bytes (262144 x 64 float32,
 // gelu, 16 values a lane: 24.2 us, 25.6 with 128 bytes).
@@ -223,9 +224,9 @@ template <typename T, int E>
 constexpr int kInFlight = E * sizeof(T) >= 48 ? 1 : E * sizeof(T) >= 32 ? 2 : 4;
 
 // L lanes hold a row, K vectors each. 8 x 1024 x 1024 x 64 bfloat16, silu, without
-// statistics: 375 us, 5.7 TB/s; 64 of 96 channels of 512 x 512: 14.8, whose lines
+// statistics: 349 us, 6.1 TB/s; 64 of 96 channels of 512 x 512: 14.0, whose lines
 // hold half as much again; 2000000 x 24 float32 58, 6.7 TB/s; one row 4. Gelu's
-// arithmetic is what bounds it in 16 bits (4194304 x 64: 238 us, silu 190).
+// arithmetic is what bounds it in 16 bits (4194304 x 64: 232 us, silu 183).
 template <typename T, int V, int L, int K, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void k_ln_rows(const Forward a) {
     constexpr int E = K * V, R = kInFlight<T, E>;
@@ -250,7 +251,7 @@ __global__ __launch_bounds__(kThreads) void k_ln_rows(const Forward a) {
         Pack<T, V> v[R][K];
         if (rows.flat && r0 + kTake <= rows.n) {
             x += r0 * rows.px_stride;
-            by_stream(L >= kStreamLanes && a.stream_in, [&](auto past) {
+            by_stream(kLongPieces<L, K> && a.stream_in, [&](auto past) {
 #pragma unroll
                 for (int i = 0; i < R; i++) {
 #pragma unroll
@@ -616,7 +617,7 @@ template <int L, bool WHOLE>
 constexpr bool kAhead = WHOLE || L >= 32;
 
 // L lanes hold a row, K vectors each, and keep the sums of their columns. 4 x 1024 x
-// 1024 x 64 bfloat16, silu: 312 us, 5.2 TB/s (gelu 348); 500000 x 100 float32 108,
+// 1024 x 64 bfloat16, silu: 308 us, 5.3 TB/s (gelu 345); 500000 x 100 float32 108,
 // 5.5 TB/s. Rows of just over a power of two of vectors leave half of the lanes
 // idle: 800000 x 130 bfloat16 186 us, 3.4 TB/s.
 template <typename T, int V, int L, int K, bool WHOLE>
@@ -653,7 +654,7 @@ __global__ __launch_bounds__(kThreads) void k_ln_bwd_rows(const Backward a) {
         if (rows.flat && r0 + kTake <= rows.n) {
             x += r0 * rows.px_stride;
             g += r0 * rows.n_ch;
-            by_stream(L >= kStreamLanes && a.stream_in, [&](auto past) {
+            by_stream(kLongPieces<L, K> && a.stream_in, [&](auto past) {
 #pragma unroll
                 for (int i = 0; i < R; i++) {
                     r.mean[i] = (a.mean + r0 + i * kSlots)[slot];
@@ -1034,7 +1035,8 @@ constexpr uint32_t kHoldElems = 1024 * 32, kHoldElemsBwd = 1024 * 16;
 
 // Bytes of results, and of inputs, from which they go past the caches. Results:
 // 1000000 x 128 bfloat16 75 us so and 90 through them. Inputs, where the caches
-// do not hold them from one call to the next: 100000 x 511 float32 68 and 79.
+// do not hold them from one call to the next: 100000 x 511 float32 68 and 79,
+// 30000000 x 8 float16 170 and 212.
 constexpr uint64_t kStreamBytes = 32ull << 20, kStreamInBytes = 256ull << 20;
 
 struct Plan {

@@ -15,8 +15,8 @@ __device__ __forceinline__ float sigmoid(float z) {
 }
 // The normal distribution's Phi(z) and e = exp(-z^2 / 2), its tail beyond |z| being
 // e times a smooth function of |z|, for 16-bit images Abramowitz and Stegun's
-// 7.1.26: erf to 1.5e-7, a rounding of a float near 1 (2 x 512 x 512 x 88 float16
-// backward: 116 us, 153 with a library erf beside the exponential).
+// 7.1.26: erf to 1.5e-7, a rounding of a float near 1 (group norm of 2 x 512 x 512 x
+// 88 float16, backward: 116 us, 153 with a library erf beside the exponential).
 template <typename T>
 __device__ __forceinline__ void gauss(float z, float& cdf, float& e) {
     e = __expf(-0.5f * z * z);
@@ -33,7 +33,7 @@ __device__ __forceinline__ void gauss(float z, float& cdf, float& e) {
 // one after the other. Near z = 0, where a function of t = 1 / (1 + a) takes every
 // rounding of t, little is added to the 1/2. The error of z Phi(z) over normal z is
 // 2.2e-8 (7.1.26: 5.6e-8; 0.5 (1 + erf) in floats: 2.5e-8), of its slope 2.6e-8
-// (6.6e-8, 2.7e-8). 2 x 512 x 512 x 88 takes 109 and 183 us with it and 104 and 181
+// (6.6e-8, 2.7e-8). Group norm of 2 x 512 x 512 x 88 takes 109 and 183 us with it, 104 and 181
 // with 7.1.26; with it float16 images would take 78 and 130, not 70 and 118.
 template <>
 __device__ __forceinline__ void gauss<float>(float z, float& cdf, float& e) {
