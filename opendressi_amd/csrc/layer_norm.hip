@@ -331,9 +331,12 @@ __global__ __launch_bounds__(kThreads) void k_ln_rows(const Forward a) {
 
 // A workgroup holds a row, K vectors a thread. HOLD: weight and bias stay in
 // registers between rows. 16384 x 4096 bfloat16: 45 us, 6.0 TB/s; 4096 x 16384
-// float32, which waits for its barriers with few workgroups: 111, 4.8 TB/s.
+// float32, which waits for its barriers with few workgroups: 110, 4.9 TB/s. 1024
+// threads with 16 values are held to 64 registers, so that a compute unit has two
+// workgroups of them (3000 x 14000 float32 61 us, 66 without).
 template <typename T, int V, int K, uint32_t THREADS, bool HOLD, bool WHOLE>
-__global__ __launch_bounds__(THREADS) void k_ln_wide(const Forward a) {
+__global__ __launch_bounds__(THREADS, THREADS == 1024 && K * V == 16 ? 8 : 1) void k_ln_wide(
+    const Forward a) {
     __shared__ float part[2][THREADS / 64];
     constexpr int E = K * V;
     const Rows& rows = a.rows;
@@ -1092,6 +1095,9 @@ Plan make_plan(uint32_t type, uint64_t rows, uint32_t n_ch, bool backward) {
         while (p.elems < (backward ? 16 : 32) && n_ch > p.elems * 256) {
             p.elems *= 2;
         }
+        if (!backward && n_ch > 8192 && n_ch <= 16 * 1024) {
+            p.elems = 16;  // 4096 x 9216 bfloat16 30 us, 45 with 32 in half the threads
+        }
         p.lanes = div_up(div_up(n_ch, p.elems), 64) * 64;
         // 512 threads for each of 256 compute units, or twice that where they hold 8 values; fewer
         // where their sums would be as much as the rows (1021 x 4096 bfloat16 16.8 us, 20.9 with
@@ -1182,11 +1188,9 @@ int forward(hipStream_t s, const Plan& p, const Forward& a, void* scratch) {
                 return for_value<16, 32>(p.elems, [&](auto elems) {
                     constexpr int K = decltype(elems)::value / V;
                     const uint32_t limit = 256 * (2048 / p.lanes);
-                    if constexpr (K * V == 32) {
-                        if (p.lanes > 256) {
-                            return launch(k_ln_wide<T, V, K, 1024, false, W>, a.rows.n, limit,
-                                          p.lanes, s, a);
-                        }
+                    if (p.lanes > 256) {
+                        return launch(k_ln_wide<T, V, K, 1024, false, W>, a.rows.n, limit, p.lanes,
+                                      s, a);
                     }
                     return launch(k_ln_wide<T, V, K, 256, true, W>, a.rows.n, limit, p.lanes, s,
                                   a);
