@@ -566,7 +566,7 @@ __device__ __forceinline__ float2 slopes(float mean, float rstd, const float (&w
         t[e] *= w[e];
         const float c = counted<WHOLE>(t[e], e % V, skip[e / V]);
         s.x += c;
-        s.y += WHOLE ? t[e] * xh[e] : counted<false>(t[e] * xh[e], e % V, skip[e / V]);
+        s.y = fmaf(c, xh[e], s.y);  // an xh that is not finite is the whole row's
     }
     return s;
 }
