@@ -613,19 +613,20 @@ __device__ __forceinline__ void write_sums(const Backward& a, uint32_t ch, uint3
     }
 }
 
-// Whether a lane reads its next row while it works on one, or else two at a time
-// (4194304 x 64 bfloat16 319 us ahead and 344 by two; 4000000 x 33 float16, gelu,
-// 314 and 282).
-template <int L, bool WHOLE>
-constexpr bool kAhead = WHOLE || L >= 32;
+// Whether a lane reads its next row while it works on one, or else two at a time:
+// the first where all lanes have values (4194304 x 64 bfloat16 308 us, 344 by two)
+// and for long rows of 32 bits (100000 x 300 63 and 68), the second in 16 bits
+// where some do not (500000 x 200 118, 129 ahead; 500000 x 248 140 and 149).
+template <int V, int L, bool WHOLE>
+constexpr bool kAhead = WHOLE || (V == 4 && L >= 32);
 
 // L lanes hold a row, K vectors each, and keep the sums of their columns. 4 x 1024 x
 // 1024 x 64 bfloat16, silu: 308 us, 5.3 TB/s (gelu 345); 500000 x 100 float32 108,
 // 5.5 TB/s. Rows of just over a power of two of vectors leave half of the lanes
-// idle: 800000 x 130 bfloat16 186 us, 3.4 TB/s.
+// idle: 800000 x 130 bfloat16 150 us, 4.2 TB/s.
 template <typename T, int V, int L, int K, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void k_ln_bwd_rows(const Backward a) {
-    constexpr int E = K * V, R = kAhead<L, WHOLE> ? 1 : 2;
+    constexpr int E = K * V, R = kAhead<V, L, WHOLE> ? 1 : 2;
     constexpr uint32_t kSlots = kThreads / L, kTake = kSlots * R, kWaves = kThreads / 64;
     __shared__ float red[kWaves][2][L * E];
     const uint32_t lane = threadIdx.x % L, slot = threadIdx.x / L;
@@ -690,12 +691,12 @@ __global__ __launch_bounds__(kThreads) void k_ln_bwd_rows(const Backward a) {
     const uint64_t step = (uint64_t)gridDim.x * kTake;
     uint64_t r0 = (uint64_t)blockIdx.x * kTake;  // there are no more workgroups than rows for them
     Raw raw;
-    if (kAhead<L, WHOLE>) {
+    if (kAhead<V, L, WHOLE>) {
         load(r0, raw);
     }
     for (; r0 < rows.n; r0 += step) {
         Raw ahead;
-        if (!kAhead<L, WHOLE>) {
+        if (!kAhead<V, L, WHOLE>) {
             load(r0, raw);
         } else if (r0 + step < rows.n) {
             load(r0 + step, ahead);
@@ -727,7 +728,7 @@ __global__ __launch_bounds__(kThreads) void k_ln_bwd_rows(const Backward a) {
                 }
             }
         }
-        if (kAhead<L, WHOLE>) {
+        if (kAhead<V, L, WHOLE>) {
             raw = ahead;
         }
     }
@@ -1055,7 +1056,7 @@ struct Plan {
 // a wave's load or store is one piece of memory (2000000 x 24 float32 forward 58
 // us, 87 with six vectors a lane); forward three, where fewer than 9 of 16 lanes
 // had one (800000 x 130 bfloat16 75 us and 84; backward the registers of three
-// cost more than the lanes: 186 us, 226 with three). Longer rows take a whole wave.
+// cost more than the lanes). Longer rows take a whole wave.
 void cut_row(Plan& p, uint32_t n_ch, bool backward) {
     const uint32_t vecs = div_up(n_ch, p.v);
     p.lanes = p.elems = 1;
@@ -1107,8 +1108,8 @@ Plan make_plan(uint32_t type, uint64_t rows, uint32_t n_ch, bool backward) {
         p.groups = (uint32_t)std::min<uint64_t>({pairs, most, std::max<uint64_t>(256, pairs / 8)});
     } else {
         cut_row(p, n_ch, backward);
-        const bool one = n_ch == p.lanes * p.elems || p.lanes >= 32;  // kAhead
-        const uint64_t take = kThreads / p.lanes * (one ? 1 : 2);
+        const bool ahead = n_ch == p.lanes * p.elems || (p.v == 4 && p.lanes >= 32);  // kAhead
+        const uint64_t take = kThreads / p.lanes * (ahead ? 1 : 2);
         // four for each compute unit: 1280, where some have five, take 400 us for 4194304 x 64
         // bfloat16, 768 345 and these 317
         p.groups = (uint32_t)std::min<uint64_t>((rows + take - 1) / take, 1024);
@@ -1237,10 +1238,13 @@ int backward(hipStream_t s, const Plan& p, const Backward& a, float2* row_part) 
     }
     return for_bool(p.whole, [&](auto whole) {
         constexpr bool W = decltype(whole)::value;
+        const auto rows = [&](auto lanes, auto iter) {
+            constexpr int L = decltype(lanes)::value, K = decltype(iter)::value;
+            return launch(k_ln_bwd_rows<T, V, L, K, W>, p.groups, ~0u, kThreads, s, a);
+        };
         if constexpr (V == 1) {
             return for_value<1, 2, 4, 8>(p.elems, [&](auto elems) {
-                return launch(k_ln_bwd_rows<T, V, 1, decltype(elems)::value, W>, p.groups, ~0u,
-                              kThreads, s, a);
+                return rows(std::integral_constant<int, 1>(), elems);
             });
         } else {
             if (p.wide) {
@@ -1262,15 +1266,13 @@ int backward(hipStream_t s, const Plan& p, const Backward& a, float2* row_part) 
             }
             if constexpr (V == 4) {
                 if (p.elems > V) {
-                    return for_value<8, 16>(p.elems, [&](auto elems) {
-                        return launch(k_ln_bwd_rows<T, V, 64, decltype(elems)::value / V, W>,
-                                      p.groups, ~0u, kThreads, s, a);
+                    return for_value<2, 4>(p.elems / V, [&](auto iter) {
+                        return rows(std::integral_constant<int, 64>(), iter);
                     });
                 }
             }
             return for_value<1, 2, 4, 8, 16, 32, 64>(p.lanes, [&](auto lanes) {
-                return launch(k_ln_bwd_rows<T, V, decltype(lanes)::value, 1, W>, p.groups, ~0u,
-                              kThreads, s, a);
+                return rows(lanes, std::integral_constant<int, 1>());
             });
         }
     });
