@@ -945,14 +945,16 @@ def layer_norm_bwd(ctx: Context, gy: torch.Tensor, x: torch.Tensor, mean: torch.
     (float32 where there is none). `need` says which of the three are wanted;
     the others are None."""
     c, code, aff, act = _layer_args(ctx, x, weight, bias, activation)
-    if gy.shape != x.shape or gy.dtype is not x.dtype or gy.get_device() != ctx.device:
-        raise ValueError(f"gy must be like x: {x.dtype} {tuple(x.shape)}, got {gy.dtype} "
+    shape, device = x.shape, ctx.device
+    if gy.shape != shape or gy.dtype is not x.dtype or gy.get_device() != device:
+        raise ValueError(f"gy must be like x: {x.dtype} {tuple(shape)}, got {gy.dtype} "
                          f"{tuple(gy.shape)} on {gy.device}")
+    lead = shape[:-1]
     for t, name in ((mean, "mean"), (rstd, "rstd")):
-        if t.dtype is not torch.float32 or t.shape != x.shape[:-1] or not t.is_contiguous() \
-                or t.get_device() != ctx.device:
-            raise ValueError(f"{name} must be packed float32 {list(x.shape[:-1])} on "
-                             f"cuda:{ctx.device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+        if t.dtype is not torch.float32 or t.shape != lead or t.get_device() != device \
+                or not t.is_contiguous():
+            raise ValueError(f"{name} must be packed float32 {list(lead)} on cuda:{device}, got "
+                             f"{t.dtype} {tuple(t.shape)} on {t.device}")
     gx = torch.empty_like(x, memory_format=torch.contiguous_format) if need[0] else None
     some = weight if weight is not None else bias
     gw, gb = (None if not wanted else x.new_empty(c, dtype=torch.float32) if some is None else

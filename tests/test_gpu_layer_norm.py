@@ -433,6 +433,35 @@ def test_captured(ctx, c):
                 assert torch.equal(p, q)
 
 
+def test_captured_through_autograd(vctx):
+    """Forward and gradients of the torch surface in one graph, replayed over new values with eager
+    calls on other leaves between them."""
+    import opendressi_amd.torch as dr
+
+    def step(leaves, gy):
+        return torch.autograd.grad(dr.layer_norm(vctx, *leaves, activation="silu"), leaves, gy)
+
+    x, gy, w, b = _inputs((4000, 48), torch.float32, 40)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step(leaves, gy)
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        out = step(leaves, gy)
+    for r in range(3):
+        new = _inputs((4000, 48), torch.float32, 41 + r)
+        with torch.no_grad():
+            for t, v in zip((x, gy, w, b), new):
+                t.copy_(v)
+        graph.replay()
+        eager = step([t.clone().requires_grad_() for t in (new[0], *new[2:])], new[1])
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, eager))
+
+
 def test_past_32_bits(ctx):
     """Rows whose elements lie past 2^32: those there are as good as the first, and the sums of
     the last rows are in the gradients of weight and bias."""
