@@ -4,6 +4,7 @@ the surface's channels-last images. No counterpart in the reference's surface.
 from __future__ import annotations
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from .. import ops as K
 from .context import RasterizeHipContext
@@ -96,10 +97,12 @@ def layer_norm(ctx: RasterizeHipContext, x: torch.Tensor, weight=None, bias=None
     act((x - mean) / sqrt(var + eps) * weight + bias), with the mean and
     variance over the C channels of each pixel, computed in float32;
     activation is "none", "relu", "silu" or "gelu". Differentiable w.r.t. x,
-    weight and bias."""
+    weight and bias, in reverse mode; forward mode's dual tensors are refused."""
     _check_tensors(x, weight, bias)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (x, weight, bias)):
+    given = [t for t in (x, weight, bias) if t is not None]
+    # a tangent of forward mode, which a Function refuses, would be lost on the short way
+    if torch.is_grad_enabled() and any(t.requires_grad for t in given) or \
+            any(unpack_dual(t).tangent is not None for t in given):
         return _LayerNormFn.apply(x, weight, bias, ctx, float(eps), activation)
     with ctx.lock:
         return K.layer_norm(ctx._ctx, *_moved(ctx.device, x, weight, bias), float(eps), activation,

@@ -1,4 +1,5 @@
 """Layer norm's and clipping's refusals, without a GPU."""
+import contextlib
 import ctypes as C
 import math
 import threading
@@ -7,9 +8,10 @@ import types
 import numpy as np
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from opendressi_amd import _lib as L
-from opendressi_amd.torch import clip
+from opendressi_amd.torch import clip, norm
 
 # never read: every call here is refused before the context is used
 CTX = C.cast(C.create_string_buffer(4096), C.c_void_p)
@@ -133,3 +135,23 @@ def test_elements_that_share_memory():
     base = torch.zeros(40)
     assert clip._apart(base[::2]) and clip._apart(base.view(4, 10)[:, 3:7].t())
     assert not clip._apart(base[:1].expand(5)) and not clip._apart(base.as_strided((5, 5), (2, 1)))
+
+
+@pytest.mark.parametrize("op", [norm.layer_norm, lambda *t: norm.group_norm(*t[:2], 1, *t[2:])],
+                         ids=["layer_norm", "group_norm"])
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("dual", range(3))
+def test_forward_mode_is_refused(monkeypatch, op, grad, dual):
+    """A dual tensor's derivative is refused, not lost; beside ordinary ones nothing changes."""
+    def kernel(ctx, x, *args, **kwargs):
+        return 2 * x, x.mean(-1), x.mean(-1)
+
+    monkeypatch.setattr(norm.K, "layer_norm", kernel)
+    monkeypatch.setattr(norm.K, "group_norm", kernel)
+    host = types.SimpleNamespace(device=torch.device("cpu"), lock=threading.RLock(), _ctx=None)
+    args = [torch.randn(4, 8), torch.ones(8), torch.zeros(8)]
+    with forward_ad.dual_level(), contextlib.nullcontext() if grad else torch.no_grad():
+        assert torch.equal(op(host, *args), 2 * args[0])
+        args[dual] = forward_ad.make_dual(args[dual], torch.ones_like(args[dual]))
+        with pytest.raises(NotImplementedError):
+            op(host, *args)
