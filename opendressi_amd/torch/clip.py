@@ -112,18 +112,19 @@ def clip_grad_norm_(ctx: RasterizeHipContext, parameters, max_norm: float,
     `parameters` is an iterable of tensors, or one; those whose grad is None
     are passed over. Gradients are float32, bfloat16 or float16, mixed as they
     come, on the context's device; no two share memory (a parameter must not
-    be there twice). max_norm inf leaves all gradients as they are. Where the
-    norm is not finite, the gradients become NaN or zero, as the formula says;
-    error_if_nonfinite waits for the norm and raises instead, with the
-    gradients as they were."""
+    be there twice). max_norm inf leaves all gradients as they are, and takes
+    those that do. Where the norm is not finite, the gradients become NaN or
+    zero, as the formula says; error_if_nonfinite waits for the norm and raises
+    instead, with the gradients as they were."""
     kind = _kind(norm_type)
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
     g = _Gradients(ctx, parameters)
-    if g.views and (not all(_apart(v) for v, _ in g.views) or
-                    len({v.data_ptr() for v in g.grads if v.numel()}) <
-                    sum(v.numel() > 0 for v in g.grads)):
+    if max_norm < math.inf and g.views and (
+            not all(_apart(v) for v, _ in g.views) or
+            len({v.data_ptr() for v in g.grads if v.numel()}) <
+            sum(v.numel() > 0 for v in g.grads)):
         raise ValueError("gradients are the same or share memory")
     if error_if_nonfinite:
         if torch.cuda.is_current_stream_capturing():

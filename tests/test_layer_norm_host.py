@@ -131,6 +131,30 @@ def test_clip_grad_norm_refuses():
         clip.grad_norm(HOST, [p], 3.0)
 
 
+@pytest.fixture
+def host(monkeypatch):
+    """A context for gradients on the host, whose calls pass for the library's: the norms of packed
+    gradients of float32, and nothing scaled."""
+    def call(self, ctx, kind, max_norm):
+        copies = {id(v): packed for v, packed in self.views}
+        return torch.cat([copies.get(id(g), g).reshape(-1) for g in self.grads]).norm()
+
+    monkeypatch.setattr(clip._Gradients, "clip", call)
+    return types.SimpleNamespace(device=types.SimpleNamespace(index=-1), lock=threading.RLock())
+
+
+def test_without_a_limit_any_gradients_are_taken(host):
+    """Nothing is written then: expanded gradients and the same twice count as they come."""
+    wide = torch.ones(4, 12)
+    p = _param(torch.ones(1, 6).expand(4, 6), (4, 6))
+    q = _param(wide[:, :6], (4, 6))
+    for params, n in (([p], 24), ([q, q], 48), ([p, q], 48)):
+        norm = clip.clip_grad_norm_(host, params, math.inf)
+        assert torch.equal(norm, clip.grad_norm(host, params)) and abs(float(norm) ** 2 - n) < 1e-3
+        with pytest.raises(ValueError):
+            clip.clip_grad_norm_(host, params, 1.0)
+
+
 def test_elements_that_share_memory():
     base = torch.zeros(40)
     assert clip._apart(base[::2]) and clip._apart(base.view(4, 10)[:, 3:7].t())
