@@ -15,6 +15,7 @@ from .._lib import NORM_2, NORM_LARGEST, check, lib
 from ..ops import TYPE_CODES, _addr
 from .context import RasterizeHipContext
 from .optim import _dense
+from .strides import shared
 
 _KINDS = {2.0: NORM_2, math.inf: NORM_LARGEST}
 
@@ -121,10 +122,9 @@ def clip_grad_norm_(ctx: RasterizeHipContext, parameters, max_norm: float,
     if not max_norm >= 0.0:
         raise ValueError(f"max_norm must not be negative, got {max_norm}")
     g = _Gradients(ctx, parameters)
-    if max_norm < math.inf and g.views and (
-            not all(_apart(v) for v, _ in g.views) or
-            len({v.data_ptr() for v in g.grads if v.numel()}) <
-            sum(v.numel() > 0 for v in g.grads)):
+    # packed ones are looked at by the call
+    if max_norm < math.inf and g.views and (not all(_apart(v) for v, _ in g.views) or
+                                            shared(g.grads, map(_dense, g.grads))):
         raise ValueError("gradients are the same or share memory")
     if error_if_nonfinite:
         if torch.cuda.is_current_stream_capturing():

@@ -2,6 +2,7 @@
 import contextlib
 import ctypes as C
 import math
+import random
 import threading
 import types
 
@@ -11,7 +12,7 @@ import torch
 from torch.autograd import forward_ad
 
 from opendressi_amd import _lib as L
-from opendressi_amd.torch import clip, norm
+from opendressi_amd.torch import clip, norm, strides
 
 # never read: every call here is refused before the context is used
 CTX = C.cast(C.create_string_buffer(4096), C.c_void_p)
@@ -153,6 +154,58 @@ def test_without_a_limit_any_gradients_are_taken(host):
         assert torch.equal(norm, clip.grad_norm(host, params)) and abs(float(norm) ** 2 - n) < 1e-3
         with pytest.raises(ValueError):
             clip.clip_grad_norm_(host, params, 1.0)
+
+
+def _some(rng, base):
+    """A strided tensor in the bytes of base, and the bytes of each of its elements."""
+    kind = rng.choice([torch.float32, torch.bfloat16])
+    flat = base.view(kind)
+    shape = [rng.choice([1, 1, 2, 3, 5]) for _ in range(rng.randint(1, 3))]
+    steps = [rng.choice([1, 2, 3, 4, 6, 7, 12, 24, 25]) for _ in shape]
+    room = len(flat) - 1 - sum(s * (n - 1) for s, n in zip(steps, shape))
+    t = flat.as_strided(shape, steps, rng.randint(0, min(room, 30)))
+    at = t.storage_offset() + sum((torch.arange(n) * s).view([-1] + [1] * (len(shape) - 1 - i))
+                                  for i, (n, s) in enumerate(zip(shape, steps)))
+    size = t.element_size()
+    return t, [int(a) * size + k for a in at.reshape(-1) for k in range(size)]
+
+
+def test_shared_memory_is_found():
+    """Against the elements' bytes counted out: nothing that shares is passed, nothing else is
+    refused."""
+    rng, base, seen = random.Random(5), torch.zeros(2400, dtype=torch.uint8), set()
+    while len(seen) < 2 or rng.random() > 2e-4:
+        made = [_some(rng, base) for _ in range(rng.randint(2, 4))]
+        made = [(t, b) for t, b in made if len(b) == len(set(b))]
+        every = [x for _, b in made for x in b]
+        want = len(every) != len(set(every))
+        dense = [clip._dense(t) for t, _ in made]
+        assert strides.shared([t for t, _ in made], dense) == want, made
+        seen.add(want)
+
+
+def test_shared_memory_of_large_tables():
+    """By addresses alone, whatever the sizes; columns of one table lie apart."""
+    wide = torch.empty(50000, 600, dtype=torch.bfloat16)
+    columns = [wide[:, 3 * i:3 * i + 3] for i in range(200)]
+    assert not strides.shared(columns, [False] * 200)
+    assert strides.shared(columns + [wide[49999, 599:]], [False] * 200 + [True])
+    assert not strides.shared([wide[::2, 1::2], wide[1::2, 1::2], wide[:, ::2]], [False] * 3)
+    assert strides.shared([wide[::2, 1::2], wide[1::2], wide[:, :1]], [False] * 3)
+
+
+def test_clip_grad_norm_refuses_shared_memory(host):
+    wide = torch.ones(4, 12)
+    flat = wide.view(-1)
+    for a, b in ((wide[:, :6], wide[:, 3:9]), (wide[:, :6], flat[13:20]), (flat[5:15], wide[:, 2:4]),
+                 (wide[:, :6], flat[36:37]), (wide[:, :6], wide[:, :6]), (wide.t()[:5], wide[2])):
+        params = [_param(a, a.shape), _param(torch.ones(7), (7,)), _param(b, b.shape)]
+        for some in (params, params[::-1]):
+            with pytest.raises(ValueError, match="share memory"):
+                clip.clip_grad_norm_(host, some, 1.0)
+    for a, b in ((wide[:, :6], wide[:, 6:]), (wide[:, :6], flat[18:24]), (wide[::2, ::2], wide[1::2]),
+                 (wide[:, ::2], wide[:, 1::2]), (wide.t()[:5], wide.t()[5:])):
+        clip.clip_grad_norm_(host, [_param(a, a.shape), _param(b, b.shape)], 1.0)
 
 
 def test_elements_that_share_memory():
