@@ -15,20 +15,9 @@ from .._lib import NORM_2, NORM_LARGEST, check, lib
 from ..ops import TYPE_CODES, _addr
 from .context import RasterizeHipContext
 from .optim import _dense
-from .strides import shared
+from .strides import apart as _apart, shared
 
 _KINDS = {2.0: NORM_2, math.inf: NORM_LARGEST}
-
-
-def _apart(t: torch.Tensor) -> bool:
-    """Whether no two of t's elements share memory, by strides that each reach
-    past all that the smaller ones span."""
-    end = 1
-    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
-        if stride < end:
-            return False
-        end += stride * (size - 1)
-    return True
 
 
 def _all_contiguous(grads) -> bool:

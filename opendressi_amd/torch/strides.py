@@ -45,6 +45,25 @@ def _solvable(terms, target: int) -> bool:
     return search(0, target)
 
 
+def apart(t: torch.Tensor) -> bool:
+    """Whether no two of t's elements share memory (and it is soon said)."""
+    dims = sorted((s, n - 1) for s, n in zip(t.stride(), t.shape) if n != 1)
+    end = 1
+    for s, u in dims:
+        if s < end:
+            break
+        end += s * u  # past all that the dimensions up to here span
+    else:
+        return True
+    # two elements at a distance of sum s d = 0, d >= 1 in one dimension and |d| <= u in the others
+    for i, (s, u) in enumerate(dims):
+        others = dims[:i] + dims[i + 1:]
+        if s == 0 or _solvable([(s, u - 1)] + [(a, 2 * v) for a, v in others],
+                               sum(a * v for a, v in others) - s):
+            return t.numel() == 0
+    return True
+
+
 class _Bytes:
     """Where a tensor's elements lie: `size` bytes from start + sum a z, 0 <= z <=
     u, on, over the terms (a, u). `dense`: they fill what they span."""

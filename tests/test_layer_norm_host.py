@@ -170,6 +170,25 @@ def _some(rng, base):
     return t, [int(a) * size + k for a in at.reshape(-1) for k in range(size)]
 
 
+def test_shared_elements_are_found():
+    """Against the elements' bytes counted out, as below."""
+    rng, base, seen = random.Random(6), torch.zeros(2400, dtype=torch.uint8), [0, 0]
+    for _ in range(5000):
+        t, at = _some(rng, base)
+        assert clip._apart(t) == (len(at) == len(set(at))), (t.shape, t.stride())
+        seen[clip._apart(t)] += 1
+    assert min(seen) > 500
+    assert clip._apart(base.as_strided((2, 4), (3, 2))) and not clip._apart(base[:1].expand(2))
+    assert not clip._apart(base.as_strided((3, 4), (3, 2)))
+    assert clip._apart(base.as_strided((3, 0), (0, 1))) and clip._apart(base.as_strided((), ()))
+
+
+def test_strides_that_cross_are_taken(host):
+    """Elements that lie apart by strides of which none reaches past the others' span."""
+    g = torch.arange(12.0).as_strided((2, 4), (3, 2))  # 0 2 4 6, 3 5 7 9
+    clip.clip_grad_norm_(host, [_param(g, (2, 4))], 1.0)
+
+
 def test_shared_memory_is_found():
     """Against the elements' bytes counted out: nothing that shares is passed, nothing else is
     refused."""
