@@ -108,7 +108,8 @@ inline uint32_t div_up(uint32_t a, uint32_t b) { return (a + b - 1) / b; }
 class DeviceScope {
 public:
     explicit DeviceScope(int device) {
-        if (hipGetDevice(&before_) != hipSuccess || before_ == device) {
+        error_ = hipGetDevice(&before_);
+        if (error_ != hipSuccess || before_ == device) {
             before_ = -1;
         } else {
             error_ = hipSetDevice(device);

@@ -1384,7 +1384,6 @@ int dressi_layer_norm_bwd(dressi_ctx* ctx, const void* gy, const void* x, uint32
     const Plan p = make_plan(type, rows.n, n_ch, true);
     const bool params = gw || gb, join = params && p.groups != 1;
     float* part = join ? (float*)((char*)scratch + row_bytes(p, rows.n)) : nullptr;
-    const DeviceScope scope(ctx->device);
     if (rows.n > 0) {
         DRESSI_REQUIRE(gy && x && mean && rstd, "layer_norm_bwd: bad arguments");
         DRESSI_REQUIRE(((uintptr_t)gy | (uintptr_t)x | (uintptr_t)gx) % type_bytes(type) == 0,
@@ -1393,7 +1392,12 @@ int dressi_layer_norm_bwd(dressi_ctx* ctx, const void* gy, const void* x, uint32
         DRESSI_REQUIRE(
             need == 0 || (scratch && ((uintptr_t)scratch & 15) == 0 && scratch_bytes >= need),
             "layer_norm_bwd: scratch too small or not aligned");
-        DRESSI_TRY_HIP(scope.error());
+    } else if (!join) {
+        return DRESSI_OK;
+    }
+    const DeviceScope scope(ctx->device);
+    DRESSI_TRY_HIP(scope.error());
+    if (rows.n > 0) {
         const Backward a{gy, x, mean, rstd, gx, part, part_stride(n_ch),
                          join ? nullptr : gw, join ? nullptr : gb, rows, aff, activation,
                          p.stream, p.stream_in};

@@ -62,6 +62,16 @@ def test_nothing_to_do():
     assert L.lib.dressi_layer_norm_scratch(0, 0, 5, 8, 1) == 0
 
 
+@pytest.mark.skipif(torch.cuda.device_count() > 0, reason="for hosts without a device")
+def test_a_device_that_cannot_be_made_current_is_reported():
+    """Before anything is launched, without rows too, whose gradients of weight and bias are zero."""
+    ctx = C.cast(C.create_string_buffer(C.string_at(C.byref(C.c_int(99)), 4) + bytes(4092), 4096),
+                 C.c_void_p)
+    for call in (lambda: _forward(ctx=ctx), lambda: _backward(ctx=ctx),
+                 lambda: _backward(ctx=ctx, items=0), lambda: _backward(ctx=ctx, px=0, gx=None)):
+        _refused(call(), "scope")
+
+
 def test_layer_norm_scratch():
     """Forward for rows beyond a workgroup alone, backward where several workgroups add to the
     weight's gradient; by the number of rows, however they are given."""
