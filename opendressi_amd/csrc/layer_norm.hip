@@ -31,6 +31,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <initializer_list>
 
 #include "internal.h"
 #include "norm_core.h"
@@ -1304,6 +1305,25 @@ Rows make_rows(uint64_t n_items, uint64_t n_px, uint32_t n_ch, uint64_t item_str
     return r;
 }
 
+// Whether the pointers lie as their types ask.
+int check_aligned(const char* what, uint32_t type, std::initializer_list<const void*> rows,
+                  uint32_t affine_type, std::initializer_list<const void*> params,
+                  std::initializer_list<const void*> stats) {
+    const auto off = [](std::initializer_list<const void*> list, size_t bytes) {
+        uintptr_t all = 0;
+        for (const void* p : list) {
+            all |= (uintptr_t)p;
+        }
+        return all % bytes != 0;
+    };
+    DRESSI_REQUIRE(!off(rows, type_bytes(type)), "%s: not aligned to its type", what);
+    DRESSI_REQUIRE(!off(params, type_bytes(affine_type)),
+                   "%s: the weight, the bias or a gradient of theirs is not aligned to its type",
+                   what);
+    DRESSI_REQUIRE(!off(stats, sizeof(float)), "%s: mean or rstd is not aligned", what);
+    return DRESSI_OK;
+}
+
 // f(a vector's type)
 template <typename F>
 int for_vec(uint32_t type, uint32_t v, F&& f) {
@@ -1348,8 +1368,10 @@ int dressi_layer_norm(dressi_ctx* ctx, const void* x, uint32_t type, uint64_t n_
         return DRESSI_OK;
     }
     DRESSI_REQUIRE(x && y && !mean == !rstd, "layer_norm: bad arguments");
-    DRESSI_REQUIRE(((uintptr_t)x | (uintptr_t)y) % type_bytes(type) == 0,
-                   "layer_norm: not aligned to its type");
+    if (int rc = check_aligned("layer_norm", type, {x, y}, affine_type, {weight, bias},
+                               {mean, rstd})) {
+        return rc;
+    }
     const Rows rows = make_rows(n_items, n_px, n_ch, item_stride, px_stride);
     const Plan p = make_plan(type, rows.n, n_ch, false);
     const size_t need = scratch_bytes_of(p, rows.n, n_ch, false);
@@ -1380,14 +1402,16 @@ int dressi_layer_norm_bwd(dressi_ctx* ctx, const void* gy, const void* x, uint32
     if (!gx && !gw && !gb) {
         return DRESSI_OK;
     }
+    if (int rc = check_aligned("layer_norm_bwd", type, {gy, x, gx}, affine_type,
+                               {weight, bias, gw, gb}, {mean, rstd})) {
+        return rc;
+    }
     const Rows rows = make_rows(n_items, n_px, n_ch, item_stride, px_stride);
     const Plan p = make_plan(type, rows.n, n_ch, true);
     const bool params = gw || gb, join = params && p.groups != 1;
     float* part = join ? (float*)((char*)scratch + row_bytes(p, rows.n)) : nullptr;
     if (rows.n > 0) {
         DRESSI_REQUIRE(gy && x && mean && rstd, "layer_norm_bwd: bad arguments");
-        DRESSI_REQUIRE(((uintptr_t)gy | (uintptr_t)x | (uintptr_t)gx) % type_bytes(type) == 0,
-                       "layer_norm_bwd: not aligned to its type");
         const size_t need = scratch_bytes_of(p, rows.n, n_ch, true);
         DRESSI_REQUIRE(
             need == 0 || (scratch && ((uintptr_t)scratch & 15) == 0 && scratch_bytes >= need),

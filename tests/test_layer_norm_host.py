@@ -56,6 +56,33 @@ def test_layer_norm_refuses():
         _refused(_backward(**bad), word)
 
 
+def _at(w=W, b=W, aff=0, mean=X, rstd=X, gw=W, gb=W, items=2, y=Y):
+    """Both calls' results with these addresses, and texts."""
+    out = []
+    for call in (lambda: L.lib.dressi_layer_norm(CTX, X, 0, items, 3, 8, 24, 8, w, b, aff, 1e-5, 0,
+                                                 None, 0, y, mean, rstd),
+                 lambda: L.lib.dressi_layer_norm_bwd(CTX, X, X, 0, items, 5000, 8, 40000, 8, w, b,
+                                                     aff, 0, mean, rstd, None, 0, Y, gw, gb)):
+        out += [call(), L.lib.dressi_last_error().decode()]
+    return out
+
+
+def test_layer_norm_refuses_what_is_not_aligned():
+    """Weight, bias and their gradients to their type, statistics to float32; the weight's type is
+    not the rows'."""
+    for bad in (dict(w=W + 1, aff=1), dict(b=W + 1, aff=2), dict(w=W + 2), dict(b=W + 2),
+                dict(mean=X + 2), dict(rstd=X + 1)):
+        forward, text, backward, other = _at(**bad)
+        assert forward != 0 and backward != 0 and "aligned" in text and "aligned" in other
+    for bad in (dict(gw=W + 1, aff=2), dict(gb=W + 1, aff=1), dict(gw=W + 2), dict(gb=W + 2)):
+        for items in (2, 0):
+            _, _, backward, text = _at(items=items, **bad)
+            assert backward != 0 and "not aligned to its type" in text
+    for fine in (dict(w=W + 2, b=W + 2, aff=1), dict(mean=X + 4, rstd=X + 8)):
+        forward, text, backward, other = _at(y=None, **fine)  # refused, but not for their addresses
+        assert "arguments" in text and "scratch" in other
+
+
 def test_nothing_to_do():
     assert _forward(items=0) == 0 and _forward(px=0) == 0
     assert _backward(gx=None, gw=None, gb=None) == 0
