@@ -859,7 +859,9 @@ int dressi_group_norm_bwd(dressi_ctx* ctx, const void* gy, const void* x,
  * NULL for 1 / 0. mean, rstd [n_items][n_px]: what the backward pass needs;
  * both may be NULL. Sums and statistics are held in 32 bits. scratch: device
  * memory of at least dressi_layer_norm_scratch bytes, aligned to 16 (NULL
- * where that is 0), used by this call only. */
+ * where that is 0), used by this call only. y may be x where that is packed
+ * and a row is at most 32768 channels, or whole vectors of 16 bytes; nothing
+ * that a call writes overlaps what it reads otherwise. */
 size_t dressi_layer_norm_scratch(uint32_t type, uint64_t n_items,
                                  uint64_t n_px, uint32_t n_ch, int backward);
 int dressi_layer_norm(dressi_ctx* ctx, const void* x, uint32_t type,
@@ -870,7 +872,9 @@ int dressi_layer_norm(dressi_ctx* ctx, const void* x, uint32_t type,
                       void* scratch, size_t scratch_bytes, void* y,
                       float* mean, float* rstd);
 /* Its gradients: gy packed -> gx packed (of `type`), gw, gb [n_ch] (of
- * affine_type); any of the three may be NULL. Sums run in a fixed order. */
+ * affine_type); any of the three may be NULL. Sums run in a fixed order. gx may
+ * be gy, or a packed x, where a row is at most 16384 channels or whole vectors
+ * of 16 bytes. */
 int dressi_layer_norm_bwd(dressi_ctx* ctx, const void* gy, const void* x,
                           uint32_t type, uint64_t n_items, uint64_t n_px,
                           uint32_t n_ch, uint64_t item_stride,
@@ -952,11 +956,11 @@ typedef struct dressi_clip_tensor {
 /* The norm of all elements of all tensors together, to `norm` on the device,
  * and each element multiplied by min(1, max_norm / (norm + 1e-6)) in place.
  * max_norm INFINITY: the norm alone, nothing is written. Where the norm is
- * not finite, the elements become what the formula gives (zero or NaN). Squares are added in
- * double, in a fixed order. No two tensors overlap where elements are
- * written. scratch: device memory of dressi_clip_norm_scratch bytes (of the
- * tensors' numbers of elements and types), aligned to 8, or NULL where that
- * is 0, used by this call only. */
+ * not finite, the elements become what the formula gives (zero or NaN).
+ * Squares are added in double, in a fixed order. No two tensors overlap where
+ * elements are written. scratch: device memory of dressi_clip_norm_scratch
+ * bytes (of the tensors' numbers of elements and types), aligned to 8, or NULL
+ * where that is 0, used by this call only. */
 size_t dressi_clip_norm_scratch(const dressi_clip_tensor* tensors,
                                 uint32_t n_tensors);
 int dressi_clip_norm(dressi_ctx* ctx, const dressi_clip_tensor* tensors,

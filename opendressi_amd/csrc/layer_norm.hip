@@ -1324,6 +1324,23 @@ int check_aligned(const char* what, uint32_t type, std::initializer_list<const v
     return DRESSI_OK;
 }
 
+// Whether results, packed, may be written while rows at `in` are read: not over
+// them, unless over each row's own values, where they are packed too and are read
+// by the lanes that write there or before a barrier: in chunks a moved-back vector
+// is not.
+int check_apart(const char* what, const void* out, const void* in, uint32_t type, const Rows& r,
+                bool packed, const Plan& p) {
+    const uintptr_t at = (uintptr_t)out, from = (uintptr_t)in;
+    const uintptr_t bytes = (uintptr_t)(r.n * r.n_ch * type_bytes(type));
+    const bool same = packed && (p.chunks == 0 || r.n_ch % p.v == 0);
+    DRESSI_REQUIRE(!out || (at == from ? same : !packed || at + bytes <= from || from + bytes <= at),
+                   "%s: results overlap what is read", what);
+    return DRESSI_OK;
+}
+bool is_packed(const Rows& r) {
+    return r.n_px == r.n && (r.n <= 1 || r.px_stride == r.n_ch);
+}
+
 // f(a vector's type)
 template <typename F>
 int for_vec(uint32_t type, uint32_t v, F&& f) {
@@ -1378,6 +1395,9 @@ int dressi_layer_norm(dressi_ctx* ctx, const void* x, uint32_t type, uint64_t n_
     DRESSI_REQUIRE(
         need == 0 || (scratch && ((uintptr_t)scratch & 15) == 0 && scratch_bytes >= need),
         "layer_norm: scratch too small or not aligned");
+    if (int rc = check_apart("layer_norm", y, x, type, rows, is_packed(rows), p)) {
+        return rc;
+    }
     const DeviceScope scope(ctx->device);
     DRESSI_TRY_HIP(scope.error());
     const Forward a{x, y, mean, rstd, rows, aff, eps, activation, p.stream, p.stream_in};
@@ -1416,6 +1436,10 @@ int dressi_layer_norm_bwd(dressi_ctx* ctx, const void* gy, const void* x, uint32
         DRESSI_REQUIRE(
             need == 0 || (scratch && ((uintptr_t)scratch & 15) == 0 && scratch_bytes >= need),
             "layer_norm_bwd: scratch too small or not aligned");
+        int rc = check_apart("layer_norm_bwd", gx, gy, type, rows, true, p);
+        if (rc || (rc = check_apart("layer_norm_bwd", gx, x, type, rows, is_packed(rows), p))) {
+            return rc;
+        }
     } else if (!join) {
         return DRESSI_OK;
     }

@@ -479,6 +479,54 @@ def test_past_32_bits(ctx):
     assert not gx[20:rows - 21].any()
 
 
+@pytest.mark.parametrize("kind", TYPES, ids=str)
+@pytest.mark.parametrize("shape", [(1001, 1), (777, 3), (5000, 33), (1301, 64), (700, 1000),
+                                   (300, 2051), (41, 8193), (30, 16384), (5, 16392), (9, 20001),
+                                   (7, 32768), (5, 40000)], ids=str)
+def test_in_place(ctx, kind, shape):
+    """Through the C interface, y over x and gx over gy or x: the bits that they have apart, or
+    refused where another lane may have written what one reads."""
+    import opendressi_amd as od
+    from opendressi_amd import _lib as L
+    from opendressi_amd import ops as K
+    x, gy, w, b = _inputs(shape, kind, 50)
+    rows, c = shape
+    code, vec = TYPES.index(kind), 4 if kind == torch.float32 else 8
+    y, mean, rstd = K.layer_norm(ctx, x, w, b, 1e-5, "silu")
+    gx, gw, gb = K.layer_norm_bwd(ctx, gy, x, mean, rstd, w, b, "silu")
+    scratch = torch.empty(max(L.lib.dressi_layer_norm_scratch(code, 1, rows, c, k) for k in (0, 1)),
+                          dtype=torch.uint8, device="cuda")
+    size = scratch.numel()
+    ctx.use_torch_stream()
+
+    def forward(x):
+        L.check(L.lib.dressi_layer_norm(
+            ctx.handle, x.data_ptr(), code, 1, rows, c, 0, c, w.data_ptr(), b.data_ptr(), 0, 1e-5,
+            L.ACT_SILU, scratch.data_ptr(), size, x.data_ptr(), None, None))
+        return x
+
+    def backward(gy, x, gx):
+        L.check(L.lib.dressi_layer_norm_bwd(
+            ctx.handle, gy.data_ptr(), x.data_ptr(), code, 1, rows, c, 0, c, w.data_ptr(),
+            b.data_ptr(), 0, L.ACT_SILU, mean.data_ptr(), rstd.data_ptr(), scratch.data_ptr(), size,
+            gx.data_ptr(), got_w.data_ptr(), got_b.data_ptr()))
+        return gx
+
+    if c <= 32768 or c % vec == 0:
+        assert torch.equal(forward(x.clone()), y)
+    else:
+        with pytest.raises(od.DressiError, match="overlap"):
+            forward(x.clone())
+    for over in (0, 1):
+        args, (got_w, got_b) = [gy.clone(), x.clone()], (torch.empty_like(w) for _ in range(2))
+        if c <= 16384 or c % vec == 0:
+            assert torch.equal(backward(*args, args[over]), gx)
+            assert torch.equal(got_w, gw) and torch.equal(got_b, gb)
+        else:
+            with pytest.raises(od.DressiError, match="overlap"):
+                backward(*args, args[over])
+
+
 def test_refusals(ctx, vctx):
     import opendressi_amd as od
     import opendressi_amd.torch as dr

@@ -83,6 +83,24 @@ def test_layer_norm_refuses_what_is_not_aligned():
         assert "arguments" in text and "scratch" in other
 
 
+def test_layer_norm_refuses_results_over_what_is_read():
+    """Over part of the rows, over rows with gaps, and in place where a row's last vector is read
+    by others than those that write it."""
+    far = 1 << 40
+    for bad in (dict(y=X + 4), dict(y=X + 188), dict(x=Y + 188), dict(y=X, step=9, item=27),
+                dict(y=X, item=25)):
+        _refused(_forward(**bad), "overlap")
+    for bad in (dict(gx=X + 4), dict(gx=X + 188), dict(gy=far, gx=X + 64), dict(gx=X - 64),
+                dict(gy=far, gx=X, step=9)):
+        _refused(_backward(**bad), "overlap")
+    for type, c in ((0, 32769), (1, 32772), (2, 50001)):
+        rows = dict(type=type, c=c, step=c, items=1, scratch=far, size=1 << 30)
+        _refused(_forward(y=X, item=3 * c, **rows), "overlap")
+        _refused(_backward(gx=X, **rows), "overlap")
+        _refused(_backward(gy=far, gx=X, **rows), "overlap")
+    _refused(_backward(gx=X, type=1, c=16387, step=16387, items=1), "overlap")
+
+
 def test_nothing_to_do():
     assert _forward(items=0) == 0 and _forward(px=0) == 0
     assert _backward(gx=None, gw=None, gb=None) == 0
