@@ -1157,6 +1157,30 @@ int for_value(uint32_t x, F&& f) {
     return f(std::integral_constant<uint32_t, FIRST>());
 }
 
+// f(values) of a row that one lane holds value by value, its length rounded up to
+// a power of two: up to 3 values of 32 bits, 7 of 16.
+template <typename T, bool WHOLE, typename F>
+int for_few(uint32_t elems, F&& f) {
+    if constexpr (sizeof(T) == 4 && WHOLE) {
+        return for_value<1, 2>(elems, f);
+    } else if constexpr (sizeof(T) == 4) {
+        return for_value<4>(elems, f);
+    } else if constexpr (WHOLE) {
+        return for_value<1, 2, 4>(elems, f);
+    } else {
+        return for_value<4, 8>(elems, f);
+    }
+}
+// f(lanes) of a row with a vector for each: one is always whole.
+template <bool WHOLE, typename F>
+int for_lanes(uint32_t lanes, F&& f) {
+    if constexpr (WHOLE) {
+        return for_value<1, 2, 4, 8, 16, 32, 64>(lanes, f);
+    } else {
+        return for_value<2, 4, 8, 16, 32, 64>(lanes, f);
+    }
+}
+
 template <typename T, int V>
 int forward(hipStream_t s, const Plan& p, const Forward& a, void* scratch) {
     if (p.chunks) {
@@ -1182,7 +1206,7 @@ int forward(hipStream_t s, const Plan& p, const Forward& a, void* scratch) {
                           s, a);
         };
         if constexpr (V == 1) {
-            return for_value<1, 2, 4, 8>(p.elems, [&](auto elems) {
+            return for_few<T, W>(p.elems, [&](auto elems) {
                 return rows(std::integral_constant<int, 1>(), elems);
             });
         } else {
@@ -1209,12 +1233,14 @@ int forward(hipStream_t s, const Plan& p, const Forward& a, void* scratch) {
                     return for_value<2, 3, 4>(p.elems / V, wave);
                 }
             }
-            if (p.elems > V) {
-                return for_value<8, 16>(p.lanes, [&](auto lanes) {
-                    return rows(lanes, std::integral_constant<int, 3 * V>());
-                });
+            if constexpr (!W) {  // 17, or 33 to 35, vectors
+                if (p.elems > V) {
+                    return for_value<8, 16>(p.lanes, [&](auto lanes) {
+                        return rows(lanes, std::integral_constant<int, 3 * V>());
+                    });
+                }
             }
-            return for_value<1, 2, 4, 8, 16, 32, 64>(p.lanes, [&](auto lanes) {
+            return for_lanes<W>(p.lanes, [&](auto lanes) {
                 return rows(lanes, std::integral_constant<int, V>());
             });
         }
@@ -1244,7 +1270,7 @@ int backward(hipStream_t s, const Plan& p, const Backward& a, float2* row_part) 
             return launch(k_ln_bwd_rows<T, V, L, K, W>, p.groups, ~0u, kThreads, s, a);
         };
         if constexpr (V == 1) {
-            return for_value<1, 2, 4, 8>(p.elems, [&](auto elems) {
+            return for_few<T, W>(p.elems, [&](auto elems) {
                 return rows(std::integral_constant<int, 1>(), elems);
             });
         } else {
@@ -1272,7 +1298,7 @@ int backward(hipStream_t s, const Plan& p, const Backward& a, float2* row_part) 
                     });
                 }
             }
-            return for_value<1, 2, 4, 8, 16, 32, 64>(p.lanes, [&](auto lanes) {
+            return for_lanes<W>(p.lanes, [&](auto lanes) {
                 return rows(lanes, std::integral_constant<int, 1>());
             });
         }
