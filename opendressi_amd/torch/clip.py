@@ -5,6 +5,7 @@ inside its own step). No counterpart in the reference's surface.
 from __future__ import annotations
 
 import math
+import operator
 from array import array
 from itertools import chain
 
@@ -59,6 +60,7 @@ class _Gradients:
                     views.append((g, g.contiguous()))
                     g = views[-1][1]
                 packed.append(g)
+        self.dense = map(operator.is_, grads, packed)  # of each, whether it is its own packed copy
         # three words an entry, as in dressi_clip_tensor
         self.table = array("Q", chain.from_iterable(zip(
             map(torch.Tensor.data_ptr, packed), map(torch.Tensor.numel, packed),
@@ -113,7 +115,7 @@ def clip_grad_norm_(ctx: RasterizeHipContext, parameters, max_norm: float,
     g = _Gradients(ctx, parameters)
     # packed ones are looked at by the call
     if max_norm < math.inf and g.views and (not all(_apart(v) for v, _ in g.views) or
-                                            shared(g.grads, map(_dense, g.grads))):
+                                            shared(g.grads, g.dense)):
         raise ValueError("gradients are the same or share memory")
     if error_if_nonfinite:
         if torch.cuda.is_current_stream_capturing():

@@ -59,9 +59,20 @@ def group_norm(ctx: RasterizeHipContext, x: torch.Tensor, groups: int, weight=No
 
 
 def _moved(dev, x, weight, bias):
-    """The three on the context's device, the last two packed."""
-    x, weight, bias = (None if t is None else t.detach().to(dev) for t in (x, weight, bias))
-    return (x, *(None if t is None else t.contiguous() for t in (weight, bias)))
+    """The three on the context's device, the last two packed; for where
+    autograd does not look."""
+    x = x.to(dev)
+    return x, *(None if t is None else t.to(dev).contiguous() for t in (weight, bias))
+
+
+def _followed(*tensors) -> bool:
+    """Whether autograd follows one of them. A tangent of forward mode, which a
+    Function refuses, would be lost on the short way past it."""
+    reverse = torch.is_grad_enabled()
+    for t in tensors:
+        if t is not None and (reverse and t.requires_grad or unpack_dual(t).tangent is not None):
+            return True
+    return False
 
 
 class _LayerNormFn(torch.autograd.Function):
@@ -99,10 +110,7 @@ def layer_norm(ctx: RasterizeHipContext, x: torch.Tensor, weight=None, bias=None
     activation is "none", "relu", "silu" or "gelu". Differentiable w.r.t. x,
     weight and bias, in reverse mode; forward mode's dual tensors are refused."""
     _check_tensors(x, weight, bias)
-    given = [t for t in (x, weight, bias) if t is not None]
-    # a tangent of forward mode, which a Function refuses, would be lost on the short way
-    if torch.is_grad_enabled() and any(t.requires_grad for t in given) or \
-            any(unpack_dual(t).tangent is not None for t in given):
+    if _followed(x, weight, bias):
         return _LayerNormFn.apply(x, weight, bias, ctx, float(eps), activation)
     with ctx.lock:
         return K.layer_norm(ctx._ctx, *_moved(ctx.device, x, weight, bias), float(eps), activation,
