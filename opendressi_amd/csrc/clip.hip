@@ -13,9 +13,12 @@
 // the die that read it, so that it finds what was read last in a cache. Where the
 // norm is below max_norm the second ends there.
 //
-// 2^28 float32 elements: 155 us for the norm, 6.9 TB/s, and 355 for the scaling,
-// 6.0 TB/s over the 2.1 GB that it reads and writes; 2^24 15 and 15; three small
-// tensors 3.7 in all (2^n: in graphs of some calls).
+// 2^28 float32 elements: 158 us for the norm, 6.8 TB/s, and 375 for the scaling,
+// 5.7 TB/s over the 2.1 GB that it reads and writes; 2^28 of 16 bits 83 and 178,
+// 6.0 TB/s; 2^24 float32 17 and 21; three small tensors 3.4 in all. These times and
+// those below are of graphs of some calls, from 48 MB of gradients on of others
+// each time, as a training step has: over the same ones again a cache would still
+// hold what the call before wrote last (2^28 float32 522 us in place of 533).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -257,8 +260,8 @@ __global__ __launch_bounds__(kThreads) void k_clip_scale(const Table tb, const d
 }
 
 // A small set: norm and scaling by one workgroup that holds all vectors.
-// `n_chunks` and `first` count vectors. 1930 elements 3.7 us, 30000 8.3: two
-// launches over 40000 take 5.8, but 4 us more of the host, which is what counts
+// `n_chunks` and `first` count vectors. 1930 elements 3.4 us, 30000 8.1: two
+// launches over 40000 take 5.6, but 4 us more of the host, which is what counts
 // outside of a graph.
 template <bool LARGEST>
 __global__ __launch_bounds__(kSmallThreads) void k_clip_small(const Table tb, double max_norm,
@@ -359,18 +362,21 @@ __global__ __launch_bounds__(kSmallThreads) void k_clip_small(const Table tb, do
     }
 }
 
-// Bytes of all tensors up to which a chunk is 4 KB and not 16: more workgroups
-// (2^22 bfloat16 8.3 us, 9.5 with chunks of 16 KB turned round; 2^22 float32 10.4
-// and 11.9 the other way).
+// Bytes of all tensors up to which a chunk is 4 KB and not 16: more workgroups (42
+// tensors of 588000 bfloat16 in all 7.5 us, 10.0 with chunks of 16 KB; 2^22 bfloat16
+// 8.2 with those, 9.4 with 4 KB).
 constexpr uint64_t kFewBytes = 4ull << 20;
 
 // Bytes that the second pass may find in the last-level cache (256 MB); the rest
-// goes past it both times. 2^28 float32: 505 us, 516 with 160 MB kept and 524 with
-// 96.
-constexpr uint64_t kKeepBytes = 224ull << 20;
+// goes past it both times. With more, what the cache held from before has to leave
+// it in between: 2^28 float32 533 us (550 with 224 MB kept, 527 with none), 2^26
+// 125 (142, 129), 2^24 38 (38, 37), and 32 where they were written just before (32,
+// 35).
+constexpr uint64_t kKeepBytes = 96ull << 20;
 
-// Workgroups of a launch: four a compute unit (2^28 float32 538 us with half of
-// them, 507 with twice as many, but 2^24 35 where these take 30).
+// Workgroups of a launch: four a compute unit (2^28 float32 533 us, the norm alone
+// 158; 541 and 186 with half of them, 527 and 167 with twice as many, but 2^24 41
+// where these take 38).
 constexpr uint32_t kGroups = 1024;
 
 int check_tensors(const dressi_clip_tensor* t, uint32_t n, bool written) {
