@@ -25,7 +25,10 @@
 // deviation that forward left, and computes z as it did: relu masks what y says.
 //
 // The times beside the choices below are those of graphs of some calls, replayed,
-// both sides in turn, statistics written.
+// both sides in turn, statistics written; from 48 MB of x on over inputs that are
+// others each time, 768 MB of x and as much of gy in all, for over the same ones
+// again a cache may hold a part (16384 x 4096 bfloat16 forward 45 us in place of
+// 54).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -214,20 +217,20 @@ struct Forward {
 // ---------------------------------------------------------------------------
 
 // Whether a wave's load is one piece of memory, or long pieces, and may go past
-// the caches: in short ones it would read lines again (4194304 x 64 bfloat16 by
-// four lanes 237 us, through the caches 219; by eight 180 and 189).
+// the caches: in short ones it would read lines again (3000000 x 130 bfloat16, three
+// vectors each by eight lanes, 456 us, through the caches 433).
 template <int L, int K>
 constexpr bool kLongPieces = K == 1 || L >= 32;
 
-// Rows that a lane has in flight, of E values each: 64 bytes (262144 x 64 float32,
-// gelu, 16 values a lane: 24.2 us, 25.6 with 128 bytes).
+// Rows that a lane has in flight, of E values each: 64 bytes (500000 x 400 float32,
+// gelu, 8 values a lane: 287 us, 318 with 128 bytes).
 template <typename T, int E>
 constexpr int kInFlight = E * sizeof(T) >= 48 ? 1 : E * sizeof(T) >= 32 ? 2 : 4;
 
 // L lanes hold a row, K vectors each. 8 x 1024 x 1024 x 64 bfloat16, silu, without
-// statistics: 349 us, 6.1 TB/s; 64 of 96 channels of 512 x 512: 14.0, whose lines
-// hold half as much again; 2000000 x 24 float32 58, 6.7 TB/s; one row 4. Gelu's
-// arithmetic is what bounds it in 16 bits (4194304 x 64: 232 us, silu 183).
+// statistics: 358 us, 6.0 TB/s; 64 of 96 channels of 512 x 512: 14.0, whose lines
+// hold half as much again; 2000000 x 24 float32 65, 5.9 TB/s; one row 3. Gelu's
+// arithmetic is what bounds it in 16 bits (4194304 x 64: 227 us, silu 175).
 template <typename T, int V, int L, int K, bool WHOLE>
 __global__ __launch_bounds__(kThreads) void k_ln_rows(const Forward a) {
     constexpr int E = K * V, R = kInFlight<T, E>;
@@ -331,10 +334,10 @@ __global__ __launch_bounds__(kThreads) void k_ln_rows(const Forward a) {
 }
 
 // A workgroup holds a row, K vectors a thread. HOLD: weight and bias stay in
-// registers between rows. 16384 x 4096 bfloat16: 45 us, 6.0 TB/s; 4096 x 16384
-// float32, which waits for its barriers with few workgroups: 110, 4.9 TB/s. 1024
+// registers between rows. 16384 x 4096 bfloat16: 54 us, 4.9 TB/s; 4096 x 16384
+// float32, which waits for its barriers with few workgroups: 105, 5.1 TB/s. 1024
 // threads with 16 values are held to 64 registers, so that a compute unit has two
-// workgroups of them (3000 x 14000 float32 61 us, 66 without).
+// workgroups of them (4000 x 15000 bfloat16 63 us, 71 without).
 template <typename T, int V, int K, uint32_t THREADS, bool HOLD, bool WHOLE>
 __global__ __launch_bounds__(THREADS, THREADS == 1024 && K * V == 16 ? 8 : 1) void k_ln_wide(
     const Forward a) {
@@ -405,7 +408,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 && K * V == 16 ? 8 : 1) vo
 // thread, in two passes: one leaves every chunk's (mean, squares about it), the
 // other joins those of its row, every wave for itself. A workgroup keeps to one
 // chunk, whose weight and bias it holds, and takes every gridDim.x-th row. 1000 x
-// 60001 bfloat16: 66 us, 5.4 TB/s over rows read twice; backward 153, 3.9.
+// 60001 bfloat16: 75 us, 4.8 TB/s over rows read twice; backward 169, 3.6.
 constexpr int kChunkElems = 32, kChunkElemsBwd = 16;  // a thread's
 
 // A thread's vectors of a chunk.
@@ -615,14 +618,15 @@ __device__ __forceinline__ void write_sums(const Backward& a, uint32_t ch, uint3
 }
 
 // Whether a lane reads its next row while it works on one, or else two at a time:
-// the first where all lanes have values (4194304 x 64 bfloat16 308 us, 344 by two)
-// and for long rows of 32 bits (100000 x 300 63 and 68), the second in 16 bits
-// where some do not (500000 x 200 118, 129 ahead; 500000 x 248 140 and 149).
+// the first where all lanes have values (4194304 x 64 bfloat16 297 us, 300 by two)
+// and for long rows of 32 bits (100000 x 300 77 and 85, 500000 x 100 108 and 112),
+// the second in 16 bits where some do not (500000 x 200 118, 129 ahead; 500000 x
+// 248 140 and 150).
 template <int V, int L, bool WHOLE>
 constexpr bool kAhead = WHOLE || (V == 4 && L >= 32);
 
 // L lanes hold a row, K vectors each, and keep the sums of their columns. 4 x 1024 x
-// 1024 x 64 bfloat16, silu: 308 us, 5.3 TB/s (gelu 345); 500000 x 100 float32 108,
+// 1024 x 64 bfloat16, silu: 299 us, 5.4 TB/s (gelu 332); 500000 x 100 float32 108,
 // 5.5 TB/s. Rows of just over a power of two of vectors leave half of the lanes
 // idle: 800000 x 130 bfloat16 150 us, 4.2 TB/s.
 template <typename T, int V, int L, int K, bool WHOLE>
@@ -1033,15 +1037,15 @@ constexpr uint32_t vec_of(uint32_t type, uint32_t n_ch) {
 
 // Values of a row up to which a wave, then a workgroup, holds it. Backward a wave
 // with two vectors of 16 bits a lane holds so many registers that there are two a
-// SIMD (65536 x 1024 bfloat16 81 us, 75 with 128 lanes a row; float32 142 and 148).
+// SIMD (65536 x 1024 bfloat16 87 us, 77 with 128 lanes a row; float32 143 and 149).
 constexpr uint32_t kWaveElems = 64 * 32;
 constexpr uint32_t wave_elems_bwd(uint32_t v) { return 64 * (v == 4 ? 16 : 8); }
 constexpr uint32_t kHoldElems = 1024 * 32, kHoldElemsBwd = 1024 * 16;
 
 // Bytes of results, and of inputs, from which they go past the caches. Results:
-// 1000000 x 128 bfloat16 75 us so and 90 through them. Inputs, where the caches
-// do not hold them from one call to the next: 100000 x 511 float32 68 and 79,
-// 30000000 x 8 float16 170 and 212.
+// 1000000 x 128 bfloat16 84 us so and 87 through them, 30000000 x 8 float16 167 and
+// 214. Inputs: 30000000 x 8 float16 167 and 216; below, where a layer before may
+// have left them in a cache, 100000 x 511 float32 takes 73 so and 71 through them.
 constexpr uint64_t kStreamBytes = 32ull << 20, kStreamInBytes = 256ull << 20;
 
 struct Plan {
@@ -1054,10 +1058,12 @@ struct Plan {
 };
 
 // Lanes and values of each for a row that a wave holds. One vector a lane, where
-// a wave's load or store is one piece of memory (2000000 x 24 float32 forward 58
-// us, 87 with six vectors a lane); forward three, where fewer than 9 of 16 lanes
-// had one (800000 x 130 bfloat16 75 us and 84; backward the registers of three
-// cost more than the lanes). Longer rows take a whole wave.
+// a wave's load or store is one piece of memory (2000000 x 24 float32 forward 65
+// us, 88 with six vectors a lane); forward three, where fewer than 9 of 16 lanes
+// had one (500000 x 264 float16 102 us, 114 with one; rows of 17 vectors gain by it
+// where a cache holds x, and lose where none does: 800000 x 130 bfloat16 78 and 80,
+// 102 and 91; backward the registers of three cost more than the lanes). Longer
+// rows take a whole wave.
 void cut_row(Plan& p, uint32_t n_ch, bool backward) {
     const uint32_t vecs = div_up(n_ch, p.v);
     p.lanes = p.elems = 1;
@@ -1098,12 +1104,12 @@ Plan make_plan(uint32_t type, uint64_t rows, uint32_t n_ch, bool backward) {
             p.elems *= 2;
         }
         if (!backward && n_ch > 8192 && n_ch <= 16 * 1024) {
-            p.elems = 16;  // 4096 x 9216 bfloat16 30 us, 45 with 32 in half the threads
+            p.elems = 16;  // 4096 x 9216 bfloat16 38 us, 52 with 32 in half the threads
         }
         p.lanes = div_up(div_up(n_ch, p.elems), 64) * 64;
         // 512 threads for each of 256 compute units, or twice that where they hold 8 values; fewer
-        // where their sums would be as much as the rows (1021 x 4096 bfloat16 16.8 us, 20.9 with
-        // 512 workgroups)
+        // where their sums would be as much as the rows (1021 x 4096 bfloat16 16.3 us, 21.2 with
+        // 512 workgroups; 1021 x 2048 11.1 and 13.8)
         const uint32_t most = (p.elems == 16 ? 256 : 512) * 256 / std::min(256u, p.lanes);
         const uint64_t pairs = p.lanes > 256 ? rows : (rows + 1) / 2;
         p.groups = (uint32_t)std::min<uint64_t>({pairs, most, std::max<uint64_t>(256, pairs / 8)});
@@ -1111,13 +1117,13 @@ Plan make_plan(uint32_t type, uint64_t rows, uint32_t n_ch, bool backward) {
         cut_row(p, n_ch, backward);
         const bool ahead = n_ch == p.lanes * p.elems || (p.v == 4 && p.lanes >= 32);  // kAhead
         const uint64_t take = kThreads / p.lanes * (ahead ? 1 : 2);
-        // four for each compute unit: 1280, where some have five, take 400 us for 4194304 x 64
-        // bfloat16, 768 345 and these 317
+        // four for each compute unit: 1280, where some have five, take 370 us for 4194304 x 64
+        // bfloat16, 768 329 and these 299
         p.groups = (uint32_t)std::min<uint64_t>((rows + take - 1) / take, 1024);
     }
     p.whole = n_ch == p.lanes * p.elems;
     // a store that does not fill lines is slower past the caches, which would have
-    // filled them (1500000 x 35 float32 in pieces of 32 bytes: 300 and 98 us)
+    // filled them (20000000 x 7 float16 backward, value by value: 667 and 392 us)
     p.stream = p.stream && (p.chunks > 0 || p.elems == p.v || p.lanes >= 8);
     return p;
 }
@@ -1201,7 +1207,7 @@ int forward(hipStream_t s, const Plan& p, const Forward& a, void* scratch) {
         const auto rows = [&](auto lanes, auto elems) {
             constexpr int L = decltype(lanes)::value, K = decltype(elems)::value / V;
             constexpr uint32_t kTake = kThreads / L * kInFlight<T, K * V>;
-            // 4194304 x 64 bfloat16: 198 us, 220 with 2048 workgroups
+            // 4194304 x 64 bfloat16: 175 us, 191 with 2048 workgroups
             return launch(k_ln_rows<T, V, L, K, W>, (a.rows.n + kTake - 1) / kTake, 16384, kThreads,
                           s, a);
         };
