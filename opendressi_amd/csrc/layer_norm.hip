@@ -1365,8 +1365,8 @@ int check_apart(const char* what, const void* out, const void* in, uint32_t type
     const uintptr_t at = (uintptr_t)out, from = (uintptr_t)in;
     const uintptr_t bytes = (uintptr_t)(r.n * r.n_ch * type_bytes(type));
     const bool same = packed && (p.chunks == 0 || r.n_ch % p.v == 0);
-    DRESSI_REQUIRE(!out || (at == from ? same : !packed || at + bytes <= from || from + bytes <= at),
-                   "%s: results overlap what is read", what);
+    const bool clear = !packed || at + bytes <= from || from + bytes <= at;
+    DRESSI_REQUIRE(!out || (at == from ? same : clear), "%s: results overlap what is read", what);
     return DRESSI_OK;
 }
 bool is_packed(const Rows& r) {
